@@ -100,7 +100,7 @@ def draw(rng):
         kv = rng.choice([1, 2, 4, 8])
         group = rng.choice([1, 2, 4, 5, 8, 16])
         batch = _logint(rng, 1, 128)
-        longest = min(_logint(rng, 1, 120000), 16384 * 64 * 512 // (batch * kv * dim))
+        longest = min(_logint(rng, 1, 120000), 16384 * 40 * 512 // (batch * kv * dim))
         return {"op": op, "batch": batch, "longest": max(1, longest), "ragged": batch > 1 and rng.random() < 0.8,
                 "q_heads": kv * group, "kv_heads": kv, "dim": dim, "page": rng.choice([16, 24, 32, 64])}
     kh = rng.choice([4, 8, 16])
