@@ -101,7 +101,9 @@ enum mcv_tuning_key {
 int mcv_set_tuning(int key, int value);
 /* Device-side error bits recorded since the last call (and cleared by it):
  * bit 0 = a bounded wait inside a kernel gave up (that kernel returned early
- * and its outputs are incomplete).  Synchronises the current device. */
+ * and its outputs are incomplete); bit 1 = an index in device memory (page,
+ * sequence row, state slot, sequence bound) was out of range and was not
+ * followed.  Synchronises the current device. */
 unsigned mcv_device_errors(void);
 int mcv_get_tuning(int key);
 
@@ -522,6 +524,136 @@ int mcv_rms_norm(const void* x, const void* gamma, void* out, int64_t rows, int6
  * fp32 g / (1 + exp(-g)) * u rounded to fp16.  Replaces silu_mul
  * (src/csrc/lib/ops.cpp:437-456, op_kernel/silu_mul_custom.cpp:63-72). */
 int mcv_silu_mul(const void* gate, const void* up, void* out, int64_t n, mcv_stream_t stream);
+
+/* ======================================================================== */
+/* Token mixing: rotary positions, paged attention, the gated delta rule      */
+/* ======================================================================== */
+/* What the decoder's layers do between their projections, for batches of
+ * sequences.  Indices that the kernels read from device memory (pages,
+ * sequence rows, state slots, sequence bounds) are checked there: one that is
+ * out of range is never followed and sets bit 1 of mcv_device_errors(). */
+
+/* fp16 rows of several heads: head h of token t starts at
+ * data + t * token_stride + h * head_stride (in elements, multiples of 8) and
+ * is contiguous; data is 16-byte aligned.  Heads of one token may not overlap. */
+typedef struct mcv_rows {
+    const void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+} mcv_rows;
+
+/* A paged key-value cache of one layer: slot s of page p holds the fp16 rows
+ * of kv head h at element p * page_stride + (h * page_size + s) * head_dim of
+ * k and of v.  A sequence's token i lies in slot i % page_size of page
+ * page_table[row][i / page_size] (int32).  Any page_size; page_stride a multiple
+ * of 8 and at least kv_heads * page_size * head_dim. */
+typedef struct mcv_kv_cache {
+    void* k;
+    void* v;
+    int64_t page_stride;
+    int32_t num_pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+} mcv_kv_cache;
+
+/* Rotary positions with several axes: frequency i < rotary_dim / 2 turns the
+ * pair (x[i], x[i + rotary_dim / 2]) of a head by
+ * 2 pi * turns[i] * position[axis[i]]; dimensions from rotary_dim on stay. */
+#define MCV_MROPE_MAX_FREQS 128
+typedef struct mcv_mrope_spec {
+    int32_t rotary_dim;
+    int32_t axes;
+    double turns[MCV_MROPE_MAX_FREQS];
+    uint8_t axis[MCV_MROPE_MAX_FREQS];
+} mcv_mrope_spec;
+
+/* Fills *spec: turns[i] = theta^(-2i / rotary_dim) / (2 pi), and the axes by
+ * `sections` (int32 [axes], adding up to rotary_dim / 2): contiguous blocks, or
+ * interleaved (axis a > 0 owns i = a, a + axes, ... below axes * sections[a],
+ * axis 0 the rest).  rotary_dim a multiple of 16 up to 256; 1 to 4 axes (one
+ * axis: ordinary rotary positions).  Host only; a caller with scaled
+ * frequencies may set turns[] itself. */
+int mcv_mrope_init(mcv_mrope_spec* spec, int rotary_dim, int axes, const int32_t* sections, int interleaved,
+                   double theta);
+
+/* Rotates x into out.  positions int32 [axes][tokens]; out is dense fp16
+ * [tokens][heads][head_dim], or x->data itself (in place, with x's strides).
+ * head_dim a multiple of 8.  Angles are taken in fp64, so far positions keep
+ * their accuracy; the rotation is fp32, rounded once. */
+int mcv_mrope(const mcv_rows* x, void* out, const mcv_mrope_spec* spec, const void* positions, int64_t tokens,
+              int64_t heads, int64_t head_dim, mcv_stream_t stream);
+
+/* Rotates q into q_out (as mcv_mrope) and k straight into the cache, and
+ * copies v there, in one launch - the step between a full-attention layer's
+ * projections and its attention, for decode batches and prompts alike.  Token t
+ * goes to place index[t] (int32) of the sequence in row seq[t] (int32; NULL:
+ * row t) of page_table [table_rows][table_cols]; a negative index writes
+ * nothing to the cache.  No two tokens of a call may share a place. */
+int mcv_mrope_append_kv(const mcv_rows* q, void* q_out, const mcv_rows* k, const mcv_rows* v,
+                        const mcv_mrope_spec* spec, const void* positions, const mcv_kv_cache* cache,
+                        const void* page_table, int64_t table_rows, int64_t table_cols, const void* seq,
+                        const void* index, int64_t tokens, int64_t q_heads, mcv_stream_t stream);
+
+/* Workspace bytes of mcv_paged_attention_decode on the current device (0 for
+ * unsupported heads); zero-fill it once, every call leaves it ready for the
+ * next.  Calls that may overlap on the GPU need workspaces of their own. */
+size_t mcv_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+
+/* out fp16 [batch][q_heads][head_dim] = softmax(scale q K^T) V of one new token
+ * per sequence over the first lengths[b] (int32) keys of its cache; query heads
+ * h * q_heads / kv_heads ... share kv head h.  lse (fp32 [batch][q_heads], may
+ * be NULL) receives log sum exp of the scaled scores.  Row b of page_table
+ * (int32 [batch][table_cols]) holds the sequence's pages; entries behind its
+ * length are not read.  A length of 0 or less gives a zero row and lse -inf; one
+ * beyond table_cols * page_size is cut to that (and sets the error bit), and
+ * a page out of range reads as zeros (and sets it).  head_dim 64, 128 or 256;
+ * batch up to 4096.  Scores, softmax and sums are fp32; the cache is read once
+ * up to 16 query heads per kv head. */
+int mcv_paged_attention_decode(const mcv_rows* q, const mcv_kv_cache* cache, const void* page_table,
+                               int64_t table_cols, const void* lengths, void* out, void* lse, int64_t batch,
+                               int64_t q_heads, float scale, void* workspace, size_t workspace_bytes,
+                               mcv_stream_t stream);
+
+/* The gated delta rule of the linear-attention layers.  Per value head, state
+ * S [key_dim][value_dim]:
+ *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q.
+ * l2_eps >= 0: q and k are first divided by sqrt(sum x^2 + l2_eps); below 0:
+ * taken as they are (keys are then expected to be of norm 1 or less).  Value
+ * heads h * v_heads / k_heads ... share key head h.  States are read from slot
+ * state_index[b] of state_in and written to the same slot of state_out, which
+ * may be state_in itself; a negative slot skips the sequence (its rows of out and
+ * its state stay as they were).  No two sequences of a call may share a slot.
+ * key_dim 64 or 128, value_dim a multiple of 16 up to 1024. */
+typedef struct mcv_gated_delta {
+    mcv_rows q, k;           /* fp16, k_heads heads of key_dim */
+    mcv_rows v;              /* fp16, v_heads heads of value_dim */
+    const void* g;           /* fp32 [tokens][v_heads], log decay */
+    const void* beta;        /* fp32 [tokens][v_heads] */
+    void* out;               /* fp16 [tokens][v_heads][value_dim] */
+    const void* state_in;    /* fp32 [slots][v_heads][key_dim][value_dim] */
+    void* state_out;         /* the same */
+    const void* state_index; /* int32 [batch], NULL: sequence b has slot b */
+    int64_t slots;
+    int32_t k_heads, v_heads, key_dim, value_dim;
+    float scale;
+    float l2_eps;
+} mcv_gated_delta;
+
+/* One token per sequence (token b belongs to sequence b): the decode step.
+ * Replaces linear_gated_delta_rule_step. */
+int mcv_gated_delta_step(const mcv_gated_delta* args, int64_t batch, mcv_stream_t stream);
+
+/* Whole prompts, packed: sequence b has tokens cu_seqlens[b] .. cu_seqlens[b+1]
+ * (int32 [batch + 1]); rows of out that belong to no sequence stay as they were.
+ * state_in NULL: sequences start from zero; state_out NULL: final states are not
+ * kept.  The workspace needs no preparation and holds nothing between calls;
+ * calls that may overlap on the GPU need workspaces of their own.
+ * Replaces linear_gated_delta_rule. */
+size_t mcv_gated_delta_workspace_size(int64_t tokens, int64_t batch, int64_t v_heads, int64_t key_dim,
+                                      int64_t value_dim);
+int mcv_gated_delta_prefill(const mcv_gated_delta* args, const void* cu_seqlens, int64_t tokens, int64_t batch,
+                            void* workspace, size_t workspace_bytes, mcv_stream_t stream);
 
 /* ======================================================================== */
 /* Decode dispatch: which weight format a projection's matmul runs on        */

@@ -11,6 +11,9 @@ unsigned take_w4a16_device_error();
 unsigned take_dense_device_error();
 unsigned take_gemm_device_error();
 unsigned take_dense_gemm_device_error();
+unsigned take_mrope_device_error();
+unsigned take_attention_device_error();
+unsigned take_gated_delta_device_error();
 
 namespace {
 thread_local std::string g_last_error;
@@ -87,7 +90,8 @@ int mcv_get_tuning(int key) { return mcv::tuning(key); }
 unsigned mcv_device_errors(void) {
     cudaDeviceSynchronize();
     return mcv::take_w4a16_device_error() | mcv::take_dense_device_error() | mcv::take_gemm_device_error() |
-           mcv::take_dense_gemm_device_error();
+           mcv::take_dense_gemm_device_error() | mcv::take_mrope_device_error() | mcv::take_attention_device_error() |
+           mcv::take_gated_delta_device_error();
 }
 
 }  // extern "C"

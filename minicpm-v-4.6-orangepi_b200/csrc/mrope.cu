@@ -1,0 +1,311 @@
+// Rotary positions with several axes (time, height, width) on the query and
+// key heads, with the keys and values written into a paged cache in the same
+// launch: what a full-attention layer does between its projections and the
+// attention of the step.
+//
+// Frequency i of R/2 turns the pair (x_i, x_{i + R/2}) by
+// pos[axis(i)] * f_i; the dimensions from R on pass unchanged.  The angle of
+// a far position (2^18 and beyond) has no correct digits left in fp32, so it is
+// kept in turns, pos * (f_i / 2 pi), in fp64 and reduced to its fraction
+// exactly before sin and cos are taken in fp32 (CUDA's sincospif).
+//
+// Bound by bytes (each row read once and written once; about 3 operations per
+// rotated element).  A block takes a few tokens: its first threads compute
+// the R/2 angles of each into shared memory, once for all heads, and find the
+// tokens' places in the cache; then all threads walk (token, head, 16-byte
+// vector) items, a rotated item being the two vectors of its halves, so that
+// every access is a 16-byte one and q may be rotated in place.
+#include "mixing.cuh"
+
+#include <cmath>
+
+namespace mcv {
+unsigned take_mrope_device_error();
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 4;   // tokens per block
+
+static __device__ unsigned g_mrope_dev_error;
+
+struct RopeArgs {
+    const __half* q;
+    const __half* k;   // null: q alone
+    const __half* v;
+    __half* q_out;
+    __half* ck;
+    __half* cv;
+    const int32_t* positions;  // [axes][tokens]
+    const int32_t* table;
+    const int32_t* seq;        // null: token t belongs to row t
+    const int32_t* index;
+    int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
+    int64_t page_stride, table_cols;
+    int tokens, q_heads, kv_heads, dim, page_size, num_pages, table_rows;
+    int per_block, in_place;
+};
+
+// Rotates eight pairs: a' = a cos - b sin, b' = b cos + a sin, in fp32, one
+// rounding each to the output's fp16.
+__device__ __forceinline__ void rotate8(uint4& a, uint4& b, const float2* cs) {
+    uint32_t* ap = &a.x;
+    uint32_t* bp = &b.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(u32_as_h2(ap[i])), y = __half22float2(u32_as_h2(bp[i]));
+        const float2 c0 = cs[2 * i], c1 = cs[2 * i + 1];
+        ap[i] = h2_as_u32(__floats2half2_rn(x.x * c0.x - y.x * c0.y, x.y * c1.x - y.y * c1.y));
+        bp[i] = h2_as_u32(__floats2half2_rn(y.x * c0.x + x.x * c0.y, y.y * c1.x + x.y * c1.y));
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) mrope_kernel(const __grid_constant__ mcv_mrope_spec spec, RopeArgs a) {
+    __shared__ float2 cs[kMaxTokens][MCV_MROPE_MAX_FREQS];
+    __shared__ int64_t place[kMaxTokens];   // element offset of the token's slot in head 0, -1: not written
+    pdl_trigger();
+    pdl_wait();
+    const int half = spec.rotary_dim / 2;
+    const int t0 = blockIdx.x * a.per_block;
+    const int nt = min(a.per_block, a.tokens - t0);
+    if (a.k && threadIdx.x >= kThreads - nt) {
+        const int t = kThreads - 1 - threadIdx.x;
+        const int i = a.index[t0 + t];
+        int64_t at = -1;
+        if (i >= 0) {
+            const int row = a.seq ? a.seq[t0 + t] : t0 + t;
+            const int64_t page = i / a.page_size;
+            int p = -1;
+            if (row >= 0 && row < a.table_rows && page < a.table_cols) p = a.table[row * a.table_cols + page];
+            if (p >= 0 && p < a.num_pages)
+                at = p * a.page_stride + static_cast<int64_t>(i - page * a.page_size) * a.dim;
+            else
+                atomicOr(&g_mrope_dev_error, kDevErrIndex);
+        }
+        place[t] = at;
+    }
+    for (int j = threadIdx.x; j < nt * half; j += kThreads) {
+        const int t = j / half, i = j - t * half;
+        const double turns = static_cast<double>(a.positions[static_cast<int64_t>(spec.axis[i]) * a.tokens + t0 + t]) *
+                             spec.turns[i];
+        float s, c;
+        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+        cs[t][i] = make_float2(c, s);
+    }
+    __syncthreads();
+
+    const int nrot = half / 8;                                 // rotated items of a head
+    const int items = nrot + (a.dim - spec.rotary_dim) / 8;    // and those that pass
+    const int heads = a.q_heads + (a.k ? 2 * a.kv_heads : 0);
+    const int per_token = heads * items;
+    for (int j = threadIdx.x; j < nt * per_token; j += kThreads) {
+        const int t = j / per_token;
+        const int r = j - t * per_token;
+        const int h = r / items, i = r - h * items;
+        const int64_t tok = t0 + t;
+        const __half* src;
+        __half* dst;
+        bool turn = true;
+        if (h < a.q_heads) {
+            src = a.q + tok * a.q_ts + h * a.q_hs;
+            dst = a.q_out + tok * a.o_ts + h * a.o_hs;
+            if (a.in_place && i >= nrot) continue;
+        } else {
+            if (place[t] < 0) continue;
+            const bool key = h < a.q_heads + a.kv_heads;
+            const int kh = h - a.q_heads - (key ? 0 : a.kv_heads);
+            src = key ? a.k + tok * a.k_ts + kh * a.k_hs : a.v + tok * a.v_ts + kh * a.v_hs;
+            dst = (key ? a.ck : a.cv) + place[t] + static_cast<int64_t>(kh) * a.page_size * a.dim;
+            turn = key;
+        }
+        const uint4* s4 = reinterpret_cast<const uint4*>(src);
+        uint4* d4 = reinterpret_cast<uint4*>(dst);
+        if (i < nrot) {
+            uint4 x = s4[i], y = s4[i + nrot];
+            if (turn) rotate8(x, y, &cs[t][i * 8]);
+            d4[i] = x;
+            d4[i + nrot] = y;
+        } else {
+            d4[i + nrot] = s4[i + nrot];
+        }
+    }
+}
+
+int check_spec(const char* who, const mcv_mrope_spec* s, int64_t dim) {
+    if (!s) return fail(MCV_ERR_NULL, std::string(who) + ": null rope specification");
+    if (s->rotary_dim < 16 || s->rotary_dim > 2 * MCV_MROPE_MAX_FREQS || s->rotary_dim % 16 || s->rotary_dim > dim)
+        return fail(MCV_ERR_SHAPE, std::string(who) + ": rotary_dim must be a multiple of 16, at most head_dim and 256");
+    if (s->axes < 1 || s->axes > 4) return fail(MCV_ERR_VALUE, std::string(who) + ": 1 to 4 axes");
+    for (int i = 0; i < s->rotary_dim / 2; ++i)
+        if (s->axis[i] >= s->axes) return fail(MCV_ERR_VALUE, std::string(who) + ": frequency with an axis beyond the last");
+    return MCV_OK;
+}
+
+// Rotating in place needs rows that do not share memory.
+int check_in_place(const char* who, const mcv_rows* x, int64_t tokens, int64_t heads, int64_t dim) {
+    const bool token_major = x->token_stride >= (heads - 1) * x->head_stride + dim;
+    const bool head_major = x->token_stride >= dim && x->head_stride >= (tokens - 1) * x->token_stride + dim;
+    if (tokens > 1 && !token_major && !head_major)
+        return fail(MCV_ERR_SHAPE, std::string(who) + ": rows rotated in place must not overlap");
+    return MCV_OK;
+}
+
+// Tokens per block: one while that fills the SMs less than twice, so that a
+// small batch spreads out; else four, which share the block's set-up.
+int tokens_per_block(int64_t tokens) { return tokens <= 8 * sm_count() ? 1 : kMaxTokens; }
+
+}  // namespace
+
+int check_rows(const char* who, const char* what, const mcv_rows* r, int64_t heads, int64_t dim) {
+    if (!r || !r->data) return fail(MCV_ERR_NULL, std::string(who) + ": null " + what);
+    if (!aligned16(r->data)) return fail(MCV_ERR_ALIGN, std::string(who) + ": " + what + " must be 16-byte aligned");
+    if (r->token_stride % 8 || r->head_stride % 8)
+        return fail(MCV_ERR_ALIGN, std::string(who) + ": strides of " + what + " must be multiples of 8 elements");
+    if (r->token_stride < 0 || r->head_stride < 0 || (heads > 1 && r->head_stride < dim))
+        return fail(MCV_ERR_SHAPE, std::string(who) + ": strides of " + what + " make rows overlap");
+    return MCV_OK;
+}
+
+int check_kv_cache(const char* who, const mcv_kv_cache* c) {
+    if (!c || !c->k || !c->v) return fail(MCV_ERR_NULL, std::string(who) + ": null cache");
+    if (!aligned16(c->k) || !aligned16(c->v)) return fail(MCV_ERR_ALIGN, std::string(who) + ": cache must be 16-byte aligned");
+    if (c->num_pages < 1 || c->page_size < 1 || c->kv_heads < 1 || c->kv_heads > 4096 || c->head_dim < 16 ||
+        c->head_dim > 1024 || c->head_dim % 8)
+        return fail(MCV_ERR_SHAPE, std::string(who) + ": bad cache dimensions");
+    if (c->page_stride % 8) return fail(MCV_ERR_ALIGN, std::string(who) + ": page stride must be a multiple of 8 elements");
+    if (c->page_stride < static_cast<int64_t>(c->kv_heads) * c->page_size * c->head_dim)
+        return fail(MCV_ERR_SHAPE, std::string(who) + ": page stride smaller than a page");
+    return MCV_OK;
+}
+
+unsigned take_mrope_device_error() {
+    unsigned v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_mrope_dev_error, sizeof(v)) != cudaSuccess) return ~0u;
+    if (v) cudaMemcpyToSymbol(g_mrope_dev_error, &zero, sizeof(zero));
+    return v;
+}
+
+}  // namespace mcv
+
+using namespace mcv;
+
+extern "C" {
+
+int mcv_mrope_init(mcv_mrope_spec* spec, int rotary_dim, int axes, const int32_t* sections, int interleaved,
+                   double theta) {
+    if (!spec || !sections) return fail(MCV_ERR_NULL, "mrope_init: null pointer");
+    if (rotary_dim < 16 || rotary_dim > 2 * MCV_MROPE_MAX_FREQS || rotary_dim % 16)
+        return fail(MCV_ERR_SHAPE, "mrope_init: rotary_dim must be a multiple of 16, at most 256");
+    if (axes < 1 || axes > 4) return fail(MCV_ERR_VALUE, "mrope_init: 1 to 4 axes");
+    if (!(theta > 1.0) || std::isinf(theta)) return fail(MCV_ERR_VALUE, "mrope_init: theta must be above 1");
+    const int half = rotary_dim / 2;
+    int64_t sum = 0;
+    for (int a = 0; a < axes; ++a) {
+        if (sections[a] < 0) return fail(MCV_ERR_VALUE, "mrope_init: negative section");
+        sum += sections[a];
+    }
+    if (sum != half) return fail(MCV_ERR_SHAPE, "mrope_init: sections must add up to rotary_dim / 2");
+    // interleaved: axis a > 0 owns frequencies a, a + axes, ... and all of them must exist
+    if (interleaved)
+        for (int a = 1; a < axes; ++a)
+            if (sections[a] > 0 && a + static_cast<int64_t>(axes) * (sections[a] - 1) >= half)
+                return fail(MCV_ERR_SHAPE, "mrope_init: an interleaved section runs past rotary_dim / 2");
+    spec->rotary_dim = rotary_dim;
+    spec->axes = axes;
+    const double two_pi = 6.283185307179586476925286766559;
+    for (int i = 0; i < MCV_MROPE_MAX_FREQS; ++i) {
+        spec->turns[i] = i < half ? std::pow(theta, -static_cast<double>(i) / half) / two_pi : 0.0;
+        int axis = 0;
+        if (i < half) {
+            if (interleaved) {
+                const int a = i % axes;
+                axis = a && i < axes * sections[a] ? a : 0;
+            } else {
+                for (int at = sections[0]; axis < axes - 1 && i >= at;) at += sections[++axis];
+            }
+        }
+        spec->axis[i] = static_cast<uint8_t>(axis);
+    }
+    return MCV_OK;
+}
+
+int mcv_mrope(const mcv_rows* x, void* out, const mcv_mrope_spec* spec, const void* positions, int64_t tokens,
+              int64_t heads, int64_t head_dim, mcv_stream_t stream) {
+    int st = check_rows("mrope", "x", x, heads, head_dim);
+    if (st) return st;
+    if (!out || !positions) return fail(MCV_ERR_NULL, "mrope: null out or positions");
+    if (!aligned16(out)) return fail(MCV_ERR_ALIGN, "mrope: out must be 16-byte aligned");
+    if (tokens < 1 || tokens > 0x7fffffffLL / 4 || heads < 1 || heads > 4096 || head_dim < 16 || head_dim > 1024 || head_dim % 8)
+        return fail(MCV_ERR_SHAPE, "mrope: bad tokens, heads or head_dim");
+    if ((st = check_spec("mrope", spec, head_dim))) return st;
+    if (x->data == out && (st = check_in_place("mrope", x, tokens, heads, head_dim))) return st;
+    RopeArgs a{};
+    a.q = static_cast<const __half*>(x->data);
+    a.q_out = static_cast<__half*>(out);
+    a.q_ts = x->token_stride;
+    a.q_hs = x->head_stride;
+    a.in_place = x->data == out;
+    // in place, out has x's strides; else it is dense
+    a.o_hs = a.in_place ? a.q_hs : head_dim;
+    a.o_ts = a.in_place ? a.q_ts : heads * head_dim;
+    a.positions = static_cast<const int32_t*>(positions);
+    a.tokens = static_cast<int>(tokens);
+    a.q_heads = static_cast<int>(heads);
+    a.dim = static_cast<int>(head_dim);
+    a.per_block = tokens_per_block(tokens);
+    const unsigned grid = static_cast<unsigned>((tokens + a.per_block - 1) / a.per_block);
+    return launch(mrope_kernel, dim3(grid), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), *spec, a);
+}
+
+int mcv_mrope_append_kv(const mcv_rows* q, void* q_out, const mcv_rows* k, const mcv_rows* v,
+                        const mcv_mrope_spec* spec, const void* positions, const mcv_kv_cache* cache,
+                        const void* page_table, int64_t table_rows, int64_t table_cols, const void* seq,
+                        const void* index, int64_t tokens, int64_t q_heads, mcv_stream_t stream) {
+    int st = check_kv_cache("mrope_append_kv", cache);
+    if (st) return st;
+    const int64_t dim = cache->head_dim;
+    if ((st = check_rows("mrope_append_kv", "q", q, q_heads, dim))) return st;
+    if ((st = check_rows("mrope_append_kv", "k", k, cache->kv_heads, dim))) return st;
+    if ((st = check_rows("mrope_append_kv", "v", v, cache->kv_heads, dim))) return st;
+    if (!q_out || !positions || !page_table || !index) return fail(MCV_ERR_NULL, "mrope_append_kv: null pointer");
+    if (!aligned16(q_out)) return fail(MCV_ERR_ALIGN, "mrope_append_kv: q_out must be 16-byte aligned");
+    if (tokens < 1 || tokens > 0x7fffffffLL / 4 || q_heads < 1 || q_heads > 4096)
+        return fail(MCV_ERR_SHAPE, "mrope_append_kv: bad tokens or q_heads");
+    if (table_rows < 1 || table_rows > 0x7fffffffLL || table_cols < 1 || table_cols > 0x7fffffffLL)
+        return fail(MCV_ERR_SHAPE, "mrope_append_kv: bad page table dimensions");
+    if (!seq && table_rows < tokens)
+        return fail(MCV_ERR_SHAPE, "mrope_append_kv: one table row per token is needed without seq");
+    if ((st = check_spec("mrope_append_kv", spec, dim))) return st;
+    if (q->data == q_out && (st = check_in_place("mrope_append_kv", q, tokens, q_heads, dim))) return st;
+    RopeArgs a{};
+    a.q = static_cast<const __half*>(q->data);
+    a.k = static_cast<const __half*>(k->data);
+    a.v = static_cast<const __half*>(v->data);
+    a.q_out = static_cast<__half*>(q_out);
+    a.ck = static_cast<__half*>(cache->k);
+    a.cv = static_cast<__half*>(cache->v);
+    a.positions = static_cast<const int32_t*>(positions);
+    a.table = static_cast<const int32_t*>(page_table);
+    a.seq = static_cast<const int32_t*>(seq);
+    a.index = static_cast<const int32_t*>(index);
+    a.q_ts = q->token_stride, a.q_hs = q->head_stride;
+    a.k_ts = k->token_stride, a.k_hs = k->head_stride;
+    a.v_ts = v->token_stride, a.v_hs = v->head_stride;
+    a.in_place = q->data == q_out;
+    a.o_hs = a.in_place ? a.q_hs : dim;
+    a.o_ts = a.in_place ? a.q_ts : q_heads * dim;
+    a.page_stride = cache->page_stride;
+    a.table_cols = table_cols;
+    a.tokens = static_cast<int>(tokens);
+    a.q_heads = static_cast<int>(q_heads);
+    a.kv_heads = cache->kv_heads;
+    a.dim = cache->head_dim;
+    a.page_size = cache->page_size;
+    a.num_pages = cache->num_pages;
+    a.table_rows = static_cast<int>(table_rows);
+    a.per_block = tokens_per_block(tokens);
+    const unsigned grid = static_cast<unsigned>((tokens + a.per_block - 1) / a.per_block);
+    return launch(mrope_kernel, dim3(grid), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), *spec, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,596 @@
+// Attention of one new token per sequence over a paged key-value cache:
+//   o = softmax(scale q K^T) V,  lse = log sum exp(scale q K^T),
+// with q_heads / kv_heads query heads sharing each key-value head.
+//
+// Bound by the cache's bytes (4 D bytes per key and kv head, read once).  The
+// products run on the warp-level tensor MMA, not for their rate but because
+// the fp32 FMAs of 8 query heads per key would take longer than the bytes do:
+// per 16 keys and 256 dimensions a warp issues 48 MMAs, a fraction of the
+// time in which its SM receives those 16 KB.
+//
+// Everything is transposed so that the few query heads are the MMA's n = 8:
+// S^T (16 keys x 8 heads) = K Q^T, and O^T (D x 8 heads) = V^T P^T.  K comes
+// as an A fragment through ldmatrix and V^T through its transposing form; S^T
+// turns into the B fragment of the second product by an 8x8 register
+// transpose.  P is split into hi + lo fp16, so that the probabilities keep 22
+// bits (the second MMA costs nothing here); scores, maxima, sums and outputs
+// are fp32.
+//
+// Work is cut evenly however ragged the batch is: all (sequence, head group)
+// rows' 16-key units form one line that is divided into one contiguous range
+// per block.  Within its range the four warps of a block take every fourth
+// unit, each through a ring of its own in shared memory that runs ahead
+// across row ends; page numbers are looked up one unit ahead of the copies.
+// At a row's end the block joins its warps' (max, sum, O).  A row that
+// lies in one block's range is written at once; of a row cut over several
+// blocks every block leaves a partial result, and the last one to arrive
+// joins them in order (in two levels of kFan, which bounds what one block has
+// to read), so results do not depend on timing.
+#include "mixing.cuh"
+
+#include <cfloat>
+
+namespace mcv {
+unsigned take_attention_device_error();
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kUnit = 16;      // keys of a unit
+constexpr int kFan = 8;        // partial results joined at a time
+constexpr int kMaxBatch = 4096;
+constexpr int kMinUnits = 4;   // least units of a block: one per warp
+
+static __device__ unsigned g_attention_dev_error;
+
+template <int D>
+struct Tile {
+    static constexpr int kStages = 3;
+    static constexpr int kRowBytes = D * 2;
+    static constexpr int kStageBytes = 2 * kUnit * kRowBytes;           // K rows, then V rows
+    static constexpr int kRingBytes = kStages * kStageBytes;            // per warp
+    static constexpr int kJoinRow = D + 4;                              // floats; spreads the heads over the banks
+    static constexpr int kJoinBytes = kWarps * 8 * kJoinRow * 4;
+    static constexpr int kSmem = kWarps * kRingBytes + kJoinBytes + 2 * kWarps * 8 * 4;
+    static constexpr int kBlocksPerSm = D == 256 ? 1 : (D == 128 ? 2 : 3);
+};
+
+struct AttnArgs {
+    const __half* q;
+    const __half* k;
+    const __half* v;
+    const int32_t* table;
+    const int32_t* lengths;
+    __half* out;
+    float* lse;
+    float* part;
+    unsigned* counters;   // [2 * grid] joins of kFan, [2 * grid] joins of those
+    int64_t q_bs, q_hs, page_stride, table_cols;
+    int batch, q_heads, kv_heads, group, head_groups, splits_of_group, num_pages, max_keys;
+    float scale_log2;
+    FastDiv page;
+};
+
+__device__ __forceinline__ int key_count(const AttnArgs& a, int b) {
+    const int n = a.lengths[b];
+    return n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n);
+}
+__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
+
+// A row of the work line: one sequence and one group of query heads.
+struct Row {
+    int64_t begin;   // first unit
+    int b, hg, keys, units;
+    __device__ __forceinline__ void next(const AttnArgs& a) {
+        begin += units;
+        if (++hg < a.head_groups) return;
+        hg = 0;
+        do {
+            ++b;
+            keys = b < a.batch ? key_count(a, b) : 0;
+        } while (b < a.batch && keys == 0);
+        units = units_of(keys);
+    }
+};
+
+__device__ __forceinline__ float scale_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2f(m - top); }
+
+template <int D, int NT>
+struct Part {
+    static constexpr int kHeads = 8 * NT;
+    static constexpr int kFloats = kHeads * (D + 2);
+    float* p;
+    __device__ __forceinline__ Part(float* base, int64_t slot) : p(base + slot * kFloats) {}
+    __device__ __forceinline__ float* m() const { return p; }
+    __device__ __forceinline__ float* l() const { return p + kHeads; }
+    __device__ __forceinline__ float* o(int head) const { return p + 2 * kHeads + head * D; }
+};
+
+// Counts this block in at *counter (after its global writes); true in the
+// last of `expected`, which leaves the counter at zero.
+__device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned expected, int* flag) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const bool last = atomicAdd(counter, 1u) == expected - 1;
+        if (last) *counter = 0;
+        *flag = last;
+    }
+    __syncthreads();
+    const bool last = *flag != 0;
+    __threadfence();
+    __syncthreads();
+    return last;
+}
+
+// Joins `n` partial results (slot_of(0..n-1), in order).  to_out: normalised
+// into the output rows; else back into slot_of(0).
+template <int D, int NT, typename SlotOf>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot_of, bool to_out, int b, int head0,
+                                           int heads) {
+    using P = Part<D, NT>;
+    constexpr int kVec = D / 4;
+    constexpr int kItems = (P::kHeads * kVec) / kThreads;
+    float4 acc[kItems];
+    float top[kItems], sum[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int item = threadIdx.x + i * kThreads;
+        const int h = item / kVec, d = (item % kVec) * 4;
+        acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        top[i] = -INFINITY;
+        sum[i] = 0.0f;
+        if (h >= heads) continue;
+        for (int s = 0; s < n; ++s) top[i] = fmaxf(top[i], __ldcg(P(a.part, slot_of(s)).m() + h));
+        for (int s = 0; s < n; ++s) {
+            const P p(a.part, slot_of(s));
+            const float w = scale_of(__ldcg(p.m() + h), top[i]);
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.o(h) + d));
+            sum[i] += w * __ldcg(p.l() + h);
+            acc[i].x += w * o.x;
+            acc[i].y += w * o.y;
+            acc[i].z += w * o.z;
+            acc[i].w += w * o.w;
+        }
+    }
+    if (to_out) {
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int item = threadIdx.x + i * kThreads;
+            const int h = item / kVec, d = (item % kVec) * 4;
+            if (h >= heads) continue;
+            const int64_t row = static_cast<int64_t>(b) * a.q_heads + head0 + h;
+            const float inv = 1.0f / sum[i];
+            const uint2 r = make_uint2(h2_as_u32(__floats2half2_rn(acc[i].x * inv, acc[i].y * inv)),
+                                       h2_as_u32(__floats2half2_rn(acc[i].z * inv, acc[i].w * inv)));
+            *reinterpret_cast<uint2*>(a.out + row * D + d) = r;
+            if (d == 0 && a.lse) a.lse[row] = (top[i] + log2f(sum[i])) * 0.6931471805599453f;
+        }
+        return;
+    }
+    __syncthreads();   // slot_of(0) is read by all before it is written
+    const P p(a.part, slot_of(0));
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int item = threadIdx.x + i * kThreads;
+        const int h = item / kVec, d = (item % kVec) * 4;
+        if (h >= heads) continue;
+        *reinterpret_cast<float4*>(p.o(h) + d) = acc[i];
+        if (d == 0) {
+            p.m()[h] = top[i];
+            p.l()[h] = sum[i];
+        }
+    }
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_kernel(const AttnArgs a) {
+    using T = Tile<D>;
+    using P = Part<D, NT>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int64_t sums[kWarps];
+    __shared__ int64_t first_begin;
+    __shared__ int first_b, flag;
+    float* join = reinterpret_cast<float*>(smem + kWarps * T::kRingBytes);
+    float* join_m = join + kWarps * 8 * T::kJoinRow;
+    float* join_l = join_m + kWarps * 8;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    pdl_trigger();
+    pdl_wait();
+
+    // sequences without keys: their rows are zero, with an empty sum
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+        const int n = a.lengths[b];
+        if (n > a.max_keys && tid == 0) atomicOr(&g_attention_dev_error, kDevErrIndex);
+        if (n > 0) continue;
+        const int64_t row = static_cast<int64_t>(b) * a.q_heads;
+        uint4* o = reinterpret_cast<uint4*>(a.out + row * D);
+        for (int i = tid; i < a.q_heads * (D / 8); i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
+        if (a.lse)
+            for (int i = tid; i < a.q_heads; i += kThreads) a.lse[row + i] = -INFINITY;
+    }
+
+    // this block's range of the work line and the row that it begins in
+    const int per_thread = (a.batch + kThreads - 1) / kThreads;
+    const int b0 = tid * per_thread, b1 = min(b0 + per_thread, a.batch);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += units_of(key_count(a, b));
+    mine *= a.head_groups;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    int64_t total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sums[w];
+        total += sums[w];
+    }
+    int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    if (per < kMinUnits) per = kMinUnits;
+    const int64_t start = per * blockIdx.x;
+    if (start >= total) return;
+    const int64_t end = min(start + per, total);
+    {
+        int64_t at = before + incl - mine;
+        if (start >= at && start < at + mine) {
+            int b = b0;
+            for (;; ++b) {
+                const int64_t n = static_cast<int64_t>(units_of(key_count(a, b))) * a.head_groups;
+                if (start < at + n) break;
+                at += n;
+            }
+            first_b = b;
+            first_begin = at;
+        }
+    }
+    __syncthreads();
+    Row row;
+    row.b = first_b;
+    row.keys = key_count(a, row.b);
+    row.units = units_of(row.keys);
+    row.hg = static_cast<int>((start - first_begin) / row.units);
+    row.begin = first_begin + static_cast<int64_t>(row.hg) * row.units;
+
+    // ---- the ring's producer side: the same lanes, running ahead ----
+    const uint32_t ring = smem_u32(smem) + warp * T::kRingBytes;
+    Row ahead = row;
+    int64_t u_ahead = start + warp;
+    int64_t src_off = 0;    // lane r < 16: element offset of the next unit's row r (K and V alike)
+    int src_ok = 0;
+    auto look_up = [&]() {
+        src_ok = 0;
+        src_off = 0;
+        if (u_ahead >= end) return;
+        while (u_ahead >= ahead.begin + ahead.units) ahead.next(a);
+        const int key = static_cast<int>(u_ahead - ahead.begin) * kUnit + (lane & 15);
+        if (key >= ahead.keys) return;
+        const uint32_t page = a.page.div(key);
+        const int p = a.table[ahead.b * a.table_cols + page];
+        if (p < 0 || p >= a.num_pages) {
+            atomicOr(&g_attention_dev_error, kDevErrIndex);
+            return;
+        }
+        const int kvh = ahead.hg / a.splits_of_group;
+        src_off = p * a.page_stride + (static_cast<int64_t>(kvh) * a.page.d + (key - page * a.page.d)) * D;
+        src_ok = 1;
+    };
+    auto issue = [&](int stage) {
+        if (u_ahead < end) {
+            constexpr int kVecs = D / 8;                 // 16-byte vectors of a row
+            constexpr int kIters = kUnit * kVecs / 32;
+            const uint32_t base = ring + stage * T::kStageBytes;
+#pragma unroll
+            for (int i = 0; i < kIters; ++i) {
+                const int item = i * 32 + lane;
+                const int r = item / kVecs, c = item % kVecs;
+                const int64_t off = __shfl_sync(0xffffffffu, src_off, r) + c * 8;
+                const bool ok = __shfl_sync(0xffffffffu, src_ok, r) != 0;
+                const uint32_t dst = base + r * T::kRowBytes + ((c ^ (r & 7)) << 4);
+                cp_async16_or_zero(dst, a.k + off, ok);
+                cp_async16_or_zero(dst + kUnit * T::kRowBytes, a.v + off, ok);
+            }
+        }
+        cp_async_commit();
+        u_ahead += kWarps;
+        look_up();
+    };
+    look_up();
+#pragma unroll
+    for (int s = 0; s < T::kStages - 1; ++s) issue(s);
+
+    // ldmatrix row addresses of this lane, before the swizzle
+    const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_vec = lane >> 4;
+    const int v_row = (lane & 7) + (lane >> 4) * 8, v_vec = (lane >> 3) & 1;
+    int stage = 0;
+    int64_t u = start + warp;
+    for (int64_t pos = start; pos < end;) {
+        const int64_t seg_end = min(row.begin + row.units, end);
+        const int kvh = row.hg / a.splits_of_group;
+        const int in_group = (row.hg % a.splits_of_group) * P::kHeads;
+        const int head0 = kvh * a.group + in_group;
+        const int heads = min(P::kHeads, a.group - in_group);
+
+        // Q^T as B fragments: lane (g, t) holds head g, dims 2t, 2t+1 (+8) of each 16
+        uint32_t qf[NT][D / 16][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int h = n * 8 + g;
+            const uint32_t* qr = reinterpret_cast<const uint32_t*>(a.q + row.b * a.q_bs + (head0 + (h < heads ? h : 0)) * a.q_hs);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                qf[n][kk][0] = h < heads ? qr[kk * 8 + t] : 0u;
+                qf[n][kk][1] = h < heads ? qr[kk * 8 + 4 + t] : 0u;
+            }
+        }
+        float acc[NT][D / 16][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.0f;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.0f;
+        }
+
+        for (; u < seg_end; u += kWarps) {
+            cp_async_wait<T::kStages - 2>();
+            __syncwarp();   // the unit has landed, and every lane is done with the stage that is filled next
+            issue(stage == 0 ? T::kStages - 1 : stage - 1);
+            const uint32_t kb = ring + stage * T::kStageBytes;
+            const uint32_t vb = kb + kUnit * T::kRowBytes;
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            {
+                // two accumulator chains: an MMA's latency is several issue slots
+                float s2[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.0f;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    uint32_t f[4];
+                    ldsm4(f, kb + k_row * T::kRowBytes + (((kk * 2 + k_vec) ^ (k_row & 7)) << 4));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma16816(kk & 1 ? s2[n] : s[n], f, qf[n][kk][0], qf[n][kk][1]);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
+            }
+            const int key = static_cast<int>(u - row.begin) * kUnit + g;
+            const bool in0 = key < row.keys, in1 = key + 8 < row.keys;
+            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                // columns 2t, 2t+1 are heads; rows g, g+8 keys
+                float top[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    s[n][c] = in0 ? s[n][c] * a.scale_log2 : -INFINITY;
+                    s[n][2 + c] = in1 ? s[n][2 + c] * a.scale_log2 : -INFINITY;
+                    float x = fmaxf(s[n][c], s[n][2 + c]);
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                    top[c] = fmaxf(m[n][c], x);
+                }
+                if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[1] > m[n][1])) {
+                    const float w0 = scale_of(m[n][0], top[0]), w1 = scale_of(m[n][1], top[1]);
+                    l[n][0] *= w0;
+                    l[n][1] *= w1;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        acc[n][i][0] *= w0;
+                        acc[n][i][1] *= w1;
+                        acc[n][i][2] *= w0;
+                        acc[n][i][3] *= w1;
+                    }
+                    m[n][0] = top[0];
+                    m[n][1] = top[1];
+                }
+                float p[4];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    // no number above -inf so far: nothing to weigh yet
+                    const float base = m[n][c] == -INFINITY ? 0.0f : m[n][c];
+                    p[c] = exp2f(s[n][c] - base);
+                    p[2 + c] = exp2f(s[n][2 + c] - base);
+                    l[n][c] += p[c] + p[2 + c];
+                }
+                uint32_t lo;
+                split_f16(p[0], p[1], ph[n][0], lo);
+                ph[n][0] = movm_t(ph[n][0]);
+                pl[n][0] = movm_t(lo);
+                split_f16(p[2], p[3], ph[n][1], lo);
+                ph[n][1] = movm_t(ph[n][1]);
+                pl[n][1] = movm_t(lo);
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t f[4];
+                ldsm4_t(f, vb + v_row * T::kRowBytes + (((i * 2 + v_vec) ^ (v_row & 7)) << 4));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16816(acc[n][i], f, ph[n][0], ph[n][1]);
+                    mma16816(acc[n][i], f, pl[n][0], pl[n][1]);
+                }
+            }
+            stage = stage + 1 == T::kStages ? 0 : stage + 1;
+        }
+
+        // ---- join the block's warps ----
+        const bool whole = row.begin >= start && row.begin + row.units <= end;
+        const int64_t c0 = row.begin / per, c1 = (row.begin + row.units - 1) / per;
+        auto slot_of_block = [&](int64_t c) { return 2 * c + (c == c0 && row.begin != c0 * per ? 1 : 0); };
+        const P mine_part(a.part, slot_of_block(blockIdx.x));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (n * 8 >= heads) break;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x = l[n][c];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                if (g == 0) {
+                    join_m[warp * 8 + 2 * t + c] = m[n][c];
+                    join_l[warp * 8 + 2 * t + c] = x;
+                }
+            }
+            float* jw = join + warp * 8 * T::kJoinRow;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    jw[(2 * t + (e & 1)) * T::kJoinRow + i * 16 + g + (e >> 1) * 8] = acc[n][i][e];
+            __syncthreads();
+            for (int item = tid; item < 8 * (D / 4); item += kThreads) {
+                const int h = item / (D / 4), d = (item % (D / 4)) * 4;
+                if (n * 8 + h >= heads) break;
+                float top = join_m[h];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, join_m[w * 8 + h]);
+                float sum = 0.0f;
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float x = scale_of(join_m[w * 8 + h], top);
+                    const float4 y = *reinterpret_cast<const float4*>(join + (w * 8 + h) * T::kJoinRow + d);
+                    sum += x * join_l[w * 8 + h];
+                    o.x += x * y.x;
+                    o.y += x * y.y;
+                    o.z += x * y.z;
+                    o.w += x * y.w;
+                }
+                if (whole) {
+                    const int64_t orow = static_cast<int64_t>(row.b) * a.q_heads + head0 + n * 8 + h;
+                    const float inv = 1.0f / sum;
+                    *reinterpret_cast<uint2*>(a.out + orow * D + d) =
+                        make_uint2(h2_as_u32(__floats2half2_rn(o.x * inv, o.y * inv)),
+                                   h2_as_u32(__floats2half2_rn(o.z * inv, o.w * inv)));
+                    if (d == 0 && a.lse) a.lse[orow] = (top + log2f(sum)) * 0.6931471805599453f;
+                } else {
+                    *reinterpret_cast<float4*>(mine_part.o(n * 8 + h) + d) = o;
+                    if (d == 0) {
+                        mine_part.m()[n * 8 + h] = top;
+                        mine_part.l()[n * 8 + h] = sum;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (!whole) {
+            const int parts = static_cast<int>(c1 - c0 + 1);
+            const int fan = static_cast<int>((blockIdx.x - c0) / kFan);
+            const int64_t f0 = c0 + static_cast<int64_t>(fan) * kFan;
+            const int in_fan = min(kFan, parts - fan * kFan);
+            const int fans = (parts + kFan - 1) / kFan;
+            if (arrive_last(a.counters + slot_of_block(f0), in_fan, &flag)) {
+                join_parts<D, NT>(a, in_fan, [&](int i) { return slot_of_block(f0 + i); }, fans == 1, row.b, head0, heads);
+                if (fans > 1 && arrive_last(a.counters + 2 * gridDim.x + slot_of_block(c0), fans, &flag))
+                    join_parts<D, NT>(a, fans, [&](int i) { return slot_of_block(c0 + static_cast<int64_t>(i) * kFan); },
+                                      true, row.b, head0, heads);
+            }
+        }
+        pos = seg_end;
+        if (pos < end) row.next(a);
+    }
+}
+
+// Query heads of one group are served by ceil(group / (8 NT)) rows; NT = 2
+// from 9 heads on, so that the cache is read once up to 16.
+int tiles_for(int64_t group) { return group <= 8 ? 1 : 2; }
+
+int blocks_per_sm(int64_t dim) { return dim == 256 ? 1 : (dim == 128 ? 2 : 3); }
+
+// The counters come first and take the same room for every head size, so that
+// calls of different shapes can share one workspace.
+size_t counter_count() { return static_cast<size_t>(sm_count()) * 4 * 3; }
+
+size_t part_floats(int64_t dim, int nt) { return static_cast<size_t>(8 * nt) * (dim + 2); }
+
+size_t workspace_bytes_for(int64_t dim, int nt) {
+    const size_t grid = static_cast<size_t>(sm_count()) * blocks_per_sm(dim);
+    return counter_count() * sizeof(unsigned) + 2 * grid * part_floats(dim, nt) * sizeof(float);
+}
+
+template <int D, int NT>
+int launch_attention(const AttnArgs& a, int grid, cudaStream_t stream) {
+    MCV_CHECK_CUDA(cudaFuncSetAttribute(attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::kSmem));
+    return launch(attention_kernel<D, NT>, dim3(grid), dim3(kThreads), Tile<D>::kSmem, stream, a);
+}
+
+}  // namespace
+
+unsigned take_attention_device_error() {
+    unsigned v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attention_dev_error, sizeof(v)) != cudaSuccess) return ~0u;
+    if (v) cudaMemcpyToSymbol(g_attention_dev_error, &zero, sizeof(zero));
+    return v;
+}
+
+}  // namespace mcv
+
+using namespace mcv;
+
+extern "C" {
+
+size_t mcv_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+    if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
+    return workspace_bytes_for(head_dim, tiles_for(q_heads / kv_heads));
+}
+
+int mcv_paged_attention_decode(const mcv_rows* q, const mcv_kv_cache* cache, const void* page_table,
+                               int64_t table_cols, const void* lengths, void* out, void* lse, int64_t batch,
+                               int64_t q_heads, float scale, void* workspace, size_t workspace_bytes,
+                               mcv_stream_t stream) {
+    int st = check_kv_cache("paged_attention_decode", cache);
+    if (st) return st;
+    const int64_t dim = cache->head_dim;
+    if (dim != 64 && dim != 128 && dim != 256)
+        return fail(MCV_ERR_SHAPE, "paged_attention_decode: head_dim must be 64, 128 or 256");
+    if ((st = check_rows("paged_attention_decode", "q", q, q_heads, dim))) return st;
+    if (!page_table || !lengths || !out) return fail(MCV_ERR_NULL, "paged_attention_decode: null pointer");
+    if (!aligned16(out)) return fail(MCV_ERR_ALIGN, "paged_attention_decode: out must be 16-byte aligned");
+    if (batch < 1 || batch > kMaxBatch) return fail(MCV_ERR_SHAPE, "paged_attention_decode: batch must be 1..4096");
+    if (q_heads < 1 || q_heads > 4096 || q_heads % cache->kv_heads)
+        return fail(MCV_ERR_SHAPE, "paged_attention_decode: q_heads must be a multiple of the cache's kv_heads");
+    if (table_cols < 1 || table_cols * cache->page_size > 0x7fffffffLL - kUnit || table_cols > 0x7fffffffLL)
+        return fail(MCV_ERR_SHAPE, "paged_attention_decode: a sequence holds fewer than 2^31 - 16 keys");
+    if (!(scale > 0.0f) || scale > FLT_MAX) return fail(MCV_ERR_VALUE, "paged_attention_decode: scale must be positive");
+    const int64_t group = q_heads / cache->kv_heads;
+    const int nt = tiles_for(group);
+    if (!workspace || workspace_bytes < workspace_bytes_for(dim, nt))
+        return fail(MCV_ERR_WORKSPACE, "paged_attention_decode: workspace missing or too small");
+    if (!aligned16(workspace)) return fail(MCV_ERR_ALIGN, "paged_attention_decode: workspace must be 16-byte aligned");
+
+    const int sms = sm_count();
+    const int64_t splits = (group + 8 * nt - 1) / (8 * nt);
+    const int64_t max_keys = table_cols * cache->page_size;
+    const int64_t most = batch * cache->kv_heads * splits * ((max_keys + kUnit - 1) / kUnit);
+    const int64_t want = (most + kMinUnits - 1) / kMinUnits;
+    const int full = sms * blocks_per_sm(dim);
+    const int grid = static_cast<int>(want < full ? want : full);
+
+    AttnArgs a{static_cast<const __half*>(q->data), static_cast<const __half*>(cache->k),
+               static_cast<const __half*>(cache->v), static_cast<const int32_t*>(page_table),
+               static_cast<const int32_t*>(lengths), static_cast<__half*>(out), static_cast<float*>(lse), nullptr, nullptr,
+               q->token_stride, q->head_stride, cache->page_stride, table_cols, static_cast<int>(batch),
+               static_cast<int>(q_heads), cache->kv_heads, static_cast<int>(group),
+               static_cast<int>(cache->kv_heads * splits), static_cast<int>(splits), cache->num_pages,
+               static_cast<int>(max_keys), scale * 1.4426950408889634f, FastDiv(static_cast<uint32_t>(cache->page_size))};
+    a.counters = static_cast<unsigned*>(workspace);
+    a.part = reinterpret_cast<float*>(a.counters + counter_count());
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dim == 256) return nt == 1 ? launch_attention<256, 1>(a, grid, s) : launch_attention<256, 2>(a, grid, s);
+    if (dim == 128) return nt == 1 ? launch_attention<128, 1>(a, grid, s) : launch_attention<128, 2>(a, grid, s);
+    return nt == 1 ? launch_attention<64, 1>(a, grid, s) : launch_attention<64, 2>(a, grid, s);
+}
+
+}  // extern "C"

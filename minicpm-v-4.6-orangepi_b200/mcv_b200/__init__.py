@@ -98,6 +98,14 @@ _SIGS = {
     "mcv_w8a8_policy_allows": [ctypes.c_char_p],
     "mcv_w8a8_policy_allows_mode": [ctypes.c_char_p, ctypes.c_char_p],
     "mcv_matmul_decode_dispatch": [_vp, _vp, _vp, _i64, _i64, _i64, _vp],
+    "mcv_mrope_init": [_vp, _int, _int, _vp, _int, ctypes.c_double],
+    "mcv_mrope": [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
+    "mcv_mrope_append_kv": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp],
+    "mcv_paged_attention_workspace_size": [_i64, _i64, _i64],
+    "mcv_paged_attention_decode": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _f32, _vp, _sz, _vp],
+    "mcv_gated_delta_step": [_vp, _i64, _vp],
+    "mcv_gated_delta_workspace_size": [_i64, _i64, _i64, _i64, _i64],
+    "mcv_gated_delta_prefill": [_vp, _vp, _i64, _i64, _vp, _sz, _vp],
 }
 _RESTYPE = {
     "mcv_status_string": ctypes.c_char_p,
@@ -111,6 +119,8 @@ _RESTYPE = {
     "mcv_lm_head_noalloc_max_bytes": _sz,
     "mcv_safetensors_count": _i64,
     "mcv_safetensors_name": ctypes.c_char_p,
+    "mcv_paged_attention_workspace_size": _sz,
+    "mcv_gated_delta_workspace_size": _sz,
 }
 EXPORTED = tuple(_SIGS)
 
@@ -178,7 +188,8 @@ TUNE_W4A16_KSPLIT_WARPS = 10
 
 
 def device_errors() -> int:
-    """Device-side error bits since the last call (bit 0: a bounded wait gave up)."""
+    """Device-side error bits since the last call (bit 0: a bounded wait gave up;
+    bit 1: an index in device memory was out of range and not followed)."""
     return int(lib().mcv_device_errors())
 
 
@@ -784,3 +795,241 @@ def matmul_decode_dispatch(x, weights: DecodeWeights, out, stream=None) -> None:
     N = out.shape[1]
     _check(lib().mcv_matmul_decode_dispatch(_ptr(x), ctypes.byref(weights), _ptr(out), M, K, N, _stream(stream)),
            "matmul_decode_dispatch")
+
+
+# ---- token mixing: rotary positions, paged attention, the gated delta rule ----
+# Strided inputs are taken as they are as long as their innermost dimension is
+# contiguous (and rows start on 16 bytes), so slices of a fused projection's
+# output need no copy.  Calls run on the tensors' device and, unless a stream is
+# given, on its current stream.
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("data", _vp), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class _KVCache(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class _MRopeSpec(ctypes.Structure):
+    _fields_ = [("rotary_dim", ctypes.c_int32), ("axes", ctypes.c_int32), ("turns", ctypes.c_double * 128),
+                ("axis", ctypes.c_uint8 * 128)]
+
+
+class _GatedDelta(ctypes.Structure):
+    _fields_ = [("q", _Rows), ("k", _Rows), ("v", _Rows), ("g", _vp), ("beta", _vp), ("out", _vp), ("state_in", _vp),
+                ("state_out", _vp), ("state_index", _vp), ("slots", _i64), ("k_heads", ctypes.c_int32),
+                ("v_heads", ctypes.c_int32), ("key_dim", ctypes.c_int32), ("value_dim", ctypes.c_int32),
+                ("scale", _f32), ("l2_eps", _f32)]
+
+
+def _f16_rows(t, what: str, device) -> _Rows:
+    """[tokens, heads, dim] fp16 with a contiguous last dimension."""
+    import torch
+    if t.dtype is not torch.float16 or t.device != device or t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] != 1):
+        raise RuntimeError(f"mcv_b200: {what} must be float16 [tokens, heads, dim] on {device} with contiguous rows")
+    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _dense(t, dtype, shape, what: str, device):
+    """Address of a contiguous tensor of this type and shape (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise RuntimeError(f"mcv_b200: {what} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _run_on(device, stream, name: str, *args) -> None:
+    """Calls mcv_<name>(*args, stream) with `device` current."""
+    import torch
+    if device.type != "cuda":
+        raise RuntimeError("mcv_b200: expected a CUDA tensor")
+    fn = getattr(lib(), "mcv_" + name)
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    if device.index == torch.cuda.current_device():
+        st = fn(*args, stream.cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, stream.cuda_stream)
+    if st != 0:
+        _check(st, name)
+
+
+class PagedKVCache:
+    """A paged key-value cache of one layer: k and v fp16 [pages, kv_heads,
+    page_size, head_dim]; pages may lie apart (any stride of the first
+    dimension, the same for k and v), each page is contiguous."""
+
+    def __init__(self, k, v):
+        import torch
+        if k.dtype is not torch.float16 or v.dtype is not torch.float16 or k.dim() != 4 or k.shape != v.shape:
+            raise RuntimeError("PagedKVCache: k and v must be float16 [pages, kv_heads, page_size, head_dim]")
+        if k.device != v.device or not k.is_cuda:
+            raise RuntimeError("PagedKVCache: k and v must be on one CUDA device")
+        _, heads, page, dim = k.shape
+        if k.stride()[1:] != (page * dim, dim, 1) or v.stride() != k.stride():
+            raise RuntimeError("PagedKVCache: pages must be contiguous and k and v laid out alike")
+        self.k, self.v = k, v
+        self._c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0), *k.shape[:1], page, heads, dim)
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda"):
+        import torch
+        kv = torch.empty(2, pages, kv_heads, page_size, head_dim, dtype=torch.float16, device=device)
+        return cls(kv[0], kv[1])
+
+
+class MRope:
+    """Rotary positions with len(sections) axes (mcv_mrope_init): `sections`
+    frequencies per axis, adding up to rotary_dim / 2, as contiguous blocks or
+    interleaved."""
+
+    def __init__(self, rotary_dim: int, sections, interleaved: bool = False, theta: float = 1.0e7):
+        self._c = _MRopeSpec()
+        self.axes = len(sections)
+        arr = (ctypes.c_int32 * max(1, self.axes))(*sections)
+        _check(lib().mcv_mrope_init(ctypes.byref(self._c), rotary_dim, self.axes, arr, int(interleaved), theta),
+               "mrope_init")
+
+
+def _rows_out(x, out, what: str):
+    """Address of a dense output of x's shape, or of x itself (in place)."""
+    if out.data_ptr() == x.data_ptr() and out.shape == x.shape and out.stride() == x.stride() and out.dtype == x.dtype:
+        return out.data_ptr()
+    return _dense(out, x.dtype, x.shape, what, x.device)
+
+
+def mrope(x, positions, rope: MRope, out, stream=None) -> None:
+    """out = x [tokens, heads, head_dim] with its rows rotated; positions int32
+    [axes, tokens]; out is dense, or x itself."""
+    import torch
+    dev = x.device
+    rows = _f16_rows(x, "x", dev)
+    n, heads, dim = x.shape
+    _run_on(dev, stream, "mrope", ctypes.byref(rows), _rows_out(x, out, "out"), ctypes.byref(rope._c),
+            _dense(positions, torch.int32, (rope.axes, n), "positions", dev), n, heads, dim)
+
+
+def mrope_append_kv(q, k, v, positions, rope: MRope, cache: PagedKVCache, page_table, index, q_out, seq=None,
+                    stream=None) -> None:
+    """q_out = q rotated, and k rotated and v written to the paged cache, in one
+    launch (mcv_mrope_append_kv).  q, k, v fp16 [tokens, heads, head_dim];
+    positions int32 [axes, tokens]; page_table int32 [rows, pages of a row];
+    index int32 [tokens]: each token's place in its sequence (negative: not
+    written); seq int32 [tokens]: its row of page_table (None: token t has row t)."""
+    import torch
+    dev, c = q.device, cache._c
+    n, heads, dim = q.shape
+    if cache.k.device != dev or dim != c.head_dim or k.shape != (n, c.kv_heads, dim) or v.shape != k.shape:
+        raise RuntimeError("mrope_append_kv: q, k, v and the cache do not fit together")
+    rq, rk, rv = _f16_rows(q, "q", dev), _f16_rows(k, "k", dev), _f16_rows(v, "v", dev)
+    if page_table.dim() != 2:
+        raise RuntimeError("mrope_append_kv: page_table must be [rows, pages]")
+    ref = ctypes.byref
+    _run_on(dev, stream, "mrope_append_kv", ref(rq), _rows_out(q, q_out, "q_out"), ref(rk), ref(rv), ref(rope._c),
+            _dense(positions, torch.int32, (rope.axes, n), "positions", dev), ref(c),
+            _dense(page_table, torch.int32, page_table.shape, "page_table", dev), page_table.shape[0],
+            page_table.shape[1], _dense(seq, torch.int32, (n,), "seq", dev),
+            _dense(index, torch.int32, (n,), "index", dev), n, heads)
+
+
+def paged_attention_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, device="cuda"):
+    """Zero-filled workspace of paged_attention_decode (of any batch); one per
+    stream that calls it."""
+    import torch
+    with torch.cuda.device(device):
+        n = lib().mcv_paged_attention_workspace_size(q_heads, kv_heads, head_dim)
+    if n == 0:
+        raise RuntimeError("paged_attention_workspace: unsupported heads or head_dim")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_attention_decode(q, cache: PagedKVCache, page_table, lengths, out, workspace, scale=None, lse=None,
+                           stream=None) -> None:
+    """Attention of one new token per sequence over its cached keys
+    (mcv_paged_attention_decode).  q fp16 [batch, q_heads, head_dim]; page_table
+    int32 [batch, pages]; lengths int32 [batch] (0: a zero row); out like q,
+    dense; lse fp32 [batch, q_heads] or None; scale defaults to head_dim^-1/2."""
+    import torch
+    dev, c = q.device, cache._c
+    b, heads, dim = q.shape
+    if cache.k.device != dev or dim != c.head_dim:
+        raise RuntimeError("paged_attention_decode: q and the cache do not fit together")
+    rows = _f16_rows(q, "q", dev)
+    if page_table.dim() != 2:
+        raise RuntimeError("paged_attention_decode: page_table must be [batch, pages]")
+    cols = page_table.shape[1]
+    if workspace.device != dev:
+        raise RuntimeError("paged_attention_decode: workspace on another device")
+    _run_on(dev, stream, "paged_attention_decode", ctypes.byref(rows), ctypes.byref(c),
+            _dense(page_table, torch.int32, (b, cols), "page_table", dev), cols,
+            _dense(lengths, torch.int32, (b,), "lengths", dev), _dense(out, torch.float16, q.shape, "out", dev),
+            _dense(lse, torch.float32, (b, heads), "lse", dev), b, heads, dim ** -0.5 if scale is None else scale,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
+def _gated_delta(q, k, v, g, beta, state, out, state_out, index, batch, scale, l2_eps) -> _GatedDelta:
+    import torch
+    dev = q.device
+    a = _GatedDelta()
+    a.q, a.k, a.v = _f16_rows(q, "q", dev), _f16_rows(k, "k", dev), _f16_rows(v, "v", dev)
+    n, kh, dk = q.shape
+    _, vh, dv = v.shape
+    if k.shape != q.shape or v.shape[0] != n:
+        raise RuntimeError("gated_delta: q, k and v do not fit together")
+    a.g = _dense(g, torch.float32, (n, vh), "g", dev)
+    a.beta = _dense(beta, torch.float32, (n, vh), "beta", dev)
+    a.out = _dense(out, torch.float16, (n, vh, dv), "out", dev)
+    any_state = state if state is not None else state_out
+    slots = any_state.shape[0] if any_state is not None else batch
+    a.state_in = _dense(state, torch.float32, (slots, vh, dk, dv), "state", dev)
+    a.state_out = _dense(state_out, torch.float32, (slots, vh, dk, dv), "state_out", dev)
+    a.state_index = _dense(index, torch.int32, (batch,), "index", dev)
+    a.slots, a.k_heads, a.v_heads, a.key_dim, a.value_dim = slots, kh, vh, dk, dv
+    a.scale = dk ** -0.5 if scale is None else scale
+    a.l2_eps = -1.0 if l2_eps is None else l2_eps
+    return a
+
+
+def gated_delta_step(q, k, v, g, beta, state, out, state_out=None, index=None, scale=None, l2_eps=None,
+                     stream=None) -> None:
+    """One token per sequence of the gated delta rule (mcv_gated_delta_step).
+    q, k fp16 [batch, k_heads, key_dim], v fp16 [batch, v_heads, value_dim], g
+    and beta fp32 [batch, v_heads], state fp32 [slots, v_heads, key_dim,
+    value_dim] (updated in place unless state_out is given), index int32 [batch]:
+    the sequences' slots (negative: skipped; None: slot b), out fp16 [batch,
+    v_heads, value_dim].  l2_eps: q and k are normalised with it first (None: not);
+    scale defaults to key_dim^-1/2."""
+    a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, q.shape[0],
+                     scale, l2_eps)
+    _run_on(q.device, stream, "gated_delta_step", ctypes.byref(a), q.shape[0])
+
+
+def gated_delta_workspace(tokens: int, batch: int, v_heads: int, key_dim: int, value_dim: int, device="cuda"):
+    """Workspace of gated_delta_prefill for up to this many tokens and sequences."""
+    import torch
+    n = lib().mcv_gated_delta_workspace_size(tokens, batch, v_heads, key_dim, value_dim)
+    if n == 0:
+        raise RuntimeError("gated_delta_workspace: unsupported dimensions")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def gated_delta_prefill(q, k, v, g, beta, cu_seqlens, state, out, workspace, state_out=None, index=None, scale=None,
+                        l2_eps=None, stream=None) -> None:
+    """Packed prompts of the gated delta rule (mcv_gated_delta_prefill): tokens
+    cu_seqlens[b] .. cu_seqlens[b+1] (int32 [batch + 1]) belong to sequence b.
+    state None: sequences start from zero.  Final states go to state_out, or back
+    into state; with neither they are not kept.  The rest as gated_delta_step."""
+    import torch
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+        raise RuntimeError("gated_delta_prefill: cu_seqlens must be [batch + 1]")
+    batch = cu_seqlens.shape[0] - 1
+    a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, batch, scale, l2_eps)
+    if workspace.device != q.device:
+        raise RuntimeError("gated_delta_prefill: workspace on another device")
+    _run_on(q.device, stream, "gated_delta_prefill", ctypes.byref(a),
+            _dense(cu_seqlens, torch.int32, (batch + 1,), "cu_seqlens", q.device), q.shape[0], batch,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size())
