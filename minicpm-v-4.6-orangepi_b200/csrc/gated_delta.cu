@@ -151,6 +151,519 @@ int run_recurrent(const DeltaArgs& a, int dk, cudaStream_t stream) {
     return launch(dk == 128 ? recurrent_kernel<128> : recurrent_kernel<64>, grid, dim3(warps * 32), 0, stream, a);
 }
 
+// ---- prompts, in chunks of 64 tokens -----------------------------------------------
+//
+// With G_i the decay summed up to token i of a chunk, S0 the state before it
+// and r the norms' reciprocals, the written rows u of the chunk solve
+//   (I + A) U = diag(beta) (V - diag(e^G r_k) K S0),
+//   A_ij = beta_i e^(G_i - G_j) r_ki r_kj k_i.k_j   (j < i),
+// and O = scale diag(e^G r_q) Q S0 + P U with P_ij = scale e^(G_i - G_j) r_qi r_kj q_i.k_j
+// (j <= i), S' = e^G_C S0 + K^T diag(e^(G_C - G_j) r_kj) U.
+//
+// chunk_kernel makes what does not need the state, for all chunks at once:
+// T = (I + A)^-1 diag(beta) and P.  scan_kernel then walks the chunks of a
+// sequence with the state in registers.
+//
+// Everything that has a 16-bit exact operand (K, Q as stored; norms, decays and
+// scales are applied to results in fp32) runs on the fp16 tensor MMA with fp32
+// accumulation.  The other operands (S, T, P, R, U) are split as hi + 2^-11 lo,
+// both fp16, the lo products in accumulators of their own: 22 bits of each
+// value, down to an absolute 2^-36, so results keep fp32's accuracy where
+// a single fp16 operand would leave 2^-11.  (State values and written rows are
+// below fp16's 65504 then; with |k| <= 1, beta <= 1 and g <= 0 they are bounded by
+// the state's start and the sum of |v|.)
+constexpr int kChunk = 64;
+constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;
+
+__device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    hi = h2_as_u32(h);
+    lo = h2_as_u32(__floats2half2_rn((x - f.x) * kLo, (y - f.y) * kLo));
+}
+
+// One chunk's share of the workspace.
+struct Chunk {
+    __half t[2][kChunk * kChunk];    // T hi, lo, by rows
+    __half p[2][kChunk * kChunk];    // P hi, lo
+    float ck[kChunk];                // e^G r_k
+    float cq[kChunk];                // scale e^G r_q
+    float cs[kChunk];                // e^(G_C - G) r_k
+    float keep;                      // e^G_C
+    float pad[31];
+};
+static_assert(sizeof(Chunk) % 128 == 0, "chunks stay aligned");
+
+// The slots of sequence b begin at cu[b] / 64 + b: ranges of ceil(len / 64) from
+// there on never overlap, since floor(x + y) >= floor(x) + floor(y).
+__device__ __forceinline__ int64_t first_chunk(int begin, int b) { return begin / kChunk + b; }
+
+// Shared-memory address of the 16-byte vector c of row r in a tile of VECS
+// vectors per row, spread so that eight rows of one column hit all banks.
+template <int VECS>
+__device__ __forceinline__ uint32_t tile_at(uint32_t base, int r, int c) {
+    return base + r * (VECS * 16) + ((c ^ (r & (VECS < 8 ? VECS - 1 : 7))) << 4);
+}
+
+template <int DK>
+__global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* chunks) {
+    constexpr int kVecs = DK / 8;
+    extern __shared__ __align__(128) unsigned char smem[];
+    float* mat = reinterpret_cast<float*>(smem + 2 * kChunk * DK * 2);     // A, rows of 68
+    constexpr int kMatRow = 68;
+    __shared__ double gsum[kChunk];
+    __shared__ float rk[kChunk], rq[kChunk], bt[kChunk];
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int h = blockIdx.y;
+    // the sequence that owns this slot: the last whose first slot is not behind it
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (first_chunk(a.cu[mid], mid) <= blockIdx.x) lo = mid;
+        else hi = mid - 1;
+    }
+    int begin, end, slot;
+    if (!sequence(a, lo, begin, end, slot)) return;
+    const int64_t local = static_cast<int64_t>(blockIdx.x) - first_chunk(begin, lo);
+    if (local < 0 || local * kChunk >= end - begin) return;
+    const int t0 = begin + static_cast<int>(local) * kChunk;
+    const int n = min(kChunk, end - t0);
+    const int kh = h / a.share;
+
+    const uint32_t ks = smem_u32(smem), qs = ks + kChunk * DK * 2;
+    for (int i = tid; i < kChunk * kVecs; i += 128) {
+        const int r = i / kVecs, c = i % kVecs;
+        const int64_t t = t0 + (r < n ? r : 0);
+        cp_async16_or_zero(tile_at<kVecs>(ks, r, c), a.k + t * a.k_ts + kh * a.k_hs + c * 8, r < n);
+        cp_async16_or_zero(tile_at<kVecs>(qs, r, c), a.q + t * a.q_ts + kh * a.q_hs + c * 8, r < n);
+    }
+    cp_async_commit();
+    if (warp == 0) {
+        // decays summed in fp64: differences of far tokens keep their digits; below
+        // -200 a decay is 0 in fp32 as it stands, and stays finite here
+        double x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 2 * lane + i;
+            const int64_t at = static_cast<int64_t>(t0 + r) * a.v_heads + h;
+            const float g = r < n ? a.g[at] : 0.0f;
+            x[i] = g < -200.0f ? -200.0f : g;
+            bt[r] = r < n ? a.beta[at] : 0.0f;
+        }
+        double s = x[0] + x[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+        }
+        gsum[2 * lane + 1] = s;
+        gsum[2 * lane] = s - x[1];
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    {
+        const int r = tid & 63;
+        const uint32_t base = tid < 64 ? ks : qs;
+        float sum = 0.0f;
+        if (a.l2_eps >= 0.0f) {
+#pragma unroll
+            for (int c = 0; c < kVecs; ++c) {
+                uint32_t x[4];
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                             : "r"(tile_at<kVecs>(base, r, c)));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = __half22float2(u32_as_h2(x[i]));
+                    sum += f.x * f.x + f.y * f.y;
+                }
+            }
+        }
+        const float norm = a.l2_eps >= 0.0f ? 1.0f / sqrtf(sum + a.l2_eps) : 1.0f;
+        (tid < 64 ? rk : rq)[r] = r < n ? norm : 0.0f;
+    }
+    __syncthreads();
+    Chunk& out = chunks[static_cast<int64_t>(blockIdx.x) * a.v_heads + h];
+    if (tid < kChunk) {
+        const double g = gsum[tid];
+        const float eg = expf(static_cast<float>(g));
+        out.ck[tid] = eg * rk[tid];
+        out.cq[tid] = eg * rq[tid] * a.scale;
+        out.cs[tid] = expf(static_cast<float>(gsum[kChunk - 1] - g)) * rk[tid];
+        if (tid == kChunk - 1) out.keep = eg;
+    }
+
+    // K K^T and Q K^T: this warp's 16 rows, columns up to the diagonal block
+    float kk[8][4], qk[8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kk[j][e] = qk[j][e] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < DK / 16; ++x) {
+        uint32_t ka[4], qa[4];
+        const int ar = warp * 16 + (lane & 15), ac = x * 2 + (lane >> 4);
+        ldsm4(ka, tile_at<kVecs>(ks, ar, ac));
+        ldsm4(qa, tile_at<kVecs>(qs, ar, ac));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > warp) break;
+            uint32_t b[4];
+            ldsm4(b, tile_at<kVecs>(ks, j * 16 + (lane & 7) + (lane >> 4) * 8, x * 2 + ((lane >> 3) & 1)));
+            mma16816(kk[2 * j], ka, b[0], b[1]);
+            mma16816(kk[2 * j + 1], ka, b[2], b[3]);
+            mma16816(qk[2 * j], qa, b[0], b[1]);
+            mma16816(qk[2 * j + 1], qa, b[2], b[3]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (j > 2 * warp + 1) break;
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            const int r = warp * 16 + (lane >> 2) + e * 4, c = j * 8 + (lane & 3) * 2;
+            float p[2], m[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float w = c + i <= r ? expf(static_cast<float>(gsum[r] - gsum[c + i])) * rk[c + i] : 0.0f;
+                p[i] = c + i <= r ? w * rq[r] * a.scale * qk[j][e + i] : 0.0f;
+                m[i] = c + i < r ? w * rk[r] * bt[r] * kk[j][e + i] : 0.0f;
+            }
+            uint32_t phi, plo;
+            split_scaled(p[0], p[1], phi, plo);
+            *reinterpret_cast<uint32_t*>(&out.p[0][r * kChunk + c]) = phi;
+            *reinterpret_cast<uint32_t*>(&out.p[1][r * kChunk + c]) = plo;
+            *reinterpret_cast<float2*>(mat + r * kMatRow + c) = make_float2(m[0], m[1]);
+        }
+    }
+    __syncthreads();
+    // column j of (I + A)^-1 by forward substitution, one thread a column:
+    // x_i = [i = j] - sum_{l < i} A_il x_l (x_l = 0 above the diagonal)
+    if (tid < kChunk) {
+        float x[kChunk];
+        const float beta = bt[tid];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            float acc[4] = {i == tid ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int l = 0; l < i; l += 4) {
+                const float4 m = *reinterpret_cast<const float4*>(mat + i * kMatRow + l);
+                acc[0] -= m.x * x[l];
+                if (l + 1 < i) acc[1] -= m.y * x[l + 1];
+                if (l + 2 < i) acc[2] -= m.z * x[l + 2];
+                if (l + 3 < i) acc[3] -= m.w * x[l + 3];
+            }
+            x[i] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+            const float t = x[i] * beta;
+            const __half th = __float2half_rn(t);
+            out.t[0][i * kChunk + tid] = th;
+            out.t[1][i * kChunk + tid] = __float2half_rn((t - __half2float(th)) * kLo);
+        }
+    }
+}
+
+// The walk.  A group of four warps owns 16 value columns of a head, a block
+// `NG` groups that share the chunk's tiles (two of them in flight).  All
+// products are taken transposed, with the 16 columns as the MMA's m, so that
+// results turn into the next product's A operand by a trip through shared
+// memory (S, R and U change hands between the warps, each of which has 16
+// tokens of a chunk and a quarter of the state's rows):
+//   R^T = V^T - (S0^T K^T) diag(ck);  U^T = R^T T^T;
+//   O^T = (S0^T Q^T) diag(cq) + U^T P^T;  S'^T = keep S0^T + (U^T diag(cs)) K.
+// Blocks of T and P above the diagonal are neither loaded nor multiplied.
+template <int DK, int NG>
+struct Scan {
+    static constexpr int kThreads = NG * 128;
+    static constexpr int kTile = kChunk * DK * 2;
+    static constexpr int kTri = kChunk * kChunk * 2;
+    static constexpr int kVRow = NG * 32;
+    static constexpr int kStage = 2 * kTile + 4 * kTri + kChunk * kVRow + 1024;
+    static constexpr int kSx = 16 * DK * 2;
+    static constexpr int kRx = 16 * kChunk * 2;
+    static constexpr int kGroup = 2 * kSx + 6 * kRx;
+    static constexpr int kSmem = 2 * kStage + NG * kGroup;
+};
+
+template <int DK, int NG>
+__global__ void __launch_bounds__(NG * 128) scan_kernel(const DeltaArgs a, const Chunk* chunks) {
+    using C = Scan<DK, NG>;
+    constexpr int kVecs = DK / 8;
+    constexpr int kN = DK / 32;       // n8 tiles of a warp's state rows
+    extern __shared__ __align__(128) unsigned char smem[];
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3, group = tid >> 7;
+    const int g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z;
+    const int kh = h / a.share;
+    const int col0 = blockIdx.x * NG * 16;
+    const int col = col0 + group * 16;
+    const bool live = col < a.dv;
+    int begin, end, slot;
+    if (!sequence(a, b, begin, end, slot)) return;
+
+    const uint32_t base = smem_u32(smem);
+    const uint32_t gx = base + 2 * C::kStage + group * C::kGroup;
+    const uint32_t s_hi = gx, s_lo = gx + C::kSx, r_hi = gx + 2 * C::kSx, r_lo = r_hi + C::kRx, u_hi = r_lo + C::kRx,
+                   u_lo = u_hi + C::kRx, w_hi = u_lo + C::kRx, w_lo = w_hi + C::kRx;
+
+    auto load = [&](int c, int stage) {
+        const uint32_t k = base + stage * C::kStage, q = k + C::kTile, tri = q + C::kTile, v = tri + 4 * C::kTri,
+                       sc = v + kChunk * C::kVRow;
+        const int t0 = begin + c * kChunk;
+        const int n = min(kChunk, end - t0);
+        const Chunk& ch = chunks[(first_chunk(begin, b) + c) * a.v_heads + h];
+        for (int i = tid; i < kChunk * kVecs; i += C::kThreads) {
+            const int r = i / kVecs, x = i % kVecs;
+            const int64_t tok = t0 + (r < n ? r : 0);
+            cp_async16_or_zero(tile_at<kVecs>(k, r, x), a.k + tok * a.k_ts + kh * a.k_hs + x * 8, r < n);
+            cp_async16_or_zero(tile_at<kVecs>(q, r, x), a.q + tok * a.q_ts + kh * a.q_hs + x * 8, r < n);
+        }
+        for (int i = tid; i < kChunk * 8; i += C::kThreads) {
+            const int r = i / 8, x = i % 8;
+            if (x / 2 > r / 16) continue;
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                cp_async16(smem + (tile_at<8>(tri + m * C::kTri, r, x) - base),
+                           (m < 2 ? ch.t[m] : ch.p[m - 2]) + r * kChunk + x * 8);
+        }
+        for (int i = tid; i < kChunk * 2 * NG; i += C::kThreads) {
+            const int r = i / (2 * NG), x = i % (2 * NG);
+            const bool ok = r < n && col0 + x * 8 < a.dv;
+            const int64_t tok = t0 + (r < n ? r : 0);
+            cp_async16_or_zero(tile_at<2 * NG>(v, r, x), a.v + tok * a.v_ts + h * a.v_hs + (ok ? col0 + x * 8 : 0), ok);
+        }
+        if (tid < 49) cp_async16(smem + (sc - base) + tid * 16, reinterpret_cast<const float4*>(ch.ck) + tid);
+        cp_async_commit();
+    };
+
+    // S^T as C fragments: rows (columns of the state) g, g + 8, columns (its rows)
+    // warp * DK / 4 + 8 n + 2t, + 1
+    float s[kN][4];
+    const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + warp * (DK / 4) + 2 * t) * a.dv + col + g;
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            s[n][e] = a.state_in && live ? a.state_in[at + static_cast<int64_t>(n * 8 + (e & 1)) * a.dv + (e >> 1) * 8] : 0.0f;
+    auto put_state = [&]() {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                uint32_t hi, lo;
+                split_scaled(s[n][e], s[n][e + 1], hi, lo);
+                const int r = g + e * 4, c = warp * kN + n;
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<kVecs>(s_hi, r, c) + t * 4), "r"(hi) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<kVecs>(s_lo, r, c) + t * 4), "r"(lo) : "memory");
+            }
+    };
+    auto put_rows = [&](uint32_t hi_at, uint32_t lo_at, const float (&x)[2][4]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                uint32_t hi, lo;
+                split_scaled(x[n][e], x[n][e + 1], hi, lo);
+                const int r = g + e * 4, c = warp * 2 + n;
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<8>(hi_at, r, c) + t * 4), "r"(hi) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<8>(lo_at, r, c) + t * 4), "r"(lo) : "memory");
+            }
+    };
+    auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); };
+    auto scale_pair = [&](uint32_t sc, int which, int n) {
+        float2 x;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(x.x), "=f"(x.y)
+                     : "r"(sc + (which * kChunk + warp * 16 + n * 8 + 2 * t) * 4));
+        return x;
+    };
+
+    const int chunks_here = (end - begin + kChunk - 1) / kChunk;
+    if (chunks_here > 0) load(0, 0);
+    put_state();
+    const int a_row = lane & 15, a_vec = lane >> 4;                                // A operand
+    const int b_row = (lane & 7) + (lane >> 4) * 8, b_vec = (lane >> 3) & 1;       // B operand, rows = n
+    for (int c = 0; c < chunks_here; ++c) {
+        cp_async_wait<0>();
+        __syncthreads();
+        if (c + 1 < chunks_here) load(c + 1, (c + 1) & 1);
+        const uint32_t k = base + (c & 1) * C::kStage, q = k + C::kTile, tri = q + C::kTile, v = tri + 4 * C::kTri,
+                       sc = v + kChunk * C::kVRow;
+        float keep;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(keep) : "r"(sc + 3 * kChunk * 4));
+
+        // ---- S0^T K^T and S0^T Q^T for this warp's tokens ----
+        float x[2][4], xl[2][4], o[2][4], ol[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = xl[n][e] = o[n][e] = ol[n][e] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; ++kk) {
+            uint32_t sh[4], sl[4], kf[4], qf[4];
+            ldsm4(sh, tile_at<kVecs>(s_hi, a_row, kk * 2 + a_vec));
+            ldsm4(sl, tile_at<kVecs>(s_lo, a_row, kk * 2 + a_vec));
+            ldsm4(kf, tile_at<kVecs>(k, warp * 16 + b_row, kk * 2 + b_vec));
+            ldsm4(qf, tile_at<kVecs>(q, warp * 16 + b_row, kk * 2 + b_vec));
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                mma16816(x[n], sh, kf[2 * n], kf[2 * n + 1]);
+                mma16816(xl[n], sl, kf[2 * n], kf[2 * n + 1]);
+                mma16816(o[n], sh, qf[2 * n], qf[2 * n + 1]);
+                mma16816(ol[n], sl, qf[2 * n], qf[2 * n + 1]);
+            }
+        }
+        uint32_t vf[4];
+        ldsm4_t(vf, tile_at<2 * NG>(v, warp * 16 + b_row, group * 2 + b_vec));
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float2 ck = scale_pair(sc, 0, n), cq = scale_pair(sc, 1, n);
+            const float2 v0 = __half22float2(u32_as_h2(vf[2 * n])), v1 = __half22float2(u32_as_h2(vf[2 * n + 1]));
+            x[n][0] = v0.x - ck.x * (x[n][0] + kLoInv * xl[n][0]);
+            x[n][1] = v0.y - ck.y * (x[n][1] + kLoInv * xl[n][1]);
+            x[n][2] = v1.x - ck.x * (x[n][2] + kLoInv * xl[n][2]);
+            x[n][3] = v1.y - ck.y * (x[n][3] + kLoInv * xl[n][3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[n][e] = (e & 1 ? cq.y : cq.x) * (o[n][e] + kLoInv * ol[n][e]);
+                ol[n][e] = 0.0f;
+            }
+        }
+        put_rows(r_hi, r_lo, x);
+        group_sync();
+
+        // ---- U^T = R^T T^T ----
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = xl[n][e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > warp) break;
+            uint32_t rh[4], rl[4], th[4], tl[4];
+            ldsm4(rh, tile_at<8>(r_hi, a_row, j * 2 + a_vec));
+            ldsm4(rl, tile_at<8>(r_lo, a_row, j * 2 + a_vec));
+            ldsm4(th, tile_at<8>(tri, warp * 16 + b_row, j * 2 + b_vec));
+            ldsm4(tl, tile_at<8>(tri + C::kTri, warp * 16 + b_row, j * 2 + b_vec));
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                mma16816(x[n], rh, th[2 * n], th[2 * n + 1]);
+                mma16816(xl[n], rl, th[2 * n], th[2 * n + 1]);
+                mma16816(xl[n], rh, tl[2 * n], tl[2 * n + 1]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] += kLoInv * xl[n][e];
+        put_rows(u_hi, u_lo, x);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float2 cs = scale_pair(sc, 2, n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] *= e & 1 ? cs.y : cs.x;
+        }
+        put_rows(w_hi, w_lo, x);
+        group_sync();
+
+        // ---- S'^T = keep S0^T + (U^T diag(cs)) K ----
+        float sl[kN][4];
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] *= keep;
+                sl[n][e] = 0.0f;
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t wh[4], wl[4];
+            ldsm4(wh, tile_at<8>(w_hi, a_row, j * 2 + a_vec));
+            ldsm4(wl, tile_at<8>(w_lo, a_row, j * 2 + a_vec));
+#pragma unroll
+            for (int p = 0; p < kN / 2; ++p) {
+                uint32_t kf[4];
+                ldsm4_t(kf, tile_at<kVecs>(k, j * 16 + a_row, warp * kN + p * 2 + a_vec));
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma16816(s[2 * p + n], wh, kf[2 * n], kf[2 * n + 1]);
+                    mma16816(sl[2 * p + n], wl, kf[2 * n], kf[2 * n + 1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] += kLoInv * sl[n][e];
+        put_state();
+
+        // ---- O^T += U^T P^T ----
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > warp) break;
+            uint32_t uh[4], ul[4], ph[4], pl[4];
+            ldsm4(uh, tile_at<8>(u_hi, a_row, j * 2 + a_vec));
+            ldsm4(ul, tile_at<8>(u_lo, a_row, j * 2 + a_vec));
+            ldsm4(ph, tile_at<8>(tri + 2 * C::kTri, warp * 16 + b_row, j * 2 + b_vec));
+            ldsm4(pl, tile_at<8>(tri + 3 * C::kTri, warp * 16 + b_row, j * 2 + b_vec));
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                mma16816(o[n], uh, ph[2 * n], ph[2 * n + 1]);
+                mma16816(ol[n], ul, ph[2 * n], ph[2 * n + 1]);
+                mma16816(ol[n], uh, pl[2 * n], pl[2 * n + 1]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int tok = begin + c * kChunk + warp * 16 + n * 8 + g;
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                // 8x8 transpose: lane (g, t) then has token g, columns 2t, 2t + 1
+                const uint32_t r = movm_t(h2_as_u32(__floats2half2_rn(o[n][e] + kLoInv * ol[n][e],
+                                                                       o[n][e + 1] + kLoInv * ol[n][e + 1])));
+                if (live && tok < end)
+                    *reinterpret_cast<uint32_t*>(a.out + (static_cast<int64_t>(tok) * a.v_heads + h) * a.dv + col + e * 4 +
+                                                 2 * t) = r;
+            }
+        }
+    }
+    if (a.state_out && live) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                a.state_out[at + static_cast<int64_t>(n * 8 + (e & 1)) * a.dv + (e >> 1) * 8] = s[n][e];
+    }
+}
+
+int64_t chunk_slots(int64_t tokens, int64_t batch) { return tokens / kChunk + batch; }
+
+template <int DK, int NG>
+int launch_scan(const DeltaArgs& a, const Chunk* chunks, cudaStream_t stream) {
+    using C = Scan<DK, NG>;
+    MCV_CHECK_CUDA(cudaFuncSetAttribute(scan_kernel<DK, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    return launch(scan_kernel<DK, NG>, dim3((a.dv / 16 + NG - 1) / NG, a.v_heads, a.batch), dim3(C::kThreads), C::kSmem,
+                  stream, a, chunks);
+}
+
+template <int DK>
+int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
+    Chunk* chunks = static_cast<Chunk*>(workspace);
+    constexpr int kSmem = 2 * kChunk * DK * 2 + kChunk * 68 * 4;
+    MCV_CHECK_CUDA(cudaFuncSetAttribute(chunk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    int st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
+                    kSmem, stream, a, chunks);
+    if (st) return st;
+    // as many column groups a block as still leave every SM a block
+    const int64_t groups = static_cast<int64_t>(a.batch) * a.v_heads * (a.dv / 16);
+    if (groups >= 4 * sm_count()) return launch_scan<DK, 4>(a, chunks, stream);
+    if (groups >= 2 * sm_count()) return launch_scan<DK, 2>(a, chunks, stream);
+    return launch_scan<DK, 1>(a, chunks, stream);
+}
+
 int fill_args(const char* who, const mcv_gated_delta* p, int64_t tokens, int64_t batch, DeltaArgs& a) {
     if (!p || !p->g || !p->beta || !p->out) return fail(MCV_ERR_NULL, std::string(who) + ": null pointer");
     if (p->key_dim != 64 && p->key_dim != 128) return fail(MCV_ERR_SHAPE, std::string(who) + ": key_dim must be 64 or 128");
@@ -220,7 +733,7 @@ int mcv_gated_delta_step(const mcv_gated_delta* args, int64_t batch, mcv_stream_
 size_t mcv_gated_delta_workspace_size(int64_t tokens, int64_t batch, int64_t v_heads, int64_t key_dim,
                                       int64_t value_dim) {
     if (tokens < 1 || batch < 1 || v_heads < 1 || (key_dim != 64 && key_dim != 128) || value_dim < 16) return 0;
-    return 16;
+    return static_cast<size_t>(chunk_slots(tokens, batch)) * v_heads * sizeof(Chunk);
 }
 
 int mcv_gated_delta_prefill(const mcv_gated_delta* args, const void* cu_seqlens, int64_t tokens, int64_t batch,
@@ -233,7 +746,8 @@ int mcv_gated_delta_prefill(const mcv_gated_delta* args, const void* cu_seqlens,
         return fail(MCV_ERR_WORKSPACE, "gated_delta_prefill: workspace missing or too small");
     if (!aligned16(workspace)) return fail(MCV_ERR_ALIGN, "gated_delta_prefill: workspace must be 16-byte aligned");
     a.cu = static_cast<const int32_t*>(cu_seqlens);
-    return run_recurrent(a, args->key_dim, static_cast<cudaStream_t>(stream));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return args->key_dim == 128 ? run_chunked<128>(a, workspace, s) : run_chunked<64>(a, workspace, s);
 }
 
 }  // extern "C"
