@@ -182,16 +182,24 @@ __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uin
     lo = h2_as_u32(__floats2half2_rn((x - f.x) * kLo, (y - f.y) * kLo));
 }
 
+// T and P are kept as their ten 16x16 blocks on and below the diagonal, block
+// (i, j) at i (i + 1) / 2 + j, each as four 8x8 matrices of 128 contiguous bytes
+// in the order in which ldmatrix takes the MMA's B operand: the address of lane l
+// is just 16 l, and no bank is hit twice.
+constexpr int kBlocks = 10;
+__host__ __device__ constexpr int block_at(int i, int j) { return (i * (i + 1) / 2 + j) * 256; }   // in elements
+
 // One chunk's share of the workspace.
 struct Chunk {
-    __half t[2][kChunk * kChunk];    // T hi, lo, by rows
-    __half p[2][kChunk * kChunk];    // P hi, lo
+    __half t[2][kBlocks * 256];      // T hi, lo
+    __half p[2][kBlocks * 256];      // P hi, lo
     float ck[kChunk];                // e^G r_k
     float cq[kChunk];                // scale e^G r_q
     float cs[kChunk];                // e^(G_C - G) r_k
     float keep;                      // e^G_C
     float pad[31];
 };
+constexpr int kChunkVecs = (4 * kBlocks * 256 * 2 + (3 * kChunk + 4) * 4) / 16;   // 16-byte vectors in use
 static_assert(sizeof(Chunk) % 128 == 0, "chunks stay aligned");
 
 // The slots of sequence b begin at cu[b] / 64 + b: ranges of ceil(len / 64) from
@@ -211,6 +219,7 @@ __global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* ch
     extern __shared__ __align__(128) unsigned char smem[];
     float* mat = reinterpret_cast<float*>(smem + 2 * kChunk * DK * 2);     // A, rows of 68
     constexpr int kMatRow = 68;
+    float* inv = mat + kChunk * kMatRow;                                   // (I + A)^-1
     __shared__ double gsum[kChunk];
     __shared__ float rk[kChunk], rq[kChunk], bt[kChunk];
     pdl_trigger();
@@ -333,53 +342,111 @@ __global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* ch
             }
             uint32_t phi, plo;
             split_scaled(p[0], p[1], phi, plo);
-            *reinterpret_cast<uint32_t*>(&out.p[0][r * kChunk + c]) = phi;
-            *reinterpret_cast<uint32_t*>(&out.p[1][r * kChunk + c]) = plo;
+            const int at = block_at(warp, j / 2) + (e + (j & 1)) * 64 + (lane >> 2) * 8 + (lane & 3) * 2;
+            *reinterpret_cast<uint32_t*>(&out.p[0][at]) = phi;
+            *reinterpret_cast<uint32_t*>(&out.p[1][at]) = plo;
             *reinterpret_cast<float2*>(mat + r * kMatRow + c) = make_float2(m[0], m[1]);
         }
     }
     __syncthreads();
-    // column j of (I + A)^-1 by forward substitution, one thread a column:
-    // x_i = [i = j] - sum_{l < i} A_il x_l (x_l = 0 above the diagonal)
+
+    // X = (I + A)^-1 by blocks of 16.  Diagonal blocks by forward substitution,
+    // one thread a column: x_i = [i = j] - sum_{l < i} A_il x_l.
     if (tid < kChunk) {
-        float x[kChunk];
-        const float beta = bt[tid];
+        const float* m = mat + (tid & ~15) * (kMatRow + 1);
+        float* xo = inv + (tid & ~15) * kMatRow + tid;
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            float acc[4] = {i == tid ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < 16; ++i) {
+            float acc[2] = {i == (tid & 15) ? 1.0f : 0.0f, 0.0f};
 #pragma unroll
-            for (int l = 0; l < i; l += 4) {
-                const float4 m = *reinterpret_cast<const float4*>(mat + i * kMatRow + l);
-                acc[0] -= m.x * x[l];
-                if (l + 1 < i) acc[1] -= m.y * x[l + 1];
-                if (l + 2 < i) acc[2] -= m.z * x[l + 2];
-                if (l + 3 < i) acc[3] -= m.w * x[l + 3];
-            }
-            x[i] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-            const float t = x[i] * beta;
-            const __half th = __float2half_rn(t);
-            out.t[0][i * kChunk + tid] = th;
-            out.t[1][i * kChunk + tid] = __float2half_rn((t - __half2float(th)) * kLo);
+            for (int l = 0; l < i; ++l) acc[l & 1] -= m[i * kMatRow + l] * x[l];
+            x[i] = acc[0] + acc[1];
+            xo[i * kMatRow] = x[i];
         }
+    }
+    __syncthreads();
+    // Block rows below: X_ij = -X_ii sum_{j <= l < i} A_il X_lj, in 4x4 tiles; the
+    // sums take the place of A's row, which is not needed any more.
+    const int tr = tid & 3, tc = tid >> 2;      // tile row within the block row, tile column
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        const bool mine = tc < 4 * i;
+        float4 y[4];
+        auto product = [&](const float* left, const float* right, int from, int to) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int l = from; l < to; l += 4) {
+                float4 b[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) b[q] = *reinterpret_cast<const float4*>(right + (l + q) * kMatRow + tc * 4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float4 w = *reinterpret_cast<const float4*>(left + (tr * 4 + r) * kMatRow + l);
+                    y[r].x += w.x * b[0].x + w.y * b[1].x + w.z * b[2].x + w.w * b[3].x;
+                    y[r].y += w.x * b[0].y + w.y * b[1].y + w.z * b[2].y + w.w * b[3].y;
+                    y[r].z += w.x * b[0].z + w.y * b[1].z + w.z * b[2].z + w.w * b[3].z;
+                    y[r].w += w.x * b[0].w + w.y * b[1].w + w.z * b[2].w + w.w * b[3].w;
+                }
+            }
+        };
+        float* sums = mat + i * 16 * kMatRow;
+        if (mine) product(sums, inv, (tc / 4) * 16, i * 16);
+        __syncthreads();
+        if (mine) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(sums + (tr * 4 + r) * kMatRow + tc * 4) = y[r];
+        }
+        __syncthreads();
+        if (mine) {
+            product(inv + i * 16 * (kMatRow + 1), sums, 0, 16);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<float4*>(inv + (i * 16 + tr * 4 + r) * kMatRow + tc * 4) =
+                    make_float4(-y[r].x, -y[r].y, -y[r].z, -y[r].w);
+        }
+        __syncthreads();
+    }
+    for (int v = tid; v < kBlocks * 32; v += 128) {
+        const int blk = v / 32, i = blk >= 6 ? 3 : (blk >= 3 ? 2 : (blk >= 1 ? 1 : 0)), j = blk - i * (i + 1) / 2;
+        const int r = i * 16 + (v & 7) + ((v >> 4) & 1) * 8, c = j * 16 + ((v >> 3) & 1) * 8;
+        uint4 hi, lo;
+        uint32_t* hp = &hi.x;
+        uint32_t* lp = &lo.x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 x = *reinterpret_cast<const float2*>(inv + r * kMatRow + c + 2 * e);
+            // above the diagonal of a diagonal block the substitution left zeros
+            split_scaled(x.x * bt[c + 2 * e], x.y * bt[c + 2 * e + 1], hp[e], lp[e]);
+        }
+        reinterpret_cast<uint4*>(out.t[0])[v] = hi;
+        reinterpret_cast<uint4*>(out.t[1])[v] = lo;
     }
 }
 
-// The walk.  A group of four warps owns 16 value columns of a head, a block
-// `NG` groups that share the chunk's tiles (two of them in flight).  All
-// products are taken transposed, with the 16 columns as the MMA's m, so that
-// results turn into the next product's A operand by a trip through shared
-// memory (S, R and U change hands between the warps, each of which has 16
-// tokens of a chunk and a quarter of the state's rows):
-//   R^T = V^T - (S0^T K^T) diag(ck);  U^T = R^T T^T;
-//   O^T = (S0^T Q^T) diag(cq) + U^T P^T;  S'^T = keep S0^T + (U^T diag(cs)) K.
-// Blocks of T and P above the diagonal are neither loaded nor multiplied.
+// The walk.  Eight warps own 16 value columns of a head: four carry the state
+// (each a quarter of its rows, in registers), four make the outputs; a block
+// has NG such groups, which share the chunk's tiles, and four warps that load the
+// next chunk's while this one's are in use.  All products are taken
+// transposed, with the 16 columns as the MMA's m:
+//   R^T = V^T - (S0^T K^T) diag(ck);  U^T = R^T T^T;  S'^T = keep S0^T + (U^T diag(cs)) K
+// by the state's warps, each for 16 tokens or a quarter of the rows, with R, U
+// and S changing hands through shared memory, and beside them
+//   O^T = (S0^T Q^T) diag(cq) + U^T P^T.
+// A product of S waits for the chunk before it, so a walk's speed is this chain of
+// three small products, not its operations; taking the outputs out of it and
+// keeping 16 columns a group makes it as short as the MMA allows.  Warp w and
+// the output warp beside it on the same scheduler take tokens 16 w and 16 (3 - w), so
+// that the triangles' work adds up to the same on each.
 template <int DK, int NG>
 struct Scan {
-    static constexpr int kThreads = NG * 128;
+    static constexpr int kThreads = NG * 256 + 128;
     static constexpr int kTile = kChunk * DK * 2;
-    static constexpr int kTri = kChunk * kChunk * 2;
-    static constexpr int kVRow = NG * 32;
-    static constexpr int kStage = 2 * kTile + 4 * kTri + kChunk * kVRow + 1024;
+    static constexpr int kTri = kBlocks * 512;
+    static constexpr int kV = 2 * kTile;
+    static constexpr int kRecord = kV + kChunk * NG * 32;
+    static constexpr int kScales = kRecord + 4 * kTri;
+    static constexpr int kStage = (kRecord + kChunkVecs * 16 + 127) / 128 * 128;
     static constexpr int kSx = 16 * DK * 2;
     static constexpr int kRx = 16 * kChunk * 2;
     static constexpr int kGroup = 2 * kSx + 6 * kRx;
@@ -387,58 +454,150 @@ struct Scan {
 };
 
 template <int DK, int NG>
-__global__ void __launch_bounds__(NG * 128) scan_kernel(const DeltaArgs a, const Chunk* chunks) {
+__global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs a, const Chunk* chunks) {
     using C = Scan<DK, NG>;
     constexpr int kVecs = DK / 8;
-    constexpr int kN = DK / 32;       // n8 tiles of a warp's state rows
+    constexpr int kN = DK / 32;       // n8 tiles of a state warp's rows
     extern __shared__ __align__(128) unsigned char smem[];
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3, group = tid >> 7;
+    const int tid = threadIdx.x, lane = tid & 31;
     const int g = lane >> 2, t = lane & 3;
     const int h = blockIdx.y, b = blockIdx.z;
-    const int kh = h / a.share;
     const int col0 = blockIdx.x * NG * 16;
-    const int col = col0 + group * 16;
-    const bool live = col < a.dv;
     int begin, end, slot;
     if (!sequence(a, b, begin, end, slot)) return;
-
+    const int chunks_here = (end - begin + kChunk - 1) / kChunk;
     const uint32_t base = smem_u32(smem);
-    const uint32_t gx = base + 2 * C::kStage + group * C::kGroup;
-    const uint32_t s_hi = gx, s_lo = gx + C::kSx, r_hi = gx + 2 * C::kSx, r_lo = r_hi + C::kRx, u_hi = r_lo + C::kRx,
-                   u_lo = u_hi + C::kRx, w_hi = u_lo + C::kRx, w_lo = w_hi + C::kRx;
 
-    auto load = [&](int c, int stage) {
-        const uint32_t k = base + stage * C::kStage, q = k + C::kTile, tri = q + C::kTile, v = tri + 4 * C::kTri,
-                       sc = v + kChunk * C::kVRow;
-        const int t0 = begin + c * kChunk;
-        const int n = min(kChunk, end - t0);
-        const Chunk& ch = chunks[(first_chunk(begin, b) + c) * a.v_heads + h];
-        for (int i = tid; i < kChunk * kVecs; i += C::kThreads) {
-            const int r = i / kVecs, x = i % kVecs;
-            const int64_t tok = t0 + (r < n ? r : 0);
-            cp_async16_or_zero(tile_at<kVecs>(k, r, x), a.k + tok * a.k_ts + kh * a.k_hs + x * 8, r < n);
-            cp_async16_or_zero(tile_at<kVecs>(q, r, x), a.q + tok * a.q_ts + kh * a.q_hs + x * 8, r < n);
-        }
-        for (int i = tid; i < kChunk * 8; i += C::kThreads) {
-            const int r = i / 8, x = i % 8;
-            if (x / 2 > r / 16) continue;
+    if (tid >= NG * 256) {
+        // ---- the loading warps: one chunk ahead ----
+        constexpr int kStep = 128 / kVecs;           // rows of one sweep of the 128 threads; a multiple of 8,
+        static_assert(kStep % 8 == 0, "swizzle");    // so a thread keeps its place in the swizzle
+        const int kh = h / a.share, lt = tid - NG * 256;
+        const int lr = lt / kVecs, lx = lt % kVecs;
+        const __half* kp = a.k + static_cast<int64_t>(begin + lr) * a.k_ts + kh * a.k_hs + lx * 8;
+        const __half* qp = a.q + static_cast<int64_t>(begin + lr) * a.q_ts + kh * a.q_hs + lx * 8;
+        const int64_t k_step = kStep * a.k_ts, q_step = kStep * a.q_ts;
+        const uint4* rec = reinterpret_cast<const uint4*>(chunks + first_chunk(begin, b) * a.v_heads + h) + lt;
+        for (int c = 0; c < chunks_here; ++c) {
+            const uint32_t stage = base + (c & 1) * C::kStage;
+            const uint32_t dst = tile_at<kVecs>(stage, lr, lx);
+            const int t0 = begin + c * kChunk;
+            const int n = min(kChunk, end - t0);
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-                cp_async16(smem + (tile_at<8>(tri + m * C::kTri, r, x) - base),
-                           (m < 2 ? ch.t[m] : ch.p[m - 2]) + r * kChunk + x * 8);
+            for (int i = 0; i < kChunk / kStep; ++i) {
+                const bool ok = i * kStep + lr < n;
+                cp_async16_or_zero(dst + i * kStep * kVecs * 16, ok ? kp : a.k, ok);
+                cp_async16_or_zero(dst + i * kStep * kVecs * 16 + C::kTile, ok ? qp : a.q, ok);
+                kp += k_step;
+                qp += q_step;
+            }
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const int item = i * 128 + lt, r = item / (2 * NG), x = item % (2 * NG);
+                const bool ok = r < n && col0 + x * 8 < a.dv;
+                cp_async16_or_zero(tile_at<2 * NG>(stage + C::kV, r, x),
+                                   ok ? a.v + static_cast<int64_t>(t0 + r) * a.v_ts + h * a.v_hs + col0 + x * 8 : a.v, ok);
+            }
+#pragma unroll
+            for (int i = 0; i < (kChunkVecs + 127) / 128; ++i)
+                if (i * 128 + lt < kChunkVecs) cp_async16_or_zero(stage + C::kRecord + (i * 128 + lt) * 16, rec + i * 128, true);
+            rec += static_cast<int64_t>(a.v_heads) * (sizeof(Chunk) / 16);
+            cp_async_commit();
+            cp_async_wait<0>();
+            __syncthreads();   // chunk c is there, and c - 1 is done with
         }
-        for (int i = tid; i < kChunk * 2 * NG; i += C::kThreads) {
-            const int r = i / (2 * NG), x = i % (2 * NG);
-            const bool ok = r < n && col0 + x * 8 < a.dv;
-            const int64_t tok = t0 + (r < n ? r : 0);
-            cp_async16_or_zero(tile_at<2 * NG>(v, r, x), a.v + tok * a.v_ts + h * a.v_hs + (ok ? col0 + x * 8 : 0), ok);
-        }
-        if (tid < 49) cp_async16(smem + (sc - base) + tid * 16, reinterpret_cast<const float4*>(ch.ck) + tid);
-        cp_async_commit();
-    };
+        return;
+    }
 
+    const int group = tid >> 8, warp = (tid >> 5) & 3;
+    const bool outputs = (tid >> 7) & 1;
+    const int col = col0 + group * 16;
+    const bool live = col < a.dv;
+    const uint32_t s_hi = base + 2 * C::kStage + group * C::kGroup, s_lo = s_hi + C::kSx, r_hi = s_lo + C::kSx,
+                   r_lo = r_hi + C::kRx, u_hi = r_lo + C::kRx, u_lo = u_hi + C::kRx, w_hi = u_lo + C::kRx,
+                   w_lo = w_hi + C::kRx;
+    const int blk = outputs ? 3 - warp : warp;       // this warp's 16 tokens of a chunk
+    const int a_row = lane & 15, a_vec = lane >> 4;                                // A operand
+    const int b_row = (lane & 7) + (lane >> 4) * 8, b_vec = (lane >> 3) & 1;       // B operand, rows = n
+    auto state_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + 2 * group) : "memory"); };
+    auto group_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(2 + 2 * group) : "memory"); };
+    auto scale_pair = [&](uint32_t sc, int which, int n) {
+        float2 x;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(x.x), "=f"(x.y)
+                     : "r"(sc + (which * kChunk + blk * 16 + n * 8 + 2 * t) * 4));
+        return x;
+    };
+    auto put = [&](uint32_t at, uint32_t x) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); };
+
+    if (outputs) {
+        for (int c = 0; c < chunks_here; ++c) {
+            __syncthreads();
+            const uint32_t stage = base + (c & 1) * C::kStage, sc = stage + C::kScales;
+            const uint32_t p_hi = stage + C::kRecord + 2 * C::kTri, p_lo = p_hi + C::kTri;
+            float o[2][4], ol[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][e] = ol[n][e] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < DK / 16; ++kk) {
+                uint32_t sh[4], sl[4], qf[4];
+                ldsm4(sh, tile_at<kVecs>(s_hi, a_row, kk * 2 + a_vec));
+                ldsm4(sl, tile_at<kVecs>(s_lo, a_row, kk * 2 + a_vec));
+                ldsm4(qf, tile_at<kVecs>(stage + C::kTile, blk * 16 + b_row, kk * 2 + b_vec));
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma16816(o[n], sh, qf[2 * n], qf[2 * n + 1]);
+                    mma16816(ol[n], sl, qf[2 * n], qf[2 * n + 1]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float2 cq = scale_pair(sc, 1, n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[n][e] = (e & 1 ? cq.y : cq.x) * (o[n][e] + kLoInv * ol[n][e]);
+                    ol[n][e] = 0.0f;
+                }
+            }
+            group_sync();       // U is there, and S0 has been read
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j > blk) break;
+                uint32_t uh[4], ul[4], ph[4], pl[4];
+                ldsm4(uh, tile_at<8>(u_hi, a_row, j * 2 + a_vec));
+                ldsm4(ul, tile_at<8>(u_lo, a_row, j * 2 + a_vec));
+                const uint32_t at = block_at(blk, j) * 2 + lane * 16;
+                ldsm4(ph, p_hi + at);
+                ldsm4(pl, p_lo + at);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma16816(o[n], uh, ph[2 * n], ph[2 * n + 1]);
+                    mma16816(ol[n], ul, ph[2 * n], ph[2 * n + 1]);
+                    mma16816(ol[n], uh, pl[2 * n], pl[2 * n + 1]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int tok = begin + c * kChunk + blk * 16 + n * 8 + g;
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    // 8x8 transpose: lane (g, t) then has token g, columns 2t, 2t + 1
+                    const uint32_t r = movm_t(h2_as_u32(__floats2half2_rn(o[n][e] + kLoInv * ol[n][e],
+                                                                           o[n][e + 1] + kLoInv * ol[n][e + 1])));
+                    if (live && tok < end)
+                        *reinterpret_cast<uint32_t*>(a.out + (static_cast<int64_t>(tok) * a.v_heads + h) * a.dv + col +
+                                                     e * 4 + 2 * t) = r;
+                }
+            }
+        }
+        return;
+    }
+
+    // ---- the state's warps ----
     // S^T as C fragments: rows (columns of the state) g, g + 8, columns (its rows)
     // warp * DK / 4 + 8 n + 2t, + 1
     float s[kN][4];
@@ -455,9 +614,8 @@ __global__ void __launch_bounds__(NG * 128) scan_kernel(const DeltaArgs a, const
             for (int e = 0; e < 4; e += 2) {
                 uint32_t hi, lo;
                 split_scaled(s[n][e], s[n][e + 1], hi, lo);
-                const int r = g + e * 4, c = warp * kN + n;
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<kVecs>(s_hi, r, c) + t * 4), "r"(hi) : "memory");
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<kVecs>(s_lo, r, c) + t * 4), "r"(lo) : "memory");
+                put(tile_at<kVecs>(s_hi, g + e * 4, warp * kN + n) + t * 4, hi);
+                put(tile_at<kVecs>(s_lo, g + e * 4, warp * kN + n) + t * 4, lo);
             }
     };
     auto put_rows = [&](uint32_t hi_at, uint32_t lo_at, const float (&x)[2][4]) {
@@ -467,87 +625,62 @@ __global__ void __launch_bounds__(NG * 128) scan_kernel(const DeltaArgs a, const
             for (int e = 0; e < 4; e += 2) {
                 uint32_t hi, lo;
                 split_scaled(x[n][e], x[n][e + 1], hi, lo);
-                const int r = g + e * 4, c = warp * 2 + n;
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<8>(hi_at, r, c) + t * 4), "r"(hi) : "memory");
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile_at<8>(lo_at, r, c) + t * 4), "r"(lo) : "memory");
+                put(tile_at<8>(hi_at, g + e * 4, warp * 2 + n) + t * 4, hi);
+                put(tile_at<8>(lo_at, g + e * 4, warp * 2 + n) + t * 4, lo);
             }
     };
-    auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); };
-    auto scale_pair = [&](uint32_t sc, int which, int n) {
-        float2 x;
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
-                     : "=f"(x.x), "=f"(x.y)
-                     : "r"(sc + (which * kChunk + warp * 16 + n * 8 + 2 * t) * 4));
-        return x;
-    };
-
-    const int chunks_here = (end - begin + kChunk - 1) / kChunk;
-    if (chunks_here > 0) load(0, 0);
     put_state();
-    const int a_row = lane & 15, a_vec = lane >> 4;                                // A operand
-    const int b_row = (lane & 7) + (lane >> 4) * 8, b_vec = (lane >> 3) & 1;       // B operand, rows = n
     for (int c = 0; c < chunks_here; ++c) {
-        cp_async_wait<0>();
         __syncthreads();
-        if (c + 1 < chunks_here) load(c + 1, (c + 1) & 1);
-        const uint32_t k = base + (c & 1) * C::kStage, q = k + C::kTile, tri = q + C::kTile, v = tri + 4 * C::kTri,
-                       sc = v + kChunk * C::kVRow;
-        float keep;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(keep) : "r"(sc + 3 * kChunk * 4));
+        const uint32_t stage = base + (c & 1) * C::kStage, sc = stage + C::kScales;
+        const uint32_t t_hi = stage + C::kRecord, t_lo = t_hi + C::kTri;
 
-        // ---- S0^T K^T and S0^T Q^T for this warp's tokens ----
-        float x[2][4], xl[2][4], o[2][4], ol[2][4];
+        // S0^T K^T for this warp's tokens
+        float x[2][4], xl[2][4];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[n][e] = xl[n][e] = o[n][e] = ol[n][e] = 0.0f;
+            for (int e = 0; e < 4; ++e) x[n][e] = xl[n][e] = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
-            uint32_t sh[4], sl[4], kf[4], qf[4];
+            uint32_t sh[4], sl[4], kf[4];
             ldsm4(sh, tile_at<kVecs>(s_hi, a_row, kk * 2 + a_vec));
             ldsm4(sl, tile_at<kVecs>(s_lo, a_row, kk * 2 + a_vec));
-            ldsm4(kf, tile_at<kVecs>(k, warp * 16 + b_row, kk * 2 + b_vec));
-            ldsm4(qf, tile_at<kVecs>(q, warp * 16 + b_row, kk * 2 + b_vec));
+            ldsm4(kf, tile_at<kVecs>(stage, blk * 16 + b_row, kk * 2 + b_vec));
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 mma16816(x[n], sh, kf[2 * n], kf[2 * n + 1]);
                 mma16816(xl[n], sl, kf[2 * n], kf[2 * n + 1]);
-                mma16816(o[n], sh, qf[2 * n], qf[2 * n + 1]);
-                mma16816(ol[n], sl, qf[2 * n], qf[2 * n + 1]);
             }
         }
         uint32_t vf[4];
-        ldsm4_t(vf, tile_at<2 * NG>(v, warp * 16 + b_row, group * 2 + b_vec));
+        ldsm4_t(vf, tile_at<2 * NG>(stage + C::kV, blk * 16 + b_row, group * 2 + b_vec));
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const float2 ck = scale_pair(sc, 0, n), cq = scale_pair(sc, 1, n);
+            const float2 ck = scale_pair(sc, 0, n);
             const float2 v0 = __half22float2(u32_as_h2(vf[2 * n])), v1 = __half22float2(u32_as_h2(vf[2 * n + 1]));
             x[n][0] = v0.x - ck.x * (x[n][0] + kLoInv * xl[n][0]);
             x[n][1] = v0.y - ck.y * (x[n][1] + kLoInv * xl[n][1]);
             x[n][2] = v1.x - ck.x * (x[n][2] + kLoInv * xl[n][2]);
             x[n][3] = v1.y - ck.y * (x[n][3] + kLoInv * xl[n][3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[n][e] = (e & 1 ? cq.y : cq.x) * (o[n][e] + kLoInv * ol[n][e]);
-                ol[n][e] = 0.0f;
-            }
         }
         put_rows(r_hi, r_lo, x);
-        group_sync();
+        state_sync();
 
-        // ---- U^T = R^T T^T ----
+        // U^T = R^T T^T
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[n][e] = xl[n][e] = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (j > warp) break;
+            if (j > blk) break;
             uint32_t rh[4], rl[4], th[4], tl[4];
             ldsm4(rh, tile_at<8>(r_hi, a_row, j * 2 + a_vec));
             ldsm4(rl, tile_at<8>(r_lo, a_row, j * 2 + a_vec));
-            ldsm4(th, tile_at<8>(tri, warp * 16 + b_row, j * 2 + b_vec));
-            ldsm4(tl, tile_at<8>(tri + C::kTri, warp * 16 + b_row, j * 2 + b_vec));
+            const uint32_t ta = block_at(blk, j) * 2 + lane * 16;
+            ldsm4(th, t_hi + ta);
+            ldsm4(tl, t_lo + ta);
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 mma16816(x[n], rh, th[2 * n], th[2 * n + 1]);
@@ -569,8 +702,9 @@ __global__ void __launch_bounds__(NG * 128) scan_kernel(const DeltaArgs a, const
         put_rows(w_hi, w_lo, x);
         group_sync();
 
-        // ---- S'^T = keep S0^T + (U^T diag(cs)) K ----
-        float sl[kN][4];
+        // S'^T = keep S0^T + (U^T diag(cs)) K
+        float keep, sl[kN][4];
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(keep) : "r"(sc + 3 * kChunk * 4));
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -586,7 +720,7 @@ __global__ void __launch_bounds__(NG * 128) scan_kernel(const DeltaArgs a, const
 #pragma unroll
             for (int p = 0; p < kN / 2; ++p) {
                 uint32_t kf[4];
-                ldsm4_t(kf, tile_at<kVecs>(k, j * 16 + a_row, warp * kN + p * 2 + a_vec));
+                ldsm4_t(kf, tile_at<kVecs>(stage, j * 16 + a_row, warp * kN + p * 2 + a_vec));
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     mma16816(s[2 * p + n], wh, kf[2 * n], kf[2 * n + 1]);
@@ -599,36 +733,6 @@ __global__ void __launch_bounds__(NG * 128) scan_kernel(const DeltaArgs a, const
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] += kLoInv * sl[n][e];
         put_state();
-
-        // ---- O^T += U^T P^T ----
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > warp) break;
-            uint32_t uh[4], ul[4], ph[4], pl[4];
-            ldsm4(uh, tile_at<8>(u_hi, a_row, j * 2 + a_vec));
-            ldsm4(ul, tile_at<8>(u_lo, a_row, j * 2 + a_vec));
-            ldsm4(ph, tile_at<8>(tri + 2 * C::kTri, warp * 16 + b_row, j * 2 + b_vec));
-            ldsm4(pl, tile_at<8>(tri + 3 * C::kTri, warp * 16 + b_row, j * 2 + b_vec));
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                mma16816(o[n], uh, ph[2 * n], ph[2 * n + 1]);
-                mma16816(ol[n], ul, ph[2 * n], ph[2 * n + 1]);
-                mma16816(ol[n], uh, pl[2 * n], pl[2 * n + 1]);
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int tok = begin + c * kChunk + warp * 16 + n * 8 + g;
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-                // 8x8 transpose: lane (g, t) then has token g, columns 2t, 2t + 1
-                const uint32_t r = movm_t(h2_as_u32(__floats2half2_rn(o[n][e] + kLoInv * ol[n][e],
-                                                                       o[n][e + 1] + kLoInv * ol[n][e + 1])));
-                if (live && tok < end)
-                    *reinterpret_cast<uint32_t*>(a.out + (static_cast<int64_t>(tok) * a.v_heads + h) * a.dv + col + e * 4 +
-                                                 2 * t) = r;
-            }
-        }
     }
     if (a.state_out && live) {
 #pragma unroll
@@ -652,15 +756,14 @@ int launch_scan(const DeltaArgs& a, const Chunk* chunks, cudaStream_t stream) {
 template <int DK>
 int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     Chunk* chunks = static_cast<Chunk*>(workspace);
-    constexpr int kSmem = 2 * kChunk * DK * 2 + kChunk * 68 * 4;
+    constexpr int kSmem = 2 * kChunk * DK * 2 + 2 * kChunk * 68 * 4;
     MCV_CHECK_CUDA(cudaFuncSetAttribute(chunk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     int st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
                     kSmem, stream, a, chunks);
     if (st) return st;
-    // as many column groups a block as still leave every SM a block
+    // two column groups a block once single ones would not all run at once
     const int64_t groups = static_cast<int64_t>(a.batch) * a.v_heads * (a.dv / 16);
-    if (groups >= 4 * sm_count()) return launch_scan<DK, 4>(a, chunks, stream);
-    if (groups >= 2 * sm_count()) return launch_scan<DK, 2>(a, chunks, stream);
+    if (groups > sm_count()) return launch_scan<DK, 2>(a, chunks, stream);
     return launch_scan<DK, 1>(a, chunks, stream);
 }
 
