@@ -213,15 +213,56 @@ __device__ __forceinline__ uint32_t tile_at(uint32_t base, int r, int c) {
     return base + r * (VECS * 16) + ((c ^ (r & (VECS < 8 ? VECS - 1 : 7))) << 4);
 }
 
+// Decays are kept in halvings, summed in fp64 and stored as the sum of two floats:
+// a difference of two far sums then loses nothing, and 2^x is one instruction.
+__device__ __forceinline__ float2 two_floats(double x) {
+    const float h = static_cast<float>(x);
+    return make_float2(h, static_cast<float>(x - h));
+}
+__device__ __forceinline__ float decay_between(float2 later, float2 earlier) {
+    return exp2f((later.x - earlier.x) + (later.y - earlier.y));
+}
+
+// 16x16 fp32 block as a product's operands.  acc + 2^-11 acc_lo += a b.
+struct Split4 {
+    uint32_t hi[4], lo[4];
+};
+__device__ __forceinline__ void mma_split(float (&acc)[2][4], float (&acc_lo)[2][4], const Split4& a, const Split4& b) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        mma16816(acc[n], a.hi, b.hi[2 * n], b.hi[2 * n + 1]);
+        mma16816(acc_lo[n], a.lo, b.hi[2 * n], b.hi[2 * n + 1]);
+        mma16816(acc_lo[n], a.hi, b.lo[2 * n], b.lo[2 * n + 1]);
+    }
+}
+// A result (C fragments of two n8 tiles) as the next product's B operand: 8x8 transposes.
+__device__ __forceinline__ void to_b(Split4& b, const float (&x)[2][4]) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            uint32_t hi, lo;
+            split_scaled(x[n][e], x[n][e + 1], hi, lo);
+            b.hi[2 * n + e / 2] = movm_t(hi);
+            b.lo[2 * n + e / 2] = movm_t(lo);
+        }
+}
+
+// Per chunk and value head.  Q K^T and K K^T by MMA, each warp 16 rows up to the
+// diagonal block; then X = (I + A)^-1 by 16x16 blocks: the diagonal ones by
+// forward substitution in fp32, one thread a column, the rest
+//   X_ij = -X_ii sum_{j <= l < i} A_il X_lj
+// by split MMAs, one warp a column of blocks, in registers - the columns do not
+// depend on each other.
 template <int DK>
-__global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* chunks) {
+__global__ void __launch_bounds__(128, 4) chunk_kernel(const DeltaArgs a, Chunk* chunks) {
     constexpr int kVecs = DK / 8;
     extern __shared__ __align__(128) unsigned char smem[];
-    float* mat = reinterpret_cast<float*>(smem + 2 * kChunk * DK * 2);     // A, rows of 68
-    constexpr int kMatRow = 68;
-    float* inv = mat + kChunk * kMatRow;                                   // (I + A)^-1
-    __shared__ double gsum[kChunk];
-    __shared__ float rk[kChunk], rq[kChunk], bt[kChunk];
+    __shared__ __align__(128) __half a_blk[2][6 * 256];     // A below the diagonal blocks, hi and lo, in MMA order
+    __shared__ __align__(128) __half x_blk[2][4 * 256];     // inverses of the diagonal blocks
+    __shared__ float diag[4][16 * 17];
+    __shared__ float4 rows[kChunk];                         // G (two floats), r_k, r_q scale
+    __shared__ float bt[kChunk];
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -242,23 +283,31 @@ __global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* ch
     const int kh = h / a.share;
 
     const uint32_t ks = smem_u32(smem), qs = ks + kChunk * DK * 2;
-    for (int i = tid; i < kChunk * kVecs; i += 128) {
-        const int r = i / kVecs, c = i % kVecs;
-        const int64_t t = t0 + (r < n ? r : 0);
-        cp_async16_or_zero(tile_at<kVecs>(ks, r, c), a.k + t * a.k_ts + kh * a.k_hs + c * 8, r < n);
-        cp_async16_or_zero(tile_at<kVecs>(qs, r, c), a.q + t * a.q_ts + kh * a.q_hs + c * 8, r < n);
+    {
+        constexpr int kStep = 128 / kVecs;
+        const int lr = tid / kVecs, lx = tid % kVecs;
+        const __half* kp = a.k + static_cast<int64_t>(t0 + lr) * a.k_ts + kh * a.k_hs + lx * 8;
+        const __half* qp = a.q + static_cast<int64_t>(t0 + lr) * a.q_ts + kh * a.q_hs + lx * 8;
+        const uint32_t dst = tile_at<kVecs>(ks, lr, lx);
+#pragma unroll
+        for (int i = 0; i < kChunk / kStep; ++i) {
+            const bool ok = i * kStep + lr < n;
+            cp_async16_or_zero(dst + i * kStep * kVecs * 16, ok ? kp : a.k, ok);
+            cp_async16_or_zero(dst + i * kStep * kVecs * 16 + kChunk * DK * 2, ok ? qp : a.q, ok);
+            kp += kStep * a.k_ts;
+            qp += kStep * a.q_ts;
+        }
     }
     cp_async_commit();
     if (warp == 0) {
-        // decays summed in fp64: differences of far tokens keep their digits; below
-        // -200 a decay is 0 in fp32 as it stands, and stays finite here
+        // below -200 a decay is 0 in fp32 as it stands, and stays finite here
         double x[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = 2 * lane + i;
             const int64_t at = static_cast<int64_t>(t0 + r) * a.v_heads + h;
             const float g = r < n ? a.g[at] : 0.0f;
-            x[i] = g < -200.0f ? -200.0f : g;
+            x[i] = (g < -200.0f ? -200.0f : g) * 1.4426950408889634074;
             bt[r] = r < n ? a.beta[at] : 0.0f;
         }
         double s = x[0] + x[1];
@@ -267,15 +316,15 @@ __global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* ch
             const double u = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += u;
         }
-        gsum[2 * lane + 1] = s;
-        gsum[2 * lane] = s - x[1];
+        *reinterpret_cast<float2*>(&rows[2 * lane].x) = two_floats(s - x[1]);
+        *reinterpret_cast<float2*>(&rows[2 * lane + 1].x) = two_floats(s);
     }
     cp_async_wait<0>();
     __syncthreads();
     {
         const int r = tid & 63;
         const uint32_t base = tid < 64 ? ks : qs;
-        float sum = 0.0f;
+        float sum[4] = {};
         if (a.l2_eps >= 0.0f) {
 #pragma unroll
             for (int c = 0; c < kVecs; ++c) {
@@ -286,25 +335,25 @@ __global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* ch
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 f = __half22float2(u32_as_h2(x[i]));
-                    sum += f.x * f.x + f.y * f.y;
+                    sum[i] += f.x * f.x + f.y * f.y;
                 }
             }
         }
-        const float norm = a.l2_eps >= 0.0f ? 1.0f / sqrtf(sum + a.l2_eps) : 1.0f;
-        (tid < 64 ? rk : rq)[r] = r < n ? norm : 0.0f;
+        float norm = a.l2_eps >= 0.0f ? 1.0f / sqrtf((sum[0] + sum[1]) + (sum[2] + sum[3]) + a.l2_eps) : 1.0f;
+        if (tid >= 64) norm *= a.scale;
+        (tid < 64 ? rows[r].z : rows[r].w) = r < n ? norm : 0.0f;
     }
     __syncthreads();
     Chunk& out = chunks[static_cast<int64_t>(blockIdx.x) * a.v_heads + h];
     if (tid < kChunk) {
-        const double g = gsum[tid];
-        const float eg = expf(static_cast<float>(g));
-        out.ck[tid] = eg * rk[tid];
-        out.cq[tid] = eg * rq[tid] * a.scale;
-        out.cs[tid] = expf(static_cast<float>(gsum[kChunk - 1] - g)) * rk[tid];
+        const float4 r = rows[tid], last = rows[kChunk - 1];
+        const float eg = exp2f(r.x + r.y);
+        out.ck[tid] = eg * r.z;
+        out.cq[tid] = eg * r.w;
+        out.cs[tid] = decay_between(make_float2(last.x, last.y), make_float2(r.x, r.y)) * r.z;
         if (tid == kChunk - 1) out.keep = eg;
     }
 
-    // K K^T and Q K^T: this warp's 16 rows, columns up to the diagonal block
     float kk[8][4], qk[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -327,100 +376,117 @@ __global__ void __launch_bounds__(128) chunk_kernel(const DeltaArgs a, Chunk* ch
             mma16816(qk[2 * j + 1], qa, b[2], b[3]);
         }
     }
+    const int g = lane >> 2, t = lane & 3;
+    const float4 row[2] = {rows[warp * 16 + g], rows[warp * 16 + g + 8]};
+    const float write[2] = {row[0].z * bt[warp * 16 + g], row[1].z * bt[warp * 16 + g + 8]};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (j > 2 * warp + 1) break;
+        const int c = j * 8 + 2 * t;
+        const float4 col[2] = {rows[c], rows[c + 1]};
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-            const int r = warp * 16 + (lane >> 2) + e * 4, c = j * 8 + (lane & 3) * 2;
+            const int r = warp * 16 + g + e * 4;
+            const float4 mine = row[e / 2];
             float p[2], m[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float w = c + i <= r ? expf(static_cast<float>(gsum[r] - gsum[c + i])) * rk[c + i] : 0.0f;
-                p[i] = c + i <= r ? w * rq[r] * a.scale * qk[j][e + i] : 0.0f;
-                m[i] = c + i < r ? w * rk[r] * bt[r] * kk[j][e + i] : 0.0f;
+                const float w = decay_between(make_float2(mine.x, mine.y), make_float2(col[i].x, col[i].y)) * col[i].z;
+                p[i] = c + i <= r ? w * mine.w * qk[j][e + i] : 0.0f;
+                m[i] = c + i < r ? w * write[e / 2] * kk[j][e + i] : 0.0f;
             }
-            uint32_t phi, plo;
-            split_scaled(p[0], p[1], phi, plo);
-            const int at = block_at(warp, j / 2) + (e + (j & 1)) * 64 + (lane >> 2) * 8 + (lane & 3) * 2;
-            *reinterpret_cast<uint32_t*>(&out.p[0][at]) = phi;
-            *reinterpret_cast<uint32_t*>(&out.p[1][at]) = plo;
-            *reinterpret_cast<float2*>(mat + r * kMatRow + c) = make_float2(m[0], m[1]);
+            uint32_t x, y;
+            split_scaled(p[0], p[1], x, y);
+            const int at = block_at(warp, j / 2) + (e + (j & 1)) * 64 + g * 8 + t * 2;
+            *reinterpret_cast<uint32_t*>(&out.p[0][at]) = x;
+            *reinterpret_cast<uint32_t*>(&out.p[1][at]) = y;
+            if (j / 2 == warp) {
+                const int dc = (j & 1) * 8 + 2 * t;
+                diag[warp][(g + e * 4) * 17 + dc] = m[0];
+                diag[warp][(g + e * 4) * 17 + dc + 1] = m[1];
+            } else {
+                // as the A operand: matrices (rows lo, k lo), (rows hi, k lo), (rows lo, k hi), (rows hi, k hi)
+                const int am = (warp * (warp - 1) / 2 + j / 2) * 256 + ((j & 1) * 2 + e / 2) * 64 + g * 8 + t * 2;
+                split_scaled(m[0], m[1], x, y);
+                *reinterpret_cast<uint32_t*>(&a_blk[0][am]) = x;
+                *reinterpret_cast<uint32_t*>(&a_blk[1][am]) = y;
+            }
         }
     }
-    __syncthreads();
+    __syncwarp();
 
-    // X = (I + A)^-1 by blocks of 16.  Diagonal blocks by forward substitution,
-    // one thread a column: x_i = [i = j] - sum_{l < i} A_il x_l.
-    if (tid < kChunk) {
-        const float* m = mat + (tid & ~15) * (kMatRow + 1);
-        float* xo = inv + (tid & ~15) * kMatRow + tid;
+    // this warp's diagonal block: lanes 0-15 take a column each,
+    // x_i = [i = j] - sum_{l < i} A_il x_l
+    if (lane < 16) {
+        const float* m = diag[warp];
+        const float beta = bt[warp * 16 + lane];
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float acc[2] = {i == (tid & 15) ? 1.0f : 0.0f, 0.0f};
+            float acc[2] = {i == lane ? 1.0f : 0.0f, 0.0f};
 #pragma unroll
-            for (int l = 0; l < i; ++l) acc[l & 1] -= m[i * kMatRow + l] * x[l];
+            for (int l = 0; l < i; ++l) acc[l & 1] -= m[i * 17 + l] * x[l];
             x[i] = acc[0] + acc[1];
-            xo[i * kMatRow] = x[i];
+            const int cc = lane >> 3, rr = i >> 3, in = (i & 7) * 8 + (lane & 7);
+            __half hi16 = __float2half_rn(x[i]);
+            x_blk[0][warp * 256 + (cc * 2 + rr) * 64 + in] = hi16;
+            x_blk[1][warp * 256 + (cc * 2 + rr) * 64 + in] = __float2half_rn((x[i] - __half2float(hi16)) * kLo);
+            const float tt = x[i] * beta;
+            hi16 = __float2half_rn(tt);
+            out.t[0][block_at(warp, warp) + (rr * 2 + cc) * 64 + in] = hi16;
+            out.t[1][block_at(warp, warp) + (rr * 2 + cc) * 64 + in] = __float2half_rn((tt - __half2float(hi16)) * kLo);
         }
     }
     __syncthreads();
-    // Block rows below: X_ij = -X_ii sum_{j <= l < i} A_il X_lj, in 4x4 tiles; the
-    // sums take the place of A's row, which is not needed any more.
-    const int tr = tid & 3, tc = tid >> 2;      // tile row within the block row, tile column
+    if (warp == 3) return;
+
+    // this warp's column of blocks; its diagonal block as a B operand (k lo, k hi of columns lo, then hi)
+    Split4 xb[3];
+    const uint32_t xs = smem_u32(x_blk), as = smem_u32(a_blk);
+    constexpr uint32_t kXLo = 4 * 512, kALo = 6 * 512;
+    ldsm4_t(xb[0].hi, xs + warp * 512 + lane * 16);
+    ldsm4_t(xb[0].lo, xs + kXLo + warp * 512 + lane * 16);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-        const bool mine = tc < 4 * i;
-        float4 y[4];
-        auto product = [&](const float* left, const float* right, int from, int to) {
+    for (int s = 1; s < 4; ++s) {
+        const int i = warp + s;         // block row
+        if (i > 3) break;
+        float y[2][4] = {}, yl[2][4] = {};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int l = from; l < to; l += 4) {
-                float4 b[4];
+        for (int l = 0; l < s; ++l) {
+            Split4 m;
+            const uint32_t at = as + (i * (i - 1) / 2 + warp + l) * 512 + lane * 16;
+            ldsm4(m.hi, at);
+            ldsm4(m.lo, at + kALo);
+            mma_split(y, yl, m, xb[l]);
+        }
 #pragma unroll
-                for (int q = 0; q < 4; ++q) b[q] = *reinterpret_cast<const float4*>(right + (l + q) * kMatRow + tc * 4);
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float4 w = *reinterpret_cast<const float4*>(left + (tr * 4 + r) * kMatRow + l);
-                    y[r].x += w.x * b[0].x + w.y * b[1].x + w.z * b[2].x + w.w * b[3].x;
-                    y[r].y += w.x * b[0].y + w.y * b[1].y + w.z * b[2].y + w.w * b[3].y;
-                    y[r].z += w.x * b[0].z + w.y * b[1].z + w.z * b[2].z + w.w * b[3].z;
-                    y[r].w += w.x * b[0].w + w.y * b[1].w + w.z * b[2].w + w.w * b[3].w;
-                }
+            for (int e = 0; e < 4; ++e) y[q][e] += kLoInv * yl[q][e];
+        Split4 yb, m;
+        to_b(yb, y);
+        ldsm4(m.hi, xs + i * 512 + lane * 16);
+        ldsm4(m.lo, xs + kXLo + i * 512 + lane * 16);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[q][e] = yl[q][e] = 0.0f;
+        mma_split(y, yl, m, yb);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const float2 beta = *reinterpret_cast<const float2*>(&bt[warp * 16 + q * 8 + 2 * t]);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                y[q][e] = -(y[q][e] + kLoInv * yl[q][e]);
+                y[q][e + 1] = -(y[q][e + 1] + kLoInv * yl[q][e + 1]);
+                uint32_t x, z;
+                split_scaled(y[q][e] * beta.x, y[q][e + 1] * beta.y, x, z);
+                const int at = block_at(i, warp) + (e + q) * 64 + g * 8 + t * 2;
+                *reinterpret_cast<uint32_t*>(&out.t[0][at]) = x;
+                *reinterpret_cast<uint32_t*>(&out.t[1][at]) = z;
             }
-        };
-        float* sums = mat + i * 16 * kMatRow;
-        if (mine) product(sums, inv, (tc / 4) * 16, i * 16);
-        __syncthreads();
-        if (mine) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) *reinterpret_cast<float4*>(sums + (tr * 4 + r) * kMatRow + tc * 4) = y[r];
         }
-        __syncthreads();
-        if (mine) {
-            product(inv + i * 16 * (kMatRow + 1), sums, 0, 16);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<float4*>(inv + (i * 16 + tr * 4 + r) * kMatRow + tc * 4) =
-                    make_float4(-y[r].x, -y[r].y, -y[r].z, -y[r].w);
-        }
-        __syncthreads();
-    }
-    for (int v = tid; v < kBlocks * 32; v += 128) {
-        const int blk = v / 32, i = blk >= 6 ? 3 : (blk >= 3 ? 2 : (blk >= 1 ? 1 : 0)), j = blk - i * (i + 1) / 2;
-        const int r = i * 16 + (v & 7) + ((v >> 4) & 1) * 8, c = j * 16 + ((v >> 3) & 1) * 8;
-        uint4 hi, lo;
-        uint32_t* hp = &hi.x;
-        uint32_t* lp = &lo.x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 x = *reinterpret_cast<const float2*>(inv + r * kMatRow + c + 2 * e);
-            // above the diagonal of a diagonal block the substitution left zeros
-            split_scaled(x.x * bt[c + 2 * e], x.y * bt[c + 2 * e + 1], hp[e], lp[e]);
-        }
-        reinterpret_cast<uint4*>(out.t[0])[v] = hi;
-        reinterpret_cast<uint4*>(out.t[1])[v] = lo;
+        if (s < 3) to_b(xb[s], y);
     }
 }
 
@@ -756,7 +822,7 @@ int launch_scan(const DeltaArgs& a, const Chunk* chunks, cudaStream_t stream) {
 template <int DK>
 int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     Chunk* chunks = static_cast<Chunk*>(workspace);
-    constexpr int kSmem = 2 * kChunk * DK * 2 + 2 * kChunk * 68 * 4;
+    constexpr int kSmem = 2 * kChunk * DK * 2;
     MCV_CHECK_CUDA(cudaFuncSetAttribute(chunk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     int st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
                     kSmem, stream, a, chunks);
