@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdio>
 #include <string>
 
@@ -81,6 +82,19 @@ int launch_clustered(void (*kernel)(KArgs...), dim3 grid, dim3 block, dim3 clust
 }
 
 int sm_count();
+
+// Allows `kernel` this much dynamic shared memory on the current device, asking
+// the runtime only the first time on each.
+template <typename Kernel>
+int allow_smem(Kernel* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    MCV_CHECK_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return MCV_OK;
+    MCV_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return MCV_OK;
+}
 
 // Cross-GPU exchange of the argmax keys through peer mailboxes (see
 // p2p.cu).  nranks <= 1 disables it.  Mailbox of rank r, in 64-bit words:

@@ -814,7 +814,9 @@ int64_t chunk_slots(int64_t tokens, int64_t batch) { return tokens / kChunk + ba
 template <int DK, int NG>
 int launch_scan(const DeltaArgs& a, const Chunk* chunks, cudaStream_t stream) {
     using C = Scan<DK, NG>;
-    MCV_CHECK_CUDA(cudaFuncSetAttribute(scan_kernel<DK, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    static std::atomic<uint64_t> done{0};
+    const int st = allow_smem(scan_kernel<DK, NG>, C::kSmem, done);
+    if (st) return st;
     return launch(scan_kernel<DK, NG>, dim3((a.dv / 16 + NG - 1) / NG, a.v_heads, a.batch), dim3(C::kThreads), C::kSmem,
                   stream, a, chunks);
 }
@@ -823,8 +825,10 @@ template <int DK>
 int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     Chunk* chunks = static_cast<Chunk*>(workspace);
     constexpr int kSmem = 2 * kChunk * DK * 2;
-    MCV_CHECK_CUDA(cudaFuncSetAttribute(chunk_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    int st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
+    static std::atomic<uint64_t> done{0};
+    int st = allow_smem(chunk_kernel<DK>, kSmem, done);
+    if (st) return st;
+    st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
                     kSmem, stream, a, chunks);
     if (st) return st;
     // two column groups a block once single ones would not all run at once

@@ -522,7 +522,9 @@ size_t workspace_bytes_for(int64_t dim, int nt) {
 
 template <int D, int NT>
 int launch_attention(const AttnArgs& a, int grid, cudaStream_t stream) {
-    MCV_CHECK_CUDA(cudaFuncSetAttribute(attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::kSmem));
+    static std::atomic<uint64_t> done{0};
+    const int st = allow_smem(attention_kernel<D, NT>, Tile<D>::kSmem, done);
+    if (st) return st;
     return launch(attention_kernel<D, NT>, dim3(grid), dim3(kThreads), Tile<D>::kSmem, stream, a);
 }
 

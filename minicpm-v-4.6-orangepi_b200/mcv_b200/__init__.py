@@ -824,36 +824,52 @@ class _GatedDelta(ctypes.Structure):
                 ("scale", _f32), ("l2_eps", _f32)]
 
 
-def _f16_rows(t, what: str, device) -> _Rows:
-    """[tokens, heads, dim] fp16 with a contiguous last dimension."""
+_ref = ctypes.byref
+
+
+# The checks below run on every call of a decode step, so they are kept to a few
+# attribute reads: tensors are compared by device index, and the current stream
+# is taken as a raw handle.
+_torch = None
+_fns = {}
+
+
+def _setup():
+    global _torch
     import torch
-    if t.dtype is not torch.float16 or t.device != device or t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] != 1):
-        raise RuntimeError(f"mcv_b200: {what} must be float16 [tokens, heads, dim] on {device} with contiguous rows")
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+    _torch = torch
+    for name in ("mrope", "mrope_append_kv", "paged_attention_decode", "gated_delta_step", "gated_delta_prefill"):
+        _fns[name] = getattr(lib(), "mcv_" + name)
+    return torch
 
 
-def _dense(t, dtype, shape, what: str, device):
+def _f16_rows(t, what: str, dev: int) -> _Rows:
+    """[tokens, heads, dim] fp16 with a contiguous last dimension."""
+    if t.dtype is not _torch.float16 or t.get_device() != dev or t.dim() != 3:
+        raise RuntimeError(f"mcv_b200: {what} must be float16 [tokens, heads, dim] on cuda:{dev}")
+    token, head, one = t.stride()
+    if one != 1 and t.shape[2] != 1:
+        raise RuntimeError(f"mcv_b200: rows of {what} must be contiguous")
+    return _Rows(t.data_ptr(), token, head)
+
+
+def _dense(t, dtype, shape, what: str, dev: int):
     """Address of a contiguous tensor of this type and shape (None: NULL)."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise RuntimeError(f"mcv_b200: {what} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise RuntimeError(f"mcv_b200: {what} must be a contiguous {dtype} tensor {list(shape)} on cuda:{dev}")
     return t.data_ptr()
 
 
-def _run_on(device, stream, name: str, *args) -> None:
-    """Calls mcv_<name>(*args, stream) with `device` current."""
-    import torch
-    if device.type != "cuda":
-        raise RuntimeError("mcv_b200: expected a CUDA tensor")
-    fn = getattr(lib(), "mcv_" + name)
-    if stream is None:
-        stream = torch.cuda.current_stream(device)
-    if device.index == torch.cuda.current_device():
-        st = fn(*args, stream.cuda_stream)
+def _run_on(dev: int, stream, name: str, *args) -> None:
+    """Calls mcv_<name>(*args, stream) with device `dev` current."""
+    handle = _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    if dev == _torch._C._cuda_getDevice():
+        st = _fns[name](*args, handle)
     else:
-        with torch.cuda.device(device):
-            st = fn(*args, stream.cuda_stream)
+        with _torch.cuda.device(dev):
+            st = _fns[name](*args, handle)
     if st != 0:
         _check(st, name)
 
@@ -873,7 +889,9 @@ class PagedKVCache:
         if k.stride()[1:] != (page * dim, dim, 1) or v.stride() != k.stride():
             raise RuntimeError("PagedKVCache: pages must be contiguous and k and v laid out alike")
         self.k, self.v = k, v
-        self._c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0), *k.shape[:1], page, heads, dim)
+        self.dev, self.kv_heads, self.head_dim = k.get_device(), heads, dim
+        self._c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0), k.shape[0], page, heads, dim)
+        self._ref = _ref(self._c)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda"):
@@ -893,23 +911,25 @@ class MRope:
         arr = (ctypes.c_int32 * max(1, self.axes))(*sections)
         _check(lib().mcv_mrope_init(ctypes.byref(self._c), rotary_dim, self.axes, arr, int(interleaved), theta),
                "mrope_init")
+        self._ref = _ref(self._c)
 
 
-def _rows_out(x, out, what: str):
+def _rows_out(x, out, what: str, dev: int):
     """Address of a dense output of x's shape, or of x itself (in place)."""
-    if out.data_ptr() == x.data_ptr() and out.shape == x.shape and out.stride() == x.stride() and out.dtype == x.dtype:
-        return out.data_ptr()
-    return _dense(out, x.dtype, x.shape, what, x.device)
+    if out is x or (out.data_ptr() == x.data_ptr() and out.shape == x.shape and out.stride() == x.stride()
+                    and out.dtype == x.dtype):
+        return x.data_ptr()
+    return _dense(out, x.dtype, x.shape, what, dev)
 
 
 def mrope(x, positions, rope: MRope, out, stream=None) -> None:
     """out = x [tokens, heads, head_dim] with its rows rotated; positions int32
     [axes, tokens]; out is dense, or x itself."""
-    import torch
-    dev = x.device
+    torch = _torch or _setup()
+    dev = x.get_device()
     rows = _f16_rows(x, "x", dev)
     n, heads, dim = x.shape
-    _run_on(dev, stream, "mrope", ctypes.byref(rows), _rows_out(x, out, "out"), ctypes.byref(rope._c),
+    _run_on(dev, stream, "mrope", _ref(rows), _rows_out(x, out, "out", dev), rope._ref,
             _dense(positions, torch.int32, (rope.axes, n), "positions", dev), n, heads, dim)
 
 
@@ -920,20 +940,17 @@ def mrope_append_kv(q, k, v, positions, rope: MRope, cache: PagedKVCache, page_t
     positions int32 [axes, tokens]; page_table int32 [rows, pages of a row];
     index int32 [tokens]: each token's place in its sequence (negative: not
     written); seq int32 [tokens]: its row of page_table (None: token t has row t)."""
-    import torch
-    dev, c = q.device, cache._c
+    torch = _torch or _setup()
+    dev, i32 = q.get_device(), torch.int32
     n, heads, dim = q.shape
-    if cache.k.device != dev or dim != c.head_dim or k.shape != (n, c.kv_heads, dim) or v.shape != k.shape:
+    if cache.dev != dev or k.shape != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or dim != cache.head_dim:
         raise RuntimeError("mrope_append_kv: q, k, v and the cache do not fit together")
-    rq, rk, rv = _f16_rows(q, "q", dev), _f16_rows(k, "k", dev), _f16_rows(v, "v", dev)
-    if page_table.dim() != 2:
-        raise RuntimeError("mrope_append_kv: page_table must be [rows, pages]")
-    ref = ctypes.byref
-    _run_on(dev, stream, "mrope_append_kv", ref(rq), _rows_out(q, q_out, "q_out"), ref(rk), ref(rv), ref(rope._c),
-            _dense(positions, torch.int32, (rope.axes, n), "positions", dev), ref(c),
-            _dense(page_table, torch.int32, page_table.shape, "page_table", dev), page_table.shape[0],
-            page_table.shape[1], _dense(seq, torch.int32, (n,), "seq", dev),
-            _dense(index, torch.int32, (n,), "index", dev), n, heads)
+    rows, cols = page_table.shape
+    _run_on(dev, stream, "mrope_append_kv", _ref(_f16_rows(q, "q", dev)), _rows_out(q, q_out, "q_out", dev),
+            _ref(_f16_rows(k, "k", dev)), _ref(_f16_rows(v, "v", dev)), rope._ref,
+            _dense(positions, i32, (rope.axes, n), "positions", dev), cache._ref,
+            _dense(page_table, i32, (rows, cols), "page_table", dev), rows, cols,
+            _dense(seq, i32, (n,), "seq", dev), _dense(index, i32, (n,), "index", dev), n, heads)
 
 
 def paged_attention_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, device="cuda"):
@@ -953,45 +970,36 @@ def paged_attention_decode(q, cache: PagedKVCache, page_table, lengths, out, wor
     (mcv_paged_attention_decode).  q fp16 [batch, q_heads, head_dim]; page_table
     int32 [batch, pages]; lengths int32 [batch] (0: a zero row); out like q,
     dense; lse fp32 [batch, q_heads] or None; scale defaults to head_dim^-1/2."""
-    import torch
-    dev, c = q.device, cache._c
+    torch = _torch or _setup()
+    dev, i32 = q.get_device(), torch.int32
     b, heads, dim = q.shape
-    if cache.k.device != dev or dim != c.head_dim:
+    if cache.dev != dev or dim != cache.head_dim:
         raise RuntimeError("paged_attention_decode: q and the cache do not fit together")
-    rows = _f16_rows(q, "q", dev)
-    if page_table.dim() != 2:
-        raise RuntimeError("paged_attention_decode: page_table must be [batch, pages]")
-    cols = page_table.shape[1]
-    if workspace.device != dev:
+    if workspace.get_device() != dev:
         raise RuntimeError("paged_attention_decode: workspace on another device")
-    _run_on(dev, stream, "paged_attention_decode", ctypes.byref(rows), ctypes.byref(c),
-            _dense(page_table, torch.int32, (b, cols), "page_table", dev), cols,
-            _dense(lengths, torch.int32, (b,), "lengths", dev), _dense(out, torch.float16, q.shape, "out", dev),
+    _, cols = page_table.shape
+    _run_on(dev, stream, "paged_attention_decode", _ref(_f16_rows(q, "q", dev)), cache._ref,
+            _dense(page_table, i32, (b, cols), "page_table", dev), cols,
+            _dense(lengths, i32, (b,), "lengths", dev), _dense(out, torch.float16, (b, heads, dim), "out", dev),
             _dense(lse, torch.float32, (b, heads), "lse", dev), b, heads, dim ** -0.5 if scale is None else scale,
-            workspace.data_ptr(), workspace.numel() * workspace.element_size())
+            workspace.data_ptr(), workspace.nbytes)
 
 
-def _gated_delta(q, k, v, g, beta, state, out, state_out, index, batch, scale, l2_eps) -> _GatedDelta:
-    import torch
-    dev = q.device
-    a = _GatedDelta()
-    a.q, a.k, a.v = _f16_rows(q, "q", dev), _f16_rows(k, "k", dev), _f16_rows(v, "v", dev)
+def _gated_delta(q, k, v, g, beta, state, out, state_out, index, batch, scale, l2_eps, dev) -> _GatedDelta:
+    torch = _torch
     n, kh, dk = q.shape
-    _, vh, dv = v.shape
-    if k.shape != q.shape or v.shape[0] != n:
+    nv, vh, dv = v.shape
+    if k.shape != (n, kh, dk) or nv != n:
         raise RuntimeError("gated_delta: q, k and v do not fit together")
-    a.g = _dense(g, torch.float32, (n, vh), "g", dev)
-    a.beta = _dense(beta, torch.float32, (n, vh), "beta", dev)
-    a.out = _dense(out, torch.float16, (n, vh, dv), "out", dev)
+    f32 = torch.float32
     any_state = state if state is not None else state_out
     slots = any_state.shape[0] if any_state is not None else batch
-    a.state_in = _dense(state, torch.float32, (slots, vh, dk, dv), "state", dev)
-    a.state_out = _dense(state_out, torch.float32, (slots, vh, dk, dv), "state_out", dev)
-    a.state_index = _dense(index, torch.int32, (batch,), "index", dev)
-    a.slots, a.k_heads, a.v_heads, a.key_dim, a.value_dim = slots, kh, vh, dk, dv
-    a.scale = dk ** -0.5 if scale is None else scale
-    a.l2_eps = -1.0 if l2_eps is None else l2_eps
-    return a
+    return _GatedDelta(
+        _f16_rows(q, "q", dev), _f16_rows(k, "k", dev), _f16_rows(v, "v", dev), _dense(g, f32, (n, vh), "g", dev),
+        _dense(beta, f32, (n, vh), "beta", dev), _dense(out, torch.float16, (n, vh, dv), "out", dev),
+        _dense(state, f32, (slots, vh, dk, dv), "state", dev), _dense(state_out, f32, (slots, vh, dk, dv), "state_out", dev),
+        _dense(index, torch.int32, (batch,), "index", dev), slots, kh, vh, dk, dv, dk ** -0.5 if scale is None else scale,
+        -1.0 if l2_eps is None else l2_eps)
 
 
 def gated_delta_step(q, k, v, g, beta, state, out, state_out=None, index=None, scale=None, l2_eps=None,
@@ -1003,9 +1011,11 @@ def gated_delta_step(q, k, v, g, beta, state, out, state_out=None, index=None, s
     the sequences' slots (negative: skipped; None: slot b), out fp16 [batch,
     v_heads, value_dim].  l2_eps: q and k are normalised with it first (None: not);
     scale defaults to key_dim^-1/2."""
-    a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, q.shape[0],
-                     scale, l2_eps)
-    _run_on(q.device, stream, "gated_delta_step", ctypes.byref(a), q.shape[0])
+    _torch or _setup()
+    dev, batch = q.get_device(), q.shape[0]
+    a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, batch, scale, l2_eps,
+                     dev)
+    _run_on(dev, stream, "gated_delta_step", _ref(a), batch)
 
 
 def gated_delta_workspace(tokens: int, batch: int, v_heads: int, key_dim: int, value_dim: int, device="cuda"):
@@ -1023,13 +1033,14 @@ def gated_delta_prefill(q, k, v, g, beta, cu_seqlens, state, out, workspace, sta
     cu_seqlens[b] .. cu_seqlens[b+1] (int32 [batch + 1]) belong to sequence b.
     state None: sequences start from zero.  Final states go to state_out, or back
     into state; with neither they are not kept.  The rest as gated_delta_step."""
-    import torch
+    torch = _torch or _setup()
+    dev = q.get_device()
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
         raise RuntimeError("gated_delta_prefill: cu_seqlens must be [batch + 1]")
-    batch = cu_seqlens.shape[0] - 1
-    a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, batch, scale, l2_eps)
-    if workspace.device != q.device:
+    if workspace.get_device() != dev:
         raise RuntimeError("gated_delta_prefill: workspace on another device")
-    _run_on(q.device, stream, "gated_delta_prefill", ctypes.byref(a),
-            _dense(cu_seqlens, torch.int32, (batch + 1,), "cu_seqlens", q.device), q.shape[0], batch,
-            workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    batch = cu_seqlens.shape[0] - 1
+    a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, batch, scale, l2_eps,
+                     dev)
+    _run_on(dev, stream, "gated_delta_prefill", _ref(a), _dense(cu_seqlens, torch.int32, (batch + 1,), "cu_seqlens", dev),
+            q.shape[0], batch, workspace.data_ptr(), workspace.nbytes)
