@@ -24,8 +24,8 @@
 // At a row's end the block joins its warps' (max, sum, O).  A row that
 // lies in one block's range is written at once; of a row cut over several
 // blocks every block leaves a partial result, and the last one to arrive
-// joins them in order (in two levels of kFan, which bounds what one block has
-// to read), so results do not depend on timing.
+// joins them in order (kFan at a time, level by level, which bounds what one
+// block has to read), so results do not depend on timing.
 #include "mixing.cuh"
 
 #include <cfloat>
@@ -39,6 +39,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;      // keys of a unit
 constexpr int kFan = 8;        // partial results joined at a time
+constexpr int kLevels = 4;     // levels of joining: kFan^4 blocks at most
 constexpr int kMaxBatch = 4096;
 constexpr int kMinUnits = 4;   // least units of a block: one per warp
 
@@ -65,7 +66,7 @@ struct AttnArgs {
     __half* out;
     float* lse;
     float* part;
-    unsigned* counters;   // [2 * grid] joins of kFan, [2 * grid] joins of those
+    unsigned* counters;   // [kLevels][2 * grid]
     int64_t q_bs, q_hs, page_stride, table_cols;
     int batch, q_heads, kv_heads, group, head_groups, splits_of_group, num_pages, max_keys;
     float scale_log2;
@@ -124,62 +125,68 @@ __device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned expected
     return last;
 }
 
-// Joins `n` partial results (slot_of(0..n-1), in order).  to_out: normalised
-// into the output rows; else back into slot_of(0).
+// Joins `n` <= kFan partial results (slot_of(0..n-1), in order).  to_out: normalised
+// into the output rows; else back into slot_of(0).  All loads of a thread are in
+// flight together; maxima and sums go through `stats` in shared memory.
 template <int D, int NT, typename SlotOf>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot_of, bool to_out, int b, int head0,
-                                           int heads) {
+                                           int heads, float2* stats) {
     using P = Part<D, NT>;
     constexpr int kVec = D / 4;
     constexpr int kItems = (P::kHeads * kVec) / kThreads;
-    float4 acc[kItems];
-    float top[kItems], sum[kItems];
+    static_assert(kFan * P::kHeads <= kThreads, "one thread loads one (max, sum)");
+    const float* part[kFan];
+#pragma unroll
+    for (int s = 0; s < kFan; ++s) part[s] = P(a.part, slot_of(s < n ? s : 0)).p;
+    {
+        const int s = threadIdx.x / P::kHeads, h = threadIdx.x % P::kHeads;
+        if (s < kFan) {
+            const P p(a.part, slot_of(s < n ? s : 0));
+            stats[threadIdx.x] = s < n && h < heads ? make_float2(__ldcg(p.m() + h), __ldcg(p.l() + h))
+                                                    : make_float2(-INFINITY, 0.0f);
+        }
+    }
+    __syncthreads();
+    const P first(a.part, slot_of(0));
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
         const int item = threadIdx.x + i * kThreads;
         const int h = item / kVec, d = (item % kVec) * 4;
-        acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        top[i] = -INFINITY;
-        sum[i] = 0.0f;
         if (h >= heads) continue;
-        for (int s = 0; s < n; ++s) top[i] = fmaxf(top[i], __ldcg(P(a.part, slot_of(s)).m() + h));
-        for (int s = 0; s < n; ++s) {
-            const P p(a.part, slot_of(s));
-            const float w = scale_of(__ldcg(p.m() + h), top[i]);
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.o(h) + d));
-            sum[i] += w * __ldcg(p.l() + h);
-            acc[i].x += w * o.x;
-            acc[i].y += w * o.y;
-            acc[i].z += w * o.z;
-            acc[i].w += w * o.w;
-        }
-    }
-    if (to_out) {
+        float4 o[kFan];
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-            const int item = threadIdx.x + i * kThreads;
-            const int h = item / kVec, d = (item % kVec) * 4;
-            if (h >= heads) continue;
+        for (int s = 0; s < kFan; ++s)
+            o[s] = s < n ? __ldcg(reinterpret_cast<const float4*>(part[s] + 2 * P::kHeads + h * D + d))
+                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kFan; ++s) top = fmaxf(top, stats[s * P::kHeads + h].x);
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int s = 0; s < kFan; ++s) {
+            const float2 ml = stats[s * P::kHeads + h];
+            const float w = scale_of(ml.x, top);
+            sum += w * ml.y;
+            acc.x += w * o[s].x;
+            acc.y += w * o[s].y;
+            acc.z += w * o[s].z;
+            acc.w += w * o[s].w;
+        }
+        if (to_out) {
             const int64_t row = static_cast<int64_t>(b) * a.q_heads + head0 + h;
-            const float inv = 1.0f / sum[i];
-            const uint2 r = make_uint2(h2_as_u32(__floats2half2_rn(acc[i].x * inv, acc[i].y * inv)),
-                                       h2_as_u32(__floats2half2_rn(acc[i].z * inv, acc[i].w * inv)));
-            *reinterpret_cast<uint2*>(a.out + row * D + d) = r;
-            if (d == 0 && a.lse) a.lse[row] = (top[i] + log2f(sum[i])) * 0.6931471805599453f;
-        }
-        return;
-    }
-    __syncthreads();   // slot_of(0) is read by all before it is written
-    const P p(a.part, slot_of(0));
-#pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-        const int item = threadIdx.x + i * kThreads;
-        const int h = item / kVec, d = (item % kVec) * 4;
-        if (h >= heads) continue;
-        *reinterpret_cast<float4*>(p.o(h) + d) = acc[i];
-        if (d == 0) {
-            p.m()[h] = top[i];
-            p.l()[h] = sum[i];
+            const float inv = 1.0f / sum;
+            *reinterpret_cast<uint2*>(a.out + row * D + d) =
+                make_uint2(h2_as_u32(__floats2half2_rn(acc.x * inv, acc.y * inv)),
+                           h2_as_u32(__floats2half2_rn(acc.z * inv, acc.w * inv)));
+            if (d == 0 && a.lse) a.lse[row] = (top + log2f(sum)) * 0.6931471805599453f;
+        } else {
+            // each element of slot_of(0) is read and written by one thread alone, and
+            // its maxima and sums were read by all before the barrier above
+            *reinterpret_cast<float4*>(first.o(h) + d) = acc;
+            if (d == 0) {
+                first.m()[h] = top;
+                first.l()[h] = sum;
+            }
         }
     }
 }
@@ -487,16 +494,18 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         }
         if (!whole) {
             const int parts = static_cast<int>(c1 - c0 + 1);
-            const int fan = static_cast<int>((blockIdx.x - c0) / kFan);
-            const int64_t f0 = c0 + static_cast<int64_t>(fan) * kFan;
-            const int in_fan = min(kFan, parts - fan * kFan);
-            const int fans = (parts + kFan - 1) / kFan;
-            if (arrive_last(a.counters + slot_of_block(f0), in_fan, &flag)) {
-                join_parts<D, NT>(a, in_fan, [&](int i) { return slot_of_block(f0 + i); }, fans == 1, row.b, head0, heads);
-                if (fans > 1 && arrive_last(a.counters + 2 * gridDim.x + slot_of_block(c0), fans, &flag))
-                    join_parts<D, NT>(a, fans, [&](int i) { return slot_of_block(c0 + static_cast<int64_t>(i) * kFan); },
-                                      true, row.b, head0, heads);
+            // kFan neighbours' results become one, kFan of those the next, ... each time by the last to arrive
+            unsigned* counters = a.counters;
+            for (int64_t step = 1;; step *= kFan, counters += 2 * gridDim.x) {
+                const int64_t f0 = c0 + (blockIdx.x - c0) / (step * kFan) * (step * kFan);
+                const int n = static_cast<int>(min(static_cast<int64_t>(kFan), (c0 + parts - f0 + step - 1) / step));
+                if (!arrive_last(counters + slot_of_block(f0), n, &flag)) break;
+                const bool all = step * kFan >= parts;
+                join_parts<D, NT>(a, n, [&](int i) { return slot_of_block(f0 + i * step); }, all, row.b, head0, heads,
+                                  reinterpret_cast<float2*>(join));
+                if (all) break;
             }
+            __syncthreads();   // join is written again
         }
         pos = seg_end;
         if (pos < end) row.next(a);
@@ -511,7 +520,7 @@ int blocks_per_sm(int64_t dim) { return dim == 256 ? 1 : (dim == 128 ? 2 : 3); }
 
 // The counters come first and take the same room for every head size, so that
 // calls of different shapes can share one workspace.
-size_t counter_count() { return static_cast<size_t>(sm_count()) * 4 * 3; }
+size_t counter_count() { return static_cast<size_t>(sm_count()) * 3 * 2 * kLevels; }
 
 size_t part_floats(int64_t dim, int nt) { return static_cast<size_t>(8 * nt) * (dim + 2); }
 
