@@ -38,8 +38,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;      // keys of a unit
-constexpr int kFan = 8;        // partial results joined at a time
-constexpr int kLevels = 4;     // levels of joining: kFan^4 blocks at most
+constexpr int kFan = 16;       // partial results joined at a time
+constexpr int kLevels = 3;     // levels of joining: kFan^3 blocks at most
 constexpr int kMaxBatch = 4096;
 constexpr int kMinUnits = 4;   // least units of a block: one per warp
 
@@ -77,6 +77,10 @@ __device__ __forceinline__ int key_count(const AttnArgs& a, int b) {
     const int n = a.lengths[b];
     return n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n);
 }
+// n / d, by a 32-bit division where n allows it (a 64-bit one is a long routine).
+__device__ __forceinline__ int64_t div_small(int64_t n, int64_t d) {
+    return ((n | d) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d;
+}
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
 
 // A row of the work line: one sequence and one group of query heads.
@@ -109,20 +113,20 @@ struct Part {
 };
 
 // Counts this block in at *counter (after its global writes); true in the
-// last of `expected`, which leaves the counter at zero.
+// last of `expected`, which leaves the counter at zero.  The barrier puts all
+// threads' writes before thread 0's fence, and its fence before all reads that
+// follow the second barrier.
 __device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned expected, int* flag) {
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+        __threadfence();
         const bool last = atomicAdd(counter, 1u) == expected - 1;
         if (last) *counter = 0;
+        __threadfence();
         *flag = last;
     }
     __syncthreads();
-    const bool last = *flag != 0;
-    __threadfence();
-    __syncthreads();
-    return last;
+    return *flag != 0;
 }
 
 // Joins `n` <= kFan partial results (slot_of(0..n-1), in order).  to_out: normalised
@@ -134,44 +138,46 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot
     using P = Part<D, NT>;
     constexpr int kVec = D / 4;
     constexpr int kItems = (P::kHeads * kVec) / kThreads;
-    static_assert(kFan * P::kHeads <= kThreads, "one thread loads one (max, sum)");
-    const float* part[kFan];
-#pragma unroll
-    for (int s = 0; s < kFan; ++s) part[s] = P(a.part, slot_of(s < n ? s : 0)).p;
-    {
-        const int s = threadIdx.x / P::kHeads, h = threadIdx.x % P::kHeads;
-        if (s < kFan) {
-            const P p(a.part, slot_of(s < n ? s : 0));
-            stats[threadIdx.x] = s < n && h < heads ? make_float2(__ldcg(p.m() + h), __ldcg(p.l() + h))
-                                                    : make_float2(-INFINITY, 0.0f);
-        }
+    constexpr int kBatch = 8;      // loads in flight per item
+    for (int i = threadIdx.x; i < kFan * P::kHeads; i += kThreads) {
+        const int s = i / P::kHeads, h = i % P::kHeads;
+        const P p(a.part, slot_of(s < n ? s : 0));
+        stats[i] = s < n && h < heads ? make_float2(__ldcg(p.m() + h), __ldcg(p.l() + h)) : make_float2(-INFINITY, 0.0f);
     }
-    __syncthreads();
     const P first(a.part, slot_of(0));
+    bool known = false;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
         const int item = threadIdx.x + i * kThreads;
         const int h = item / kVec, d = (item % kVec) * 4;
-        if (h >= heads) continue;
-        float4 o[kFan];
-#pragma unroll
-        for (int s = 0; s < kFan; ++s)
-            o[s] = s < n ? __ldcg(reinterpret_cast<const float4*>(part[s] + 2 * P::kHeads + h * D + d))
-                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int s = 0; s < kFan; ++s) top = fmaxf(top, stats[s * P::kHeads + h].x);
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int s = 0; s < kFan; ++s) {
-            const float2 ml = stats[s * P::kHeads + h];
-            const float w = scale_of(ml.x, top);
-            sum += w * ml.y;
-            acc.x += w * o[s].x;
-            acc.y += w * o[s].y;
-            acc.z += w * o[s].z;
-            acc.w += w * o[s].w;
+        for (int s0 = 0; s0 < kFan; s0 += kBatch) {
+            float4 o[kBatch];
+#pragma unroll
+            for (int s = 0; s < kBatch; ++s)
+                o[s] = s0 + s < n && h < heads
+                           ? __ldcg(reinterpret_cast<const float4*>(P(a.part, slot_of(s0 + s)).o(h) + d))
+                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (!known) __syncthreads();    // stats, while the first loads are on their way
+            known = true;
+            if (s0 == 0) {
+#pragma unroll
+                for (int s = 0; s < kFan; ++s) top = fmaxf(top, stats[s * P::kHeads + h].x);
+            }
+#pragma unroll
+            for (int s = 0; s < kBatch; ++s) {
+                const float2 ml = stats[(s0 + s) * P::kHeads + h];
+                const float w = scale_of(ml.x, top);
+                sum += w * ml.y;
+                acc.x += w * o[s].x;
+                acc.y += w * o[s].y;
+                acc.z += w * o[s].z;
+                acc.w += w * o[s].w;
+            }
         }
+        if (h >= heads) continue;
         if (to_out) {
             const int64_t row = static_cast<int64_t>(b) * a.q_heads + head0 + h;
             const float inv = 1.0f / sum;
@@ -208,16 +214,18 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
     pdl_wait();
 
     // sequences without keys: their rows are zero, with an empty sum
-    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-        const int n = a.lengths[b];
-        if (n > a.max_keys && tid == 0) atomicOr(&g_attention_dev_error, kDevErrIndex);
-        if (n > 0) continue;
-        const int64_t row = static_cast<int64_t>(b) * a.q_heads;
-        uint4* o = reinterpret_cast<uint4*>(a.out + row * D);
-        for (int i = tid; i < a.q_heads * (D / 8); i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
-        if (a.lse)
-            for (int i = tid; i < a.q_heads; i += kThreads) a.lse[row + i] = -INFINITY;
-    }
+    auto empty_rows = [&]() {
+        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+            const int n = a.lengths[b];
+            if (n > a.max_keys && tid == 0) atomicOr(&g_attention_dev_error, kDevErrIndex);
+            if (n > 0) continue;
+            const int64_t row = static_cast<int64_t>(b) * a.q_heads;
+            uint4* o = reinterpret_cast<uint4*>(a.out + row * D);
+            for (int i = tid; i < a.q_heads * (D / 8); i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
+            if (a.lse)
+                for (int i = tid; i < a.q_heads; i += kThreads) a.lse[row + i] = -INFINITY;
+        }
+    };
 
     // this block's range of the work line and the row that it begins in
     const int per_thread = (a.batch + kThreads - 1) / kThreads;
@@ -239,10 +247,13 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         if (w < warp) before += sums[w];
         total += sums[w];
     }
-    int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    int64_t per = div_small(total + gridDim.x - 1, gridDim.x);
     if (per < kMinUnits) per = kMinUnits;
     const int64_t start = per * blockIdx.x;
-    if (start >= total) return;
+    if (start >= total) {
+        empty_rows();
+        return;
+    }
     const int64_t end = min(start + per, total);
     {
         int64_t at = before + incl - mine;
@@ -262,55 +273,84 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
     row.b = first_b;
     row.keys = key_count(a, row.b);
     row.units = units_of(row.keys);
-    row.hg = static_cast<int>((start - first_begin) / row.units);
+    row.hg = static_cast<int>(div_small(start - first_begin, row.units));
     row.begin = first_begin + static_cast<int64_t>(row.hg) * row.units;
 
     // ---- the ring's producer side: the same lanes, running ahead ----
     const uint32_t ring = smem_u32(smem) + warp * T::kRingBytes;
     Row ahead = row;
-    int64_t u_ahead = start + warp;
-    int64_t src_off = 0;    // lane r < 16: element offset of the next unit's row r (K and V alike)
-    int src_ok = 0;
-    auto look_up = [&]() {
-        src_ok = 0;
-        src_off = 0;
-        if (u_ahead >= end) return;
-        while (u_ahead >= ahead.begin + ahead.units) ahead.next(a);
-        const int key = static_cast<int>(u_ahead - ahead.begin) * kUnit + (lane & 15);
-        if (key >= ahead.keys) return;
-        const uint32_t page = a.page.div(key);
-        const int p = a.table[ahead.b * a.table_cols + page];
-        if (p < 0 || p >= a.num_pages) {
-            atomicOr(&g_attention_dev_error, kDevErrIndex);
-            return;
-        }
-        const int kvh = ahead.hg / a.splits_of_group;
-        src_off = p * a.page_stride + (static_cast<int64_t>(kvh) * a.page.d + (key - page * a.page.d)) * D;
-        src_ok = 1;
+    int64_t u_look = start + warp, u_ahead = u_look;
+    struct Look {       // row r of a unit, in lanes r and r + 16
+        int64_t off;    // element offset within the page (K and V alike)
+        int page;
+        bool row;       // there is such a row
     };
-    auto issue = [&](int stage) {
+    auto look_up = [&]() {
+        Look x{0, 0, false};
+        const int64_t u = u_look;
+        u_look += kWarps;
+        if (u >= end) return x;
+        while (u >= ahead.begin + ahead.units) ahead.next(a);
+        const int key = static_cast<int>(u - ahead.begin) * kUnit + (lane & 15);
+        if (key >= ahead.keys) return x;
+        const uint32_t page = a.page.div(key);
+        x.page = a.table[ahead.b * a.table_cols + page];
+        const int kvh = ahead.hg / a.splits_of_group;
+        x.off = (static_cast<int64_t>(kvh) * a.page.d + (key - page * a.page.d)) * D;
+        x.row = true;
+        return x;
+    };
+    auto issue = [&](int stage, const Look& x) {
         if (u_ahead < end) {
             constexpr int kVecs = D / 8;                 // 16-byte vectors of a row
             constexpr int kIters = kUnit * kVecs / 32;
             const uint32_t base = ring + stage * T::kStageBytes;
+            const bool inside = x.page >= 0 && x.page < a.num_pages;
+            if (x.row && !inside) atomicOr(&g_attention_dev_error, kDevErrIndex);
+            const int64_t src = x.off + (inside ? x.page : 0) * a.page_stride;
+            const int ok = x.row && inside;
 #pragma unroll
             for (int i = 0; i < kIters; ++i) {
                 const int item = i * 32 + lane;
                 const int r = item / kVecs, c = item % kVecs;
-                const int64_t off = __shfl_sync(0xffffffffu, src_off, r) + c * 8;
-                const bool ok = __shfl_sync(0xffffffffu, src_ok, r) != 0;
+                const int64_t off = __shfl_sync(0xffffffffu, src, r) + c * 8;
+                const bool take = __shfl_sync(0xffffffffu, ok, r) != 0;
                 const uint32_t dst = base + r * T::kRowBytes + ((c ^ (r & 7)) << 4);
-                cp_async16_or_zero(dst, a.k + off, ok);
-                cp_async16_or_zero(dst + kUnit * T::kRowBytes, a.v + off, ok);
+                cp_async16_or_zero(dst, a.k + off, take);
+                cp_async16_or_zero(dst + kUnit * T::kRowBytes, a.v + off, take);
             }
         }
         cp_async_commit();
         u_ahead += kWarps;
-        look_up();
     };
-    look_up();
+
+    // Q^T as B fragments: lane (g, t) holds head g, dims 2t, 2t+1 (+8) of each 16
+    uint32_t qf[NT][D / 16][2];
+    auto load_q = [&](const Row& r) {
+        const int in_group = (r.hg % a.splits_of_group) * P::kHeads;
+        const int head0 = (r.hg / a.splits_of_group) * a.group + in_group;
+        const int heads = min(P::kHeads, a.group - in_group);
 #pragma unroll
-    for (int s = 0; s < T::kStages - 1; ++s) issue(s);
+        for (int n = 0; n < NT; ++n) {
+            const int h = n * 8 + g;
+            const uint32_t* qr = reinterpret_cast<const uint32_t*>(a.q + r.b * a.q_bs + (head0 + (h < heads ? h : 0)) * a.q_hs);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                qf[n][kk][0] = h < heads ? qr[kk * 8 + t] : 0u;
+                qf[n][kk][1] = h < heads ? qr[kk * 8 + 4 + t] : 0u;
+            }
+        }
+    };
+    // pages are looked up two units ahead of their copies, queries a row ahead
+    Look look0 = look_up(), look1 = look_up();
+    load_q(row);
+#pragma unroll
+    for (int s = 0; s < T::kStages - 1; ++s) {
+        issue(s, look0);
+        look0 = look1;
+        look1 = look_up();
+    }
+    empty_rows();
 
     // ldmatrix row addresses of this lane, before the swizzle
     const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_vec = lane >> 4;
@@ -324,18 +364,6 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         const int head0 = kvh * a.group + in_group;
         const int heads = min(P::kHeads, a.group - in_group);
 
-        // Q^T as B fragments: lane (g, t) holds head g, dims 2t, 2t+1 (+8) of each 16
-        uint32_t qf[NT][D / 16][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int h = n * 8 + g;
-            const uint32_t* qr = reinterpret_cast<const uint32_t*>(a.q + row.b * a.q_bs + (head0 + (h < heads ? h : 0)) * a.q_hs);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                qf[n][kk][0] = h < heads ? qr[kk * 8 + t] : 0u;
-                qf[n][kk][1] = h < heads ? qr[kk * 8 + 4 + t] : 0u;
-            }
-        }
         float acc[NT][D / 16][4];
         float m[NT][2], l[NT][2];
 #pragma unroll
@@ -349,7 +377,9 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         for (; u < seg_end; u += kWarps) {
             cp_async_wait<T::kStages - 2>();
             __syncwarp();   // the unit has landed, and every lane is done with the stage that is filled next
-            issue(stage == 0 ? T::kStages - 1 : stage - 1);
+            issue(stage == 0 ? T::kStages - 1 : stage - 1, look0);
+            look0 = look1;
+            look1 = look_up();
             const uint32_t kb = ring + stage * T::kStageBytes;
             const uint32_t vb = kb + kUnit * T::kRowBytes;
             float s[NT][4];
@@ -432,9 +462,15 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
             stage = stage + 1 == T::kStages ? 0 : stage + 1;
         }
 
+        Row next = row;
+        if (seg_end < end) {
+            next.next(a);
+            load_q(next);
+        }
+
         // ---- join the block's warps ----
         const bool whole = row.begin >= start && row.begin + row.units <= end;
-        const int64_t c0 = row.begin / per, c1 = (row.begin + row.units - 1) / per;
+        const int64_t c0 = div_small(row.begin, per), c1 = div_small(row.begin + row.units - 1, per);
         auto slot_of_block = [&](int64_t c) { return 2 * c + (c == c0 && row.begin != c0 * per ? 1 : 0); };
         const P mine_part(a.part, slot_of_block(blockIdx.x));
 #pragma unroll
@@ -508,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
             __syncthreads();   // join is written again
         }
         pos = seg_end;
-        if (pos < end) row.next(a);
+        row = next;
     }
 }
 
