@@ -113,85 +113,104 @@ struct Part {
 };
 
 // Counts this block in at *counter (after its global writes); true in the
-// last of `expected`, which leaves the counter at zero.  The barrier puts all
-// threads' writes before thread 0's fence, and its fence before all reads that
-// follow the second barrier.
+// last of `expected`, which leaves the counter at zero.  The barriers and the
+// acquire-release addition order all threads' writes before it and all
+// reads after it, on both sides.
 __device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned expected, int* flag) {
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();
-        const bool last = atomicAdd(counter, 1u) == expected - 1;
-        if (last) *counter = 0;
-        __threadfence();
-        *flag = last;
+        unsigned before;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+        if (before == expected - 1) *counter = 0;
+        *flag = before == expected - 1;
     }
     __syncthreads();
     return *flag != 0;
 }
 
 // Joins `n` <= kFan partial results (slot_of(0..n-1), in order).  to_out: normalised
-// into the output rows; else back into slot_of(0).  All loads of a thread are in
-// flight together; maxima and sums go through `stats` in shared memory.
+// into the output rows; else back into slot_of(0).  `stats` (kFan + 1 rows of
+// heads, shared memory) holds the maxima and sums, then the weights.  Four
+// results' elements are in flight at once per thread; the loop stays rolled, since
+// its instructions are fetched for one use.
 template <int D, int NT, typename SlotOf>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot_of, bool to_out, int b, int head0,
                                            int heads, float2* stats) {
     using P = Part<D, NT>;
     constexpr int kVec = D / 4;
     constexpr int kItems = (P::kHeads * kVec) / kThreads;
-    constexpr int kBatch = 8;      // loads in flight per item
+    constexpr int kBatch = kItems > 4 ? 2 : 4;
+    float4 acc[kItems], o[kBatch][kItems];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) {
+            const float4* src = reinterpret_cast<const float4*>(P(a.part, slot_of(min(s0 + s, n - 1))).o(0)) + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < kItems; ++i)
+                // heads of a group that ends before the tile were never written
+                o[s][i] = (static_cast<int>(threadIdx.x) + i * kThreads) / kVec < heads ? __ldcg(src + i * kThreads)
+                                                                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    fetch(0);
     for (int i = threadIdx.x; i < kFan * P::kHeads; i += kThreads) {
         const int s = i / P::kHeads, h = i % P::kHeads;
-        const P p(a.part, slot_of(s < n ? s : 0));
+        const P p(a.part, slot_of(min(s, n - 1)));
         stats[i] = s < n && h < heads ? make_float2(__ldcg(p.m() + h), __ldcg(p.l() + h)) : make_float2(-INFINITY, 0.0f);
     }
+    __syncthreads();
+    if (threadIdx.x < P::kHeads) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kFan; ++s) top = fmaxf(top, stats[s * P::kHeads + threadIdx.x].x);
+#pragma unroll
+        for (int s = 0; s < kFan; ++s) {
+            float2& x = stats[s * P::kHeads + threadIdx.x];
+            x.x = scale_of(x.x, top);
+            sum += x.x * x.y;
+        }
+        stats[kFan * P::kHeads + threadIdx.x] = make_float2(top, sum);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int s0 = 0;;) {
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s)
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                const float w = s0 + s < n ? stats[(s0 + s) * P::kHeads + (threadIdx.x + i * kThreads) / kVec].x : 0.0f;
+                acc[i].x += w * o[s][i].x;
+                acc[i].y += w * o[s][i].y;
+                acc[i].z += w * o[s][i].z;
+                acc[i].w += w * o[s][i].w;
+            }
+        s0 += kBatch;
+        if (s0 >= n) break;
+        fetch(s0);
+    }
     const P first(a.part, slot_of(0));
-    bool known = false;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
         const int item = threadIdx.x + i * kThreads;
         const int h = item / kVec, d = (item % kVec) * 4;
-        float top = -INFINITY, sum = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int s0 = 0; s0 < kFan; s0 += kBatch) {
-            float4 o[kBatch];
-#pragma unroll
-            for (int s = 0; s < kBatch; ++s)
-                o[s] = s0 + s < n && h < heads
-                           ? __ldcg(reinterpret_cast<const float4*>(P(a.part, slot_of(s0 + s)).o(h) + d))
-                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (!known) __syncthreads();    // stats, while the first loads are on their way
-            known = true;
-            if (s0 == 0) {
-#pragma unroll
-                for (int s = 0; s < kFan; ++s) top = fmaxf(top, stats[s * P::kHeads + h].x);
-            }
-#pragma unroll
-            for (int s = 0; s < kBatch; ++s) {
-                const float2 ml = stats[(s0 + s) * P::kHeads + h];
-                const float w = scale_of(ml.x, top);
-                sum += w * ml.y;
-                acc.x += w * o[s].x;
-                acc.y += w * o[s].y;
-                acc.z += w * o[s].z;
-                acc.w += w * o[s].w;
-            }
-        }
         if (h >= heads) continue;
+        const float2 all = stats[kFan * P::kHeads + h];
         if (to_out) {
             const int64_t row = static_cast<int64_t>(b) * a.q_heads + head0 + h;
-            const float inv = 1.0f / sum;
+            const float inv = 1.0f / all.y;
             *reinterpret_cast<uint2*>(a.out + row * D + d) =
-                make_uint2(h2_as_u32(__floats2half2_rn(acc.x * inv, acc.y * inv)),
-                           h2_as_u32(__floats2half2_rn(acc.z * inv, acc.w * inv)));
-            if (d == 0 && a.lse) a.lse[row] = (top + log2f(sum)) * 0.6931471805599453f;
+                make_uint2(h2_as_u32(__floats2half2_rn(acc[i].x * inv, acc[i].y * inv)),
+                           h2_as_u32(__floats2half2_rn(acc[i].z * inv, acc[i].w * inv)));
+            if (d == 0 && a.lse) a.lse[row] = (all.x + log2f(all.y)) * 0.6931471805599453f;
         } else {
             // each element of slot_of(0) is read and written by one thread alone, and
-            // its maxima and sums were read by all before the barrier above
-            *reinterpret_cast<float4*>(first.o(h) + d) = acc;
+            // its maxima and sums were read by all before the barriers above
+            *reinterpret_cast<float4*>(first.o(h) + d) = acc[i];
             if (d == 0) {
-                first.m()[h] = top;
-                first.l()[h] = sum;
+                first.m()[h] = all.x;
+                first.l()[h] = all.y;
             }
         }
     }
@@ -227,54 +246,117 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         }
     };
 
-    // this block's range of the work line and the row that it begins in
-    const int per_thread = (a.batch + kThreads - 1) / kThreads;
-    const int b0 = tid * per_thread, b1 = min(b0 + per_thread, a.batch);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units_of(key_count(a, b));
-    mine *= a.head_groups;
-    int64_t incl = mine;
+    // ---- this block's range of the work line and the row that it begins in ----
+    // Thread i counts a few sequences; up to 32, every warp counts them all by itself.
+    const bool few = a.batch <= 32;
+    const int per_thread = few ? 1 : (a.batch + kThreads - 1) / kThreads;
+    const int b0 = (few ? lane : tid) * per_thread, b1 = min(b0 + per_thread, a.batch);
+    auto block_scan = [&](int64_t mine, int64_t& total) {      // exclusive sum before this thread
+        int64_t incl = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += u;
-    }
-    if (lane == 31) sums[warp] = incl;
-    __syncthreads();
-    int64_t total = 0, before = 0;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        total = __shfl_sync(0xffffffffu, incl, 31);
+        if (few) return incl - mine;
+        __syncthreads();
+        if (lane == 31) sums[warp] = incl;
+        __syncthreads();
+        int64_t before = 0;
+        total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += sums[w];
-        total += sums[w];
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+        }
+        return before + incl - mine;
+    };
+    int64_t units = 0, rows = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int n = units_of(key_count(a, b));
+        units += n;
+        rows += n > 0;
     }
+    units *= a.head_groups;
+    rows *= a.head_groups;
+    int64_t total, total_rows;
+    int64_t before = block_scan(units, total);
+    block_scan(rows, total_rows);
+    // Ranges of the line are even, but a block whose range crosses a row's end joins
+    // two rows, which a short call waits for.  With few rows each is divided by
+    // itself: no block has more than `aligned` units and no more blocks are
+    // needed, since sum ceil(n_r / p) <= total / p + rows.  Taken where it costs a
+    // block at most 128 KB more than the even ranges; joining twice was seen to
+    // take as long as 4 us, that many bytes' time.
     int64_t per = div_small(total + gridDim.x - 1, gridDim.x);
     if (per < kMinUnits) per = kMinUnits;
-    const int64_t start = per * blockIdx.x;
+    const int64_t spare = static_cast<int64_t>(gridDim.x) - total_rows;
+    int64_t aligned = spare > 0 ? div_small(total + spare - 1, spare) : 0;
+    if (aligned < kMinUnits) aligned = kMinUnits;
+    const bool by_row = spare > 0 && (aligned - per) * D <= 2048;
+    // what a sequence takes of the line: its units, or its blocks
+    auto weight = [&](int b) {
+        const int n = units_of(key_count(a, b));
+        return static_cast<int64_t>(a.head_groups) * (by_row ? div_small(n + aligned - 1, aligned) : n);
+    };
+    int64_t mine = units;
+    if (by_row) {
+        mine = 0;
+        for (int b = b0; b < b1; ++b) mine += weight(b);
+        before = block_scan(mine, total);
+    }
+    int64_t start = by_row ? blockIdx.x : per * blockIdx.x;
     if (start >= total) {
         empty_rows();
         return;
     }
-    const int64_t end = min(start + per, total);
-    {
-        int64_t at = before + incl - mine;
-        if (start >= at && start < at + mine) {
-            int b = b0;
-            for (;; ++b) {
-                const int64_t n = static_cast<int64_t>(units_of(key_count(a, b))) * a.head_groups;
-                if (start < at + n) break;
-                at += n;
-            }
-            first_b = b;
-            first_begin = at;
+    int64_t end = by_row ? 0 : min(start + per, total);
+    const bool owner = start >= before && start < before + mine;
+    int row_b = b0;
+    if (owner) {
+        for (;; ++row_b) {
+            const int64_t n = weight(row_b);
+            if (start < before + n) break;
+            before += n;
         }
     }
-    __syncthreads();
+    if (few) {
+        const int from = __ffs(__ballot_sync(0xffffffffu, owner)) - 1;
+        row_b = __shfl_sync(0xffffffffu, row_b, from);
+        before = __shfl_sync(0xffffffffu, before, from);
+    } else {
+        if (owner) {
+            first_b = row_b;
+            first_begin = before;
+        }
+        __syncthreads();
+        row_b = first_b;
+        before = first_begin;
+    }
     Row row;
-    row.b = first_b;
+    row.b = row_b;
     row.keys = key_count(a, row.b);
     row.units = units_of(row.keys);
-    row.hg = static_cast<int>(div_small(start - first_begin, row.units));
-    row.begin = first_begin + static_cast<int64_t>(row.hg) * row.units;
+    int row_part = 0, row_parts = 0;      // by_row: this block's share of its row
+    if (by_row) {
+        const int blocks = static_cast<int>(div_small(row.units + aligned - 1, aligned));
+        const int at = static_cast<int>(start - before);
+        row.hg = at / blocks;
+        row_part = at - row.hg * blocks;
+        const int share = (row.units + blocks - 1) / blocks;
+        row_parts = (row.units + share - 1) / share;
+        row.begin = 0;
+        start = static_cast<int64_t>(row_part) * share;
+        end = min(start + share, static_cast<int64_t>(row.units));
+        if (start >= end) {
+            empty_rows();
+            return;
+        }
+    } else {
+        row.hg = static_cast<int>(div_small(start - before, row.units));
+        row.begin = before + static_cast<int64_t>(row.hg) * row.units;
+    }
 
     // ---- the ring's producer side: the same lanes, running ahead ----
     const uint32_t ring = smem_u32(smem) + warp * T::kRingBytes;
@@ -470,8 +552,11 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
 
         // ---- join the block's warps ----
         const bool whole = row.begin >= start && row.begin + row.units <= end;
-        const int64_t c0 = div_small(row.begin, per), c1 = div_small(row.begin + row.units - 1, per);
-        auto slot_of_block = [&](int64_t c) { return 2 * c + (c == c0 && row.begin != c0 * per ? 1 : 0); };
+        // the row's blocks are c0 .. c0 + parts - 1; a row that begins inside c0's range uses its second slot
+        const int64_t c0 = by_row ? static_cast<int64_t>(blockIdx.x) - row_part : div_small(row.begin, per);
+        const int parts = by_row ? row_parts : static_cast<int>(div_small(row.begin + row.units - 1, per) - c0 + 1);
+        const bool second = !by_row && row.begin != c0 * per;
+        auto slot_of_block = [&](int64_t c) { return 2 * c + (second && c == c0 ? 1 : 0); };
         const P mine_part(a.part, slot_of_block(blockIdx.x));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -529,7 +614,6 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
             __syncthreads();
         }
         if (!whole) {
-            const int parts = static_cast<int>(c1 - c0 + 1);
             // kFan neighbours' results become one, kFan of those the next, ... each time by the last to arrive
             unsigned* counters = a.counters;
             for (int64_t step = 1;; step *= kFan, counters += 2 * gridDim.x) {
