@@ -608,7 +608,9 @@ size_t mcv_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int
  * length are not read.  A length of 0 or less gives a zero row and lse -inf; one
  * beyond table_cols * page_size is cut to that (and sets the error bit), and
  * a page out of range reads as zeros (and sets it).  head_dim 64, 128 or 256;
- * batch up to 4096.  Scores, softmax and sums are fp32; the cache is read once
+ * batch up to 4096; batch * kv_heads * table_cols * page_size / 16 (twice that
+ * from 17 query heads per kv head on, and so forth) below 2^31; k and v within
+ * 64 GB each.  Scores, softmax and sums are fp32; the cache is read once
  * up to 16 query heads per kv head. */
 int mcv_paged_attention_decode(const mcv_rows* q, const mcv_kv_cache* cache, const void* page_table,
                                int64_t table_cols, const void* lengths, void* out, void* lse, int64_t batch,

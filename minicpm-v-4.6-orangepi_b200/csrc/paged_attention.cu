@@ -67,7 +67,8 @@ struct AttnArgs {
     float* lse;
     float* part;
     unsigned* counters;   // [kLevels][2 * grid]
-    int64_t q_bs, q_hs, page_stride, table_cols;
+    int64_t q_bs, q_hs, table_cols;
+    uint32_t page_vecs;      // 16-byte vectors from page to page
     int batch, q_heads, kv_heads, group, head_groups, splits_of_group, num_pages, max_keys;
     float scale_log2;
     FastDiv page;
@@ -77,15 +78,11 @@ __device__ __forceinline__ int key_count(const AttnArgs& a, int b) {
     const int n = a.lengths[b];
     return n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n);
 }
-// n / d, by a 32-bit division where n allows it (a 64-bit one is a long routine).
-__device__ __forceinline__ int64_t div_small(int64_t n, int64_t d) {
-    return ((n | d) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d;
-}
 __device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
 
 // A row of the work line: one sequence and one group of query heads.
 struct Row {
-    int64_t begin;   // first unit
+    int begin;       // first unit
     int b, hg, keys, units;
     __device__ __forceinline__ void next(const AttnArgs& a) {
         begin += units;
@@ -130,17 +127,18 @@ __device__ __forceinline__ bool arrive_last(unsigned* counter, unsigned expected
 
 // Joins `n` <= kFan partial results (slot_of(0..n-1), in order).  to_out: normalised
 // into the output rows; else back into slot_of(0).  `stats` (kFan + 1 rows of
-// heads, shared memory) holds the maxima and sums, then the weights.  Four
-// results' elements are in flight at once per thread; the loop stays rolled, since
-// its instructions are fetched for one use.
+// heads, shared memory) holds the maxima, then the weights.  Eight results'
+// elements are in flight at once per thread (four with 16 heads of 256).
 template <int D, int NT, typename SlotOf>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot_of, bool to_out, int b, int head0,
                                            int heads, float2* stats) {
     using P = Part<D, NT>;
     constexpr int kVec = D / 4;
     constexpr int kItems = (P::kHeads * kVec) / kThreads;
-    constexpr int kBatch = kItems > 4 ? 2 : 4;
+    constexpr int kRounds = kFan * P::kHeads / kThreads;
+    constexpr int kBatch = kItems > 4 ? 4 : 8;
     float4 acc[kItems], o[kBatch][kItems];
+    float sum[kItems];
     auto fetch = [&](int s0) {
 #pragma unroll
         for (int s = 0; s < kBatch; ++s) {
@@ -148,43 +146,58 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot
 #pragma unroll
             for (int i = 0; i < kItems; ++i)
                 // heads of a group that ends before the tile were never written
-                o[s][i] = (static_cast<int>(threadIdx.x) + i * kThreads) / kVec < heads ? __ldcg(src + i * kThreads)
-                                                                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                o[s][i] = s0 + s < n && (static_cast<int>(threadIdx.x) + i * kThreads) / kVec < heads
+                              ? __ldcg(src + i * kThreads)
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
     };
-    fetch(0);
-    for (int i = threadIdx.x; i < kFan * P::kHeads; i += kThreads) {
-        const int s = i / P::kHeads, h = i % P::kHeads;
+    float m[kRounds], l[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const int i = threadIdx.x + r * kThreads, s = i / P::kHeads, h = i % P::kHeads;
         const P p(a.part, slot_of(min(s, n - 1)));
-        stats[i] = s < n && h < heads ? make_float2(__ldcg(p.m() + h), __ldcg(p.l() + h)) : make_float2(-INFINITY, 0.0f);
+        const bool there = s < n && h < heads;
+        m[r] = there ? __ldcg(p.m() + h) : -INFINITY;
+        l[r] = there ? __ldcg(p.l() + h) : 0.0f;
+    }
+    fetch(0);
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) stats[threadIdx.x + r * kThreads].x = m[r];
+    __syncthreads();
+    float top[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const int h = threadIdx.x % P::kHeads;
+        top[r] = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < kFan; ++s) top[r] = fmaxf(top[r], stats[s * P::kHeads + h].x);
     }
     __syncthreads();
-    if (threadIdx.x < P::kHeads) {
-        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kFan; ++s) top = fmaxf(top, stats[s * P::kHeads + threadIdx.x].x);
-#pragma unroll
-        for (int s = 0; s < kFan; ++s) {
-            float2& x = stats[s * P::kHeads + threadIdx.x];
-            x.x = scale_of(x.x, top);
-            sum += x.x * x.y;
-        }
-        stats[kFan * P::kHeads + threadIdx.x] = make_float2(top, sum);
+    for (int r = 0; r < kRounds; ++r) {
+        const float w = scale_of(m[r], top[r]);
+        stats[threadIdx.x + r * kThreads] = make_float2(w, w * l[r]);
+        if (r == 0 && threadIdx.x < P::kHeads) stats[kFan * P::kHeads + threadIdx.x].x = top[r];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < kItems; ++i) {
+        acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        sum[i] = 0.0f;
+    }
 #pragma unroll 1
     for (int s0 = 0;;) {
 #pragma unroll
         for (int s = 0; s < kBatch; ++s)
 #pragma unroll
             for (int i = 0; i < kItems; ++i) {
-                const float w = s0 + s < n ? stats[(s0 + s) * P::kHeads + (threadIdx.x + i * kThreads) / kVec].x : 0.0f;
-                acc[i].x += w * o[s][i].x;
-                acc[i].y += w * o[s][i].y;
-                acc[i].z += w * o[s][i].z;
-                acc[i].w += w * o[s][i].w;
+                // weights behind the last result are zero
+                const float2 w = stats[(s0 + s) * P::kHeads + (threadIdx.x + i * kThreads) / kVec];
+                sum[i] += w.y;
+                acc[i].x += w.x * o[s][i].x;
+                acc[i].y += w.x * o[s][i].y;
+                acc[i].z += w.x * o[s][i].z;
+                acc[i].w += w.x * o[s][i].w;
             }
         s0 += kBatch;
         if (s0 >= n) break;
@@ -196,7 +209,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot
         const int item = threadIdx.x + i * kThreads;
         const int h = item / kVec, d = (item % kVec) * 4;
         if (h >= heads) continue;
-        const float2 all = stats[kFan * P::kHeads + h];
+        const float2 all = make_float2(stats[kFan * P::kHeads + h].x, sum[i]);
         if (to_out) {
             const int64_t row = static_cast<int64_t>(b) * a.q_heads + head0 + h;
             const float inv = 1.0f / all.y;
@@ -221,9 +234,8 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
     using T = Tile<D>;
     using P = Part<D, NT>;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int64_t sums[kWarps];
-    __shared__ int64_t first_begin;
-    __shared__ int first_b, flag;
+    __shared__ int2 sums[kWarps], first;
+    __shared__ int flag;
     float* join = reinterpret_cast<float*>(smem + kWarps * T::kRingBytes);
     float* join_m = join + kWarps * 8 * T::kJoinRow;
     float* join_l = join_m + kWarps * 8;
@@ -251,72 +263,75 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
     const bool few = a.batch <= 32;
     const int per_thread = few ? 1 : (a.batch + kThreads - 1) / kThreads;
     const int b0 = (few ? lane : tid) * per_thread, b1 = min(b0 + per_thread, a.batch);
-    auto block_scan = [&](int64_t mine, int64_t& total) {      // exclusive sum before this thread
-        int64_t incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += u;
-        }
-        total = __shfl_sync(0xffffffffu, incl, 31);
-        if (few) return incl - mine;
-        __syncthreads();
-        if (lane == 31) sums[warp] = incl;
-        __syncthreads();
-        int64_t before = 0;
-        total = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) before += sums[w];
-            total += sums[w];
-        }
-        return before + incl - mine;
-    };
-    int64_t units = 0, rows = 0;
+    int units = 0, rows = 0;
     for (int b = b0; b < b1; ++b) {
         const int n = units_of(key_count(a, b));
         units += n;
         rows += n > 0;
     }
-    units *= a.head_groups;
-    rows *= a.head_groups;
-    int64_t total, total_rows;
-    int64_t before = block_scan(units, total);
-    block_scan(rows, total_rows);
+    int total = __reduce_add_sync(0xffffffffu, units) * a.head_groups;
+    int total_rows = __reduce_add_sync(0xffffffffu, rows) * a.head_groups;
+    if (!few) {
+        if (lane == 0) sums[warp] = make_int2(total, total_rows);
+        __syncthreads();
+        total = total_rows = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            total += sums[w].x;
+            total_rows += sums[w].y;
+        }
+        __syncthreads();
+    }
     // Ranges of the line are even, but a block whose range crosses a row's end joins
     // two rows, which a short call waits for.  With few rows each is divided by
-    // itself: no block has more than `aligned` units and no more blocks are
-    // needed, since sum ceil(n_r / p) <= total / p + rows.  Taken where it costs a
-    // block at most 128 KB more than the even ranges; joining twice was seen to
-    // take as long as 4 us, that many bytes' time.
-    int64_t per = div_small(total + gridDim.x - 1, gridDim.x);
-    if (per < kMinUnits) per = kMinUnits;
-    const int64_t spare = static_cast<int64_t>(gridDim.x) - total_rows;
-    int64_t aligned = spare > 0 ? div_small(total + spare - 1, spare) : 0;
-    if (aligned < kMinUnits) aligned = kMinUnits;
-    const bool by_row = spare > 0 && (aligned - per) * D <= 2048;
+    // itself: with total / (blocks - rows) units a block there are blocks enough, since
+    // sum ceil(n_r / p) <= total / p + rows.  Taken where it costs a block at most
+    // 128 KB more than the even ranges, total rows / (blocks (blocks - rows)) units:
+    // joining twice was seen to take as long as 4 us, that many bytes' time.
+    const int grid = gridDim.x, spare = grid - total_rows;
+    const bool by_row = spare > 0 && static_cast<int64_t>(total) * total_rows * D <= static_cast<int64_t>(grid) * spare * 2048;
+    const int div = by_row ? spare : grid;
+    const int per = max(kMinUnits, (total + div - 1) / div);     // units of a block
     // what a sequence takes of the line: its units, or its blocks
     auto weight = [&](int b) {
         const int n = units_of(key_count(a, b));
-        return static_cast<int64_t>(a.head_groups) * (by_row ? div_small(n + aligned - 1, aligned) : n);
+        return a.head_groups * (by_row ? (n + per - 1) / per : n);
     };
-    int64_t mine = units;
+    int mine = units * a.head_groups;
     if (by_row) {
         mine = 0;
         for (int b = b0; b < b1; ++b) mine += weight(b);
-        before = block_scan(mine, total);
     }
-    int64_t start = by_row ? blockIdx.x : per * blockIdx.x;
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += u;
+    }
+    if (few) {
+        total = __shfl_sync(0xffffffffu, before, 31);
+    } else {
+        if (lane == 31) sums[warp].x = before;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += sums[w].x;
+            total += sums[w].x;
+        }
+    }
+    before -= mine;
+    int start = by_row ? blockIdx.x : min(static_cast<int64_t>(per) * blockIdx.x, static_cast<int64_t>(total));
     if (start >= total) {
         empty_rows();
         return;
     }
-    int64_t end = by_row ? 0 : min(start + per, total);
+    int end = by_row ? 0 : min(static_cast<int64_t>(start) + per, static_cast<int64_t>(total));
     const bool owner = start >= before && start < before + mine;
     int row_b = b0;
     if (owner) {
         for (;; ++row_b) {
-            const int64_t n = weight(row_b);
+            const int n = weight(row_b);
             if (start < before + n) break;
             before += n;
         }
@@ -326,13 +341,10 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         row_b = __shfl_sync(0xffffffffu, row_b, from);
         before = __shfl_sync(0xffffffffu, before, from);
     } else {
-        if (owner) {
-            first_b = row_b;
-            first_begin = before;
-        }
+        if (owner) first = make_int2(row_b, before);
         __syncthreads();
-        row_b = first_b;
-        before = first_begin;
+        row_b = first.x;
+        before = first.y;
     }
     Row row;
     row.b = row_b;
@@ -340,66 +352,66 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
     row.units = units_of(row.keys);
     int row_part = 0, row_parts = 0;      // by_row: this block's share of its row
     if (by_row) {
-        const int blocks = static_cast<int>(div_small(row.units + aligned - 1, aligned));
-        const int at = static_cast<int>(start - before);
+        const int blocks = (row.units + per - 1) / per;
+        const int at = start - before;
         row.hg = at / blocks;
         row_part = at - row.hg * blocks;
         const int share = (row.units + blocks - 1) / blocks;
         row_parts = (row.units + share - 1) / share;
         row.begin = 0;
-        start = static_cast<int64_t>(row_part) * share;
-        end = min(start + share, static_cast<int64_t>(row.units));
+        start = row_part * share;
+        end = min(start + share, row.units);
         if (start >= end) {
             empty_rows();
             return;
         }
     } else {
-        row.hg = static_cast<int>(div_small(start - before, row.units));
-        row.begin = before + static_cast<int64_t>(row.hg) * row.units;
+        row.hg = (start - before) / row.units;
+        row.begin = before + row.hg * row.units;
     }
 
     // ---- the ring's producer side: the same lanes, running ahead ----
+    constexpr int kVecs = D / 8;     // 16-byte vectors of a row
     const uint32_t ring = smem_u32(smem) + warp * T::kRingBytes;
     Row ahead = row;
-    int64_t u_look = start + warp, u_ahead = u_look;
-    struct Look {       // row r of a unit, in lanes r and r + 16
-        int64_t off;    // element offset within the page (K and V alike)
+    int u_look = start + warp, u_ahead = u_look;
+    constexpr uint32_t kNone = 0xffffffffu;
+    struct Look {          // row r of a unit, in lanes r and r + 16
+        uint32_t at;       // place within the page in 16-byte vectors, kNone: no such row
         int page;
-        bool row;       // there is such a row
     };
     auto look_up = [&]() {
-        Look x{0, 0, false};
-        const int64_t u = u_look;
+        Look x{kNone, 0};
+        const int u = u_look;
         u_look += kWarps;
         if (u >= end) return x;
         while (u >= ahead.begin + ahead.units) ahead.next(a);
-        const int key = static_cast<int>(u - ahead.begin) * kUnit + (lane & 15);
+        const int key = (u - ahead.begin) * kUnit + (lane & 15);
         if (key >= ahead.keys) return x;
         const uint32_t page = a.page.div(key);
         x.page = a.table[ahead.b * a.table_cols + page];
         const int kvh = ahead.hg / a.splits_of_group;
-        x.off = (static_cast<int64_t>(kvh) * a.page.d + (key - page * a.page.d)) * D;
-        x.row = true;
+        x.at = (kvh * a.page.d + (key - page * a.page.d)) * kVecs;
         return x;
     };
     auto issue = [&](int stage, const Look& x) {
         if (u_ahead < end) {
-            constexpr int kVecs = D / 8;                 // 16-byte vectors of a row
-            constexpr int kIters = kUnit * kVecs / 32;
             const uint32_t base = ring + stage * T::kStageBytes;
-            const bool inside = x.page >= 0 && x.page < a.num_pages;
-            if (x.row && !inside) atomicOr(&g_attention_dev_error, kDevErrIndex);
-            const int64_t src = x.off + (inside ? x.page : 0) * a.page_stride;
-            const int ok = x.row && inside;
+            uint32_t src = kNone;      // the row's first vector in k and v
+            if (x.at != kNone) {
+                if (x.page >= 0 && x.page < a.num_pages) src = x.page * a.page_vecs + x.at;
+                else atomicOr(&g_attention_dev_error, kDevErrIndex);
+            }
 #pragma unroll
-            for (int i = 0; i < kIters; ++i) {
+            for (int i = 0; i < kUnit * kVecs / 32; ++i) {
                 const int item = i * 32 + lane;
                 const int r = item / kVecs, c = item % kVecs;
-                const int64_t off = __shfl_sync(0xffffffffu, src, r) + c * 8;
-                const bool take = __shfl_sync(0xffffffffu, ok, r) != 0;
+                const uint32_t off = __shfl_sync(0xffffffffu, src, r);
+                const bool take = off != kNone;
+                const uint64_t bytes = static_cast<uint64_t>(take ? off + c : 0) * 16;
                 const uint32_t dst = base + r * T::kRowBytes + ((c ^ (r & 7)) << 4);
-                cp_async16_or_zero(dst, a.k + off, take);
-                cp_async16_or_zero(dst + kUnit * T::kRowBytes, a.v + off, take);
+                cp_async16_or_zero(dst, reinterpret_cast<const char*>(a.k) + bytes, take);
+                cp_async16_or_zero(dst + kUnit * T::kRowBytes, reinterpret_cast<const char*>(a.v) + bytes, take);
             }
         }
         cp_async_commit();
@@ -426,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
     // pages are looked up two units ahead of their copies, queries a row ahead
     Look look0 = look_up(), look1 = look_up();
     load_q(row);
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < T::kStages - 1; ++s) {
         issue(s, look0);
         look0 = look1;
@@ -438,9 +450,9 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
     const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_vec = lane >> 4;
     const int v_row = (lane & 7) + (lane >> 4) * 8, v_vec = (lane >> 3) & 1;
     int stage = 0;
-    int64_t u = start + warp;
-    for (int64_t pos = start; pos < end;) {
-        const int64_t seg_end = min(row.begin + row.units, end);
+    int u = start + warp;
+    for (int pos = start; pos < end;) {
+        const int seg_end = min(row.begin + row.units, end);
         const int kvh = row.hg / a.splits_of_group;
         const int in_group = (row.hg % a.splits_of_group) * P::kHeads;
         const int head0 = kvh * a.group + in_group;
@@ -484,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
             }
-            const int key = static_cast<int>(u - row.begin) * kUnit + g;
+            const int key = (u - row.begin) * kUnit + g;
             const bool in0 = key < row.keys, in1 = key + 8 < row.keys;
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
@@ -553,10 +565,10 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         // ---- join the block's warps ----
         const bool whole = row.begin >= start && row.begin + row.units <= end;
         // the row's blocks are c0 .. c0 + parts - 1; a row that begins inside c0's range uses its second slot
-        const int64_t c0 = by_row ? static_cast<int64_t>(blockIdx.x) - row_part : div_small(row.begin, per);
-        const int parts = by_row ? row_parts : static_cast<int>(div_small(row.begin + row.units - 1, per) - c0 + 1);
+        const int c0 = by_row ? static_cast<int>(blockIdx.x) - row_part : row.begin / per;
+        const int parts = by_row ? row_parts : (row.begin + row.units - 1) / per - c0 + 1;
         const bool second = !by_row && row.begin != c0 * per;
-        auto slot_of_block = [&](int64_t c) { return 2 * c + (second && c == c0 ? 1 : 0); };
+        auto slot_of_block = [&](int c) { return 2 * c + (second && c == c0 ? 1 : 0); };
         const P mine_part(a.part, slot_of_block(blockIdx.x));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -616,9 +628,9 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
         if (!whole) {
             // kFan neighbours' results become one, kFan of those the next, ... each time by the last to arrive
             unsigned* counters = a.counters;
-            for (int64_t step = 1;; step *= kFan, counters += 2 * gridDim.x) {
-                const int64_t f0 = c0 + (blockIdx.x - c0) / (step * kFan) * (step * kFan);
-                const int n = static_cast<int>(min(static_cast<int64_t>(kFan), (c0 + parts - f0 + step - 1) / step));
+            for (int step = 1;; step *= kFan, counters += 2 * gridDim.x) {
+                const int f0 = c0 + (static_cast<int>(blockIdx.x) - c0) / (step * kFan) * (step * kFan);
+                const int n = min(kFan, (c0 + parts - f0 + step - 1) / step);
                 if (!arrive_last(counters + slot_of_block(f0), n, &flag)) break;
                 const bool all = step * kFan >= parts;
                 join_parts<D, NT>(a, n, [&](int i) { return slot_of_block(f0 + i * step); }, all, row.b, head0, heads,
@@ -705,6 +717,10 @@ int mcv_paged_attention_decode(const mcv_rows* q, const mcv_kv_cache* cache, con
     const int64_t splits = (group + 8 * nt - 1) / (8 * nt);
     const int64_t max_keys = table_cols * cache->page_size;
     const int64_t most = batch * cache->kv_heads * splits * ((max_keys + kUnit - 1) / kUnit);
+    if (most > 0x7fffffffLL - kMinUnits)
+        return fail(MCV_ERR_SHAPE, "paged_attention_decode: batch x kv heads x table capacity / 16 must stay below 2^31");
+    if (static_cast<uint64_t>(cache->num_pages) * static_cast<uint64_t>(cache->page_stride / 8) >= 0xffffffffull)
+        return fail(MCV_ERR_SHAPE, "paged_attention_decode: k and v may span 64 GB each");
     const int64_t want = (most + kMinUnits - 1) / kMinUnits;
     const int full = sms * blocks_per_sm(dim);
     const int grid = static_cast<int>(want < full ? want : full);
@@ -712,7 +728,7 @@ int mcv_paged_attention_decode(const mcv_rows* q, const mcv_kv_cache* cache, con
     AttnArgs a{static_cast<const __half*>(q->data), static_cast<const __half*>(cache->k),
                static_cast<const __half*>(cache->v), static_cast<const int32_t*>(page_table),
                static_cast<const int32_t*>(lengths), static_cast<__half*>(out), static_cast<float*>(lse), nullptr, nullptr,
-               q->token_stride, q->head_stride, cache->page_stride, table_cols, static_cast<int>(batch),
+               q->token_stride, q->head_stride, table_cols, static_cast<uint32_t>(cache->page_stride / 8), static_cast<int>(batch),
                static_cast<int>(q_heads), cache->kv_heads, static_cast<int>(group),
                static_cast<int>(cache->kv_heads * splits), static_cast<int>(splits), cache->num_pages,
                static_cast<int>(max_keys), scale * 1.4426950408889634f, FastDiv(static_cast<uint32_t>(cache->page_size))};
