@@ -5,7 +5,6 @@
 // with q and k divided by sqrt(sum x^2 + eps) first when asked.  Value heads
 // h * v_heads / k_heads ... share key head h.
 #include "mixing.cuh"
-#include "tcgen05.cuh"
 
 #include <cmath>
 
@@ -184,21 +183,26 @@ __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uin
     lo = h2_as_u32(__floats2half2_rn((x - f.x) * kLo, (y - f.y) * kLo));
 }
 
-// One chunk's share of the workspace: T (rows 0-63) over P T (rows 64-127), hi and
-// lo, as the shared-memory image of an MMA operand (rows of 128 bytes, 16-byte
-// pieces exchanged by the row's low bits: the 128-byte swizzle), and the scales.
+// One chunk's share of the workspace: T and P T, hi and lo, and the scales.  Of the
+// two matrices only the 16x16 blocks on and below the diagonal are kept, as 8x8
+// matrices of 128 contiguous bytes, 2 i + 2 of them for each of the two groups of
+// eight rows of block row i: fragments are written and read whole, ldmatrix
+// hits no bank twice, and a chunk is one copy.
+constexpr int kTri = 40 * 64;        // elements of a triangle
 struct Chunk {
-    __half tp[2][128 * kChunk];
+    __half tp[2][2][kTri];           // [hi, lo][T, P T]
     float ck[kChunk];                // e^G r_k
     float cq[kChunk];                // scale e^G r_q
     float cs[kChunk];                // e^(G_C - G) r_k
     float keep;                      // e^G_C
     float pad[63];
 };
-static_assert(sizeof(Chunk) == 33 * 1024, "a chunk is copied whole");
-
-// Byte offset of element (r, c) in a tile of 128-byte rows under the 128-byte swizzle.
-__device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((((c >> 3) ^ r) & 7) << 4) + (c & 7) * 2; }
+static_assert(sizeof(Chunk) % 128 == 0, "chunks stay aligned");
+constexpr uint32_t kChunkBytes = 4 * kTri * 2 + (3 * kChunk + 4) * 4;      // in use
+__host__ __device__ constexpr int tri_at(int r, int c) {
+    const int i = r >> 4;
+    return (2 * i * (i + 1) + ((r >> 3) & 1) * (2 * i + 2) + (c >> 3)) * 64 + (r & 7) * 8 + (c & 7);
+}
 
 // The slots of sequence b begin at cu[b] / 64 + b: ranges of ceil(len / 64) from
 // there on never overlap, since floor(x + y) >= floor(x) + floor(y).
@@ -253,14 +257,14 @@ __device__ __forceinline__ void to_b(Split4& b, const float (&x)[2][4]) {
 // by split MMAs, one warp a column of blocks, in registers - the columns do not
 // depend on each other - and so P X.
 template <int DK>
-__global__ void __launch_bounds__(128, 4) chunk_kernel(const DeltaArgs a, Chunk* chunks) {
+__global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk* chunks) {
     constexpr int kVecs = DK / 8;
-    extern __shared__ __align__(128) unsigned char smem[];  // K and Q, later the record's image
+    extern __shared__ __align__(128) unsigned char smem[];  // K and Q, then the blocks
     // 16x16 blocks, hi and lo, each as four 8x8 matrices in ldmatrix's order for an A operand
-    __shared__ __align__(128) __half a_blk[2][6 * 256];     // A below the diagonal blocks
-    __shared__ __align__(128) __half p_blk[2][10 * 256];    // P on and below the diagonal
-    __shared__ __align__(128) __half x_blk[2][4 * 256];     // inverses of the diagonal blocks
-    __shared__ float diag[4][16 * 17];
+    __half* a_blk = reinterpret_cast<__half*>(smem);         // [2][6 blocks]: A below the diagonal blocks
+    __half* p_blk = a_blk + 2 * 6 * 256;                      // [2][10]: P on and below the diagonal
+    __half* x_blk = p_blk + 2 * 10 * 256;                     // [2][4]: inverses of the diagonal blocks
+    float* diag = reinterpret_cast<float*>(x_blk + 2 * 4 * 256);   // [4][16 * 17]: A's diagonal blocks
     __shared__ float4 rows[kChunk];                         // G (two floats), r_k, r_q scale
     __shared__ float bt[kChunk];
     pdl_trigger();
@@ -376,6 +380,7 @@ __global__ void __launch_bounds__(128, 4) chunk_kernel(const DeltaArgs a, Chunk*
             mma16816(qk[2 * j + 1], qa, b[2], b[3]);
         }
     }
+    __syncthreads();     // K and Q are not read any more
     const int g = lane >> 2, t = lane & 3;
     const float4 row[2] = {rows[warp * 16 + g], rows[warp * 16 + g + 8]};
     const float write[2] = {row[0].z * bt[warp * 16 + g], row[1].z * bt[warp * 16 + g + 8]};
@@ -400,17 +405,17 @@ __global__ void __launch_bounds__(128, 4) chunk_kernel(const DeltaArgs a, Chunk*
             uint32_t x, y;
             split_scaled(p[0], p[1], x, y);
             const int at = (warp * (warp + 1) / 2 + j / 2) * 256 + in;
-            *reinterpret_cast<uint32_t*>(&p_blk[0][at]) = x;
-            *reinterpret_cast<uint32_t*>(&p_blk[1][at]) = y;
+            *reinterpret_cast<uint32_t*>(p_blk + at) = x;
+            *reinterpret_cast<uint32_t*>(p_blk + 10 * 256 + at) = y;
             if (j / 2 == warp) {
-                const int dc = (j & 1) * 8 + 2 * t;
-                diag[warp][(g + e * 4) * 17 + dc] = m[0];
-                diag[warp][(g + e * 4) * 17 + dc + 1] = m[1];
+                float* d = diag + warp * 16 * 17 + (g + e * 4) * 17 + (j & 1) * 8 + 2 * t;
+                d[0] = m[0];
+                d[1] = m[1];
             } else {
                 const int am = (warp * (warp - 1) / 2 + j / 2) * 256 + in;
                 split_scaled(m[0], m[1], x, y);
-                *reinterpret_cast<uint32_t*>(&a_blk[0][am]) = x;
-                *reinterpret_cast<uint32_t*>(&a_blk[1][am]) = y;
+                *reinterpret_cast<uint32_t*>(a_blk + am) = x;
+                *reinterpret_cast<uint32_t*>(a_blk + 6 * 256 + am) = y;
             }
         }
     }
@@ -418,226 +423,155 @@ __global__ void __launch_bounds__(128, 4) chunk_kernel(const DeltaArgs a, Chunk*
 
     // this warp's diagonal block: lanes 0-15 take a column each,
     // x_i = [i = j] - sum_{l < i} A_il x_l
-    float xc[16];
     if (lane < 16) {
-        const float* m = diag[warp];
+        const float* m = diag + warp * 16 * 17;
+        const float beta = bt[warp * 16 + lane];
+        float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float acc[2] = {i == lane ? 1.0f : 0.0f, 0.0f};
 #pragma unroll
-            for (int l = 0; l < i; ++l) acc[l & 1] -= m[i * 17 + l] * xc[l];
-            xc[i] = acc[0] + acc[1];
+            for (int l = 0; l < i; ++l) acc[l & 1] -= m[i * 17 + l] * x[l];
+            x[i] = acc[0] + acc[1];
             const int at = warp * 256 + ((lane >> 3) * 2 + (i >> 3)) * 64 + (i & 7) * 8 + (lane & 7);
-            const __half hi16 = __float2half_rn(xc[i]);
-            x_blk[0][at] = hi16;
-            x_blk[1][at] = __float2half_rn((xc[i] - __half2float(hi16)) * kLo);
+            __half hi16 = __float2half_rn(x[i]);
+            x_blk[at] = hi16;
+            x_blk[4 * 256 + at] = __float2half_rn((x[i] - __half2float(hi16)) * kLo);
+            const float y = x[i] * beta;
+            const int to = tri_at(warp * 16 + i, warp * 16 + lane);
+            hi16 = __float2half_rn(y);
+            out.tp[0][0][to] = hi16;
+            out.tp[1][0][to] = __float2half_rn((y - __half2float(hi16)) * kLo);
         }
     }
-    __syncthreads();     // K and Q are not read any more: the image takes their place
+    __syncthreads();
 
-    unsigned char* image = smem;
-    constexpr int kImageLo = 128 * kChunk * 2;
-    for (int i = tid; i < 6 * 32 * 2 * 2; i += 128) {     // blocks above the diagonal
-        const int blk = i / 128, half = (i >> 6) & 1, lo_part = (i >> 5) & 1, r = (i >> 1) & 15, c = i & 1;
-        const int bi = blk >= 5 ? 2 : (blk >= 3 ? 1 : 0), bj = blk >= 5 ? 3 : (blk >= 3 ? blk - 1 : blk + 1);
-        *reinterpret_cast<uint4*>(image + lo_part * kImageLo + sw128(half * 64 + bi * 16 + r, bj * 16 + c * 8)) =
-            make_uint4(0, 0, 0, 0);
-    }
-    if (lane < 16) {
-        const float beta = bt[warp * 16 + lane];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float x = xc[i] * beta;
-            const __half hi16 = __float2half_rn(x);
-            const uint32_t at = sw128(warp * 16 + i, warp * 16 + lane);
-            *reinterpret_cast<__half*>(image + at) = hi16;
-            *reinterpret_cast<__half*>(image + kImageLo + at) = __float2half_rn((x - __half2float(hi16)) * kLo);
-        }
-    }
     // this warp's column of blocks; its diagonal block as a B operand (k lo, k hi of columns lo, then hi)
-    {
-        Split4 xb[4];
-        const uint32_t xs = smem_u32(x_blk), as = smem_u32(a_blk), ps = smem_u32(p_blk);
-        constexpr uint32_t kXLo = 4 * 512, kALo = 6 * 512, kPLo = 10 * 512;
-        const float2 beta[2] = {*reinterpret_cast<const float2*>(&bt[warp * 16 + 2 * t]),
-                                *reinterpret_cast<const float2*>(&bt[warp * 16 + 8 + 2 * t])};
-        auto put_block = [&](int row0, const float (&y)[2][4]) {      // times beta, into columns of this warp
+    Split4 xb[4];
+    const uint32_t as = smem_u32(a_blk), ps = smem_u32(p_blk), xs = smem_u32(x_blk);
+    constexpr uint32_t kXLo = 4 * 512, kALo = 6 * 512, kPLo = 10 * 512;
+    const float2 beta[2] = {*reinterpret_cast<const float2*>(&bt[warp * 16 + 2 * t]),
+                            *reinterpret_cast<const float2*>(&bt[warp * 16 + 8 + 2 * t])};
+    auto put_block = [&](int which, int row0, const float (&y)[2][4]) {      // times beta, into columns of this warp
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    uint32_t x, z;
-                    split_scaled(y[q][e] * beta[q].x, y[q][e + 1] * beta[q].y, x, z);
-                    const uint32_t at = sw128(row0 + g + e * 4, warp * 16 + q * 8 + 2 * t);
-                    *reinterpret_cast<uint32_t*>(image + at) = x;
-                    *reinterpret_cast<uint32_t*>(image + kImageLo + at) = z;
-                }
-        };
-        ldsm4_t(xb[0].hi, xs + warp * 512 + lane * 16);
-        ldsm4_t(xb[0].lo, xs + kXLo + warp * 512 + lane * 16);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int i = warp + s;         // block row
-            if (i > 3) break;
-            if (s > 0) {
-                float y[2][4] = {}, yl[2][4] = {};
-#pragma unroll
-                for (int l = 0; l < s; ++l) {
-                    Split4 m;
-                    const uint32_t at = as + (i * (i - 1) / 2 + warp + l) * 512 + lane * 16;
-                    ldsm4(m.hi, at);
-                    ldsm4(m.lo, at + kALo);
-                    mma_split(y, yl, m, xb[l]);
-                }
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[q][e] += kLoInv * yl[q][e];
-                Split4 yb, m;
-                to_b(yb, y);
-                ldsm4(m.hi, xs + i * 512 + lane * 16);
-                ldsm4(m.lo, xs + kXLo + i * 512 + lane * 16);
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[q][e] = yl[q][e] = 0.0f;
-                mma_split(y, yl, m, yb);
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[q][e] = -(y[q][e] + kLoInv * yl[q][e]);
-                put_block(i * 16, y);
-                to_b(xb[s], y);
+            for (int e = 0; e < 4; e += 2) {
+                uint32_t x, z;
+                split_scaled(y[q][e] * beta[q].x, y[q][e + 1] * beta[q].y, x, z);
+                const int at = tri_at(row0 + g + e * 4, warp * 16 + q * 8 + 2 * t);
+                *reinterpret_cast<uint32_t*>(&out.tp[0][which][at]) = x;
+                *reinterpret_cast<uint32_t*>(&out.tp[1][which][at]) = z;
             }
+    };
+    ldsm4_t(xb[0].hi, xs + warp * 512 + lane * 16);
+    ldsm4_t(xb[0].lo, xs + kXLo + warp * 512 + lane * 16);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const int i = warp + s;         // block row
+        if (i > 3) break;
+        if (s > 0) {
             float y[2][4] = {}, yl[2][4] = {};
 #pragma unroll
-            for (int l = 0; l <= s; ++l) {
+            for (int l = 0; l < s; ++l) {
                 Split4 m;
-                const uint32_t at = ps + (i * (i + 1) / 2 + warp + l) * 512 + lane * 16;
+                const uint32_t at = as + (i * (i - 1) / 2 + warp + l) * 512 + lane * 16;
                 ldsm4(m.hi, at);
-                ldsm4(m.lo, at + kPLo);
+                ldsm4(m.lo, at + kALo);
                 mma_split(y, yl, m, xb[l]);
             }
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[q][e] += kLoInv * yl[q][e];
-            put_block(64 + i * 16, y);
-        }
-    }
-    __syncthreads();
-    uint4* to = reinterpret_cast<uint4*>(out.tp);
+            Split4 yb, m;
+            to_b(yb, y);
+            ldsm4(m.hi, xs + i * 512 + lane * 16);
+            ldsm4(m.lo, xs + kXLo + i * 512 + lane * 16);
 #pragma unroll
-    for (int i = 0; i < 2 * kImageLo / 16 / 128; ++i) to[i * 128 + tid] = reinterpret_cast<const uint4*>(image)[i * 128 + tid];
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[q][e] = yl[q][e] = 0.0f;
+            mma_split(y, yl, m, yb);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[q][e] = -(y[q][e] + kLoInv * yl[q][e]);
+            put_block(0, i * 16, y);
+            to_b(xb[s], y);
+        }
+        float y[2][4] = {}, yl[2][4] = {};
+#pragma unroll
+        for (int l = 0; l <= s; ++l) {
+            Split4 m;
+            const uint32_t at = ps + (i * (i + 1) / 2 + warp + l) * 512 + lane * 16;
+            ldsm4(m.hi, at);
+            ldsm4(m.lo, at + kPLo);
+            mma_split(y, yl, m, xb[l]);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[q][e] += kLoInv * yl[q][e];
+        put_block(1, i * 16, y);
+    }
 }
 
-// The walk, on the tcgen05 tensor cores.  A group of eight warps owns CW value
-// columns of a head; a block has NG groups, which share the chunk's tiles, and four
-// warps that load them ahead.  Per chunk and group three products, each with M =
-// 128 rows and N = 2 CW columns (the hi and the lo half of a split operand side by
-// side, so that the other operand is read once for both):
-//   D1 = [K; Q] S0        rows 0-63 give R = V - diag(ck) K S0, rows 64-127 the outputs' first part
-//   D2 = [T; P T] R       rows 0-63 give U, rows 64-127 the outputs' second part
-//   D3 = K^T diag(cs) U   the state's new part; K's tile serves as its own transpose (M-major operand)
-// A row of a product belongs to one thread of each of the group's two
-// warpgroups (half of the columns each), so every scale is a thread's own and the
-// state stays in registers, CW / 2 values per thread.  Between products only R, U
-// or S goes through shared memory, in the layout of the next B operand.
-//
-// A walk's speed is this chain, not its operations: three times issue, MMA (about
-// 32 clocks per 16 of K, the reading of the 128-row operand) and a pass over the
-// accumulator.  So a small call takes CW = 16 (most blocks), a large one two groups
-// of 32 columns per block, whose chains interleave on one tensor core.
-template <int DK, int CW, int NG>
-struct Walk {
+// The walk.  Eight warps own 16 value columns of a head: four carry the state
+// (each a quarter of its rows, in registers), four make the outputs; a block
+// has NG such groups, which share the chunk's tiles, and four warps that load the
+// next chunk's while this one's are in use.  All products are taken
+// transposed, with the 16 columns as the MMA's m:
+//   R^T = V^T - (S0^T K^T) diag(ck);  U^T = R^T T^T;  S'^T = keep S0^T + (U^T diag(cs)) K
+// by the state's warps, each for 16 tokens or a quarter of the rows, with R, U
+// and S changing hands through shared memory, and beside them
+//   O^T = (S0^T Q^T) diag(cq) + R^T (P T)^T.
+// A product of S waits for the chunk before it, so a walk's speed is this chain of
+// three small products, not its operations; taking the outputs out of it and
+// keeping 16 columns a group makes it as short as the MMA allows.  Warp w and
+// the output warp beside it on the same scheduler take tokens 16 w and 16 (3 - w), so
+// that the triangles' work adds up to the same on each.
+template <int DK, int NG>
+struct Scan {
     static constexpr int kThreads = NG * 256 + 128;
-    static constexpr int kSub = DK / 64;                   // 64 columns of K, Q: one 128-byte tile
-    static constexpr int kTile = 128 * 128;                // 128 rows of 128 bytes
-    static constexpr int kRec = kSub * kTile;              // offset of the chunk's record in a stage
-    static constexpr int kVRow = NG * CW * 2;
-    static constexpr int kV = kRec + sizeof(Chunk);
-    static constexpr int kStage = (kV + kChunk * kVRow + 1023) / 1024 * 1024;
-    static constexpr int kBTile = 2 * CW * 128;            // a B operand with K = 64
-    static constexpr int kGroup = (kSub + 1) * kBTile;     // S, then R and U in turn
-    static constexpr int kStages = NG * CW == 16 ? 3 : 2;
-    static constexpr int kSmem = kStages * kStage + NG * kGroup + 1024;
-    static constexpr int kAcc = 2 * CW;                    // tensor-memory columns of an accumulator
-    static constexpr int kTmem = NG * 3 * kAcc <= 128 ? 128 : (NG * 3 * kAcc <= 256 ? 256 : 512);
-    static_assert(kSmem <= 232448 - 256, "shared memory");
+    static constexpr int kTile = kChunk * DK * 2;
+    static constexpr int kRecord = 2 * kTile;
+    static constexpr int kLoPart = 2 * kTri * 2;                 // from the record's hi to its lo
+    static constexpr int kScales = kRecord + 2 * kLoPart;
+    static constexpr int kV = kRecord + sizeof(Chunk);
+    static constexpr int kStage = kV + kChunk * NG * 32;
+    static constexpr int kSx = 16 * DK * 2;
+    static constexpr int kRx = 16 * kChunk * 2;
+    static constexpr int kGroup = 2 * kSx + 4 * kRx;
+    static constexpr int kSmem = 2 * kStage + NG * kGroup;
 };
 
-// CT consecutive fp32 columns of this warp's 32 lanes.
-template <int CT>
-__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[CT]) {
-    static_assert(CT == 8 || CT == 16, "");
-    uint32_t r[CT];
-    if constexpr (CT == 8)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                     : "r"(addr));
-    else
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-            : "r"(addr));
-#pragma unroll
-    for (int i = 0; i < CT; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-template <int DK, int CW, int NG>
-__global__ void __launch_bounds__(NG * 256 + 128, 1) walk_kernel(const DeltaArgs a, const Chunk* chunks) {
-    using C = Walk<DK, CW, NG>;
+template <int DK, int NG>
+__global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs a, const Chunk* chunks) {
+    using C = Scan<DK, NG>;
     constexpr int kVecs = DK / 8;
-    constexpr int CT = CW / 2;        // columns of a thread
-    extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], made[NG];
-    __shared__ uint32_t tmem_slot;
-    const int tid = threadIdx.x, lane = tid & 31;
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
-    if (tid < 32) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
-                     "r"(C::kTmem)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    if (tid == 32) {
-        for (int i = 0; i < C::kStages; ++i) {
-            mbar_init(&full[i], 129);      // the loading threads, and the announcement of the bulk copy
-            mbar_init(&empty[i], NG);
-        }
-        for (int i = 0; i < NG; ++i) mbar_init(&made[i], 1);
+    constexpr int kN = DK / 32;       // n8 tiles of a state warp's rows
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t landed[2];
+    if (threadIdx.x == 0) {
+        mbar_init(&landed[0], 1);
+        mbar_init(&landed[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    pdl_trigger();
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    pdl_trigger();
     pdl_wait();
-
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int g = lane >> 2, t = lane & 3;
     const int h = blockIdx.y, b = blockIdx.z;
-    const int col0 = blockIdx.x * NG * CW;
-    int begin = 0, end = 0, slot = 0;
-    const bool valid = sequence(a, b, begin, end, slot);
-    const int chunks_here = valid ? (end - begin + kChunk - 1) / kChunk : 0;
-    // Every wait is bounded.  A thread whose wait gave up records it and goes on
-    // without waiting, so that all barriers still meet and the block ends.
-    bool dead = false;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity)) {
-            dead = true;
-            atomicOr(&g_gated_delta_dev_error, kDevErrTimeout);
-        }
-    };
-    auto arrive = [](uint64_t* bar) {
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-    };
+    const int col0 = blockIdx.x * NG * 16;
+    int begin, end, slot;
+    if (!sequence(a, b, begin, end, slot)) return;
+    const int chunks_here = (end - begin + kChunk - 1) / kChunk;
+    const uint32_t base = smem_u32(smem);
 
     if (tid >= NG * 256) {
-        // ---- the loading warps ----
+        // ---- the loading warps: one chunk ahead ----
         constexpr int kStep = 128 / kVecs;           // rows of one sweep of the 128 threads; a multiple of 8,
         static_assert(kStep % 8 == 0, "swizzle");    // so a thread keeps its place in the swizzle
         const int kh = h / a.share, lt = tid - NG * 256;
@@ -646,233 +580,297 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) walk_kernel(const DeltaArgs
         const __half* qp = a.q + static_cast<int64_t>(begin + lr) * a.q_ts + kh * a.q_hs + lx * 8;
         const int64_t k_step = kStep * a.k_ts, q_step = kStep * a.q_ts;
         const Chunk* rec = chunks + first_chunk(begin, b) * a.v_heads + h;
+        bool dead = false;
         for (int c = 0; c < chunks_here; ++c) {
-            const int st = c % C::kStages;
-            if (c >= C::kStages) wait(&empty[st], (c / C::kStages - 1) & 1);
-            const uint32_t stage = base + st * C::kStage;
+            const uint32_t stage = base + (c & 1) * C::kStage;
             if (lt == 0) {
-                mbar_expect_tx(&full[st], sizeof(Chunk));
-                bulk_load(smem + st * C::kStage + C::kRec, rec, sizeof(Chunk), &full[st]);
+                fence_proxy_async_smem();      // the stage's reads come before the copy into it
+                mbar_expect_tx(&landed[c & 1], kChunkBytes);
+                bulk_load(smem + (c & 1) * C::kStage + C::kRecord, rec, kChunkBytes, &landed[c & 1]);
             }
             rec += a.v_heads;
-            const uint32_t dst = stage + (lx >> 3) * C::kTile + sw128(lr, (lx & 7) * 8);
+            const uint32_t dst = tile_at<kVecs>(stage, lr, lx);
             const int t0 = begin + c * kChunk;
             const int n = min(kChunk, end - t0);
 #pragma unroll
             for (int i = 0; i < kChunk / kStep; ++i) {
                 const bool ok = i * kStep + lr < n;
-                cp_async16_or_zero(dst + i * kStep * 128, ok ? kp : a.k, ok);
-                cp_async16_or_zero(dst + (kChunk + i * kStep) * 128, ok ? qp : a.q, ok);
+                cp_async16_or_zero(dst + i * kStep * kVecs * 16, ok ? kp : a.k, ok);
+                cp_async16_or_zero(dst + i * kStep * kVecs * 16 + C::kTile, ok ? qp : a.q, ok);
                 kp += k_step;
                 qp += q_step;
             }
-            constexpr int kVV = NG * CW / 8;      // 16-byte vectors of a row of V
 #pragma unroll
-            for (int i = 0; i < kChunk * kVV / 128; ++i) {
-                const int item = i * 128 + lt, r = item / kVV, x = item % kVV;
+            for (int i = 0; i < NG; ++i) {
+                const int item = i * 128 + lt, r = item / (2 * NG), x = item % (2 * NG);
                 const bool ok = r < n && col0 + x * 8 < a.dv;
-                cp_async16_or_zero(tile_at<kVV>(stage + C::kV, r, x),
+                cp_async16_or_zero(tile_at<2 * NG>(stage + C::kV, r, x),
                                    ok ? a.v + static_cast<int64_t>(t0 + r) * a.v_ts + h * a.v_hs + col0 + x * 8 : a.v, ok);
             }
             cp_async_commit();
             cp_async_wait<0>();
-            fence_proxy_async_smem();      // the MMAs read through the async proxy
-            arrive(&full[st]);
-        }
-        // bulk copies land before the block's shared memory goes
-        if (lt == 0)
-            for (int c = max(0, chunks_here - C::kStages); c < chunks_here; ++c) wait(&full[c % C::kStages], (c / C::kStages) & 1);
-    } else {
-        const int group = tid >> 8, gt = tid & 255, half = gt >> 7, quarter = (tid >> 5) & 3;
-        const int row = quarter * 32 + lane;          // of every product
-        const int tok = row & 63;
-        const bool state_row = quarter < 2;           // of D1 and D2: a token's state part, or its output part
-        const int colg = group * CW + half * CT;      // first column of this thread within the block
-        const int col = col0 + colg;
-        const bool live = col < a.dv;                 // value_dim is a multiple of 16: CT columns are in or out together
-        const uint32_t bt = base + C::kStages * C::kStage + group * C::kGroup, rt = bt + C::kSub * C::kBTile;
-        const uint32_t acc = tmem + group * 3 * C::kAcc;
-        const uint32_t acc_lane = acc + (static_cast<uint32_t>(quarter * 32) << 16) + half * CT;
-        auto rows_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + 2 * group) : "memory"); };
-        auto group_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(2 + 2 * group) : "memory"); };
-        // a split value as element k of rows n (hi) and CW + n (lo) of a B tile
-        auto put = [&](uint32_t tile, int n, int k, float x) {
-            const __half hi = __float2half_rn(x);
-            const __half lo = __float2half_rn((x - __half2float(hi)) * kLo);
-            const uint32_t at = tile + sw128(n, k);
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(__half_as_ushort(hi)) : "memory");
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + CW * 128), "h"(__half_as_ushort(lo)) : "memory");
-        };
-        // a product's hi + 2^-11 lo for this thread's row and columns
-        auto take = [&](int d, float (&x)[CT]) {
-            float lo[CT];
-            tmem_ld<CT>(acc_lane + d * C::kAcc, x);
-            tmem_ld<CT>(acc_lane + d * C::kAcc + CW, lo);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < CT; ++i) x[i] += kLoInv * lo[i];
-        };
-
-        // this thread's row of the state
-        float s[CT];
-        const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + row) * a.dv + col;
-        const bool has_state = row < DK && live && valid;
-#pragma unroll
-        for (int i = 0; i < CT; i += 4) {
-            const float4 x = a.state_in && has_state ? *reinterpret_cast<const float4*>(a.state_in + at + i)
-                                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            s[i] = x.x, s[i + 1] = x.y, s[i + 2] = x.z, s[i + 3] = x.w;
-        }
-        auto put_state = [&]() {
-            if (row < DK) {
-#pragma unroll
-                for (int i = 0; i < CT; ++i) put(bt + (row >> 6) * C::kBTile, half * CT + i, row & 63, s[i]);
+            if (lt == 0 && !dead && !mbar_wait(&landed[c & 1], (c >> 1) & 1)) {
+                dead = true;      // gives up waiting, not the barriers: the block still ends
+                atomicOr(&g_gated_delta_dev_error, kDevErrTimeout);
             }
-            fence_proxy_async_smem();
-            tc_fence_before();
-            group_sync();
-        };
-        put_state();
-
-        constexpr uint32_t kWide = instr_desc_f16(128, 2 * CW), kNarrow = instr_desc_f16(128, CW);
-        constexpr uint32_t kMajorM = kWide | (1u << 15);      // A stored with M contiguous
-        uint32_t phase = 0;
-        for (int c = 0; c < chunks_here; ++c) {
-            const int st = c % C::kStages;
-            const uint32_t stage = base + st * C::kStage;
-            const float* scales = reinterpret_cast<const float*>(smem + st * C::kStage + C::kRec + sizeof(__half) * 2 * 128 * kChunk);
-            wait(&full[st], (c / C::kStages) & 1);
-            if (gt == 0) {
-                tc_fence_after();
-#pragma unroll
-                for (int j = 0; j < DK / 16; ++j)
-                    mma_f16_ss(acc, smem_desc_sw128(stage + (j / 4) * C::kTile + (j % 4) * 32),
-                               smem_desc_sw128(bt + (j / 4) * C::kBTile + (j % 4) * 32), kWide, j > 0);
-                mma_commit(&made[group]);
-            }
-            __syncwarp();
-            // what the pass over D1 needs, while the MMAs run
-            const float scale = scales[(state_row ? 0 : kChunk) + tok], cs = scales[2 * kChunk + tok], keep = scales[3 * kChunk];
-            uint4 vv[CT / 8];
-#pragma unroll
-            for (int i = 0; i < CT / 8; ++i)
-                vv[i] = *reinterpret_cast<const uint4*>(smem + (tile_at<NG * CW / 8>(stage + C::kV, tok, colg / 8 + i) - base));
-            wait(&made[group], phase);
-            phase ^= 1;
-            __syncwarp();
-            tc_fence_after();
-            float x[CT], o[CT];
-            take(0, x);
-            tc_fence_before();
-            if (state_row) {
-#pragma unroll
-                for (int i = 0; i < CT; i += 2) {
-                    const float2 v = __half22float2(u32_as_h2((&vv[i / 8].x)[(i & 7) / 2]));
-                    put(rt, half * CT + i, tok, v.x - scale * x[i]);
-                    put(rt, half * CT + i + 1, tok, v.y - scale * x[i + 1]);
-                }
-                fence_proxy_async_smem();
-                rows_sync();
-                if (gt == 0) {
-                    tc_fence_after();
-                    const uint32_t tp = stage + C::kRec;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint64_t r = smem_desc_sw128(rt + j * 32);
-                        mma_f16_ss(acc + C::kAcc, smem_desc_sw128(tp + j * 32), r, kWide, j > 0);
-                        mma_f16_ss(acc + C::kAcc + CW, smem_desc_sw128(tp + C::kTile + j * 32), r, kNarrow, 1);
-                    }
-                    mma_commit(&made[group]);
-                }
-                __syncwarp();
-            } else {
-#pragma unroll
-                for (int i = 0; i < CT; ++i) o[i] = scale * x[i];
-            }
-            wait(&made[group], phase);
-            phase ^= 1;
-            __syncwarp();
-            tc_fence_after();
-            take(1, x);
-            tc_fence_before();
-            if (state_row) {
-#pragma unroll
-                for (int i = 0; i < CT; ++i) put(rt, half * CT + i, tok, cs * x[i]);
-                fence_proxy_async_smem();
-                rows_sync();
-                if (gt == 0) {
-                    tc_fence_after();
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        // K^T: blocks of 64 rows lie a tile apart (with 64 of them, the second block is Q's, its
-                        // results unused), groups of 8 tokens 1024 bytes
-                        const uint64_t kt = (smem_desc_sw128(stage + j * 2048) & ~(static_cast<uint64_t>(0x3fff) << 16)) |
-                                            (static_cast<uint64_t>((C::kSub == 2 ? C::kTile : 8192) >> 4) << 16);
-                        mma_f16_ss(acc + 2 * C::kAcc, kt, smem_desc_sw128(rt + j * 32), kMajorM, j > 0);
-                    }
-                    mma_commit(&made[group]);
-                }
-                __syncwarp();
-            } else {
-                const int token = begin + c * kChunk + tok;
-                if (live && token < end) {
-                    uint32_t r[CT / 2];
-#pragma unroll
-                    for (int i = 0; i < CT; i += 2) r[i / 2] = h2_as_u32(__floats2half2_rn(o[i] + x[i], o[i + 1] + x[i + 1]));
-                    uint4* to = reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(token) * a.v_heads + h) * a.dv + col);
-#pragma unroll
-                    for (int i = 0; i < CT / 8; ++i) to[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
-                }
-            }
-            wait(&made[group], phase);
-            phase ^= 1;
-            __syncwarp();
-            tc_fence_after();
-            take(2, x);
-#pragma unroll
-            for (int i = 0; i < CT; ++i) s[i] = keep * s[i] + x[i];
-            put_state();
-            if (gt == 0) arrive(&empty[st]);
+            __syncthreads();   // chunk c is there, and c - 1 is done with
         }
-        if (a.state_out && has_state) {
-#pragma unroll
-            for (int i = 0; i < CT; i += 4)
-                *reinterpret_cast<float4*>(a.state_out + at + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
-        }
+        return;
     }
-    tc_fence_before();
-    __syncthreads();
-    if (tid < 32)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+
+    const int group = tid >> 8, warp = (tid >> 5) & 3;
+    const bool outputs = (tid >> 7) & 1;
+    const int col = col0 + group * 16;
+    const bool live = col < a.dv;
+    const uint32_t s_hi = base + 2 * C::kStage + group * C::kGroup, s_lo = s_hi + C::kSx, r_hi = s_lo + C::kSx,
+                   r_lo = r_hi + C::kRx, w_hi = r_lo + C::kRx, w_lo = w_hi + C::kRx;
+    const int blk = outputs ? 3 - warp : warp;       // this warp's 16 tokens of a chunk
+    const int a_row = lane & 15, a_vec = lane >> 4;                                // A operand
+    const int b_row = (lane & 7) + (lane >> 4) * 8, b_vec = (lane >> 3) & 1;       // B operand, rows = n
+    // this warp's block row of a triangle of the record: its start, and the lane's row address in a 16x16 block
+    const uint32_t tri_row = 2 * blk * (blk + 1) * 128 + (lane >> 4) * (2 * blk + 2) * 128 + ((lane >> 3) & 1) * 128 + (lane & 7) * 16;
+    auto state_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + 2 * group) : "memory"); };
+    auto group_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(2 + 2 * group) : "memory"); };
+    auto scale_pair = [&](uint32_t sc, int which, int n) {
+        float2 x;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(x.x), "=f"(x.y)
+                     : "r"(sc + (which * kChunk + blk * 16 + n * 8 + 2 * t) * 4));
+        return x;
+    };
+    auto put = [&](uint32_t at, uint32_t x) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); };
+
+    if (outputs) {
+        for (int c = 0; c < chunks_here; ++c) {
+            __syncthreads();
+            const uint32_t stage = base + (c & 1) * C::kStage, sc = stage + C::kScales;
+            const uint32_t p_hi = stage + C::kRecord + kTri * 2 + tri_row;
+            float o[2][4], ol[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][e] = ol[n][e] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < DK / 16; ++kk) {
+                uint32_t sh[4], sl[4], qf[4];
+                ldsm4(sh, tile_at<kVecs>(s_hi, a_row, kk * 2 + a_vec));
+                ldsm4(sl, tile_at<kVecs>(s_lo, a_row, kk * 2 + a_vec));
+                ldsm4(qf, tile_at<kVecs>(stage + C::kTile, blk * 16 + b_row, kk * 2 + b_vec));
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma16816(o[n], sh, qf[2 * n], qf[2 * n + 1]);
+                    mma16816(ol[n], sl, qf[2 * n], qf[2 * n + 1]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float2 cq = scale_pair(sc, 1, n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[n][e] = (e & 1 ? cq.y : cq.x) * (o[n][e] + kLoInv * ol[n][e]);
+                    ol[n][e] = 0.0f;
+                }
+            }
+            group_sync();       // R is there, and S0 has been read
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j > blk) break;
+                uint32_t rh[4], rl[4], ph[4], pl[4];
+                ldsm4(rh, tile_at<8>(r_hi, a_row, j * 2 + a_vec));
+                ldsm4(rl, tile_at<8>(r_lo, a_row, j * 2 + a_vec));
+                ldsm4(ph, p_hi + j * 256);
+                ldsm4(pl, p_hi + C::kLoPart + j * 256);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma16816(o[n], rh, ph[2 * n], ph[2 * n + 1]);
+                    mma16816(ol[n], rl, ph[2 * n], ph[2 * n + 1]);
+                    mma16816(ol[n], rh, pl[2 * n], pl[2 * n + 1]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int tok = begin + c * kChunk + blk * 16 + n * 8 + g;
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    // 8x8 transpose: lane (g, t) then has token g, columns 2t, 2t + 1
+                    const uint32_t r = movm_t(h2_as_u32(__floats2half2_rn(o[n][e] + kLoInv * ol[n][e],
+                                                                           o[n][e + 1] + kLoInv * ol[n][e + 1])));
+                    if (live && tok < end)
+                        *reinterpret_cast<uint32_t*>(a.out + (static_cast<int64_t>(tok) * a.v_heads + h) * a.dv + col +
+                                                     e * 4 + 2 * t) = r;
+                }
+            }
+        }
+        return;
+    }
+
+    // ---- the state's warps ----
+    // S^T as C fragments: rows (columns of the state) g, g + 8, columns (its rows)
+    // warp * DK / 4 + 8 n + 2t, + 1
+    float s[kN][4];
+    const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + warp * (DK / 4) + 2 * t) * a.dv + col + g;
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            s[n][e] = a.state_in && live ? a.state_in[at + static_cast<int64_t>(n * 8 + (e & 1)) * a.dv + (e >> 1) * 8] : 0.0f;
+    auto put_state = [&]() {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                uint32_t hi, lo;
+                split_scaled(s[n][e], s[n][e + 1], hi, lo);
+                put(tile_at<kVecs>(s_hi, g + e * 4, warp * kN + n) + t * 4, hi);
+                put(tile_at<kVecs>(s_lo, g + e * 4, warp * kN + n) + t * 4, lo);
+            }
+    };
+    auto put_rows = [&](uint32_t hi_at, uint32_t lo_at, const float (&x)[2][4]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                uint32_t hi, lo;
+                split_scaled(x[n][e], x[n][e + 1], hi, lo);
+                put(tile_at<8>(hi_at, g + e * 4, warp * 2 + n) + t * 4, hi);
+                put(tile_at<8>(lo_at, g + e * 4, warp * 2 + n) + t * 4, lo);
+            }
+    };
+    put_state();
+    for (int c = 0; c < chunks_here; ++c) {
+        __syncthreads();
+        const uint32_t stage = base + (c & 1) * C::kStage, sc = stage + C::kScales;
+        const uint32_t t_hi = stage + C::kRecord + tri_row;
+
+        // S0^T K^T for this warp's tokens
+        float x[2][4], xl[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = xl[n][e] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; ++kk) {
+            uint32_t sh[4], sl[4], kf[4];
+            ldsm4(sh, tile_at<kVecs>(s_hi, a_row, kk * 2 + a_vec));
+            ldsm4(sl, tile_at<kVecs>(s_lo, a_row, kk * 2 + a_vec));
+            ldsm4(kf, tile_at<kVecs>(stage, blk * 16 + b_row, kk * 2 + b_vec));
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                mma16816(x[n], sh, kf[2 * n], kf[2 * n + 1]);
+                mma16816(xl[n], sl, kf[2 * n], kf[2 * n + 1]);
+            }
+        }
+        uint32_t vf[4];
+        ldsm4_t(vf, tile_at<2 * NG>(stage + C::kV, blk * 16 + b_row, group * 2 + b_vec));
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float2 ck = scale_pair(sc, 0, n);
+            const float2 v0 = __half22float2(u32_as_h2(vf[2 * n])), v1 = __half22float2(u32_as_h2(vf[2 * n + 1]));
+            x[n][0] = v0.x - ck.x * (x[n][0] + kLoInv * xl[n][0]);
+            x[n][1] = v0.y - ck.y * (x[n][1] + kLoInv * xl[n][1]);
+            x[n][2] = v1.x - ck.x * (x[n][2] + kLoInv * xl[n][2]);
+            x[n][3] = v1.y - ck.y * (x[n][3] + kLoInv * xl[n][3]);
+        }
+        put_rows(r_hi, r_lo, x);
+        group_sync();
+
+        // U^T = R^T T^T
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = xl[n][e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > blk) break;
+            uint32_t rh[4], rl[4], th[4], tl[4];
+            ldsm4(rh, tile_at<8>(r_hi, a_row, j * 2 + a_vec));
+            ldsm4(rl, tile_at<8>(r_lo, a_row, j * 2 + a_vec));
+            ldsm4(th, t_hi + j * 256);
+            ldsm4(tl, t_hi + C::kLoPart + j * 256);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                mma16816(x[n], rh, th[2 * n], th[2 * n + 1]);
+                mma16816(xl[n], rl, th[2 * n], th[2 * n + 1]);
+                mma16816(xl[n], rh, tl[2 * n], tl[2 * n + 1]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float2 cs = scale_pair(sc, 2, n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = (e & 1 ? cs.y : cs.x) * (x[n][e] + kLoInv * xl[n][e]);
+        }
+        put_rows(w_hi, w_lo, x);
+        state_sync();
+
+        // S'^T = keep S0^T + (U^T diag(cs)) K
+        float keep, sl[kN][4];
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(keep) : "r"(sc + 3 * kChunk * 4));
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] *= keep;
+                sl[n][e] = 0.0f;
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t wh[4], wl[4];
+            ldsm4(wh, tile_at<8>(w_hi, a_row, j * 2 + a_vec));
+            ldsm4(wl, tile_at<8>(w_lo, a_row, j * 2 + a_vec));
+#pragma unroll
+            for (int p = 0; p < kN / 2; ++p) {
+                uint32_t kf[4];
+                ldsm4_t(kf, tile_at<kVecs>(stage, j * 16 + a_row, warp * kN + p * 2 + a_vec));
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    mma16816(s[2 * p + n], wh, kf[2 * n], kf[2 * n + 1]);
+                    mma16816(sl[2 * p + n], wl, kf[2 * n], kf[2 * n + 1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] += kLoInv * sl[n][e];
+        put_state();
+    }
+    if (a.state_out && live) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                a.state_out[at + static_cast<int64_t>(n * 8 + (e & 1)) * a.dv + (e >> 1) * 8] = s[n][e];
+    }
 }
 
 int64_t chunk_slots(int64_t tokens, int64_t batch) { return tokens / kChunk + batch; }
 
-template <int DK, int CW, int NG>
-int launch_walk(const DeltaArgs& a, const Chunk* chunks, cudaStream_t stream) {
-    using C = Walk<DK, CW, NG>;
+template <int DK, int NG>
+int launch_scan(const DeltaArgs& a, const Chunk* chunks, cudaStream_t stream) {
+    using C = Scan<DK, NG>;
     static std::atomic<uint64_t> done{0};
-    const int st = allow_smem(walk_kernel<DK, CW, NG>, C::kSmem, done);
+    const int st = allow_smem(scan_kernel<DK, NG>, C::kSmem, done);
     if (st) return st;
-    return launch(walk_kernel<DK, CW, NG>, dim3((a.dv + NG * CW - 1) / (NG * CW), a.v_heads, a.batch), dim3(C::kThreads),
-                  C::kSmem, stream, a, chunks);
+    return launch(scan_kernel<DK, NG>, dim3((a.dv / 16 + NG - 1) / NG, a.v_heads, a.batch), dim3(C::kThreads), C::kSmem,
+                  stream, a, chunks);
 }
 
 template <int DK>
 int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     Chunk* chunks = static_cast<Chunk*>(workspace);
-    constexpr int kSmem = 32768;      // K and Q (at most 64 rows of 256 bytes each), then the record's image
+    // K and Q, then the blocks in their place
+    constexpr int kSmem = 2 * kChunk * DK * 2 > 24832 ? 2 * kChunk * DK * 2 : 24832;
     static std::atomic<uint64_t> done{0};
     int st = allow_smem(chunk_kernel<DK>, kSmem, done);
     if (st) return st;
     st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
-                kSmem, stream, a, chunks);
+                    kSmem, stream, a, chunks);
     if (st) return st;
-    // the narrowest blocks that still all run at once
-    const int64_t heads = static_cast<int64_t>(a.batch) * a.v_heads;
-    if (heads * ((a.dv + 15) / 16) <= sm_count()) return launch_walk<DK, 16, 1>(a, chunks, stream);
-    if (heads * ((a.dv + 31) / 32) <= sm_count()) return launch_walk<DK, 32, 1>(a, chunks, stream);
-    return launch_walk<DK, 32, 2>(a, chunks, stream);
+    // two column groups a block once single ones would not all run at once
+    const int64_t groups = static_cast<int64_t>(a.batch) * a.v_heads * (a.dv / 16);
+    if (groups > sm_count()) return launch_scan<DK, 2>(a, chunks, stream);
+    return launch_scan<DK, 1>(a, chunks, stream);
 }
 
 int fill_args(const char* who, const mcv_gated_delta* p, int64_t tokens, int64_t batch, DeltaArgs& a) {
