@@ -5,8 +5,10 @@
 // with q and k divided by sqrt(sum x^2 + eps) first when asked.  Value heads
 // h * v_heads / k_heads ... share key head h.
 #include "mixing.cuh"
+#include "tcgen05.cuh"
 
 #include <cmath>
+#include <cstdlib>
 
 namespace mcv {
 unsigned take_gated_delta_device_error();
@@ -183,22 +185,26 @@ __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uin
     lo = h2_as_u32(__floats2half2_rn((x - f.x) * kLo, (y - f.y) * kLo));
 }
 
-// One chunk's share of the workspace: T and P T, hi and lo, and the scales.  Of the
+// One chunk's share of the workspace: T and P T (its rows for q of norm 1 or less),
+// both at most 1 in magnitude and kept times 2^14 as hi + lo, and the scales.  Of the
 // two matrices only the 16x16 blocks on and below the diagonal are kept, as 8x8
 // matrices of 128 contiguous bytes, 2 i + 2 of them for each of the two groups of
 // eight rows of block row i: fragments are written and read whole, ldmatrix
 // hits no bank twice, and a chunk is one copy.
 constexpr int kTri = 40 * 64;        // elements of a triangle
+constexpr float kTriScale = 16384.0f;
 struct Chunk {
     __half tp[2][2][kTri];           // [hi, lo][T, P T]
     float ck[kChunk];                // e^G r_k
     float cq[kChunk];                // scale e^G r_q
-    float cs[kChunk];                // e^(G_C - G) r_k
+    float cs[kChunk];                // e^(G_C - G) r_k 2^-14
+    float oq[kChunk];                // scale r_q |q's row in P T|^-1 2^-14
     float keep;                      // e^G_C
     float pad[63];
 };
 static_assert(sizeof(Chunk) % 128 == 0, "chunks stay aligned");
-constexpr uint32_t kChunkBytes = 4 * kTri * 2 + (3 * kChunk + 4) * 4;      // in use
+constexpr uint32_t kTriBytes = 4 * kTri * 2, kScaleBytes = (4 * kChunk + 4) * 4;
+constexpr uint32_t kChunkBytes = kTriBytes + kScaleBytes;      // in use
 __host__ __device__ constexpr int tri_at(int r, int c) {
     const int i = r >> 4;
     return (2 * i * (i + 1) + ((r >> 3) & 1) * (2 * i + 2) + (c >> 3)) * 64 + (r & 7) * 8 + (c & 7);
@@ -265,8 +271,8 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
     __half* p_blk = a_blk + 2 * 6 * 256;                      // [2][10]: P on and below the diagonal
     __half* x_blk = p_blk + 2 * 10 * 256;                     // [2][4]: inverses of the diagonal blocks
     float* diag = reinterpret_cast<float*>(x_blk + 2 * 4 * 256);   // [4][16 * 17]: A's diagonal blocks
-    __shared__ float4 rows[kChunk];                         // G (two floats), r_k, r_q scale
-    __shared__ float bt[kChunk];
+    __shared__ float4 rows[kChunk];                         // G (two floats), r_k, r of q's row
+    __shared__ float bt[kChunk], qn[kChunk];                // beta; scale of an output over that of q's row
     pdl_trigger();
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -329,7 +335,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
         const int r = tid & 63;
         const uint32_t base = tid < 64 ? ks : qs;
         float sum[4] = {};
-        if (a.l2_eps >= 0.0f) {
+        if (a.l2_eps >= 0.0f || tid >= 64) {
 #pragma unroll
             for (int c = 0; c < kVecs; ++c) {
                 uint32_t x[4];
@@ -343,9 +349,15 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
                 }
             }
         }
-        float norm = a.l2_eps >= 0.0f ? 1.0f / sqrtf((sum[0] + sum[1]) + (sum[2] + sum[3]) + a.l2_eps) : 1.0f;
-        if (tid >= 64) norm *= a.scale;
-        (tid < 64 ? rows[r].z : rows[r].w) = r < n ? norm : 0.0f;
+        const float square = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (tid < 64) {
+            rows[r].z = r < n ? (a.l2_eps >= 0.0f ? 1.0f / sqrtf(square + a.l2_eps) : 1.0f) : 0.0f;
+        } else {
+            // P's rows are made for q of norm 1 or less, whether or not q is to be normalised
+            const float norm = a.l2_eps >= 0.0f ? sqrtf(square + a.l2_eps) : (square > 0.0f ? sqrtf(square) : 1.0f);
+            rows[r].w = r < n ? 1.0f / norm : 0.0f;
+            qn[r] = a.scale * (a.l2_eps >= 0.0f ? 1.0f : norm);
+        }
     }
     __syncthreads();
     Chunk& out = chunks[static_cast<int64_t>(blockIdx.x) * a.v_heads + h];
@@ -353,8 +365,9 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
         const float4 r = rows[tid], last = rows[kChunk - 1];
         const float eg = exp2f(r.x + r.y);
         out.ck[tid] = eg * r.z;
-        out.cq[tid] = eg * r.w;
-        out.cs[tid] = decay_between(make_float2(last.x, last.y), make_float2(r.x, r.y)) * r.z;
+        out.cq[tid] = eg * r.w * qn[tid];
+        out.cs[tid] = decay_between(make_float2(last.x, last.y), make_float2(r.x, r.y)) * r.z * (1.0f / kTriScale);
+        out.oq[tid] = qn[tid] * (1.0f / kTriScale);
         if (tid == kChunk - 1) out.keep = eg;
     }
 
@@ -437,11 +450,11 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
             __half hi16 = __float2half_rn(x[i]);
             x_blk[at] = hi16;
             x_blk[4 * 256 + at] = __float2half_rn((x[i] - __half2float(hi16)) * kLo);
-            const float y = x[i] * beta;
+            const float y = x[i] * beta * kTriScale;
             const int to = tri_at(warp * 16 + i, warp * 16 + lane);
             hi16 = __float2half_rn(y);
             out.tp[0][0][to] = hi16;
-            out.tp[1][0][to] = __float2half_rn((y - __half2float(hi16)) * kLo);
+            out.tp[1][0][to] = __float2half_rn(y - __half2float(hi16));
         }
     }
     __syncthreads();
@@ -450,15 +463,16 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
     Split4 xb[4];
     const uint32_t as = smem_u32(a_blk), ps = smem_u32(p_blk), xs = smem_u32(x_blk);
     constexpr uint32_t kXLo = 4 * 512, kALo = 6 * 512, kPLo = 10 * 512;
-    const float2 beta[2] = {*reinterpret_cast<const float2*>(&bt[warp * 16 + 2 * t]),
-                            *reinterpret_cast<const float2*>(&bt[warp * 16 + 8 + 2 * t])};
-    auto put_block = [&](int which, int row0, const float (&y)[2][4]) {      // times beta, into columns of this warp
+    float2 beta[2] = {*reinterpret_cast<const float2*>(&bt[warp * 16 + 2 * t]),
+                      *reinterpret_cast<const float2*>(&bt[warp * 16 + 8 + 2 * t])};
+    beta[0].x *= kTriScale, beta[0].y *= kTriScale, beta[1].x *= kTriScale, beta[1].y *= kTriScale;
+    auto put_block = [&](int which, int row0, const float (&y)[2][4]) {      // times beta 2^14, into columns of this warp
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
                 uint32_t x, z;
-                split_scaled(y[q][e] * beta[q].x, y[q][e + 1] * beta[q].y, x, z);
+                split_f16(y[q][e] * beta[q].x, y[q][e + 1] * beta[q].y, x, z);
                 const int at = tri_at(row0 + g + e * 4, warp * 16 + q * 8 + 2 * t);
                 *reinterpret_cast<uint32_t*>(&out.tp[0][which][at]) = x;
                 *reinterpret_cast<uint32_t*>(&out.tp[1][which][at]) = z;
@@ -645,11 +659,11 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
             __syncthreads();
             const uint32_t stage = base + (c & 1) * C::kStage, sc = stage + C::kScales;
             const uint32_t p_hi = stage + C::kRecord + kTri * 2 + tri_row;
-            float o[2][4], ol[2][4];
+            float o[2][4], ol[2][4], x[2][4];
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[n][e] = ol[n][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) o[n][e] = ol[n][e] = x[n][e] = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < DK / 16; ++kk) {
                 uint32_t sh[4], sl[4], qf[4];
@@ -682,19 +696,20 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
                 ldsm4(pl, p_hi + C::kLoPart + j * 256);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    mma16816(o[n], rh, ph[2 * n], ph[2 * n + 1]);
+                    mma16816(x[n], rh, ph[2 * n], ph[2 * n + 1]);
                     mma16816(ol[n], rl, ph[2 * n], ph[2 * n + 1]);
-                    mma16816(ol[n], rh, pl[2 * n], pl[2 * n + 1]);
+                    mma16816(x[n], rh, pl[2 * n], pl[2 * n + 1]);
                 }
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const int tok = begin + c * kChunk + blk * 16 + n * 8 + g;
+                const float2 oq = scale_pair(sc, 3, n);
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
                     // 8x8 transpose: lane (g, t) then has token g, columns 2t, 2t + 1
-                    const uint32_t r = movm_t(h2_as_u32(__floats2half2_rn(o[n][e] + kLoInv * ol[n][e],
-                                                                           o[n][e + 1] + kLoInv * ol[n][e + 1])));
+                    const uint32_t r = movm_t(h2_as_u32(__floats2half2_rn(o[n][e] + oq.x * (x[n][e] + kLoInv * ol[n][e]),
+                                                                           o[n][e + 1] + oq.y * (x[n][e + 1] + kLoInv * ol[n][e + 1]))));
                     if (live && tok < end)
                         *reinterpret_cast<uint32_t*>(a.out + (static_cast<int64_t>(tok) * a.v_heads + h) * a.dv + col +
                                                      e * 4 + 2 * t) = r;
@@ -791,7 +806,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
             for (int n = 0; n < 2; ++n) {
                 mma16816(x[n], rh, th[2 * n], th[2 * n + 1]);
                 mma16816(xl[n], rl, th[2 * n], th[2 * n + 1]);
-                mma16816(xl[n], rh, tl[2 * n], tl[2 * n + 1]);
+                mma16816(x[n], rh, tl[2 * n], tl[2 * n + 1]);
             }
         }
 #pragma unroll
@@ -805,7 +820,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 
         // S'^T = keep S0^T + (U^T diag(cs)) K
         float keep, sl[kN][4];
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(keep) : "r"(sc + 3 * kChunk * 4));
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(keep) : "r"(sc + 4 * kChunk * 4));
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -844,6 +859,459 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
     }
 }
 
+// ---- the same walk on the tcgen05 tensor cores, for many heads -----------------------
+//
+// One block per head (128 value columns), the columns as the MMA's M = 128 rows, so
+// that every product has N = 128 and runs at the tensor core's rate:
+//   D1 = S^T [K; Q]^T;  D2 = R^T [T; P T]^T;  D3 = W^T K  with W = diag(cs) U,
+// S^T as a tensor-memory operand, R^T and W^T in shared memory, K's tile of
+// tokens by rows serving both as [K; Q] and, read with N contiguous, as W's
+// factor.  A row of an accumulator, one value column, belongs to one thread of
+// each of two warpgroups (half of the tokens, half of the state's rows, in
+// registers), which turn D1 into R, D2 into W and D3 into the next S; a third
+// warpgroup writes the outputs from the other halves of D1 and D2 beside them; a
+// fourth loads the next chunk; one thread issues the MMAs, 16 of K at a time as
+// soon as that part of an operand is there.
+//
+// Here a split operand is hi + lo in one scale and one accumulator, so its row is
+// first multiplied by a power of two that puts a bound of the chunk's values at
+// 2^9: |S'|, |R| and |U| <= sqrt(Dk) max|S| + (C + 1) max|v| for the row (the
+// state's update is a contraction), with S taken a chunk earlier and that chunk's
+// C max|v| added, so that the bound is there before the state is.  Values
+// down to 2^-12 of it keep 22 bits, smaller ones an absolute 2^-34 of it; 2^6 above it
+// stays below fp16's end.
+template <int DK>
+struct Walk {
+    static constexpr int kLoaders = 96;           // three warps
+    static constexpr int kThreads = 512;          // state 8 warps, outputs 4, loading 3, MMA issue 1
+    static constexpr int kSub = DK / 64;          // 128-byte tiles of 64 dims
+    static constexpr int kTile = 128 * 128;
+    static constexpr int kTp = kSub * kTile;      // [K; Q], then [T; P T] hi, lo: 128 rows of 64, in 8x8 matrices
+    static constexpr int kV = kTp + 2 * kTile;    // 64 tokens of 128 values
+    static constexpr int kScales = kV + kChunk * 256;
+    static constexpr int kStage = kScales + 2048;
+    static constexpr int kR = 2 * kStage;         // R, then W: hi and lo tiles of 128 rows of 64 tokens
+    static constexpr int kSmem = kR + 2 * kTile + 1024;
+    static constexpr int kHalf = DK / 2;          // state rows of a thread
+    static constexpr int kBatches = kHalf / 16;
+    // tensor-memory columns
+    static constexpr uint32_t kD1 = 0, kD2 = 128, kD3 = 256, kSHi = 384, kSLo = 448;
+    static_assert(kScaleBytes <= 2048 && kSmem <= 232448 - 5120, "shared memory");
+};
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+// 16 columns of this warp's 32 lanes, to be waited for with tmem_wait.
+__device__ __forceinline__ void tmem_get(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+// Waits for all tmem_get so far; `r` are the ones used next.
+template <int N>
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// The power of two that takes a bound of a row's values to 2^9 .. 2^10, and its inverse.
+__device__ __forceinline__ float2 row_scale(float bound) {
+    const int e = min(max(136 - static_cast<int>((__float_as_uint(bound) >> 23) & 255u), -100), 100);
+    return make_float2(__uint_as_float(static_cast<uint32_t>(127 + e) << 23), __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
+}
+
+// K-major operand of 8x8 matrices of 128 bytes without swizzle: the next 8 of K 128
+// bytes on, the next 8 rows 1024.
+__device__ __forceinline__ uint64_t smem_desc_plain(uint32_t saddr) {
+    return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>(128 >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
+}
+
+template <int DK>
+__global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const DeltaArgs a, const Chunk* chunks) {
+    using C = Walk<DK>;
+    constexpr int kVecs = DK / 8;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t full[2], empty[2], s_ready[4], r_ready[2], w_ready[2], made[3], o_done, scaled;
+    __shared__ float2 most[3][2][128];      // [in turn][half][row]: max|S|, max|v|
+    __shared__ uint32_t tmem_slot;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
+    if (warp == 15) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&full[i], C::kLoaders + 1);      // the loading threads, and the announcement of the bulk copies
+            mbar_init(&empty[i], 13);      // state and output warps, and the MMAs
+            mbar_init(&r_ready[i], 8);
+            mbar_init(&w_ready[i], 8);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&s_ready[i], 8);
+        for (int i = 0; i < 3; ++i) mbar_init(&made[i], 1);
+        mbar_init(&o_done, 4);
+        mbar_init(&scaled, 8);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_trigger();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait();
+
+    const int h = blockIdx.y, b = blockIdx.z, col0 = blockIdx.x * 128;
+    int begin = 0, end = 0, slot = 0;
+    const bool valid = sequence(a, b, begin, end, slot);
+    const int chunks_here = valid ? (end - begin + kChunk - 1) / kChunk : 0;
+    // Every wait is bounded, by one lane for its warp.  A lane whose wait gave up
+    // records it and goes on without waiting, so that all barriers still meet
+    // and the block ends.
+    bool dead = false;
+    auto wait_one = [&](uint64_t* bar, uint32_t parity) {
+        if (!dead && !mbar_wait(bar, parity & 1)) {
+            dead = true;
+            atomicOr(&g_gated_delta_dev_error, kDevErrTimeout);
+        }
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (lane == 0) wait_one(bar, parity);
+        __syncwarp();
+    };
+    auto scales_of = [&](int c) { return reinterpret_cast<const float*>(smem + (c & 1) * C::kStage + C::kScales); };
+    // The k-th bound and its scale, k = 0 for the state at the start, c + 1 for chunk c; row_v: max|v| of the
+    // chunk before, taken along.
+    auto scale_of = [&](int k, int row, float& row_v) {
+        const float2 x = most[k % 3][0][row], y = most[k % 3][1][row];
+        const float v = fmaxf(x.y, y.y);
+        const float bound = (DK == 128 ? 11.4f : 8.1f) * fmaxf(x.x, y.x) + kChunk * row_v + (kChunk + 1) * v;
+        row_v = v;
+        return row_scale(bound);
+    };
+
+    if (warp < 8) {
+        // ---- the state ----
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int col = col0 + row;
+        const bool live = col < a.dv && valid;
+        const uint32_t lane_at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        float s[C::kHalf];
+        const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + half * C::kHalf) * a.dv + col;
+        float most_s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C::kHalf; ++i) {
+            s[i] = a.state_in && live ? a.state_in[at + static_cast<int64_t>(i) * a.dv] : 0.0f;
+            most_s = fmaxf(most_s, fabsf(s[i]));
+        }
+        // batch b of this half: 16 state rows, hi and lo, as tensor-memory operand
+        auto put_state = [&](int b, float scale) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) split_f16(s[b * 16 + 2 * i] * scale, s[b * 16 + 2 * i + 1] * scale, hi[i], lo[i]);
+            tmem_st8(lane_at + C::kSHi + half * (C::kHalf / 2) + b * 8, hi);
+            tmem_st8(lane_at + C::kSLo + half * (C::kHalf / 2) + b * 8, lo);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_ready[b]);
+        };
+        // 16 values of tokens half * 32 + 16 b .. as part of row `row` of the R / W tiles
+        auto put_row = [&](int b, const float (&x)[16], uint64_t* ready) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) split_f16(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t to = C::kR + row * 128 + (((half * 4 + b * 2 + i) ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(smem + to) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+                *reinterpret_cast<uint4*>(smem + to + C::kTile) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+            }
+            fence_proxy_async_smem();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ready[b]);
+        };
+        float row_v = 0.0f;
+        auto agree = [&](int k, float v) {      // with the thread of the other half; the outputs follow
+            most[k % 3][half][row] = make_float2(most_s, v);
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (lane == 0) mbar_arrive(&scaled);
+            return scale_of(k, row, row_v);
+        };
+        most[0][half][row] = make_float2(most_s, 0.0f);
+        asm volatile("bar.sync 3, 384;" ::: "memory");      // with the outputs
+        // this thread's 32 tokens of its value column
+        __half2 v[16];
+        auto load_v = [&](int c) {
+            wait(&full[c & 1], c >> 1);
+            const __half* p = reinterpret_cast<const __half*>(smem + (c & 1) * C::kStage + C::kV + half * 32 * 256) + row;
+            float most_v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                v[i] = __halves2half2(p[i * 256], p[i * 256 + 128]);
+                const float2 f = __half22float2(v[i]);
+                most_v = fmaxf(most_v, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+            return most_v;
+        };
+        float2 in_s = scale_of(0, row, row_v), now = in_s;      // scales of the state operand in use, of this chunk
+#pragma unroll
+        for (int b = 0; b < C::kBatches; ++b) put_state(b, in_s.x);
+        if (chunks_here > 0) now = agree(1, load_v(0));
+
+        for (int c = 0; c < chunks_here; ++c) {
+            const float* sc = scales_of(c);
+            const float keep = sc[4 * kChunk], f = now.x * in_s.y;
+            uint32_t d[2][16];
+            wait(&made[0], c);
+            tc_fence_after();
+            tmem_get(lane_at + C::kD1 + half * 32, d[0]);
+            tmem_get(lane_at + C::kD1 + half * 32 + 16, d[1]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                tmem_wait(d[b]);
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 ck = *reinterpret_cast<const float4*>(sc + half * 32 + b * 16 + i);
+                    const float2 v0 = __half22float2(v[b * 8 + i / 2]), v1 = __half22float2(v[b * 8 + i / 2 + 1]);
+                    x[i] = v0.x * now.x - ck.x * (f * __uint_as_float(d[b][i]));
+                    x[i + 1] = v0.y * now.x - ck.y * (f * __uint_as_float(d[b][i + 1]));
+                    x[i + 2] = v1.x * now.x - ck.z * (f * __uint_as_float(d[b][i + 2]));
+                    x[i + 3] = v1.y * now.x - ck.w * (f * __uint_as_float(d[b][i + 3]));
+                }
+                put_row(b, x, r_ready);
+            }
+            wait(&made[1], c);
+            tc_fence_after();
+            tmem_get(lane_at + C::kD2 + half * 32, d[0]);
+            tmem_get(lane_at + C::kD2 + half * 32 + 16, d[1]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                tmem_wait(d[b]);
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 cs = *reinterpret_cast<const float4*>(sc + 2 * kChunk + half * 32 + b * 16 + i);
+                    x[i] = cs.x * __uint_as_float(d[b][i]);
+                    x[i + 1] = cs.y * __uint_as_float(d[b][i + 1]);
+                    x[i + 2] = cs.z * __uint_as_float(d[b][i + 2]);
+                    x[i + 3] = cs.w * __uint_as_float(d[b][i + 3]);
+                }
+                put_row(b, x, w_ready);
+            }
+            if (lane == 0) mbar_arrive(&empty[c & 1]);
+            // while the last product is made: the next chunk's values and scale
+            float2 next = now;
+            if (c + 1 < chunks_here) next = agree(c + 2, load_v(c + 1));
+            wait(&made[2], c);
+            tc_fence_after();
+            most_s = 0.0f;
+            tmem_get(lane_at + C::kD3 + half * C::kHalf, d[0]);
+#pragma unroll
+            for (int b = 0; b < C::kBatches; ++b) {
+                tmem_wait(d[b & 1]);
+                if (b + 1 < C::kBatches) tmem_get(lane_at + C::kD3 + half * C::kHalf + (b + 1) * 16, d[(b + 1) & 1]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float& y = s[b * 16 + i];
+                    y = keep * y + now.y * __uint_as_float(d[b & 1][i]);
+                    most_s = fmaxf(most_s, fabsf(y));
+                }
+                put_state(b, now.x);
+            }
+            in_s = now;
+            now = next;
+        }
+        if (a.state_out && live) {
+#pragma unroll
+            for (int i = 0; i < C::kHalf; ++i) a.state_out[at + static_cast<int64_t>(i) * a.dv] = s[i];
+        }
+    } else if (warp < 12) {
+        // ---- the outputs ----
+        const int row = (warp & 3) * 32 + lane;
+        const int col = col0 + row;
+        const uint32_t lane_at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        float row_v = 0.0f;
+        asm volatile("bar.sync 3, 384;" ::: "memory");
+        float in_s = scale_of(0, row, row_v).y;
+        // "done" also says that the next chunk's scale has been seen, so the state cannot get ahead by two
+        if (chunks_here > 0) wait(&scaled, 0);
+        if (lane == 0) mbar_arrive(&o_done);
+        const int odd = lane & 1;
+        // two lanes swap values: the even one writes both columns of the first of two tokens, the odd one of the second
+        const int64_t step = 2 * static_cast<int64_t>(a.v_heads) * a.dv;
+        __half* to = a.out + ((static_cast<int64_t>(begin) + odd) * a.v_heads + h) * a.dv + (col & ~1);
+        for (int c = 0; c < chunks_here; ++c) {
+            const float* sc = scales_of(c);
+            wait(&full[c & 1], c >> 1);
+            const float in_r = scale_of(c + 1, row, row_v).y;
+            wait(&made[1], c);
+            tc_fence_after();
+            const int left = col < a.dv ? end - begin - c * kChunk - odd : 0;      // of this lane's tokens
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                uint32_t x[16], y[16];
+                tmem_get(lane_at + C::kD1 + 64 + b * 16, x);
+                tmem_get(lane_at + C::kD2 + 64 + b * 16, y);
+                tmem_wait(x);
+                tmem_wait(y);
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 cq = *reinterpret_cast<const float4*>(sc + kChunk + b * 16 + i);
+                    const float4 oq = *reinterpret_cast<const float4*>(sc + 3 * kChunk + b * 16 + i);
+                    const float* cp = &cq.x;
+                    const float* op = &oq.x;
+                    float o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[e] = cp[e] * (in_s * __uint_as_float(x[i + e])) + op[e] * (in_r * __uint_as_float(y[i + e]));
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float other = __shfl_xor_sync(0xffffffffu, odd ? o[e] : o[e + 1], 1);
+                        if (b * 16 + i + e < left)
+                            *reinterpret_cast<__half2*>(to) = odd ? __floats2half2_rn(other, o[e + 1]) : __floats2half2_rn(o[e], other);
+                        to += step;
+                    }
+                }
+            }
+            in_s = in_r;
+            if (c + 1 < chunks_here) wait(&scaled, c + 1);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&o_done);
+                mbar_arrive(&empty[c & 1]);
+            }
+        }
+    } else if (warp < 15) {
+        // ---- loading ----
+        const int kh = h / a.share, lt = tid - 12 * 32;
+        const __half* k0 = a.k + kh * a.k_hs;
+        const __half* q0 = a.q + kh * a.q_hs;
+        const __half* v0 = a.v + h * a.v_hs + col0;
+        const Chunk* rec = chunks + first_chunk(begin, b) * a.v_heads + h;
+        // 32 runs of 8x8 matrices (two parts, two matrices, eight groups of rows) from the record's packed
+        // triangles to their places among zeros, and the scales: eleven copies per warp, since a warp's
+        // lanes issue theirs one by one
+        const int run = (lt >> 5) * 11 + lane, part = run >> 4, which = (run >> 3) & 1, rg = run & 7;
+        const bool scales = run == 32;
+        const uint32_t run_to = scales ? C::kScales : C::kTp + part * C::kTile + (which * 8 + rg) * 1024;
+        const uint32_t run_bytes = scales ? kScaleBytes : (2 * (rg >> 1) + 2) * 128;
+        const uint32_t run_from = scales ? kTriBytes : ((part * 2 + which) * kTri + tri_at(rg * 8, 0)) * 2;
+        for (int i = lt; i < 2 * 2 * C::kTile / 16; i += C::kLoaders) {
+            const int st = i / (2 * C::kTile / 16), at = i % (2 * C::kTile / 16);
+            *reinterpret_cast<uint4*>(smem + st * C::kStage + C::kTp + at * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        asm volatile("bar.sync 2, 96;" ::: "memory");      // zeros first, copies behind them
+        for (int c = 0; c < chunks_here; ++c) {
+            const int st = c & 1;
+            if (c >= 2) wait(&empty[st], (c >> 1) - 1);
+            const uint32_t stage = base + st * C::kStage;
+            fence_proxy_async_smem();      // the stage's reads come before the copies into it
+            if (lt == 0) mbar_expect_tx(&full[st], kChunkBytes);
+            if (lane < 11) bulk_load(smem + st * C::kStage + run_to, reinterpret_cast<const char*>(rec) + run_from, run_bytes, &full[st]);
+            rec += a.v_heads;
+            const int t0 = begin + c * kChunk;
+            const int n = min(kChunk, end - t0);
+#pragma unroll 4
+            for (int i = lt; i < kChunk * kVecs; i += C::kLoaders) {
+                const int r = i / kVecs, x = i % kVecs;
+                const bool ok = r < n;
+                const int64_t tok = t0 + (ok ? r : 0);
+                const uint32_t dst = stage + (x >> 3) * C::kTile + r * 128 + (((x & 7) ^ (r & 7)) << 4);
+                cp_async16_or_zero(dst, k0 + tok * a.k_ts + x * 8, ok);
+                cp_async16_or_zero(dst + kChunk * 128, q0 + tok * a.q_ts + x * 8, ok);
+            }
+#pragma unroll 4
+            for (int i = lt; i < kChunk * 16; i += C::kLoaders) {
+                const int r = i >> 4, x = i & 15;
+                const bool ok = r < n && col0 + x * 8 < a.dv;
+                cp_async16_or_zero(stage + C::kV + r * 256 + x * 16, ok ? v0 + static_cast<int64_t>(t0 + r) * a.v_ts + x * 8 : a.v, ok);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_proxy_async_smem();      // the MMAs read through the async proxy
+            mbar_arrive(&full[st]);
+        }
+        // the bulk copies have landed before the block's shared memory goes
+        if (lane == 0)
+            for (int c = max(0, chunks_here - 2); c < chunks_here; ++c) wait_one(&full[c & 1], c >> 1);
+    } else if (lane == 0) {
+        // ---- MMA issue ----
+        constexpr uint32_t kIdesc = instr_desc_f16(128, 128), kIdescT = instr_desc_f16(128, DK) | (1u << 16);   // B with N contiguous
+        // descriptors count in 16 bytes; all are constants away from these
+        const uint64_t tiles = smem_desc_sw128(base), rh = smem_desc_sw128(base + C::kR), rl = rh + (C::kTile >> 4);
+        const uint64_t tri = smem_desc_plain(base + C::kTp);
+        // K by tokens: groups of eight 1024 bytes apart, the second 64 dims a tile on
+        const uint64_t turned = (tiles & ~(static_cast<uint64_t>(0x3fff) << 16)) | (static_cast<uint64_t>(C::kTile >> 4) << 16);
+        for (int c = 0; c < chunks_here; ++c) {
+            const uint64_t st = static_cast<uint64_t>((c & 1) * (C::kStage >> 4));
+            const uint64_t kq = tiles + st, tp = tri + st, kt = turned + st;
+            wait_one(&full[c & 1], c >> 1);
+            wait_one(&o_done, c);      // the outputs have read D1 and D2
+#pragma unroll
+            for (int b = 0; b < C::kBatches; ++b) {
+                wait_one(&s_ready[b], c);
+                tc_fence_after();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int k = half * C::kBatches + b;
+                    const uint64_t off = ((k / 4) * C::kTile + (k % 4) * 32) >> 4;
+                    mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, kq + off, kIdesc, b + half > 0);
+                    mma_f16_ts(tmem + C::kD1, tmem + C::kSLo + k * 8, kq + off, kIdesc, 1);
+                }
+            }
+            mma_commit(&made[0]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                wait_one(&r_ready[b], c);
+                tc_fence_after();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int k = half * 2 + b;
+                    mma_f16_ss(tmem + C::kD2, rh + k * 2, tp + k * 16, kIdesc, b + half > 0);
+                    mma_f16_ss(tmem + C::kD2, rl + k * 2, tp + k * 16, kIdesc, 1);
+                    mma_f16_ss(tmem + C::kD2, rh + k * 2, tp + (C::kTile >> 4) + k * 16, kIdesc, 1);
+                }
+            }
+            mma_commit(&made[1]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                wait_one(&w_ready[b], c);
+                tc_fence_after();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int k = half * 2 + b;
+                    mma_f16_ss(tmem + C::kD3, rh + k * 2, kt + k * 128, kIdescT, b + half > 0);
+                    mma_f16_ss(tmem + C::kD3, rl + k * 2, kt + k * 128, kIdescT, 1);
+                }
+            }
+            mma_commit(&made[2]);
+            mma_commit(&empty[c & 1]);
+        }
+        // every MMA has ended before its operands and tensor memory go
+        if (chunks_here > 0) wait_one(&made[2], chunks_here - 1);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+int g_force = getenv("MCV_FORCE") ? atoi(getenv("MCV_FORCE")) : 0;
 int64_t chunk_slots(int64_t tokens, int64_t batch) { return tokens / kChunk + batch; }
 
 template <int DK, int NG>
@@ -869,6 +1337,12 @@ int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     if (st) return st;
     // two column groups a block once single ones would not all run at once
     const int64_t groups = static_cast<int64_t>(a.batch) * a.v_heads * (a.dv / 16);
+    if (g_force == 3 || (g_force == 0 && groups > 2 * sm_count())) {
+        static std::atomic<uint64_t> done_walk{0};
+        if ((st = allow_smem(walk_kernel<DK>, Walk<DK>::kSmem, done_walk))) return st;
+        return launch(walk_kernel<DK>, dim3((a.dv + 127) / 128, a.v_heads, a.batch), dim3(Walk<DK>::kThreads), Walk<DK>::kSmem,
+                      stream, a, chunks);
+    }
     if (groups > sm_count()) return launch_scan<DK, 2>(a, chunks, stream);
     return launch_scan<DK, 1>(a, chunks, stream);
 }
