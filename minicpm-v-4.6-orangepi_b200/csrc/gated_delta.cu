@@ -179,10 +179,9 @@ constexpr int kChunk = 64;
 constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;
 
 __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = h2_as_u32(h);
-    lo = h2_as_u32(__floats2half2_rn((x - f.x) * kLo, (y - f.y) * kLo));
+    hi = h2_as_u32(__floats2half2_rn(x, y));
+    fma2_f16_f32(x, y, hi, 0xbc00bc00u);      // - 1 hi
+    lo = h2_as_u32(__floats2half2_rn(x * kLo, y * kLo));
 }
 
 // One chunk's share of the workspace: T and P T (its rows for q of norm 1 or less),
@@ -864,39 +863,43 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 // One block per head (128 value columns), the columns as the MMA's M = 128 rows, so
 // that every product has N = 128 and runs at the tensor core's rate:
 //   D1 = S^T [K; Q]^T;  D2 = R^T [T; P T]^T;  D3 = W^T K  with W = diag(cs) U,
-// S^T as a tensor-memory operand, R^T and W^T in shared memory, K's tile of
+// the left operands from tensor memory (S^T, then R^T and W^T in its place: a
+// shared-memory operand each side would take all of its bandwidth), K's tile of
 // tokens by rows serving both as [K; Q] and, read with N contiguous, as W's
-// factor.  A row of an accumulator, one value column, belongs to one thread of
-// each of two warpgroups (half of the tokens, half of the state's rows, in
-// registers), which turn D1 into R, D2 into W and D3 into the next S; a third
-// warpgroup writes the outputs from the other halves of D1 and D2 beside them; a
-// fourth loads the next chunk; one thread issues the MMAs, 16 of K at a time as
-// soon as that part of an operand is there.
+// factor.  The state itself lives in D3: keep S is put there before the product
+// adds to it.  A row of an accumulator, one value column, belongs to one
+// thread of each of four warpgroups (a quarter of the tokens and of the state's
+// rows each), which turn D1 into R, D2 into W and D3 into the next S; four warps
+// write the outputs from the other halves of D1 and D2 beside them, three load
+// the next chunk, one thread issues the MMAs, 16 of K at a time as soon as that
+// part of an operand is there.  The passes over the accumulators are what a chunk
+// waits for, so they are short rolled loops (straight code is fetched more slowly
+// than it runs) on many warps.
 //
-// Here a split operand is hi + lo in one scale and one accumulator, so its row is
-// first multiplied by a power of two that puts a bound of the chunk's values at
-// 2^9: |S'|, |R| and |U| <= sqrt(Dk) max|S| + (C + 1) max|v| for the row (the
-// state's update is a contraction), with S taken a chunk earlier and that chunk's
-// C max|v| added, so that the bound is there before the state is.  Values
-// down to 2^-12 of it keep 22 bits, smaller ones an absolute 2^-34 of it; 2^6 above it
-// stays below fp16's end.
+// Here a split operand is hi + lo in one scale and one accumulator, so a row's values
+// are first multiplied by a power of two that keeps a bound of all of a chunk's,
+// |S|, |S'|, |R|, |U| <= sqrt(Dk) max|S| + (C + 1) max|v|, between 2^4 and 2^13 (the
+// state's update is a contraction).  max|S| is measured every fourth chunk and
+// raised by C max|v| for each chunk since, so that the scale is there before the
+// state is; the state stays in its scale in registers.  Values down to 2^-12 of
+// the bound keep 20 bits or more, smaller ones an absolute 2^-29 of it at worst, and
+// a factor of 8 above it stays below fp16's end.
 template <int DK>
 struct Walk {
     static constexpr int kLoaders = 96;           // three warps
-    static constexpr int kThreads = 512;          // state 8 warps, outputs 4, loading 3, MMA issue 1
+    static constexpr int kThreads = 768;          // state 16 warps, outputs 4, loading 3, MMA issue 1
     static constexpr int kSub = DK / 64;          // 128-byte tiles of 64 dims
     static constexpr int kTile = 128 * 128;
     static constexpr int kTp = kSub * kTile;      // [K; Q], then [T; P T] hi, lo: 128 rows of 64, in 8x8 matrices
     static constexpr int kV = kTp + 2 * kTile;    // 64 tokens of 128 values
     static constexpr int kScales = kV + kChunk * 256;
     static constexpr int kStage = kScales + 2048;
-    static constexpr int kR = 2 * kStage;         // R, then W: hi and lo tiles of 128 rows of 64 tokens
-    static constexpr int kSmem = kR + 2 * kTile + 1024;
-    static constexpr int kHalf = DK / 2;          // state rows of a thread
-    static constexpr int kBatches = kHalf / 16;
+    static constexpr int kSmem = 2 * kStage + 1024;
+    static constexpr int kPart = DK / 4;          // state rows of a thread
+    static constexpr int kBatches = kPart / 16;
     // tensor-memory columns
-    static constexpr uint32_t kD1 = 0, kD2 = 128, kD3 = 256, kSHi = 384, kSLo = 448;
-    static_assert(kScaleBytes <= 2048 && kSmem <= 232448 - 5120, "shared memory");
+    static constexpr uint32_t kD1 = 0, kD2 = 128, kD3 = 256, kSHi = 384, kSLo = 448, kRHi = 384, kRLo = 416;
+    static_assert(kScaleBytes <= 2048 && kSmem <= 232448 - 16384, "shared memory");
 };
 
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
@@ -941,27 +944,27 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     using C = Walk<DK>;
     constexpr int kVecs = DK / 8;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[2], empty[2], s_ready[4], r_ready[2], w_ready[2], made[3], o_done, scaled;
-    __shared__ float2 most[3][2][128];      // [in turn][half][row]: max|S|, max|v|
+    __shared__ __align__(8) uint64_t full[2], empty[2], s_ready[2], r_ready, w_ready, made[3], o_done, scaled;
+    __shared__ float2 most[3][4][128];      // [chunk % 3][part][row]: max|S|, max|v|
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = smem_raw + (base - smem_u32(smem_raw));
-    if (warp == 15) {
+    if (warp == 23) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&full[i], C::kLoaders + 1);      // the loading threads, and the announcement of the bulk copies
-            mbar_init(&empty[i], 13);      // state and output warps, and the MMAs
-            mbar_init(&r_ready[i], 8);
-            mbar_init(&w_ready[i], 8);
+            mbar_init(&empty[i], 21);      // state and output warps, and the MMAs
+            mbar_init(&s_ready[i], 16);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&s_ready[i], 8);
+        mbar_init(&r_ready, 16);
+        mbar_init(&w_ready, 16);
         for (int i = 0; i < 3; ++i) mbar_init(&made[i], 1);
         mbar_init(&o_done, 4);
-        mbar_init(&scaled, 8);
+        mbar_init(&scaled, 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_trigger();
@@ -990,162 +993,169 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         __syncwarp();
     };
     auto scales_of = [&](int c) { return reinterpret_cast<const float*>(smem + (c & 1) * C::kStage + C::kScales); };
-    // The k-th bound and its scale, k = 0 for the state at the start, c + 1 for chunk c; row_v: max|v| of the
-    // chunk before, taken along.
-    auto scale_of = [&](int k, int row, float& row_v) {
-        const float2 x = most[k % 3][0][row], y = most[k % 3][1][row];
-        const float v = fmaxf(x.y, y.y);
-        const float bound = (DK == 128 ? 11.4f : 8.1f) * fmaxf(x.x, y.x) + kChunk * row_v + (kChunk + 1) * v;
-        row_v = v;
-        return row_scale(bound);
+    // A row's scale and its inverse, chunk by chunk.
+    struct Scale {
+        float s = 0.0f, v = 0.0f;      // bound of the state before the chunk; max|v| of the chunk
+        float2 now = make_float2(0.0f, 0.0f);
+        __device__ __forceinline__ float2 next(int c, const float2 (&most)[4][128], int row) {
+            float2 m = most[0][row];
+#pragma unroll
+            for (int p = 1; p < 4; ++p) m = make_float2(fmaxf(m.x, most[p][row].x), fmaxf(m.y, most[p][row].y));
+            // measured at the start and behind chunks 0, 4, 8, ..., known one chunk later
+            if (c == 0 || (c >= 2 && (c & 3) == 2)) s = (DK == 128 ? 11.4f : 8.1f) * m.x;
+            s += kChunk * v;
+            v = m.y;
+            const float bound = s + (kChunk + 1) * v, at = bound * now.x;
+            if (!(at >= 16.0f && at < 8192.0f)) now = row_scale(bound);
+            return now;
+        }
     };
 
-    if (warp < 8) {
+    if (warp < 16) {
         // ---- the state ----
-        const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int part = warp >> 2, row = (warp & 3) * 32 + lane;
         const int col = col0 + row;
         const bool live = col < a.dv && valid;
         const uint32_t lane_at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        float s[C::kHalf];
-        const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + half * C::kHalf) * a.dv + col;
+        const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + part * C::kPart) * a.dv + col;
+        const unsigned char* v_at = smem + C::kV + part * 16 * 256 + row * 2;      // this thread's 16 tokens
         float most_s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < C::kHalf; ++i) {
-            s[i] = a.state_in && live ? a.state_in[at + static_cast<int64_t>(i) * a.dv] : 0.0f;
-            most_s = fmaxf(most_s, fabsf(s[i]));
-        }
-        // batch b of this half: 16 state rows, hi and lo, as tensor-memory operand
-        auto put_state = [&](int b, float scale) {
+        // 16 state rows of this part (batch b) as hi and lo operand, and times `keep` where the product adds to them
+        auto put_state = [&](int b, const float (&x)[16], float keep) {
             uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) split_f16(s[b * 16 + 2 * i] * scale, s[b * 16 + 2 * i + 1] * scale, hi[i], lo[i]);
-            tmem_st8(lane_at + C::kSHi + half * (C::kHalf / 2) + b * 8, hi);
-            tmem_st8(lane_at + C::kSLo + half * (C::kHalf / 2) + b * 8, lo);
+            for (int i = 0; i < 8; ++i) split_f16(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+            tmem_st8(lane_at + C::kSHi + part * (C::kPart / 2) + b * 8, hi);
+            tmem_st8(lane_at + C::kSLo + part * (C::kPart / 2) + b * 8, lo);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) hi[i] = __float_as_uint(keep * x[e * 8 + i]);
+                tmem_st8(lane_at + C::kD3 + part * C::kPart + b * 16 + e * 8, hi);
+            }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_ready[b]);
         };
-        // 16 values of tokens half * 32 + 16 b .. as part of row `row` of the R / W tiles
-        auto put_row = [&](int b, const float (&x)[16], uint64_t* ready) {
+        // R or W of this part's 16 tokens
+        auto put_row = [&](const float (&x)[16], uint64_t* ready) {
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) split_f16(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t to = C::kR + row * 128 + (((half * 4 + b * 2 + i) ^ (row & 7)) << 4);
-                *reinterpret_cast<uint4*>(smem + to) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-                *reinterpret_cast<uint4*>(smem + to + C::kTile) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-            }
-            fence_proxy_async_smem();
+            tmem_st8(lane_at + C::kRHi + part * 8, hi);
+            tmem_st8(lane_at + C::kRLo + part * 8, lo);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ready[b]);
+            if (lane == 0) mbar_arrive(ready);
         };
-        float row_v = 0.0f;
-        auto agree = [&](int k, float v) {      // with the thread of the other half; the outputs follow
-            most[k % 3][half][row] = make_float2(most_s, v);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (lane == 0) mbar_arrive(&scaled);
-            return scale_of(k, row, row_v);
-        };
-        most[0][half][row] = make_float2(most_s, 0.0f);
-        asm volatile("bar.sync 3, 384;" ::: "memory");      // with the outputs
-        // this thread's 32 tokens of its value column
-        __half2 v[16];
-        auto load_v = [&](int c) {
+        auto most_v = [&](int c) {
             wait(&full[c & 1], c >> 1);
-            const __half* p = reinterpret_cast<const __half*>(smem + (c & 1) * C::kStage + C::kV + half * 32 * 256) + row;
-            float most_v = 0.0f;
+            const unsigned char* p = v_at + (c & 1) * C::kStage;
+            __half m = __float2half_rn(0.0f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                v[i] = __halves2half2(p[i * 256], p[i * 256 + 128]);
-                const float2 f = __half22float2(v[i]);
-                most_v = fmaxf(most_v, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-            return most_v;
+            for (int i = 0; i < 16; ++i) m = __hmax(m, __habs(*reinterpret_cast<const __half*>(p + i * 256)));
+            return __half2float(m);
         };
-        float2 in_s = scale_of(0, row, row_v), now = in_s;      // scales of the state operand in use, of this chunk
+        Scale scale;
+        auto agree = [&](int c, float v) {      // with the row's other threads; the outputs follow
+            most[c % 3][part][row] = make_float2(most_s, v);
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            if (lane == 0) mbar_arrive(&scaled);
+            return scale.next(c, most[c % 3], row);
+        };
+        float2 now = make_float2(1.0f, 1.0f);      // registers and operands of chunk c are in its scale
+        if (chunks_here == 0 && a.state_out && live) {
+            for (int i = 0; i < C::kPart; ++i)
+                a.state_out[at + static_cast<int64_t>(i) * a.dv] = a.state_in ? a.state_in[at + static_cast<int64_t>(i) * a.dv] : 0.0f;
+        }
+        if (chunks_here > 0) {
+            float x[C::kBatches][16];
 #pragma unroll
-        for (int b = 0; b < C::kBatches; ++b) put_state(b, in_s.x);
-        if (chunks_here > 0) now = agree(1, load_v(0));
-
-        for (int c = 0; c < chunks_here; ++c) {
-            const float* sc = scales_of(c);
-            const float keep = sc[4 * kChunk], f = now.x * in_s.y;
-            uint32_t d[2][16];
-            wait(&made[0], c);
-            tc_fence_after();
-            tmem_get(lane_at + C::kD1 + half * 32, d[0]);
-            tmem_get(lane_at + C::kD1 + half * 32 + 16, d[1]);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                tmem_wait(d[b]);
-                float x[16];
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float4 ck = *reinterpret_cast<const float4*>(sc + half * 32 + b * 16 + i);
-                    const float2 v0 = __half22float2(v[b * 8 + i / 2]), v1 = __half22float2(v[b * 8 + i / 2 + 1]);
-                    x[i] = v0.x * now.x - ck.x * (f * __uint_as_float(d[b][i]));
-                    x[i + 1] = v0.y * now.x - ck.y * (f * __uint_as_float(d[b][i + 1]));
-                    x[i + 2] = v1.x * now.x - ck.z * (f * __uint_as_float(d[b][i + 2]));
-                    x[i + 3] = v1.y * now.x - ck.w * (f * __uint_as_float(d[b][i + 3]));
-                }
-                put_row(b, x, r_ready);
+            for (int i = 0; i < C::kPart; ++i) {
+                x[i / 16][i % 16] = a.state_in && live ? a.state_in[at + static_cast<int64_t>(i) * a.dv] : 0.0f;
+                most_s = fmaxf(most_s, fabsf(x[i / 16][i % 16]));
             }
-            wait(&made[1], c);
-            tc_fence_after();
-            tmem_get(lane_at + C::kD2 + half * 32, d[0]);
-            tmem_get(lane_at + C::kD2 + half * 32 + 16, d[1]);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                tmem_wait(d[b]);
-                float x[16];
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float4 cs = *reinterpret_cast<const float4*>(sc + 2 * kChunk + half * 32 + b * 16 + i);
-                    x[i] = cs.x * __uint_as_float(d[b][i]);
-                    x[i + 1] = cs.y * __uint_as_float(d[b][i + 1]);
-                    x[i + 2] = cs.z * __uint_as_float(d[b][i + 2]);
-                    x[i + 3] = cs.w * __uint_as_float(d[b][i + 3]);
-                }
-                put_row(b, x, w_ready);
-            }
-            if (lane == 0) mbar_arrive(&empty[c & 1]);
-            // while the last product is made: the next chunk's values and scale
-            float2 next = now;
-            if (c + 1 < chunks_here) next = agree(c + 2, load_v(c + 1));
-            wait(&made[2], c);
-            tc_fence_after();
-            most_s = 0.0f;
-            tmem_get(lane_at + C::kD3 + half * C::kHalf, d[0]);
+            now = agree(0, most_v(0));
+            const float keep = scales_of(0)[4 * kChunk];
 #pragma unroll
             for (int b = 0; b < C::kBatches; ++b) {
-                tmem_wait(d[b & 1]);
-                if (b + 1 < C::kBatches) tmem_get(lane_at + C::kD3 + half * C::kHalf + (b + 1) * 16, d[(b + 1) & 1]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float& y = s[b * 16 + i];
-                    y = keep * y + now.y * __uint_as_float(d[b & 1][i]);
-                    most_s = fmaxf(most_s, fabsf(y));
-                }
-                put_state(b, now.x);
+                for (int i = 0; i < 16; ++i) x[b][i] *= now.x;
+                put_state(b, x[b], keep);
             }
-            in_s = now;
+        }
+
+#pragma unroll 1
+        for (int c = 0; c < chunks_here; ++c) {
+            const float* sc = scales_of(c) + part * 16;
+            float x[16];
+            wait(&made[0], c);
+            tc_fence_after();
+            tmem_ld16(lane_at + C::kD1 + part * 16, x);
+            const unsigned char* vp = v_at + (c & 1) * C::kStage;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4 ck = *reinterpret_cast<const float4*>(sc + i);
+                const float* cp = &ck.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[i + e] = __half2float(*reinterpret_cast<const __half*>(vp + (i + e) * 256)) * now.x - cp[e] * x[i + e];
+            }
+            put_row(x, &r_ready);
+            wait(&made[1], c);
+            tc_fence_after();
+            tmem_ld16(lane_at + C::kD2 + part * 16, x);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4 cs = *reinterpret_cast<const float4*>(sc + 2 * kChunk + i);
+                x[i] *= cs.x, x[i + 1] *= cs.y, x[i + 2] *= cs.z, x[i + 3] *= cs.w;
+            }
+            put_row(x, &w_ready);
+            if (lane == 0) mbar_arrive(&empty[c & 1]);
+            // while the last product is made: the next chunk's scale and decay
+            const bool last = c + 1 == chunks_here;
+            float2 next = now;
+            float keep = 0.0f;
+            if (!last) {
+                next = agree(c + 1, most_v(c + 1));
+                keep = scales_of(c + 1)[4 * kChunk];
+            }
+            const float change = next.x * now.y;
+            const bool changes = __any_sync(0xffffffffu, change != 1.0f), measure = (c & 3) == 0;
+            if (measure) most_s = 0.0f;
+            wait(&made[2], c);
+            tc_fence_after();
+#pragma unroll 1
+            for (int b = 0; b < C::kBatches; ++b) {
+                tmem_ld16(lane_at + C::kD3 + part * C::kPart + b * 16, x);
+                if (measure) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) most_s = fmaxf(most_s, fabsf(x[i]));
+                }
+                if (last) {
+                    if (a.state_out && live) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) a.state_out[at + static_cast<int64_t>(b * 16 + i) * a.dv] = x[i] * now.y;
+                    }
+                    continue;
+                }
+                if (changes) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] *= change;
+                }
+                put_state(b, x, keep);
+            }
+            if (measure) most_s *= now.y;
             now = next;
         }
-        if (a.state_out && live) {
-#pragma unroll
-            for (int i = 0; i < C::kHalf; ++i) a.state_out[at + static_cast<int64_t>(i) * a.dv] = s[i];
-        }
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ---- the outputs ----
         const int row = (warp & 3) * 32 + lane;
         const int col = col0 + row;
         const uint32_t lane_at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        float row_v = 0.0f;
-        asm volatile("bar.sync 3, 384;" ::: "memory");
-        float in_s = scale_of(0, row, row_v).y;
+        Scale scale;
         // "done" also says that the next chunk's scale has been seen, so the state cannot get ahead by two
         if (chunks_here > 0) wait(&scaled, 0);
         if (lane == 0) mbar_arrive(&o_done);
@@ -1156,37 +1166,36 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         for (int c = 0; c < chunks_here; ++c) {
             const float* sc = scales_of(c);
             wait(&full[c & 1], c >> 1);
-            const float in_r = scale_of(c + 1, row, row_v).y;
+            const float unit = scale.next(c, most[c % 3], row).y;
             wait(&made[1], c);
             tc_fence_after();
             const int left = col < a.dv ? end - begin - c * kChunk - odd : 0;      // of this lane's tokens
-#pragma unroll
+#pragma unroll 1
             for (int b = 0; b < 4; ++b) {
                 uint32_t x[16], y[16];
                 tmem_get(lane_at + C::kD1 + 64 + b * 16, x);
                 tmem_get(lane_at + C::kD2 + 64 + b * 16, y);
+                float cq[16], oq[16], o[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    *reinterpret_cast<float4*>(cq + i) = *reinterpret_cast<const float4*>(sc + kChunk + b * 16 + i);
+                    *reinterpret_cast<float4*>(oq + i) = *reinterpret_cast<const float4*>(sc + 3 * kChunk + b * 16 + i);
+                }
                 tmem_wait(x);
                 tmem_wait(y);
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const float4 cq = *reinterpret_cast<const float4*>(sc + kChunk + b * 16 + i);
-                    const float4 oq = *reinterpret_cast<const float4*>(sc + 3 * kChunk + b * 16 + i);
-                    const float* cp = &cq.x;
-                    const float* op = &oq.x;
-                    float o[4];
+                for (int i = 0; i < 16; ++i) o[i] = unit * (cq[i] * __uint_as_float(x[i]) + oq[i] * __uint_as_float(y[i]));
+                __half2 r[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        o[e] = cp[e] * (in_s * __uint_as_float(x[i + e])) + op[e] * (in_r * __uint_as_float(y[i + e]));
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const float other = __shfl_xor_sync(0xffffffffu, odd ? o[e] : o[e + 1], 1);
-                        if (b * 16 + i + e < left)
-                            *reinterpret_cast<__half2*>(to) = odd ? __floats2half2_rn(other, o[e + 1]) : __floats2half2_rn(o[e], other);
-                        to += step;
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const float other = __shfl_xor_sync(0xffffffffu, odd ? o[2 * i] : o[2 * i + 1], 1);
+                    r[i] = odd ? __floats2half2_rn(other, o[2 * i + 1]) : __floats2half2_rn(o[2 * i], other);
                 }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (b * 16 + 2 * i < left) *reinterpret_cast<__half2*>(to + i * step) = r[i];
+                to += 8 * step;
             }
-            in_s = in_r;
             if (c + 1 < chunks_here) wait(&scaled, c + 1);
             tc_fence_before();
             __syncwarp();
@@ -1195,9 +1204,9 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 mbar_arrive(&empty[c & 1]);
             }
         }
-    } else if (warp < 15) {
+    } else if (warp < 23) {
         // ---- loading ----
-        const int kh = h / a.share, lt = tid - 12 * 32;
+        const int kh = h / a.share, lt = tid - 20 * 32;
         const __half* k0 = a.k + kh * a.k_hs;
         const __half* q0 = a.q + kh * a.q_hs;
         const __half* v0 = a.v + h * a.v_hs + col0;
@@ -1226,7 +1235,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             rec += a.v_heads;
             const int t0 = begin + c * kChunk;
             const int n = min(kChunk, end - t0);
-#pragma unroll 4
+#pragma unroll 2
             for (int i = lt; i < kChunk * kVecs; i += C::kLoaders) {
                 const int r = i / kVecs, x = i % kVecs;
                 const bool ok = r < n;
@@ -1235,7 +1244,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 cp_async16_or_zero(dst, k0 + tok * a.k_ts + x * 8, ok);
                 cp_async16_or_zero(dst + kChunk * 128, q0 + tok * a.q_ts + x * 8, ok);
             }
-#pragma unroll 4
+#pragma unroll 2
             for (int i = lt; i < kChunk * 16; i += C::kLoaders) {
                 const int r = i >> 4, x = i & 15;
                 const bool ok = r < n && col0 + x * 8 < a.dv;
@@ -1253,7 +1262,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         // ---- MMA issue ----
         constexpr uint32_t kIdesc = instr_desc_f16(128, 128), kIdescT = instr_desc_f16(128, DK) | (1u << 16);   // B with N contiguous
         // descriptors count in 16 bytes; all are constants away from these
-        const uint64_t tiles = smem_desc_sw128(base), rh = smem_desc_sw128(base + C::kR), rl = rh + (C::kTile >> 4);
+        const uint64_t tiles = smem_desc_sw128(base);
         const uint64_t tri = smem_desc_plain(base + C::kTp);
         // K by tokens: groups of eight 1024 bytes apart, the second 64 dims a tile on
         const uint64_t turned = (tiles & ~(static_cast<uint64_t>(0x3fff) << 16)) | (static_cast<uint64_t>(C::kTile >> 4) << 16);
@@ -1267,37 +1276,29 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 wait_one(&s_ready[b], c);
                 tc_fence_after();
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int k = half * C::kBatches + b;
+                for (int part = 0; part < 4; ++part) {
+                    const int k = part * C::kBatches + b;
                     const uint64_t off = ((k / 4) * C::kTile + (k % 4) * 32) >> 4;
-                    mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, kq + off, kIdesc, b + half > 0);
+                    mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, kq + off, kIdesc, b + part > 0);
                     mma_f16_ts(tmem + C::kD1, tmem + C::kSLo + k * 8, kq + off, kIdesc, 1);
                 }
             }
             mma_commit(&made[0]);
+            wait_one(&r_ready, c);
+            tc_fence_after();
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                wait_one(&r_ready[b], c);
-                tc_fence_after();
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int k = half * 2 + b;
-                    mma_f16_ss(tmem + C::kD2, rh + k * 2, tp + k * 16, kIdesc, b + half > 0);
-                    mma_f16_ss(tmem + C::kD2, rl + k * 2, tp + k * 16, kIdesc, 1);
-                    mma_f16_ss(tmem + C::kD2, rh + k * 2, tp + (C::kTile >> 4) + k * 16, kIdesc, 1);
-                }
+            for (int k = 0; k < 4; ++k) {
+                mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + k * 16, kIdesc, k > 0);
+                mma_f16_ts(tmem + C::kD2, tmem + C::kRLo + k * 8, tp + k * 16, kIdesc, 1);
+                mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + (C::kTile >> 4) + k * 16, kIdesc, 1);
             }
             mma_commit(&made[1]);
+            wait_one(&w_ready, c);
+            tc_fence_after();
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                wait_one(&w_ready[b], c);
-                tc_fence_after();
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int k = half * 2 + b;
-                    mma_f16_ss(tmem + C::kD3, rh + k * 2, kt + k * 128, kIdescT, b + half > 0);
-                    mma_f16_ss(tmem + C::kD3, rl + k * 2, kt + k * 128, kIdescT, 1);
-                }
+            for (int k = 0; k < 4; ++k) {
+                mma_f16_ts(tmem + C::kD3, tmem + C::kRHi + k * 8, kt + k * 128, kIdescT, 1);
+                mma_f16_ts(tmem + C::kD3, tmem + C::kRLo + k * 8, kt + k * 128, kIdescT, 1);
             }
             mma_commit(&made[2]);
             mma_commit(&empty[c & 1]);
@@ -1308,7 +1309,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 23) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 int g_force = getenv("MCV_FORCE") ? atoi(getenv("MCV_FORCE")) : 0;

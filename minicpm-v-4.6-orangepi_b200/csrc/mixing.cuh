@@ -75,12 +75,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 
 // x, y as two fp16 pairs hi + lo: x - (hi + lo) is at most 2^-22 |x| (and 2^-25
 // where lo is subnormal), so that a product of hi and lo with fp16 operands
-// keeps fp32's accuracy.
+// keeps fp32's accuracy.  The remainder is exact, in one mixed-precision FMA.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = h2_as_u32(h);
-    lo = h2_as_u32(__floats2half2_rn(x - f.x, y - f.y));
+    hi = h2_as_u32(__floats2half2_rn(x, y));
+    fma2_f16_f32(x, y, hi, 0xbc00bc00u);      // - 1 hi
+    lo = h2_as_u32(__floats2half2_rn(x, y));
 }
 
 }  // namespace mcv
