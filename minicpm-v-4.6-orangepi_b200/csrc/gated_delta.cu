@@ -8,7 +8,6 @@
 #include "tcgen05.cuh"
 
 #include <cmath>
-#include <cstdlib>
 
 namespace mcv {
 unsigned take_gated_delta_device_error();
@@ -907,6 +906,22 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
+// Waits for an mbarrier phase suspended, 10 ms at a time and 200 times at most.
+__device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < 200; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(10000000u)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
 // 16 columns of this warp's 32 lanes, to be waited for with tmem_wait.
 __device__ __forceinline__ void tmem_get(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
@@ -978,19 +993,20 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     int begin = 0, end = 0, slot = 0;
     const bool valid = sequence(a, b, begin, end, slot);
     const int chunks_here = valid ? (end - begin + kChunk - 1) / kChunk : 0;
-    // Every wait is bounded, by one lane for its warp.  A lane whose wait gave up
-    // records it and goes on without waiting, so that all barriers still meet
-    // and the block ends.
+    // Every wait is bounded.  A thread whose wait gave up records it and goes on
+    // without waiting, so that all barriers still meet and the block ends.  Warps
+    // wait whole and suspended: one lane of each of 23 asking again and again took
+    // a fifth of a chunk's time from the thread that issues, which alone does ask.
     bool dead = false;
-    auto wait_one = [&](uint64_t* bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity & 1)) {
-            dead = true;
-            atomicOr(&g_gated_delta_dev_error, kDevErrTimeout);
-        }
+    auto gave_up = [&]() {
+        dead = true;
+        atomicOr(&g_gated_delta_dev_error, kDevErrTimeout);
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (lane == 0) wait_one(bar, parity);
-        __syncwarp();
+        if (!dead && !mbar_wait_suspended(bar, parity & 1)) gave_up();
+    };
+    auto wait_one = [&](uint64_t* bar, uint32_t parity) {
+        if (!dead && !mbar_wait(bar, parity & 1)) gave_up();
     };
     auto scales_of = [&](int c) { return reinterpret_cast<const float*>(smem + (c & 1) * C::kStage + C::kScales); };
     // A row's scale and its inverse, chunk by chunk.
@@ -1256,8 +1272,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             mbar_arrive(&full[st]);
         }
         // the bulk copies have landed before the block's shared memory goes
-        if (lane == 0)
-            for (int c = max(0, chunks_here - 2); c < chunks_here; ++c) wait_one(&full[c & 1], c >> 1);
+        for (int c = max(0, chunks_here - 2); c < chunks_here; ++c) wait(&full[c & 1], c >> 1);
     } else if (lane == 0) {
         // ---- MMA issue ----
         constexpr uint32_t kIdesc = instr_desc_f16(128, 128), kIdescT = instr_desc_f16(128, DK) | (1u << 16);   // B with N contiguous
@@ -1271,22 +1286,22 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             const uint64_t kq = tiles + st, tp = tri + st, kt = turned + st;
             wait_one(&full[c & 1], c >> 1);
             wait_one(&o_done, c);      // the outputs have read D1 and D2
-#pragma unroll
+            // rolled: each instruction of straight code would be fetched for one use
+#pragma unroll 1
             for (int b = 0; b < C::kBatches; ++b) {
                 wait_one(&s_ready[b], c);
                 tc_fence_after();
-#pragma unroll
-                for (int part = 0; part < 4; ++part) {
-                    const int k = part * C::kBatches + b;
-                    const uint64_t off = ((k / 4) * C::kTile + (k % 4) * 32) >> 4;
-                    mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, kq + off, kIdesc, b + part > 0);
-                    mma_f16_ts(tmem + C::kD1, tmem + C::kSLo + k * 8, kq + off, kIdesc, 1);
+#pragma unroll 1
+                for (int k = b; k < DK / 16; k += C::kBatches) {
+                    const uint64_t d = kq + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
+                    mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, d, kIdesc, k > 0);
+                    mma_f16_ts(tmem + C::kD1, tmem + C::kSLo + k * 8, d, kIdesc, 1);
                 }
             }
             mma_commit(&made[0]);
             wait_one(&r_ready, c);
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < 4; ++k) {
                 mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + k * 16, kIdesc, k > 0);
                 mma_f16_ts(tmem + C::kD2, tmem + C::kRLo + k * 8, tp + k * 16, kIdesc, 1);
@@ -1295,7 +1310,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             mma_commit(&made[1]);
             wait_one(&w_ready, c);
             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < 4; ++k) {
                 mma_f16_ts(tmem + C::kD3, tmem + C::kRHi + k * 8, kt + k * 128, kIdescT, 1);
                 mma_f16_ts(tmem + C::kD3, tmem + C::kRLo + k * 8, kt + k * 128, kIdescT, 1);
@@ -1304,7 +1319,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             mma_commit(&empty[c & 1]);
         }
         // every MMA has ended before its operands and tensor memory go
-        if (chunks_here > 0) wait_one(&made[2], chunks_here - 1);
+        if (chunks_here > 0) wait(&made[2], chunks_here - 1);
     }
     __syncwarp();
     tc_fence_before();
@@ -1312,7 +1327,6 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     if (warp == 23) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-int g_force = getenv("MCV_FORCE") ? atoi(getenv("MCV_FORCE")) : 0;
 int64_t chunk_slots(int64_t tokens, int64_t batch) { return tokens / kChunk + batch; }
 
 template <int DK, int NG>
@@ -1336,15 +1350,18 @@ int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
                     kSmem, stream, a, chunks);
     if (st) return st;
-    // two column groups a block once single ones would not all run at once
-    const int64_t groups = static_cast<int64_t>(a.batch) * a.v_heads * (a.dv / 16);
-    if (g_force == 3 || (g_force == 0 && groups > 2 * sm_count())) {
+    // One column group a block while those all run at once (a chunk then takes 1.4 us), else two (2.5 us), unless
+    // whole heads on the other walk (4.0 us) get through in less, which they do from twice as many rounds on.
+    const int64_t heads = static_cast<int64_t>(a.batch) * a.v_heads;
+    const int sms = sm_count();
+    if (heads * (a.dv / 16) > sms) {
+        const int64_t pairs = (heads * ((a.dv + 31) / 32) + sms - 1) / sms, whole = (heads * ((a.dv + 127) / 128) + sms - 1) / sms;
+        if (pairs * 5 <= whole * 8) return launch_scan<DK, 2>(a, chunks, stream);
         static std::atomic<uint64_t> done_walk{0};
         if ((st = allow_smem(walk_kernel<DK>, Walk<DK>::kSmem, done_walk))) return st;
         return launch(walk_kernel<DK>, dim3((a.dv + 127) / 128, a.v_heads, a.batch), dim3(Walk<DK>::kThreads), Walk<DK>::kSmem,
                       stream, a, chunks);
     }
-    if (groups > sm_count()) return launch_scan<DK, 2>(a, chunks, stream);
     return launch_scan<DK, 1>(a, chunks, stream);
 }
 

@@ -461,6 +461,49 @@ def test_delta_prefill(cuda, lens, hk, hv, dk, dv, start):
     assert torch.equal(out, out2)
 
 
+@pytest.mark.parametrize("lens,hk,hv,dk,dv", [
+    ([130, 64, 1, 0, 257], 8, 16, 128, 128), ([65] * 12, 8, 16, 64, 64), ([200, 70], 48, 48, 64, 144),
+    ([449, 321], 24, 48, 128, 16), ([100] * 40, 2, 4, 128, 96)])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -9, 2.0 ** 7])
+def test_delta_prefill_many_heads(cuda, lens, hk, hv, dk, dv, scale):
+    """Enough heads for the walk that takes whole ones; values and states of
+    very different sizes from head to head and within a sequence."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(sum(lens) + dv)
+    b, n = len(lens), sum(lens)
+    q, k, v, gl, beta = delta_inputs(torch, g, n, hk, hv, dk, dv)
+    v = v * (scale * 2.0 ** torch.randint(-6, 6, (1, hv, 1), generator=g, device="cuda").float()).half()
+    v[n // 2:] *= 0.125
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    index = torch.randperm(b + 1, generator=g, device="cuda")[:b].int()
+    state = randn(g, b + 1, hv, dk, dv, dtype=torch.float32) * scale
+    new, out = torch.full_like(state, 9.0), torch.empty(n, hv, dv, dtype=torch.float16, device="cuda")
+    ws = mcv.gated_delta_workspace(n, b, hv, dk, dv)
+    ws.fill_(255)
+    mcv.device_errors()
+    mcv.gated_delta_prefill(q, k, v, gl, beta, cu, state, out, ws, state_out=new, index=index, l2_eps=1e-6)
+    assert mcv.device_errors() == 0
+    at = 0
+    for i, ln in enumerate(lens):
+        slot = int(index[i])
+        if ln == 0:
+            assert torch.equal(new[slot], state[slot])
+        else:
+            delta_check(torch, [x[at:at + ln] for x in (q, k, v, gl, beta)], state[slot], out[at:at + ln], new[slot], dk ** -0.5,
+                        1e-6, f"sequence {i}")
+        at += ln
+    # in place, without a state at the start, and as given keys and queries
+    inplace, out2 = state.clone(), torch.empty_like(out)
+    mcv.gated_delta_prefill(q, k, v, gl, beta, cu, inplace, out2, ws, index=index, l2_eps=1e-6)
+    assert torch.equal(out, out2) and torch.equal(inplace[index.long()], new[index.long()])
+    kn, qs = (k / 16).contiguous(), (q * 3).contiguous()
+    first = torch.empty(b, hv, dk, dv, device="cuda")
+    mcv.gated_delta_prefill(qs, kn, v, gl, beta, cu, None, out2, ws, state_out=first, scale=0.5)
+    zero = torch.zeros(hv, dk, dv, device="cuda")
+    delta_check(torch, [x[:lens[0]] for x in (qs, kn, v, gl, beta)], zero, out2[:lens[0]], first[0], 0.5, None, "as given")
+
+
 @pytest.mark.parametrize("kind", ["forget", "keep", "write", "none", "mixed"])
 def test_delta_prefill_gates(cuda, kind):
     """Decays that erase everything (also -inf), none at all, full and no
