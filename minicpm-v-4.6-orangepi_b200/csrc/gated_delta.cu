@@ -225,8 +225,13 @@ __device__ __forceinline__ float2 two_floats(double x) {
     const float h = static_cast<float>(x);
     return make_float2(h, static_cast<float>(x - h));
 }
+__device__ __forceinline__ float pow2(float x) {       // below 2^-126: 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float decay_between(float2 later, float2 earlier) {
-    return exp2f((later.x - earlier.x) + (later.y - earlier.y));
+    return pow2((later.x - earlier.x) + (later.y - earlier.y));
 }
 
 // 16x16 fp32 block as a product's operands.  acc + 2^-11 acc_lo += a b.
@@ -241,35 +246,39 @@ __device__ __forceinline__ void mma_split(float (&acc)[2][4], float (&acc_lo)[2]
         mma16816(acc_lo[n], a.hi, b.lo[2 * n], b.lo[2 * n + 1]);
     }
 }
-// A result (C fragments of two n8 tiles) as the next product's B operand: 8x8 transposes.
-__device__ __forceinline__ void to_b(Split4& b, const float (&x)[2][4]) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            uint32_t hi, lo;
-            split_scaled(x[n][e], x[n][e + 1], hi, lo);
-            b.hi[2 * n + e / 2] = movm_t(hi);
-            b.lo[2 * n + e / 2] = movm_t(lo);
-        }
-}
+// Per chunk and value head, four warps.
+//
+// Q K^T and K K^T by MMA in 16x16 blocks on and below the diagonal, three or two
+// per warp, one of them on the diagonal.  Below it a decay e^(G_r - G_c) is split at
+// the row block's start into a factor of the row and one of the column, neither
+// above 1 where g <= 0, so that an element costs a product and not an exponential.
+//
+// Then X = (I + A)^-1: the diagonal blocks by forward substitution in fp32, one
+// thread a column; the others by split MMAs (operands hi + 2^-11 lo), first
+// X_10 and X_32, then the lower left quarter -X_B (A_BA X_A), so that no warp
+// waits for more than four steps; and P X beside and behind them.
+//
+// Bound by its instructions (about 1.5 us a chunk and SM for 53 KB, which would
+// take 1.2): 512 threads a SM had the loads and the steps' latencies showing.
+template <int DK>
+struct ChunkSmem {
+    static constexpr int kKQ = 2 * kChunk * DK * 2;
+    static constexpr int kA = 0, kP = kA + 6 * 1024, kX = kP + 10 * 1024, kY = kX + 10 * 1024, kDiag = kY + 4 * 1024;
+    static constexpr int kDiagRow = 20;                    // floats
+    static constexpr int kWork = kDiag + 4 * 16 * kDiagRow * 4;
+    static constexpr int kBytes = kKQ > kWork ? kKQ : kWork;
+};
 
-// Per chunk and value head.  Q K^T and K K^T by MMA, each warp 16 rows up to the
-// diagonal block; then X = (I + A)^-1 by 16x16 blocks: the diagonal ones by
-// forward substitution in fp32, one thread a column, the rest
-//   X_ij = -X_ii sum_{j <= l < i} A_il X_lj
-// by split MMAs, one warp a column of blocks, in registers - the columns do not
-// depend on each other - and so P X.
 template <int DK>
 __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk* chunks) {
+    using M = ChunkSmem<DK>;
     constexpr int kVecs = DK / 8;
-    extern __shared__ __align__(128) unsigned char smem[];  // K and Q, then the blocks
-    // 16x16 blocks, hi and lo, each as four 8x8 matrices in ldmatrix's order for an A operand
-    __half* a_blk = reinterpret_cast<__half*>(smem);         // [2][6 blocks]: A below the diagonal blocks
-    __half* p_blk = a_blk + 2 * 6 * 256;                      // [2][10]: P on and below the diagonal
-    __half* x_blk = p_blk + 2 * 10 * 256;                     // [2][4]: inverses of the diagonal blocks
-    float* diag = reinterpret_cast<float*>(x_blk + 2 * 4 * 256);   // [4][16 * 17]: A's diagonal blocks
+    // K and Q; then blocks of 16x16, hi and lo of 512 bytes, each as four 8x8 matrices in ldmatrix's order for
+    // an A operand: (rows lo, k lo), (rows hi, k lo), (rows lo, k hi), (rows hi, k hi)
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float4 rows[kChunk];                         // G (two floats), r_k, r of q's row
+    __shared__ float2 row_by[kChunk];                       // factors of a row below the diagonal: of A, of P
+    __shared__ float col_by[96];                            // factors of columns 0 .. 16 i - 1 for row block i = 1, 2, 3
     __shared__ float bt[kChunk], qn[kChunk];                // beta; scale of an output over that of q's row
     pdl_trigger();
     pdl_wait();
@@ -290,7 +299,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
     const int n = min(kChunk, end - t0);
     const int kh = h / a.share;
 
-    const uint32_t ks = smem_u32(smem), qs = ks + kChunk * DK * 2;
+    const uint32_t base = smem_u32(smem), ks = base, qs = ks + kChunk * DK * 2;
     {
         constexpr int kStep = 128 / kVecs;
         const int lr = tid / kVecs, lx = tid % kVecs;
@@ -331,7 +340,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
     __syncthreads();
     {
         const int r = tid & 63;
-        const uint32_t base = tid < 64 ? ks : qs;
+        const uint32_t from = tid < 64 ? ks : qs;
         float sum[4] = {};
         if (a.l2_eps >= 0.0f || tid >= 64) {
 #pragma unroll
@@ -339,7 +348,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
                 uint32_t x[4];
                 asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                              : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                             : "r"(tile_at<kVecs>(base, r, c)));
+                             : "r"(tile_at<kVecs>(from, r, c)));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 f = __half22float2(u32_as_h2(x[i]));
@@ -359,174 +368,245 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
     }
     __syncthreads();
     Chunk& out = chunks[static_cast<int64_t>(blockIdx.x) * a.v_heads + h];
+    auto g_at = [&](int r) { return *reinterpret_cast<const float2*>(&rows[r].x); };
     if (tid < kChunk) {
-        const float4 r = rows[tid], last = rows[kChunk - 1];
-        const float eg = exp2f(r.x + r.y);
+        const float4 r = rows[tid];
+        const float eg = pow2(r.x + r.y);
         out.ck[tid] = eg * r.z;
         out.cq[tid] = eg * r.w * qn[tid];
-        out.cs[tid] = decay_between(make_float2(last.x, last.y), make_float2(r.x, r.y)) * r.z * (1.0f / kTriScale);
+        out.cs[tid] = decay_between(g_at(kChunk - 1), make_float2(r.x, r.y)) * r.z * (1.0f / kTriScale);
         out.oq[tid] = qn[tid] * (1.0f / kTriScale);
         if (tid == kChunk - 1) out.keep = eg;
+        if (tid >= 16) {
+            const float f = decay_between(make_float2(r.x, r.y), g_at((tid & ~15) - 1));
+            row_by[tid] = make_float2(f * r.z * bt[tid], f * r.w);
+        }
+    }
+    if (tid >= 32) {
+        const int i = tid - 32;
+        const int block = i < 16 ? 1 : (i < 48 ? 2 : 3), c = i - (block == 1 ? 0 : (block == 2 ? 16 : 48));
+        col_by[i] = decay_between(g_at(block * 16 - 1), g_at(c)) * rows[c].z;
     }
 
-    float kk[8][4], qk[8][4];
+    // this warp's blocks: two in one row of blocks, and with warps 0 and 2 a third; the last on the diagonal
+    const int row01 = warp == 0 ? 3 : (warp == 1 ? 3 : (warp == 2 ? 2 : 1)), col0 = warp == 1 ? 2 : 0;
+    const bool third = !(warp & 1);
+    const int own = warp == 0 ? 0 : 4 - warp;         // its diagonal block: 0, 3, 2, 1
+    float kk[3][2][4], qk[3][2][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 3; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kk[j][e] = qk[j][e] = 0.0f;
+        for (int e = 0; e < 8; ++e) kk[j][e >> 2][e & 3] = qk[j][e >> 2][e & 3] = 0.0f;
+    const int a_row = lane & 15, a_vec = lane >> 4, b_row = (lane & 7) + (lane >> 4) * 8, b_vec = (lane >> 3) & 1;
 #pragma unroll
     for (int x = 0; x < DK / 16; ++x) {
-        uint32_t ka[4], qa[4];
-        const int ar = warp * 16 + (lane & 15), ac = x * 2 + (lane >> 4);
-        ldsm4(ka, tile_at<kVecs>(ks, ar, ac));
-        ldsm4(qa, tile_at<kVecs>(qs, ar, ac));
+        uint32_t ka[4], qa[4], b[4];
+        ldsm4(ka, tile_at<kVecs>(ks, row01 * 16 + a_row, x * 2 + a_vec));
+        ldsm4(qa, tile_at<kVecs>(qs, row01 * 16 + a_row, x * 2 + a_vec));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > warp) break;
-            uint32_t b[4];
-            ldsm4(b, tile_at<kVecs>(ks, j * 16 + (lane & 7) + (lane >> 4) * 8, x * 2 + ((lane >> 3) & 1)));
-            mma16816(kk[2 * j], ka, b[0], b[1]);
-            mma16816(kk[2 * j + 1], ka, b[2], b[3]);
-            mma16816(qk[2 * j], qa, b[0], b[1]);
-            mma16816(qk[2 * j + 1], qa, b[2], b[3]);
+        for (int j = 0; j < 3; ++j) {
+            if (j == 2) {
+                if (!third) break;
+                if (warp == 0) {
+                    ldsm4(ka, tile_at<kVecs>(ks, a_row, x * 2 + a_vec));
+                    ldsm4(qa, tile_at<kVecs>(qs, a_row, x * 2 + a_vec));
+                }
+            }
+            ldsm4(b, tile_at<kVecs>(ks, (j < 2 ? col0 + j : own) * 16 + b_row, x * 2 + b_vec));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                mma16816(kk[j][q], ka, b[2 * q], b[2 * q + 1]);
+                mma16816(qk[j][q], qa, b[2 * q], b[2 * q + 1]);
+            }
         }
     }
     __syncthreads();     // K and Q are not read any more
     const int g = lane >> 2, t = lane & 3;
-    const float4 row[2] = {rows[warp * 16 + g], rows[warp * 16 + g + 8]};
-    const float write[2] = {row[0].z * bt[warp * 16 + g], row[1].z * bt[warp * 16 + g + 8]};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if (j > 2 * warp + 1) break;
-        const int c = j * 8 + 2 * t;
-        const float4 col[2] = {rows[c], rows[c + 1]};
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            const int r = warp * 16 + g + e * 4;
-            const float4 mine = row[e / 2];
-            float p[2], m[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float w = decay_between(make_float2(mine.x, mine.y), make_float2(col[i].x, col[i].y)) * col[i].z;
-                p[i] = c + i <= r ? w * mine.w * qk[j][e + i] : 0.0f;
-                m[i] = c + i < r ? w * write[e / 2] * kk[j][e + i] : 0.0f;
-            }
-            // matrices of a block: (rows lo, k lo), (rows hi, k lo), (rows lo, k hi), (rows hi, k hi)
-            const int in = ((j & 1) * 2 + e / 2) * 64 + g * 8 + t * 2;
-            uint32_t x, y;
-            split_scaled(p[0], p[1], x, y);
-            const int at = (warp * (warp + 1) / 2 + j / 2) * 256 + in;
-            *reinterpret_cast<uint32_t*>(p_blk + at) = x;
-            *reinterpret_cast<uint32_t*>(p_blk + 10 * 256 + at) = y;
-            if (j / 2 == warp) {
-                float* d = diag + warp * 16 * 17 + (g + e * 4) * 17 + (j & 1) * 8 + 2 * t;
-                d[0] = m[0];
-                d[1] = m[1];
-            } else {
-                const int am = (warp * (warp - 1) / 2 + j / 2) * 256 + in;
-                split_scaled(m[0], m[1], x, y);
-                *reinterpret_cast<uint32_t*>(a_blk + am) = x;
-                *reinterpret_cast<uint32_t*>(a_blk + 6 * 256 + am) = y;
-            }
-        }
-    }
-    __syncwarp();
-
-    // this warp's diagonal block: lanes 0-15 take a column each,
-    // x_i = [i = j] - sum_{l < i} A_il x_l
-    if (lane < 16) {
-        const float* m = diag + warp * 16 * 17;
-        const float beta = bt[warp * 16 + lane];
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float acc[2] = {i == lane ? 1.0f : 0.0f, 0.0f};
-#pragma unroll
-            for (int l = 0; l < i; ++l) acc[l & 1] -= m[i * 17 + l] * x[l];
-            x[i] = acc[0] + acc[1];
-            const int at = warp * 256 + ((lane >> 3) * 2 + (i >> 3)) * 64 + (i & 7) * 8 + (lane & 7);
-            __half hi16 = __float2half_rn(x[i]);
-            x_blk[at] = hi16;
-            x_blk[4 * 256 + at] = __float2half_rn((x[i] - __half2float(hi16)) * kLo);
-            const float y = x[i] * beta * kTriScale;
-            const int to = tri_at(warp * 16 + i, warp * 16 + lane);
-            hi16 = __float2half_rn(y);
-            out.tp[0][0][to] = hi16;
-            out.tp[1][0][to] = __float2half_rn(y - __half2float(hi16));
-        }
-    }
-    __syncthreads();
-
-    // this warp's column of blocks; its diagonal block as a B operand (k lo, k hi of columns lo, then hi)
-    Split4 xb[4];
-    const uint32_t as = smem_u32(a_blk), ps = smem_u32(p_blk), xs = smem_u32(x_blk);
-    constexpr uint32_t kXLo = 4 * 512, kALo = 6 * 512, kPLo = 10 * 512;
-    float2 beta[2] = {*reinterpret_cast<const float2*>(&bt[warp * 16 + 2 * t]),
-                      *reinterpret_cast<const float2*>(&bt[warp * 16 + 8 + 2 * t])};
-    beta[0].x *= kTriScale, beta[0].y *= kTriScale, beta[1].x *= kTriScale, beta[1].y *= kTriScale;
-    auto put_block = [&](int which, int row0, const float (&y)[2][4]) {      // times beta 2^14, into columns of this warp
+    // values of an accumulator as block `to` in shared memory
+    auto put = [&](int to, const float (&x)[2][4]) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
-                uint32_t x, z;
-                split_f16(y[q][e] * beta[q].x, y[q][e + 1] * beta[q].y, x, z);
-                const int at = tri_at(row0 + g + e * 4, warp * 16 + q * 8 + 2 * t);
-                *reinterpret_cast<uint32_t*>(&out.tp[0][which][at]) = x;
-                *reinterpret_cast<uint32_t*>(&out.tp[1][which][at]) = z;
+                uint32_t u, l;
+                split_scaled(x[q][e], x[q][e + 1], u, l);
+                uint32_t* at = reinterpret_cast<uint32_t*>(smem + to + (q * 2 + e / 2) * 128 + g * 16 + t * 4);
+                at[0] = u;
+                at[128] = l;
             }
     };
-    ldsm4_t(xb[0].hi, xs + warp * 512 + lane * 16);
-    ldsm4_t(xb[0].lo, xs + kXLo + warp * 512 + lane * 16);
+    auto tri = [](int i, int j) { return (i * (i + 1) / 2 + j) * 1024; };      // of P and X
+    auto below = [](int i, int j) { return (i * (i - 1) / 2 + j) * 1024; };    // of A
+    float* diag = reinterpret_cast<float*>(smem + M::kDiag) + own * 16 * M::kDiagRow;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int i = warp + s;         // block row
-        if (i > 3) break;
-        if (s > 0) {
-            float y[2][4] = {}, yl[2][4] = {};
+    for (int j = 0; j < 3; ++j) {
+        if (j == 2 && !third) break;
+        const int bi = j < 2 ? row01 : own, bj = j < 2 ? col0 + j : own;
+        if (bi != bj) {
+            const float* cb = col_by + (bi == 1 ? 0 : (bi == 2 ? 16 : 48)) + bj * 16 + 2 * t;
 #pragma unroll
-            for (int l = 0; l < s; ++l) {
-                Split4 m;
-                const uint32_t at = as + (i * (i - 1) / 2 + warp + l) * 512 + lane * 16;
-                ldsm4(m.hi, at);
-                ldsm4(m.lo, at + kALo);
-                mma_split(y, yl, m, xb[l]);
+            for (int e = 0; e < 4; e += 2) {
+                const float2 rb = row_by[bi * 16 + g + e * 4];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const float2 c = *reinterpret_cast<const float2*>(cb + q * 8);
+                    kk[j][q][e] *= rb.x * c.x, kk[j][q][e + 1] *= rb.x * c.y;
+                    qk[j][q][e] *= rb.y * c.x, qk[j][q][e + 1] *= rb.y * c.y;
+                }
             }
+            put(M::kA + below(bi, bj), kk[j]);
+        } else {
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
+            for (int e = 0; e < 4; e += 2) {
+                const int r = g + e * 4;
+                const float4 mine = rows[bi * 16 + r];
+                const float write = mine.z * bt[bi * 16 + r];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[q][e] += kLoInv * yl[q][e];
-            Split4 yb, m;
-            to_b(yb, y);
-            ldsm4(m.hi, xs + i * 512 + lane * 16);
-            ldsm4(m.lo, xs + kXLo + i * 512 + lane * 16);
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[q][e] = yl[q][e] = 0.0f;
-            mma_split(y, yl, m, yb);
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[q][e] = -(y[q][e] + kLoInv * yl[q][e]);
-            put_block(0, i * 16, y);
-            to_b(xb[s], y);
+                    for (int i = 0; i < 2; ++i) {
+                        const int c = q * 8 + 2 * t + i;
+                        const float4 col = rows[bi * 16 + c];
+                        const float w = decay_between(make_float2(mine.x, mine.y), make_float2(col.x, col.y)) * col.z;
+                        diag[r * M::kDiagRow + c] = c < r ? w * write * kk[j][q][e + i] : 0.0f;
+                        qk[j][q][e + i] = c <= r ? w * mine.w * qk[j][q][e + i] : 0.0f;
+                    }
+            }
         }
-        float y[2][4] = {}, yl[2][4] = {};
+        put(M::kP + tri(bi, bj), qk[j]);
+    }
+    __syncwarp();
+
+    // the diagonal block: lanes 0-15 take a column each, x_i = [i = j] - sum_{l < i} A_il x_l
+    if (lane < 16) {
+        float x[16];
 #pragma unroll
-        for (int l = 0; l <= s; ++l) {
-            Split4 m;
-            const uint32_t at = ps + (i * (i + 1) / 2 + warp + l) * 512 + lane * 16;
-            ldsm4(m.hi, at);
-            ldsm4(m.lo, at + kPLo);
-            mma_split(y, yl, m, xb[l]);
+        for (int i = 0; i < 16; ++i) {
+            float acc[4] = {i == lane ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int l = 0; l < i; l += 4) {
+                const float4 m = *reinterpret_cast<const float4*>(diag + i * M::kDiagRow + l);     // zeros from l = i on
+                acc[0] -= m.x * x[l];
+                if (l + 1 < i) acc[1] -= m.y * x[l + 1];
+                if (l + 2 < i) acc[2] -= m.z * x[l + 2];
+                if (l + 3 < i) acc[3] -= m.w * x[l + 3];
+            }
+            x[i] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
         }
+        __syncwarp(0xffffu);      // all of A's block has been read
+#pragma unroll
+        for (int i = 0; i < 16; ++i) diag[i * M::kDiagRow + lane] = x[i];
+    }
+    __syncwarp();
+
+    float y[2][4], yl[2][4];
+    auto start = [&]() {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[q][e] += kLoInv * yl[q][e];
-        put_block(1, i * 16, y);
+            for (int e = 0; e < 4; ++e) y[q][e] = yl[q][e] = 0.0f;
+    };
+    // (y, yl) += block at `left` times block at `right`
+    auto times = [&](int left, int right) {
+        Split4 l, r;
+        ldsm4(l.hi, base + left + lane * 16);
+        ldsm4(l.lo, base + left + 512 + lane * 16);
+        ldsm4_t(r.hi, base + right + lane * 16);
+        ldsm4_t(r.lo, base + right + 512 + lane * 16);
+        mma_split(y, yl, l, r);
+    };
+    auto finish = [&](float sign) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[q][e] = sign * (y[q][e] + kLoInv * yl[q][e]);
+    };
+    // y times beta 2^14 as block (i, j) of the record's T (0) or P T (1)
+    auto record = [&](int which, int i, int j) {
+        const int in = 2 * i * (i + 1) * 64 + j * 128 + g * 8 + t * 2;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const float2 b = *reinterpret_cast<const float2*>(&bt[j * 16 + q * 8 + 2 * t]);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                uint32_t u, l;
+                split_f16(y[q][e] * (b.x * kTriScale), y[q][e + 1] * (b.y * kTriScale), u, l);
+                const int at = in + (e / 2) * (2 * i + 2) * 64 + q * 64;
+                *reinterpret_cast<uint32_t*>(&out.tp[0][which][at]) = u;
+                *reinterpret_cast<uint32_t*>(&out.tp[1][which][at]) = l;
+            }
+        }
+    };
+    auto put_x = [&](int i, int j) {
+        put(M::kX + tri(i, j), y);
+        record(0, i, j);
+    };
+    auto p_times = [&](int i, int j) {
+        start();
+#pragma unroll 1
+        for (int l = j; l <= i; ++l) times(M::kP + tri(i, l), M::kX + tri(l, j));
+        finish(1.0f);
+        record(1, i, j);
+    };
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[q][e] = diag[(g + (e >> 1) * 8) * M::kDiagRow + q * 8 + 2 * t + (e & 1)];
+    put_x(own, own);
+    __syncthreads();
+    auto y_at = [](int i, int j) { return M::kY + ((i - 2) * 2 + j) * 1024; };
+    if (warp < 2) {          // X_10, X_32; the products go through shared memory of Y_20, Y_30
+        const int i = warp == 0 ? 1 : 3, j = i - 1;
+        start();
+        times(M::kA + below(i, j), M::kX + tri(j, j));
+        finish(1.0f);
+        put(y_at(2 + warp, 0), y);
+        __syncwarp();
+        start();
+        times(M::kX + tri(i, i), y_at(2 + warp, 0));
+        finish(-1.0f);
+        put_x(i, j);
+    } else {                 // Y_21, Y_31
+        start();
+        times(M::kA + below(warp, 1), M::kX + tri(1, 1));
+        finish(1.0f);
+        put(y_at(warp, 1), y);
     }
+    __syncthreads();
+    if (warp < 2) {          // Y_20, Y_30
+        start();
+        times(M::kA + below(2 + warp, 0), M::kX + tri(0, 0));
+        times(M::kA + below(2 + warp, 1), M::kX + tri(1, 0));
+        finish(1.0f);
+        put(y_at(2 + warp, 0), y);
+    } else {                 // X_21, X_31
+        start();
+        if (warp == 3) times(M::kX + tri(3, 2), y_at(2, 1));
+        times(M::kX + tri(warp, warp), y_at(warp, 1));
+        finish(-1.0f);
+        put_x(warp, 1);
+    }
+    __syncthreads();
+    if (warp < 2) {          // X_20, X_30
+        start();
+        if (warp == 1) times(M::kX + tri(3, 2), y_at(2, 0));
+        times(M::kX + tri(2 + warp, 2 + warp), y_at(2 + warp, 0));
+        finish(-1.0f);
+        put_x(2 + warp, 0);
+    } else if (warp == 2) {
+        p_times(3, 1);
+        p_times(2, 1);
+    } else {
+        p_times(1, 0);
+        p_times(0, 0);
+        p_times(1, 1);
+        p_times(2, 2);
+    }
+    __syncthreads();
+    if (warp == 0) p_times(3, 0);
+    else if (warp == 1) p_times(2, 0);
+    else if (warp == 2) p_times(3, 2);
+    else p_times(3, 3);
 }
 
 // The walk.  Eight warps own 16 value columns of a head: four carry the state
@@ -1342,8 +1422,7 @@ int launch_scan(const DeltaArgs& a, const Chunk* chunks, cudaStream_t stream) {
 template <int DK>
 int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     Chunk* chunks = static_cast<Chunk*>(workspace);
-    // K and Q, then the blocks in their place
-    constexpr int kSmem = 2 * kChunk * DK * 2 > 24832 ? 2 * kChunk * DK * 2 : 24832;
+    constexpr int kSmem = ChunkSmem<DK>::kBytes;
     static std::atomic<uint64_t> done{0};
     int st = allow_smem(chunk_kernel<DK>, kSmem, done);
     if (st) return st;
