@@ -10,11 +10,16 @@
 // exactly before sin and cos are taken in fp32 (CUDA's sincospif).
 //
 // Bound by bytes (each row read once and written once; about 3 operations per
-// rotated element).  A block takes a few tokens: its first threads compute
-// the R/2 angles of each into shared memory, once for all heads, and find the
-// tokens' places in the cache; then all threads walk (token, head, 16-byte
-// vector) items, a rotated item being the two vectors of its halves, so that
-// every access is a 16-byte one and q may be rotated in place.
+// rotated element) as long as the addresses cost little: a row of 64, 128 or 256
+// lies across 8, 16 or 32 lanes, so that every access is 16 bytes of a full line
+// and the two halves of a pair meet by a shuffle.  A warp has one token: it
+// requests the token's rows, computes the R/2 angles with one lane each while they
+// are on their way, and keeps the eight pairs of each lane's place for all heads.
+// With few tokens up to eight warps share one, a part of the heads each.
+// Other head sizes go through a kernel that deals out items.
+// 8191 tokens of 8 + 2 + 2 heads of 256 (101 MB, 15.4 us at the copy rate): 25.4 us; with all
+// sizes dealt out as items, whose divisions cost more than the rows, 31.6; with four rows on
+// their way and twice the warps 27.4.
 #include "mixing.cuh"
 
 #include <cmath>
@@ -26,6 +31,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 4;   // tokens per block
+
+constexpr int kWarps = kThreads / 32;
+constexpr int kQRows = 8, kKvRows = 2;      // steps of q, and of k and v, on their way at once
 
 static __device__ unsigned g_mrope_dev_error;
 
@@ -43,7 +51,10 @@ struct RopeArgs {
     int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
     int64_t page_stride, table_cols;
     int tokens, q_heads, kv_heads, dim, page_size, num_pages, table_rows;
-    int per_block, in_place;
+    FastDiv page{1};
+    int per_block;             // tokens of a block
+    int share;                 // log2 of the warps that share a token
+    int in_place;              // q is its own output
 };
 
 // Rotates eight pairs: a' = a cos - b sin, b' = b cos + a sin, in fp32, one
@@ -60,6 +71,129 @@ __device__ __forceinline__ void rotate8(uint4& a, uint4& b, const float2* cs) {
     }
 }
 
+// Element offset of the token's slot in head 0 of the cache, -1: not written.
+__device__ __forceinline__ int64_t place_of(const RopeArgs& a, int tok) {
+    const int i = a.index[tok];
+    if (i < 0) return -1;
+    const int row = a.seq ? a.seq[tok] : tok;
+    const int page = a.page.div(i);
+    int p = -1;
+    if (row >= 0 && row < a.table_rows && page < a.table_cols) p = a.table[row * a.table_cols + page];
+    if (p >= 0 && p < a.num_pages) return p * a.page_stride + static_cast<int64_t>(i - page * a.page_size) * a.dim;
+    atomicOr(&g_mrope_dev_error, kDevErrIndex);
+    return -1;
+}
+__device__ __forceinline__ float2 turn_of(const mcv_mrope_spec& spec, const RopeArgs& a, int tok, int i) {
+    const double turns = static_cast<double>(a.positions[static_cast<int64_t>(spec.axis[i]) * a.tokens + tok]) * spec.turns[i];
+    float s, c;
+    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+    return make_float2(c, s);
+}
+
+// One step of rows: this lane's vector `x` and its partner's half, mine cos -+ other
+// sin in fp32, one rounding to the output's fp16 (s carries the sign).
+__device__ __forceinline__ void turn_vector(uint4& x, bool turn, int partner, const float (&c)[8], const float (&s)[8]) {
+    uint32_t* xp = &x.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t other = __shfl_sync(0xffffffffu, xp[i], partner);
+        const float2 m = __half22float2(u32_as_h2(xp[i])), o = __half22float2(u32_as_h2(other));
+        const uint32_t y = h2_as_u32(__floats2half2_rn(m.x * c[2 * i] + o.x * s[2 * i], m.y * c[2 * i + 1] + o.y * s[2 * i + 1]));
+        xp[i] = turn ? y : xp[i];
+    }
+}
+
+template <int VECS>
+__global__ void __launch_bounds__(kThreads, 2) mrope_rows_kernel(const __grid_constant__ mcv_mrope_spec spec, const RopeArgs a) {
+    constexpr int kPer = 32 / VECS;      // rows of a step
+    __shared__ float2 turns[kWarps][VECS * 4];
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int id = blockIdx.x * kWarps + warp;
+    const int tok = id >> a.share, mine = id & ((1 << a.share) - 1);
+    if (tok >= a.tokens) return;
+    const int sub = lane / VECS, vec = lane % VECS, step = kPer << a.share;
+    const int half = spec.rotary_dim / 2, nrot = half / 8;
+    const bool turned = vec < 2 * nrot, first = vec < nrot;
+
+    // rows q0 + r step of q, and so of k and v, whose steps the sharing warps take on from q's
+    const int q0 = mine * kPer + sub;
+    const int q_heads = a.in_place && !turned ? 0 : a.q_heads;      // what passes in place is there already
+    const uint4* qp = reinterpret_cast<const uint4*>(a.q + tok * a.q_ts + q0 * a.q_hs) + vec;
+    const int64_t qs = step * a.q_hs / 8;
+    uint4 xq[kQRows], xk[kKvRows], xv[kKvRows];
+#pragma unroll
+    for (int r = 0; r < kQRows; ++r) xq[r] = q0 + r * step < q_heads ? __ldg(qp + r * qs) : make_uint4(0, 0, 0, 0);
+    const uint4 *kp = nullptr, *vp = nullptr;
+    int64_t ks = 0, vs = 0, place = -1;
+    const int shift = (a.q_heads + kPer - 1) / kPer, kv0 = ((mine - shift) & ((1 << a.share) - 1)) * kPer + sub;
+    if (a.k) {
+        kp = reinterpret_cast<const uint4*>(a.k + tok * a.k_ts + kv0 * a.k_hs) + vec;
+        vp = reinterpret_cast<const uint4*>(a.v + tok * a.v_ts + kv0 * a.v_hs) + vec;
+        ks = step * a.k_hs / 8;
+        vs = step * a.v_hs / 8;
+#pragma unroll
+        for (int r = 0; r < kKvRows; ++r) {
+            const bool there = kv0 + r * step < a.kv_heads;
+            xk[r] = there ? __ldg(kp + r * ks) : make_uint4(0, 0, 0, 0);
+            xv[r] = there ? __ldg(vp + r * vs) : make_uint4(0, 0, 0, 0);
+        }
+        place = place_of(a, tok);
+    }
+    for (int i = lane; i < half; i += 32) turns[warp][i] = turn_of(spec, a, tok, i);
+    __syncwarp();
+    const int partner = turned ? (first ? lane + nrot : lane - nrot) : lane;
+    float c[8] = {}, s[8] = {};
+    if (turned) {
+        const float4* from = reinterpret_cast<const float4*>(&turns[warp][(first ? vec : vec - nrot) * 8]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 y = from[i];
+            c[2 * i] = y.x, c[2 * i + 1] = y.z;
+            s[2 * i] = first ? -y.y : y.y, s[2 * i + 1] = first ? -y.w : y.w;
+        }
+    }
+    uint4* op = reinterpret_cast<uint4*>(a.q_out + tok * a.o_ts + q0 * a.o_hs) + vec;
+    const int64_t os = step * a.o_hs / 8;
+    for (int base = 0;;) {
+#pragma unroll
+        for (int r = 0; r < kQRows; ++r) {
+            turn_vector(xq[r], turned, partner, c, s);
+            if (q0 + base + r * step < q_heads) op[r * os] = xq[r];
+        }
+        base += kQRows * step;
+        if (base >= a.q_heads) break;
+        qp += kQRows * qs;
+        op += kQRows * os;
+#pragma unroll
+        for (int r = 0; r < kQRows; ++r) xq[r] = q0 + base + r * step < q_heads ? __ldg(qp + r * qs) : make_uint4(0, 0, 0, 0);
+    }
+    if (place < 0) return;
+    const int64_t head = static_cast<int64_t>(a.page_size) * a.dim, cs = step * head / 8;
+    uint4* kc = reinterpret_cast<uint4*>(a.ck + place + kv0 * head) + vec;
+    uint4* vc = reinterpret_cast<uint4*>(a.cv + place + kv0 * head) + vec;
+    for (int base = 0;;) {
+#pragma unroll
+        for (int r = 0; r < kKvRows; ++r) {
+            turn_vector(xk[r], turned, partner, c, s);
+            if (kv0 + base + r * step < a.kv_heads) {
+                kc[r * cs] = xk[r];
+                vc[r * cs] = xv[r];
+            }
+        }
+        base += kKvRows * step;
+        if (base >= a.kv_heads) break;
+        kp += kKvRows * ks, vp += kKvRows * vs, kc += kKvRows * cs, vc += kKvRows * cs;
+#pragma unroll
+        for (int r = 0; r < kKvRows; ++r) {
+            const bool there = kv0 + base + r * step < a.kv_heads;
+            xk[r] = there ? __ldg(kp + r * ks) : make_uint4(0, 0, 0, 0);
+            xv[r] = there ? __ldg(vp + r * vs) : make_uint4(0, 0, 0, 0);
+        }
+    }
+}
+
 __global__ void __launch_bounds__(kThreads) mrope_kernel(const __grid_constant__ mcv_mrope_spec spec, RopeArgs a) {
     __shared__ float2 cs[kMaxTokens][MCV_MROPE_MAX_FREQS];
     __shared__ int64_t place[kMaxTokens];   // element offset of the token's slot in head 0, -1: not written
@@ -70,27 +204,11 @@ __global__ void __launch_bounds__(kThreads) mrope_kernel(const __grid_constant__
     const int nt = min(a.per_block, a.tokens - t0);
     if (a.k && threadIdx.x >= kThreads - nt) {
         const int t = kThreads - 1 - threadIdx.x;
-        const int i = a.index[t0 + t];
-        int64_t at = -1;
-        if (i >= 0) {
-            const int row = a.seq ? a.seq[t0 + t] : t0 + t;
-            const int64_t page = i / a.page_size;
-            int p = -1;
-            if (row >= 0 && row < a.table_rows && page < a.table_cols) p = a.table[row * a.table_cols + page];
-            if (p >= 0 && p < a.num_pages)
-                at = p * a.page_stride + static_cast<int64_t>(i - page * a.page_size) * a.dim;
-            else
-                atomicOr(&g_mrope_dev_error, kDevErrIndex);
-        }
-        place[t] = at;
+        place[t] = place_of(a, t0 + t);
     }
     for (int j = threadIdx.x; j < nt * half; j += kThreads) {
         const int t = j / half, i = j - t * half;
-        const double turns = static_cast<double>(a.positions[static_cast<int64_t>(spec.axis[i]) * a.tokens + t0 + t]) *
-                             spec.turns[i];
-        float s, c;
-        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-        cs[t][i] = make_float2(c, s);
+        cs[t][i] = turn_of(spec, a, t0 + t, i);
     }
     __syncthreads();
 
@@ -150,9 +268,23 @@ int check_in_place(const char* who, const mcv_rows* x, int64_t tokens, int64_t h
     return MCV_OK;
 }
 
-// Tokens per block: one while that fills the SMs less than twice, so that a
-// small batch spreads out; else four, which share the block's set-up.
-int tokens_per_block(int64_t tokens) { return tokens <= 8 * sm_count() ? 1 : kMaxTokens; }
+int launch_mrope(const mcv_mrope_spec& spec, RopeArgs& a, cudaStream_t stream) {
+    const int64_t sms = sm_count();
+    if (a.dim == 64 || a.dim == 128 || a.dim == 256) {
+        // eight warps a token while they all run at once, else as many as have their rows on their way at once
+        const int per = 256 / a.dim, q_steps = (a.q_heads + per - 1) / per, kv_steps = a.k ? (a.kv_heads + per - 1) / per : 0;
+        a.share = 0;
+        while (a.share < 3 && (q_steps > kQRows << a.share || kv_steps > kKvRows << a.share)) ++a.share;
+        if (static_cast<int64_t>(a.tokens) * 8 <= sms * 2 * kWarps) a.share = 3;
+        const unsigned grid = static_cast<unsigned>(((static_cast<int64_t>(a.tokens) << a.share) + kWarps - 1) / kWarps);
+        return launch(a.dim == 64 ? mrope_rows_kernel<8> : (a.dim == 128 ? mrope_rows_kernel<16> : mrope_rows_kernel<32>),
+                      dim3(grid), dim3(kThreads), 0, stream, spec, a);
+    }
+    // one token a block while that fills the SMs less than twice, else four, which share the block's set-up
+    a.per_block = a.tokens <= 8 * sms ? 1 : kMaxTokens;
+    const unsigned grid = static_cast<unsigned>((a.tokens + a.per_block - 1) / a.per_block);
+    return launch(mrope_kernel, dim3(grid), dim3(kThreads), 0, stream, spec, a);
+}
 
 }  // namespace
 
@@ -252,9 +384,7 @@ int mcv_mrope(const mcv_rows* x, void* out, const mcv_mrope_spec* spec, const vo
     a.tokens = static_cast<int>(tokens);
     a.q_heads = static_cast<int>(heads);
     a.dim = static_cast<int>(head_dim);
-    a.per_block = tokens_per_block(tokens);
-    const unsigned grid = static_cast<unsigned>((tokens + a.per_block - 1) / a.per_block);
-    return launch(mrope_kernel, dim3(grid), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), *spec, a);
+    return launch_mrope(*spec, a, static_cast<cudaStream_t>(stream));
 }
 
 int mcv_mrope_append_kv(const mcv_rows* q, void* q_out, const mcv_rows* k, const mcv_rows* v,
@@ -301,11 +431,10 @@ int mcv_mrope_append_kv(const mcv_rows* q, void* q_out, const mcv_rows* k, const
     a.kv_heads = cache->kv_heads;
     a.dim = cache->head_dim;
     a.page_size = cache->page_size;
+    a.page = FastDiv(static_cast<uint32_t>(cache->page_size));
     a.num_pages = cache->num_pages;
     a.table_rows = static_cast<int>(table_rows);
-    a.per_block = tokens_per_block(tokens);
-    const unsigned grid = static_cast<unsigned>((tokens + a.per_block - 1) / a.per_block);
-    return launch(mrope_kernel, dim3(grid), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), *spec, a);
+    return launch_mrope(*spec, a, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
