@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -828,10 +829,13 @@ _ref = ctypes.byref
 
 
 # The checks below run on every call of a decode step, so they are kept to a few
-# attribute reads: tensors are compared by device index, and the current stream
-# is taken as a raw handle.
+# attribute reads: tensors are compared by device index, the current stream is
+# taken as a raw handle, and the C structures are packed as bytes (a ctypes
+# structure takes several times as long to fill).
 _torch = None
 _fns = {}
+_pack_rows = struct.Struct("@3q").pack                # mcv_rows
+_pack_delta = struct.Struct("@9q6Pq4i2f").pack        # mcv_gated_delta
 
 
 def _setup():
@@ -843,14 +847,15 @@ def _setup():
     return torch
 
 
-def _f16_rows(t, what: str, dev: int) -> _Rows:
-    """[tokens, heads, dim] fp16 with a contiguous last dimension."""
-    if t.dtype is not _torch.float16 or t.get_device() != dev or t.dim() != 3:
+def _f16_rows(t, what: str, dev: int):
+    """Address, token and head stride of [tokens, heads, dim] fp16 with contiguous rows."""
+    stride = t.stride()
+    if t.dtype is not _torch.float16 or len(stride) != 3 or t.get_device() != dev:
         raise RuntimeError(f"mcv_b200: {what} must be float16 [tokens, heads, dim] on cuda:{dev}")
-    token, head, one = t.stride()
+    token, head, one = stride
     if one != 1 and t.shape[2] != 1:
         raise RuntimeError(f"mcv_b200: rows of {what} must be contiguous")
-    return _Rows(t.data_ptr(), token, head)
+    return t.data_ptr(), token, head
 
 
 def _dense(t, dtype, shape, what: str, dev: int):
@@ -927,9 +932,9 @@ def mrope(x, positions, rope: MRope, out, stream=None) -> None:
     [axes, tokens]; out is dense, or x itself."""
     torch = _torch or _setup()
     dev = x.get_device()
-    rows = _f16_rows(x, "x", dev)
+    rows = _pack_rows(*_f16_rows(x, "x", dev))
     n, heads, dim = x.shape
-    _run_on(dev, stream, "mrope", _ref(rows), _rows_out(x, out, "out", dev), rope._ref,
+    _run_on(dev, stream, "mrope", rows, _rows_out(x, out, "out", dev), rope._ref,
             _dense(positions, torch.int32, (rope.axes, n), "positions", dev), n, heads, dim)
 
 
@@ -946,8 +951,8 @@ def mrope_append_kv(q, k, v, positions, rope: MRope, cache: PagedKVCache, page_t
     if cache.dev != dev or k.shape != (n, cache.kv_heads, cache.head_dim) or v.shape != k.shape or dim != cache.head_dim:
         raise RuntimeError("mrope_append_kv: q, k, v and the cache do not fit together")
     rows, cols = page_table.shape
-    _run_on(dev, stream, "mrope_append_kv", _ref(_f16_rows(q, "q", dev)), _rows_out(q, q_out, "q_out", dev),
-            _ref(_f16_rows(k, "k", dev)), _ref(_f16_rows(v, "v", dev)), rope._ref,
+    _run_on(dev, stream, "mrope_append_kv", _pack_rows(*_f16_rows(q, "q", dev)), _rows_out(q, q_out, "q_out", dev),
+            _pack_rows(*_f16_rows(k, "k", dev)), _pack_rows(*_f16_rows(v, "v", dev)), rope._ref,
             _dense(positions, i32, (rope.axes, n), "positions", dev), cache._ref,
             _dense(page_table, i32, (rows, cols), "page_table", dev), rows, cols,
             _dense(seq, i32, (n,), "seq", dev), _dense(index, i32, (n,), "index", dev), n, heads)
@@ -978,28 +983,32 @@ def paged_attention_decode(q, cache: PagedKVCache, page_table, lengths, out, wor
     if workspace.get_device() != dev:
         raise RuntimeError("paged_attention_decode: workspace on another device")
     _, cols = page_table.shape
-    _run_on(dev, stream, "paged_attention_decode", _ref(_f16_rows(q, "q", dev)), cache._ref,
+    _run_on(dev, stream, "paged_attention_decode", _pack_rows(*_f16_rows(q, "q", dev)), cache._ref,
             _dense(page_table, i32, (b, cols), "page_table", dev), cols,
             _dense(lengths, i32, (b,), "lengths", dev), _dense(out, torch.float16, (b, heads, dim), "out", dev),
             _dense(lse, torch.float32, (b, heads), "lse", dev), b, heads, dim ** -0.5 if scale is None else scale,
             workspace.data_ptr(), workspace.nbytes)
 
 
-def _gated_delta(q, k, v, g, beta, state, out, state_out, index, batch, scale, l2_eps, dev) -> _GatedDelta:
+def _gated_delta(q, k, v, g, beta, state, out, state_out, index, batch, scale, l2_eps, dev) -> bytes:
+    """An mcv_gated_delta."""
     torch = _torch
     n, kh, dk = q.shape
     nv, vh, dv = v.shape
-    if k.shape != (n, kh, dk) or nv != n:
+    if k.shape != q.shape or nv != n:
         raise RuntimeError("gated_delta: q, k and v do not fit together")
     f32 = torch.float32
     any_state = state if state is not None else state_out
     slots = any_state.shape[0] if any_state is not None else batch
-    return _GatedDelta(
-        _f16_rows(q, "q", dev), _f16_rows(k, "k", dev), _f16_rows(v, "v", dev), _dense(g, f32, (n, vh), "g", dev),
-        _dense(beta, f32, (n, vh), "beta", dev), _dense(out, torch.float16, (n, vh, dv), "out", dev),
-        _dense(state, f32, (slots, vh, dk, dv), "state", dev), _dense(state_out, f32, (slots, vh, dk, dv), "state_out", dev),
-        _dense(index, torch.int32, (batch,), "index", dev), slots, kh, vh, dk, dv, dk ** -0.5 if scale is None else scale,
-        -1.0 if l2_eps is None else l2_eps)
+    gates, states = (n, vh), (slots, vh, dk, dv)
+    return _pack_delta(
+        *_f16_rows(q, "q", dev), *_f16_rows(k, "k", dev), *_f16_rows(v, "v", dev), _dense(g, f32, gates, "g", dev) or 0,
+        _dense(beta, f32, gates, "beta", dev) or 0, _dense(out, torch.float16, (n, vh, dv), "out", dev) or 0,
+        _dense(state, f32, states, "state", dev) or 0,
+        0 if state_out is None else (_dense(state_out, f32, states, "state_out", dev) if state_out is not state
+                                     else state.data_ptr()),
+        _dense(index, torch.int32, (batch,), "index", dev) or 0, slots, kh, vh, dk, dv,
+        dk ** -0.5 if scale is None else scale, -1.0 if l2_eps is None else l2_eps)
 
 
 def gated_delta_step(q, k, v, g, beta, state, out, state_out=None, index=None, scale=None, l2_eps=None,
@@ -1015,7 +1024,7 @@ def gated_delta_step(q, k, v, g, beta, state, out, state_out=None, index=None, s
     dev, batch = q.get_device(), q.shape[0]
     a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, batch, scale, l2_eps,
                      dev)
-    _run_on(dev, stream, "gated_delta_step", _ref(a), batch)
+    _run_on(dev, stream, "gated_delta_step", a, batch)
 
 
 def gated_delta_workspace(tokens: int, batch: int, v_heads: int, key_dim: int, value_dim: int, device="cuda"):
@@ -1042,5 +1051,5 @@ def gated_delta_prefill(q, k, v, g, beta, cu_seqlens, state, out, workspace, sta
     batch = cu_seqlens.shape[0] - 1
     a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, batch, scale, l2_eps,
                      dev)
-    _run_on(dev, stream, "gated_delta_prefill", _ref(a), _dense(cu_seqlens, torch.int32, (batch + 1,), "cu_seqlens", dev),
+    _run_on(dev, stream, "gated_delta_prefill", a, _dense(cu_seqlens, torch.int32, (batch + 1,), "cu_seqlens", dev),
             q.shape[0], batch, workspace.data_ptr(), workspace.nbytes)

@@ -96,7 +96,9 @@ def test_mrope(cuda, tokens, heads, dim, rotary, sections, interleaved):
 
 
 @pytest.mark.parametrize("tokens,hq,hk,dim,rotary,page", [(1, 8, 2, 256, 64, 16), (33, 4, 4, 64, 32, 7),
-                                                          (2000, 6, 1, 128, 128, 24), (9, 2, 2, 256, 64, 1)])
+                                                          (2000, 6, 1, 128, 128, 24), (9, 2, 2, 256, 64, 1),
+                                                          (700, 72, 20, 256, 64, 16), (50, 40, 33, 64, 64, 8),
+                                                          (1500, 12, 3, 80, 48, 16), (3, 2, 1, 512, 256, 4)])
 def test_mrope_append_kv(cuda, tokens, hq, hk, dim, rotary, page):
     """Scattered tokens of several sequences, some not written; slots that no
     token has stay as they were."""

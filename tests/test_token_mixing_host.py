@@ -3,6 +3,7 @@ touch a device, and the rope specification is filled as documented.  Status
 codes: 1 null, 2 shape, 3 alignment, 6 workspace, 7 value."""
 import ctypes
 import math
+import struct
 
 import pytest
 
@@ -173,3 +174,15 @@ def test_python_checks():
         mcv_b200.mrope(x, pos, rope, torch.zeros(3, 2, 72).half()[:, :, :64])
     with pytest.raises(mcv_b200.McvError):
         mcv_b200.MRope(64, [30])
+
+
+def test_packed_structures():
+    """The bytes that the binding passes are the C structures of the header."""
+    assert struct.calcsize("@3q") == ctypes.sizeof(mcv_b200._Rows)
+    assert struct.calcsize("@9q6Pq4i2f") == ctypes.sizeof(mcv_b200._GatedDelta)
+    assert mcv_b200._pack_rows(F, 24, 8) == bytes(mcv_b200._Rows(F, 24, 8))
+    a = mcv_b200._GatedDelta()
+    a.q, a.k, a.v = (mcv_b200._Rows(10 * i, 10 * i + 1, 10 * i + 2) for i in (1, 2, 3))
+    a.g, a.beta, a.out, a.state_in, a.state_out, a.state_index = 40, 50, 60, 70, 80, 90
+    a.slots, a.k_heads, a.v_heads, a.key_dim, a.value_dim, a.scale, a.l2_eps = 5, 6, 7, 8, 9, 0.5, 0.25
+    assert mcv_b200._pack_delta(10, 11, 12, 20, 21, 22, 30, 31, 32, 40, 50, 60, 70, 80, 90, 5, 6, 7, 8, 9, 0.5, 0.25) == bytes(a)
