@@ -989,6 +989,13 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // Waits for an mbarrier phase suspended, 10 ms at a time and 200 times at most.
 __device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
@@ -1356,8 +1363,10 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         }
         // the bulk copies have landed before the block's shared memory goes
         for (int c = max(0, chunks_here - 2); c < chunks_here; ++c) wait(&full[c & 1], c >> 1);
-    } else if (lane == 0) {
+    } else {
         // ---- MMA issue ----
+        // The warp stays together and an elected lane issues: 36 clocks an MMA beside 23 busy warps (74 from a
+        // branch of lane 0, 130 from a rolled loop).
         constexpr uint32_t kIdesc = instr_desc_f16(128, 128), kIdescT = instr_desc_f16(128, DK) | (1u << 16);   // B with N contiguous
         // descriptors count in 16 bytes; all are constants away from these
         const uint64_t tiles = smem_desc_sw128(base);
@@ -1369,40 +1378,48 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             const uint64_t kq = tiles + st, tp = tri + st, kt = turned + st;
             wait_one(&full[c & 1], c >> 1);
             wait_one(&o_done, c);      // the outputs have read D1 and D2
-            // rolled: each instruction of straight code would be fetched for one use
-#pragma unroll 1
+#pragma unroll
             for (int b = 0; b < C::kBatches; ++b) {
                 wait_one(&s_ready[b], c);
                 tc_fence_after();
-#pragma unroll 1
-                for (int k = b; k < DK / 16; k += C::kBatches) {
-                    const uint64_t d = kq + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
-                    mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, d, kIdesc, k > 0);
-                    mma_f16_ts(tmem + C::kD1, tmem + C::kSLo + k * 8, d, kIdesc, 1);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = b; k < DK / 16; k += C::kBatches) {
+                        const uint64_t d = kq + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
+                        mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, d, kIdesc, k > 0);
+                        mma_f16_ts(tmem + C::kD1, tmem + C::kSLo + k * 8, d, kIdesc, 1);
+                    }
+                    if (b == C::kBatches - 1) mma_commit(&made[0]);
                 }
+                __syncwarp();
             }
-            mma_commit(&made[0]);
             wait_one(&r_ready, c);
             tc_fence_after();
-#pragma unroll 1
-            for (int k = 0; k < 4; ++k) {
-                mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + k * 16, kIdesc, k > 0);
-                mma_f16_ts(tmem + C::kD2, tmem + C::kRLo + k * 8, tp + k * 16, kIdesc, 1);
-                mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + (C::kTile >> 4) + k * 16, kIdesc, 1);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + k * 16, kIdesc, k > 0);
+                    mma_f16_ts(tmem + C::kD2, tmem + C::kRLo + k * 8, tp + k * 16, kIdesc, 1);
+                    mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + (C::kTile >> 4) + k * 16, kIdesc, 1);
+                }
+                mma_commit(&made[1]);
             }
-            mma_commit(&made[1]);
+            __syncwarp();
             wait_one(&w_ready, c);
             tc_fence_after();
-#pragma unroll 1
-            for (int k = 0; k < 4; ++k) {
-                mma_f16_ts(tmem + C::kD3, tmem + C::kRHi + k * 8, kt + k * 128, kIdescT, 1);
-                mma_f16_ts(tmem + C::kD3, tmem + C::kRLo + k * 8, kt + k * 128, kIdescT, 1);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    mma_f16_ts(tmem + C::kD3, tmem + C::kRHi + k * 8, kt + k * 128, kIdescT, 1);
+                    mma_f16_ts(tmem + C::kD3, tmem + C::kRLo + k * 8, kt + k * 128, kIdescT, 1);
+                }
+                mma_commit(&made[2]);
+                mma_commit(&empty[c & 1]);
             }
-            mma_commit(&made[2]);
-            mma_commit(&empty[c & 1]);
+            __syncwarp();
         }
         // every MMA has ended before its operands and tensor memory go
-        if (chunks_here > 0) wait(&made[2], chunks_here - 1);
+        if (chunks_here > 0) wait_one(&made[2], chunks_here - 1);
     }
     __syncwarp();
     tc_fence_before();
