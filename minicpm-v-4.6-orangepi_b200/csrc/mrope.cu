@@ -17,9 +17,10 @@
 // are on their way, and keeps the eight pairs of each lane's place for all heads.
 // With few tokens up to eight warps share one, a part of the heads each.
 // Other head sizes go through a kernel that deals out items.
-// 8191 tokens of 8 + 2 + 2 heads of 256 (101 MB, 15.4 us at the copy rate): 25.4 us; with all
-// sizes dealt out as items, whose divisions cost more than the rows, 31.6; with four rows on
-// their way and twice the warps 27.4.
+// 8191 tokens of 8 + 2 + 2 heads of 256 (101 MB, 15.4 us at the copy rate): 21.7 us; in blocks of
+// eight warps 25.4, with all sizes dealt out as items, whose divisions cost more than the rows, 31.6.
+// What is left is latency: a warp's rows, place and angles are one chain of about 5 us, and the registers
+// that hold the rows on their way leave an SM 18 to 20 warps.
 #include "mixing.cuh"
 
 #include <cmath>
@@ -32,7 +33,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 4;   // tokens per block
 
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarps = 2;       // of a block of whole rows: small ones take each other's places without a wait
 constexpr int kQRows = 8, kKvRows = 2;      // steps of q, and of k and v, on their way at once
 
 static __device__ unsigned g_mrope_dev_error;
@@ -103,15 +104,17 @@ __device__ __forceinline__ void turn_vector(uint4& x, bool turn, int partner, co
     }
 }
 
-template <int VECS>
-__global__ void __launch_bounds__(kThreads, 2) mrope_rows_kernel(const __grid_constant__ mcv_mrope_spec spec, const RopeArgs a) {
+// BLOCKS resident: 8 leave a thread the 128 registers that hold all its rows on their way (200 tokens of 16 + 2 + 2
+// heads 4.7 us, with 9 5.2); 9 hide more of the tokens' latency when there are many (8191 tokens 21.7 us, with 8 24.1).
+template <int VECS, int BLOCKS>
+__global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const __grid_constant__ mcv_mrope_spec spec, const RopeArgs a) {
     constexpr int kPer = 32 / VECS;      // rows of a step
     __shared__ float2 turns[kWarps][VECS * 4];
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int id = blockIdx.x * kWarps + warp;
-    const int tok = id >> a.share, mine = id & ((1 << a.share) - 1);
+    const unsigned id = blockIdx.x * kWarps + warp;     // fewer than 2^29 tokens by at most eight warps
+    const int tok = static_cast<int>(id >> a.share), mine = id & ((1 << a.share) - 1);
     if (tok >= a.tokens) return;
     const int sub = lane / VECS, vec = lane % VECS, step = kPer << a.share;
     const int half = spec.rotary_dim / 2, nrot = half / 8;
@@ -275,10 +278,13 @@ int launch_mrope(const mcv_mrope_spec& spec, RopeArgs& a, cudaStream_t stream) {
         const int per = 256 / a.dim, q_steps = (a.q_heads + per - 1) / per, kv_steps = a.k ? (a.kv_heads + per - 1) / per : 0;
         a.share = 0;
         while (a.share < 3 && (q_steps > kQRows << a.share || kv_steps > kKvRows << a.share)) ++a.share;
-        if (static_cast<int64_t>(a.tokens) * 8 <= sms * 2 * kWarps) a.share = 3;
+        if (static_cast<int64_t>(a.tokens) * 8 <= sms * 8 * kWarps) a.share = 3;
         const unsigned grid = static_cast<unsigned>(((static_cast<int64_t>(a.tokens) << a.share) + kWarps - 1) / kWarps);
-        return launch(a.dim == 64 ? mrope_rows_kernel<8> : (a.dim == 128 ? mrope_rows_kernel<16> : mrope_rows_kernel<32>),
-                      dim3(grid), dim3(kThreads), 0, stream, spec, a);
+        if (grid > sms * 8)
+            return launch(a.dim == 64 ? mrope_rows_kernel<8, 9> : (a.dim == 128 ? mrope_rows_kernel<16, 9> : mrope_rows_kernel<32, 9>),
+                          dim3(grid), dim3(kWarps * 32), 0, stream, spec, a);
+        return launch(a.dim == 64 ? mrope_rows_kernel<8, 8> : (a.dim == 128 ? mrope_rows_kernel<16, 8> : mrope_rows_kernel<32, 8>),
+                      dim3(grid), dim3(kWarps * 32), 0, stream, spec, a);
     }
     // one token a block while that fills the SMs less than twice, else four, which share the block's set-up
     a.per_block = a.tokens <= 8 * sms ? 1 : kMaxTokens;
