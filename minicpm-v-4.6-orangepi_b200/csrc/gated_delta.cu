@@ -26,7 +26,7 @@ struct DeltaArgs {
     const float* state_in;    // null: zeros
     float* state_out;         // null: not kept
     const int32_t* index;     // null: sequence b has slot b
-    const int32_t* cu;        // null: sequence b is token b
+    const int32_t* cu;        // prompts: sequence b has tokens cu[b] .. cu[b + 1] - 1
     int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
     int batch, tokens, slots, v_heads, share, dv;
     float scale, l2_eps;
@@ -35,8 +35,8 @@ struct DeltaArgs {
 // The tokens and the state slot of sequence b; false: nothing to do.
 __device__ __forceinline__ bool sequence(const DeltaArgs& a, int b, int& begin, int& end, int& slot) {
     slot = a.index ? a.index[b] : b;
-    begin = a.cu ? a.cu[b] : b;
-    end = a.cu ? a.cu[b + 1] : b + 1;
+    begin = a.cu[b];
+    end = a.cu[b + 1];
     if (slot < 0) return false;
     if (slot >= a.slots || begin < 0 || end < begin || end > a.tokens) {
         if (threadIdx.x == 0) atomicOr(&g_gated_delta_dev_error, kDevErrIndex);
@@ -45,19 +45,18 @@ __device__ __forceinline__ bool sequence(const DeltaArgs& a, int b, int& begin, 
     return true;
 }
 
-// ---- one token after the other -------------------------------------------------
+// ---- one token per sequence -----------------------------------------------------
 //
-// Bound by the state's bytes (8 Dk Dv per head and token step, read and written
-// once; 7 operations per element).  A warp keeps 16 columns of a head's state in
-// registers - 8 lane groups take every eighth row, four lanes a 64-byte row
-// piece - and works without any block-wide step: the products S^T k and S^T q
-// are taken in one pass over the old state, since
-// S_new^T q = e^g S^T q + (k.q) u.
+// Bound by the state's bytes (8 Dk Dv per head, read and written once; 7 operations
+// per element).  A warp keeps 16 columns of a head's state in registers - 8 lane
+// groups take every eighth row, four lanes a 64-byte row piece - and works
+// without any block-wide step: the products S^T k and S^T q are taken in one
+// pass over the old state, since S_new^T q = e^g S^T q + (k.q) u.
 constexpr int kCols = 16;
 constexpr int kStepWarps = 2;
 
 template <int DK>
-__global__ void __launch_bounds__(kStepWarps * 32) recurrent_kernel(const DeltaArgs a) {
+__global__ void __launch_bounds__(kStepWarps * 32) step_kernel(const DeltaArgs a) {
     constexpr int kRows = DK / 8;    // rows of a lane
     constexpr int kPer = DK / 32;    // q, k elements of a lane
     __shared__ float2 kq[kStepWarps][DK];
@@ -66,93 +65,88 @@ __global__ void __launch_bounds__(kStepWarps * 32) recurrent_kernel(const DeltaA
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = (blockIdx.x * (blockDim.x >> 5) + warp) * kCols + (lane & 3) * 4;
     const int rg = lane >> 2;
-    const int b = blockIdx.z, h = blockIdx.y;
-    int begin, end, slot;
-    if (!sequence(a, b, begin, end, slot) || col >= a.dv) return;
+    const int64_t b = blockIdx.z;
+    const int h = blockIdx.y, slot = a.index ? a.index[b] : static_cast<int>(b);
+    if (slot < 0 || col >= a.dv) return;
+    if (slot >= a.slots) {
+        if (threadIdx.x == 0) atomicOr(&g_gated_delta_dev_error, kDevErrIndex);
+        return;
+    }
     const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + rg) * a.dv + col;
     float4 s[kRows];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
-        s[i] = a.state_in ? *reinterpret_cast<const float4*>(a.state_in + at + static_cast<int64_t>(i) * 8 * a.dv)
-                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < kRows; ++i) s[i] = *reinterpret_cast<const float4*>(a.state_in + at + static_cast<int64_t>(i) * 8 * a.dv);
     const int kh = h / a.share;
-    for (int64_t t = begin; t < end; ++t) {
-        const __half* qp = a.q + t * a.q_ts + kh * a.q_hs + lane * kPer;
-        const __half* kp = a.k + t * a.k_ts + kh * a.k_hs + lane * kPer;
-        const uint2 vv = *reinterpret_cast<const uint2*>(a.v + t * a.v_ts + h * a.v_hs + col);
-        const float decay = expf(a.g[t * a.v_heads + h]), beta = a.beta[t * a.v_heads + h];
-        float qx[kPer], kx[kPer];
+    const __half* qp = a.q + b * a.q_ts + kh * a.q_hs + lane * kPer;
+    const __half* kp = a.k + b * a.k_ts + kh * a.k_hs + lane * kPer;
+    const uint2 vv = *reinterpret_cast<const uint2*>(a.v + b * a.v_ts + h * a.v_hs + col);
+    const float decay = expf(a.g[b * a.v_heads + h]), beta = a.beta[b * a.v_heads + h];
+    float qx[kPer], kx[kPer];
 #pragma unroll
-        for (int i = 0; i < kPer; i += 2) {
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(qp + i));
-            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(kp + i));
-            qx[i] = x.x, qx[i + 1] = x.y, kx[i] = y.x, kx[i + 1] = y.y;
-        }
-        float qq = 0.0f, kk = 0.0f, qk = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            qq += qx[i] * qx[i];
-            kk += kx[i] * kx[i];
-            qk += qx[i] * kx[i];
-        }
-        qk = warp_sum(qk);
-        float rq = a.scale, rk = 1.0f;
-        if (a.l2_eps >= 0.0f) {
-            rq *= 1.0f / sqrtf(warp_sum(qq) + a.l2_eps);
-            rk = 1.0f / sqrtf(warp_sum(kk) + a.l2_eps);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) kq[warp][lane * kPer + i] = make_float2(kx[i] * rk, qx[i] * rq);
-        __syncwarp();
-        float ks[4] = {}, qs[4] = {};
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const float2 w = kq[warp][rg + 8 * i];
-            ks[0] += w.x * s[i].x, ks[1] += w.x * s[i].y, ks[2] += w.x * s[i].z, ks[3] += w.x * s[i].w;
-            qs[0] += w.y * s[i].x, qs[1] += w.y * s[i].y, qs[2] += w.y * s[i].z, qs[3] += w.y * s[i].w;
-        }
-        const float2 v01 = __half22float2(u32_as_h2(vv.x)), v23 = __half22float2(u32_as_h2(vv.y));
-        const float v[4] = {v01.x, v01.y, v23.x, v23.y};
-        float u[4], o[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                ks[c] += __shfl_xor_sync(0xffffffffu, ks[c], x);
-                qs[c] += __shfl_xor_sync(0xffffffffu, qs[c], x);
-            }
-            u[c] = beta * (v[c] - decay * ks[c]);
-            o[c] = decay * qs[c] + qk * rq * rk * u[c];
-        }
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const float k = kq[warp][rg + 8 * i].x;
-            s[i].x = decay * s[i].x + k * u[0];
-            s[i].y = decay * s[i].y + k * u[1];
-            s[i].z = decay * s[i].z + k * u[2];
-            s[i].w = decay * s[i].w + k * u[3];
-        }
-        if (rg == 0)
-            *reinterpret_cast<uint2*>(a.out + (t * a.v_heads + h) * a.dv + col) =
-                make_uint2(h2_as_u32(__floats2half2_rn(o[0], o[1])), h2_as_u32(__floats2half2_rn(o[2], o[3])));
+    for (int i = 0; i < kPer; i += 2) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(qp + i));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(kp + i));
+        qx[i] = x.x, qx[i + 1] = x.y, kx[i] = y.x, kx[i + 1] = y.y;
     }
-    if (a.state_out) {
+    float qq = 0.0f, kk = 0.0f, qk = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
-            *reinterpret_cast<float4*>(a.state_out + at + static_cast<int64_t>(i) * 8 * a.dv) = s[i];
+    for (int i = 0; i < kPer; ++i) {
+        qq += qx[i] * qx[i];
+        kk += kx[i] * kx[i];
+        qk += qx[i] * kx[i];
     }
+    qk = warp_sum(qk);
+    float rq = a.scale, rk = 1.0f;
+    if (a.l2_eps >= 0.0f) {
+        rq *= 1.0f / sqrtf(warp_sum(qq) + a.l2_eps);
+        rk = 1.0f / sqrtf(warp_sum(kk) + a.l2_eps);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) kq[warp][lane * kPer + i] = make_float2(kx[i] * rk, qx[i] * rq);
+    __syncwarp();
+    float ks[4] = {}, qs[4] = {};
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const float2 w = kq[warp][rg + 8 * i];
+        ks[0] += w.x * s[i].x, ks[1] += w.x * s[i].y, ks[2] += w.x * s[i].z, ks[3] += w.x * s[i].w;
+        qs[0] += w.y * s[i].x, qs[1] += w.y * s[i].y, qs[2] += w.y * s[i].z, qs[3] += w.y * s[i].w;
+    }
+    const float2 v01 = __half22float2(u32_as_h2(vv.x)), v23 = __half22float2(u32_as_h2(vv.y));
+    const float v[4] = {v01.x, v01.y, v23.x, v23.y};
+    float u[4], o[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+            ks[c] += __shfl_xor_sync(0xffffffffu, ks[c], x);
+            qs[c] += __shfl_xor_sync(0xffffffffu, qs[c], x);
+        }
+        u[c] = beta * (v[c] - decay * ks[c]);
+        o[c] = decay * qs[c] + qk * rq * rk * u[c];
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const float k = kq[warp][rg + 8 * i].x;
+        s[i].x = decay * s[i].x + k * u[0];
+        s[i].y = decay * s[i].y + k * u[1];
+        s[i].z = decay * s[i].z + k * u[2];
+        s[i].w = decay * s[i].w + k * u[3];
+        *reinterpret_cast<float4*>(a.state_out + at + static_cast<int64_t>(i) * 8 * a.dv) = s[i];
+    }
+    if (rg == 0)
+        *reinterpret_cast<uint2*>(a.out + (b * a.v_heads + h) * a.dv + col) =
+            make_uint2(h2_as_u32(__floats2half2_rn(o[0], o[1])), h2_as_u32(__floats2half2_rn(o[2], o[3])));
 }
 
-int run_recurrent(const DeltaArgs& a, int dk, cudaStream_t stream) {
+int run_step(const DeltaArgs& a, int dk, cudaStream_t stream) {
     // Two warps a block (one while that leaves SMs without a block): a block's registers are only free for the
     // next when its last warp ends, and with eight warps a block 160 sequences of 32 heads took 114 us instead of
-    // 101 (654 MB, 100 at the copy rate).
+    // 99 (654 MB, 100 at the copy rate).
     const int cols = a.dv / kCols;
     int warps = cols > 1 ? kStepWarps : 1;
     if (static_cast<int64_t>(a.batch) * a.v_heads * ((cols + warps - 1) / warps) < 2 * sm_count()) warps = 1;
     const dim3 grid((cols + warps - 1) / warps, a.v_heads, a.batch);
-    return launch(dk == 128 ? recurrent_kernel<128> : recurrent_kernel<64>, grid, dim3(warps * 32), 0, stream, a);
+    return launch(dk == 128 ? step_kernel<128> : step_kernel<64>, grid, dim3(warps * 32), 0, stream, a);
 }
 
 // ---- prompts, in chunks of 64 tokens -----------------------------------------------
@@ -175,8 +169,8 @@ int run_recurrent(const DeltaArgs& a, int dk, cudaStream_t stream) {
 // both fp16, the lo products in accumulators of their own: 22 bits of each
 // value, down to an absolute 2^-36, so results keep fp32's accuracy where
 // a single fp16 operand would leave 2^-11.  (State values and written rows are
-// below fp16's 65504 then; with |k| <= 1, beta <= 1 and g <= 0 they are bounded by
-// the state's start and the sum of |v|.)
+// below fp16's 65504 then; with |k| <= 1, beta <= 2 and g <= 0 they are bounded by
+// the state's start and twice the sum of |v|.)
 constexpr int kChunk = 64;
 constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;
 
@@ -187,19 +181,19 @@ __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uin
 }
 
 // One chunk's share of the workspace: T and P T (its rows for q of norm 1 or less),
-// both at most 1 in magnitude and kept times 2^14 as hi + lo, and the scales.  Of the
+// both at most 4 in magnitude (1 with beta <= 1) and kept times 2^13 as hi + lo, and the scales.  Of the
 // two matrices only the 16x16 blocks on and below the diagonal are kept, as 8x8
 // matrices of 128 contiguous bytes, 2 i + 2 of them for each of the two groups of
 // eight rows of block row i: fragments are written and read whole, ldmatrix
 // hits no bank twice, and a chunk is one copy.
 constexpr int kTri = 40 * 64;        // elements of a triangle
-constexpr float kTriScale = 16384.0f;
+constexpr float kTriScale = 8192.0f;
 struct Chunk {
     __half tp[2][2][kTri];           // [hi, lo][T, P T]
     float ck[kChunk];                // e^G r_k
     float cq[kChunk];                // scale e^G r_q
-    float cs[kChunk];                // e^(G_C - G) r_k 2^-14
-    float oq[kChunk];                // scale r_q |q's row in P T|^-1 2^-14
+    float cs[kChunk];                // e^(G_C - G) r_k 2^-13
+    float oq[kChunk];                // scale r_q |q's row in P T|^-1 2^-13
     float keep;                      // e^G_C
     float pad[63];
 };
@@ -261,8 +255,10 @@ __device__ __forceinline__ void mma_split(float (&acc)[2][4], float (&acc_lo)[2]
 // X_10 and X_32, then the lower left quarter -X_B (A_BA X_A), so that no warp
 // waits for more than four steps; and P X beside and behind them.
 //
-// Bound by its instructions (about 1.5 us a chunk and SM for 53 KB, which would
-// take 1.2): 512 threads a SM had the loads and the steps' latencies showing.
+// 8256 chunks of 64 tokens (16 heads of 128, 409 MB with what stays in L2): 136 us, 2.4 us a chunk and
+// SM, where the copy rate would take 67.  Bound by its instructions and shared memory: 9200 warp
+// instructions a chunk, issued in 54 % of the cycles, shared memory busy in 67 %, DRAM in 37 %
+// (152 us before the triangle's blocks were dealt out evenly, 262 with a warp a block row).
 template <int DK>
 struct ChunkSmem {
     static constexpr int kKQ = 2 * kChunk * DK * 2;
@@ -524,7 +520,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[q][e] = sign * (y[q][e] + kLoInv * yl[q][e]);
     };
-    // y times beta 2^14 as block (i, j) of the record's T (0) or P T (1)
+    // y times beta 2^13 as block (i, j) of the record's T (0) or P T (1)
     auto record = [&](int which, int i, int j) {
         const int in = 2 * i * (i + 1) * 64 + j * 128 + g * 8 + t * 2;
 #pragma unroll
@@ -1527,7 +1523,7 @@ int mcv_gated_delta_step(const mcv_gated_delta* args, int64_t batch, mcv_stream_
     int st = fill_args("gated_delta_step", args, batch, batch, a);
     if (st) return st;
     if (!a.state_in || !a.state_out) return fail(MCV_ERR_NULL, "gated_delta_step: null state");
-    return run_recurrent(a, args->key_dim, static_cast<cudaStream_t>(stream));
+    return run_step(a, args->key_dim, static_cast<cudaStream_t>(stream));
 }
 
 size_t mcv_gated_delta_workspace_size(int64_t tokens, int64_t batch, int64_t v_heads, int64_t key_dim,

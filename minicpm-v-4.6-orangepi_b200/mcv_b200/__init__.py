@@ -1041,7 +1041,8 @@ def gated_delta_prefill(q, k, v, g, beta, cu_seqlens, state, out, workspace, sta
     """Packed prompts of the gated delta rule (mcv_gated_delta_prefill): tokens
     cu_seqlens[b] .. cu_seqlens[b+1] (int32 [batch + 1]) belong to sequence b.
     state None: sequences start from zero.  Final states go to state_out, or back
-    into state; with neither they are not kept.  The rest as gated_delta_step."""
+    into state; with neither they are not kept.  g <= 0 and 0 <= beta <= 2.  The
+    rest as gated_delta_step."""
     torch = _torch or _setup()
     dev = q.get_device()
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
