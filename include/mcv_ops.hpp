@@ -287,6 +287,148 @@ int64_t lm_head_greedy_index_w8a8(const T& x, const T& embed_int8, const T& embe
     return idx;
 }
 
+/* ---- Token mixing -------------------------------------------------------
+ * Over dense tensors; rows that lie apart (a slice of a wider projection) go
+ * through the C calls, whose mcv_rows carry strides. */
+namespace detail {
+template <class T>
+mcv_rows heads_of(const T& t, const char* what) {   /* [tokens, heads, head_dim] */
+    if (t.shape().size() != 3) throw Error(MCV_ERR_SHAPE, std::string(what) + ": expected [tokens, heads, head_dim]");
+    return mcv_rows{t.data(), t.shape()[1] * t.shape()[2], t.shape()[2]};
+}
+template <class T>
+void need_shape(const T& t, const std::vector<int64_t>& shape, const char* what) {
+    if (t.shape() != shape) throw Error(MCV_ERR_SHAPE, std::string(what) + ": shapes do not fit together");
+}
+}  // namespace detail
+
+/* A layer's paged cache from its fp16 tensors [pages, kv_heads, page_size, head_dim]. */
+template <class T>
+mcv_kv_cache paged_kv_cache(T& k, T& v) {
+    if (k.shape().size() != 4 || k.shape() != v.shape())
+        throw Error(MCV_ERR_SHAPE, "paged_kv_cache: k and v must be [pages, kv_heads, page_size, head_dim]");
+    const auto& s = k.shape();
+    for (int64_t n : s)
+        if (n < 1 || n > 0x7fffffff) throw Error(MCV_ERR_SHAPE, "paged_kv_cache: bad dimensions");
+    return mcv_kv_cache{k.data(), v.data(), s[1] * s[2] * s[3], static_cast<int32_t>(s[0]), static_cast<int32_t>(s[2]),
+                        static_cast<int32_t>(s[1]), static_cast<int32_t>(s[3])};
+}
+
+/* out = x with its rotary positions; positions int32 [axes, tokens]. */
+template <class T>
+void mrope(const T& x, const T& positions, const mcv_mrope_spec& spec, T& out, cudaStream_t stream, bool sync = false) {
+    const mcv_rows rows = detail::heads_of(x, "mrope");
+    const auto& s = x.shape();
+    detail::need_shape(out, s, "mrope");
+    detail::need_shape(positions, {spec.axes, s[0]}, "mrope");
+    check(mcv_mrope(&rows, out.data(), &spec, positions.data(), s[0], s[1], s[2], stream), "mrope");
+    finish(stream, sync, "mrope");
+}
+
+/* q_out = q rotated; k rotated and v written to the cache (mcv_mrope_append_kv);
+ * `seq` nullptr: token t belongs to row t of page_table [rows, pages]. */
+template <class T>
+void mrope_append_kv(const T& q, const T& k, const T& v, const T& positions, const mcv_mrope_spec& spec,
+                     const mcv_kv_cache& cache, const T& page_table, const T* seq, const T& index, T& q_out,
+                     cudaStream_t stream, bool sync = false) {
+    const mcv_rows qr = detail::heads_of(q, "mrope_append_kv"), kr = detail::heads_of(k, "mrope_append_kv"),
+                   vr = detail::heads_of(v, "mrope_append_kv");
+    const int64_t n = q.shape()[0];
+    detail::need_shape(q, {n, q.shape()[1], cache.head_dim}, "mrope_append_kv");
+    detail::need_shape(k, {n, cache.kv_heads, cache.head_dim}, "mrope_append_kv");
+    detail::need_shape(v, k.shape(), "mrope_append_kv");
+    detail::need_shape(q_out, q.shape(), "mrope_append_kv");
+    detail::need_shape(positions, {spec.axes, n}, "mrope_append_kv");
+    detail::need_shape(index, {n}, "mrope_append_kv");
+    if (seq) detail::need_shape(*seq, {n}, "mrope_append_kv");
+    detail::need_rank2(page_table, "mrope_append_kv");
+    check(mcv_mrope_append_kv(&qr, q_out.data(), &kr, &vr, &spec, positions.data(), &cache, page_table.data(),
+                              page_table.shape()[0], page_table.shape()[1], seq ? seq->data() : nullptr, index.data(), n,
+                              q.shape()[1], stream),
+          "mrope_append_kv");
+    finish(stream, sync, "mrope_append_kv");
+}
+
+/* One new token per sequence over the cache (mcv_paged_attention_decode); `lse`
+ * may be nullptr; `workspace` holds mcv_paged_attention_workspace_size bytes,
+ * zero-filled once. */
+template <class T>
+void paged_attention_decode(const T& q, const mcv_kv_cache& cache, const T& page_table, const T& lengths, float scale,
+                            T& out, T* lse, void* workspace, size_t workspace_bytes, cudaStream_t stream,
+                            bool sync = false) {
+    const mcv_rows qr = detail::heads_of(q, "paged_attention_decode");
+    const int64_t b = q.shape()[0], heads = q.shape()[1];
+    detail::need_shape(q, {b, heads, cache.head_dim}, "paged_attention_decode");
+    detail::need_shape(out, q.shape(), "paged_attention_decode");
+    detail::need_shape(lengths, {b}, "paged_attention_decode");
+    detail::need_rank2(page_table, "paged_attention_decode");
+    detail::need_shape(page_table, {b, page_table.shape()[1]}, "paged_attention_decode");
+    if (lse) detail::need_shape(*lse, {b, heads}, "paged_attention_decode");
+    check(mcv_paged_attention_decode(&qr, &cache, page_table.data(), page_table.shape()[1], lengths.data(), out.data(),
+                                     lse ? lse->data() : nullptr, b, heads, scale, workspace, workspace_bytes, stream),
+          "paged_attention_decode");
+    finish(stream, sync, "paged_attention_decode");
+}
+
+namespace detail {
+template <class T>
+mcv_gated_delta delta_of(const T& q, const T& k, const T& v, const T& g, const T& beta, const T* state_in, T* state_out,
+                         const T* state_index, int64_t batch, float scale, float l2_eps, T& out, const char* what) {
+    mcv_gated_delta a{};
+    a.q = heads_of(q, what), a.k = heads_of(k, what), a.v = heads_of(v, what);
+    const int64_t n = q.shape()[0], dk = q.shape()[2], vh = v.shape()[1], dv = v.shape()[2];
+    need_shape(k, q.shape(), what);
+    need_shape(v, {n, vh, dv}, what);
+    need_shape(g, {n, vh}, what);
+    need_shape(beta, {n, vh}, what);
+    need_shape(out, v.shape(), what);
+    const T* any = state_in ? state_in : state_out;
+    a.slots = any && !any->shape().empty() ? any->shape()[0] : batch;
+    if (state_in) need_shape(*state_in, {a.slots, vh, dk, dv}, what);
+    if (state_out) need_shape(*state_out, {a.slots, vh, dk, dv}, what);
+    if (state_index) need_shape(*state_index, {batch}, what);
+    if (q.shape()[1] > 0x7fffffff || vh > 0x7fffffff || dk > 0x7fffffff || dv > 0x7fffffff)
+        throw Error(MCV_ERR_SHAPE, std::string(what) + ": bad dimensions");
+    a.g = g.data(), a.beta = beta.data(), a.out = out.data();
+    a.state_in = state_in ? state_in->data() : nullptr;
+    a.state_out = state_out ? state_out->data() : nullptr;
+    a.state_index = state_index ? state_index->data() : nullptr;
+    a.k_heads = static_cast<int32_t>(q.shape()[1]), a.v_heads = static_cast<int32_t>(vh);
+    a.key_dim = static_cast<int32_t>(dk), a.value_dim = static_cast<int32_t>(dv);
+    a.scale = scale, a.l2_eps = l2_eps;
+    return a;
+}
+}  // namespace detail
+
+/* One token per sequence of the gated delta rule (mcv_gated_delta_step);
+ * state_out may be state_in; state_index nullptr: sequence b has slot b. */
+template <class T>
+void gated_delta_step(const T& q, const T& k, const T& v, const T& g, const T& beta, const T& state_in, T& state_out,
+                      const T* state_index, float scale, float l2_eps, T& out, cudaStream_t stream, bool sync = false) {
+    if (q.shape().empty()) throw Error(MCV_ERR_SHAPE, "gated_delta_step: expected [tokens, heads, head_dim]");
+    const int64_t batch = q.shape()[0];
+    const mcv_gated_delta a = detail::delta_of(q, k, v, g, beta, &state_in, &state_out, state_index, batch, scale,
+                                               l2_eps, out, "gated_delta_step");
+    check(mcv_gated_delta_step(&a, batch, stream), "gated_delta_step");
+    finish(stream, sync, "gated_delta_step");
+}
+
+/* Packed prompts (mcv_gated_delta_prefill); cu_seqlens int32 [batch + 1];
+ * state_in, state_out and state_index may be nullptr; `workspace` holds
+ * mcv_gated_delta_workspace_size bytes. */
+template <class T>
+void gated_delta_prefill(const T& q, const T& k, const T& v, const T& g, const T& beta, const T& cu_seqlens,
+                         const T* state_in, T* state_out, const T* state_index, float scale, float l2_eps, T& out,
+                         void* workspace, size_t workspace_bytes, cudaStream_t stream, bool sync = false) {
+    if (cu_seqlens.shape().size() != 1) throw Error(MCV_ERR_SHAPE, "gated_delta_prefill: cu_seqlens must be [batch + 1]");
+    const int64_t batch = cu_seqlens.shape()[0] - 1;
+    const mcv_gated_delta a = detail::delta_of(q, k, v, g, beta, state_in, state_out, state_index, batch, scale, l2_eps,
+                                               out, "gated_delta_prefill");
+    check(mcv_gated_delta_prefill(&a, cu_seqlens.data(), q.shape()[0], batch, workspace, workspace_bytes, stream),
+          "gated_delta_prefill");
+    finish(stream, sync, "gated_delta_prefill");
+}
+
 }  // namespace mcv_ops
 
 #endif
