@@ -828,47 +828,34 @@ class _GatedDelta(ctypes.Structure):
 _ref = ctypes.byref
 
 
-# The checks below run on every call of a decode step, so they are kept to a few
-# attribute reads: tensors are compared by device index, the current stream is
+# The checks below run on every call of a decode step, so they are kept short: tensors
+# are looked at by a native module (csrc/tensors.cpp), the current stream is
 # taken as a raw handle, and the C structures are packed as bytes (a ctypes
 # structure takes several times as long to fill).
 _torch = None
+_f16_rows = _dense = _rows_out = None                  # of the native module
 _fns = {}
 _pack_rows = struct.Struct("@3q").pack                # mcv_rows
 _pack_delta = struct.Struct("@9q6Pq4i2f").pack        # mcv_gated_delta
 
 
 def _setup():
-    global _torch
+    global _torch, _f16_rows, _dense, _rows_out
     import torch
-    _torch = torch
+    try:
+        from . import _tensors
+    except ImportError as e:
+        raise RuntimeError("mcv_b200/_tensors.so not built; run __graft_entry__.build()") from e
+    _torch, _f16_rows, _dense, _rows_out = torch, _tensors.rows, _tensors.dense, _tensors.rows_out
     for name in ("mrope", "mrope_append_kv", "paged_attention_decode", "gated_delta_step", "gated_delta_prefill"):
         _fns[name] = getattr(lib(), "mcv_" + name)
     return torch
 
 
-def _f16_rows(t, what: str, dev: int):
-    """Address, token and head stride of [tokens, heads, dim] fp16 with contiguous rows."""
-    stride = t.stride()
-    if t.dtype is not _torch.float16 or len(stride) != 3 or t.get_device() != dev:
-        raise RuntimeError(f"mcv_b200: {what} must be float16 [tokens, heads, dim] on cuda:{dev}")
-    token, head, one = stride
-    if one != 1 and t.shape[2] != 1:
-        raise RuntimeError(f"mcv_b200: rows of {what} must be contiguous")
-    return t.data_ptr(), token, head
-
-
-def _dense(t, dtype, shape, what: str, dev: int):
-    """Address of a contiguous tensor of this type and shape (None: NULL)."""
-    if t is None:
-        return None
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
-        raise RuntimeError(f"mcv_b200: {what} must be a contiguous {dtype} tensor {list(shape)} on cuda:{dev}")
-    return t.data_ptr()
-
-
 def _run_on(dev: int, stream, name: str, *args) -> None:
     """Calls mcv_<name>(*args, stream) with device `dev` current."""
+    if dev < 0:
+        raise RuntimeError(f"{name}: tensors must be on a CUDA device")
     handle = _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
     if dev == _torch._C._cuda_getDevice():
         st = _fns[name](*args, handle)
@@ -917,14 +904,6 @@ class MRope:
         _check(lib().mcv_mrope_init(ctypes.byref(self._c), rotary_dim, self.axes, arr, int(interleaved), theta),
                "mrope_init")
         self._ref = _ref(self._c)
-
-
-def _rows_out(x, out, what: str, dev: int):
-    """Address of a dense output of x's shape, or of x itself (in place)."""
-    if out is x or (out.data_ptr() == x.data_ptr() and out.shape == x.shape and out.stride() == x.stride()
-                    and out.dtype == x.dtype):
-        return x.data_ptr()
-    return _dense(out, x.dtype, x.shape, what, dev)
 
 
 def mrope(x, positions, rope: MRope, out, stream=None) -> None:
@@ -980,8 +959,8 @@ def paged_attention_decode(q, cache: PagedKVCache, page_table, lengths, out, wor
     b, heads, dim = q.shape
     if cache.dev != dev or dim != cache.head_dim:
         raise RuntimeError("paged_attention_decode: q and the cache do not fit together")
-    if workspace.get_device() != dev:
-        raise RuntimeError("paged_attention_decode: workspace on another device")
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        raise RuntimeError("paged_attention_decode: workspace must be contiguous and on q's device")
     _, cols = page_table.shape
     _run_on(dev, stream, "paged_attention_decode", _pack_rows(*_f16_rows(q, "q", dev)), cache._ref,
             _dense(page_table, i32, (b, cols), "page_table", dev), cols,
@@ -1047,8 +1026,8 @@ def gated_delta_prefill(q, k, v, g, beta, cu_seqlens, state, out, workspace, sta
     dev = q.get_device()
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
         raise RuntimeError("gated_delta_prefill: cu_seqlens must be [batch + 1]")
-    if workspace.get_device() != dev:
-        raise RuntimeError("gated_delta_prefill: workspace on another device")
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        raise RuntimeError("gated_delta_prefill: workspace must be contiguous and on q's device")
     batch = cu_seqlens.shape[0] - 1
     a = _gated_delta(q, k, v, g, beta, state, out, state if state_out is None else state_out, index, batch, scale, l2_eps,
                      dev)
