@@ -8,6 +8,7 @@
 #include "tcgen05.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace mcv {
 unsigned take_gated_delta_device_error();
@@ -182,10 +183,10 @@ __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uin
 
 // One chunk's share of the workspace: T and P T (its rows for q of norm 1 or less),
 // both at most 4 in magnitude (1 with beta <= 1) and kept times 2^13 as hi + lo, and the scales.  Of the
-// two matrices only the 16x16 blocks on and below the diagonal are kept, as 8x8
-// matrices of 128 contiguous bytes, 2 i + 2 of them for each of the two groups of
-// eight rows of block row i: fragments are written and read whole, ldmatrix
-// hits no bank twice, and a chunk is one copy.
+// two matrices only the 16x16 blocks on and below the diagonal are kept, block column
+// after block column, each block as four 8x8 matrices of 128 contiguous bytes:
+// fragments are written and read whole, ldmatrix hits no bank twice, a block
+// column is an MMA's operand of 64 - 16 j rows, and a chunk is one copy.
 constexpr int kTri = 40 * 64;        // elements of a triangle
 constexpr float kTriScale = 8192.0f;
 struct Chunk {
@@ -200,10 +201,9 @@ struct Chunk {
 static_assert(sizeof(Chunk) % 128 == 0, "chunks stay aligned");
 constexpr uint32_t kTriBytes = 4 * kTri * 2, kScaleBytes = (4 * kChunk + 4) * 4;
 constexpr uint32_t kChunkBytes = kTriBytes + kScaleBytes;      // in use
-__host__ __device__ constexpr int tri_at(int r, int c) {
-    const int i = r >> 4;
-    return (2 * i * (i + 1) + ((r >> 3) & 1) * (2 * i + 2) + (c >> 3)) * 64 + (r & 7) * 8 + (c & 7);
-}
+// Block (i, j) of a triangle, in blocks of 512 bytes; i counts on from column j's start.
+__host__ __device__ constexpr int tri_column(int j) { return j * (9 - j) / 2; }
+__host__ __device__ constexpr int tri_block(int i, int j) { return tri_column(j) + i - j; }
 
 // The slots of sequence b begin at cu[b] / 64 + b: ranges of ceil(len / 64) from
 // there on never overlap, since floor(x + y) >= floor(x) + floor(y).
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
     };
     // y times beta 2^13 as block (i, j) of the record's T (0) or P T (1)
     auto record = [&](int which, int i, int j) {
-        const int in = 2 * i * (i + 1) * 64 + j * 128 + g * 8 + t * 2;
+        const int in = tri_block(i, j) * 256 + g * 8 + t * 2;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const float2 b = *reinterpret_cast<const float2*>(&bt[j * 16 + q * 8 + 2 * t]);
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
             for (int e = 0; e < 4; e += 2) {
                 uint32_t u, l;
                 split_f16(y[q][e] * (b.x * kTriScale), y[q][e + 1] * (b.y * kTriScale), u, l);
-                const int at = in + (e / 2) * (2 * i + 2) * 64 + q * 64;
+                const int at = in + (e / 2) * 128 + q * 64;
                 *reinterpret_cast<uint32_t*>(&out.tp[0][which][at]) = u;
                 *reinterpret_cast<uint32_t*>(&out.tp[1][which][at]) = l;
             }
@@ -718,8 +718,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
     const int blk = outputs ? 3 - warp : warp;       // this warp's 16 tokens of a chunk
     const int a_row = lane & 15, a_vec = lane >> 4;                                // A operand
     const int b_row = (lane & 7) + (lane >> 4) * 8, b_vec = (lane >> 3) & 1;       // B operand, rows = n
-    // this warp's block row of a triangle of the record: its start, and the lane's row address in a 16x16 block
-    const uint32_t tri_row = 2 * blk * (blk + 1) * 128 + (lane >> 4) * (2 * blk + 2) * 128 + ((lane >> 3) & 1) * 128 + (lane & 7) * 16;
+    const uint32_t tri_row = blk * 512 + lane * 16;       // this lane's row of block (blk, j) of a triangle, from block (0, j)
     auto state_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + 2 * group) : "memory"); };
     auto group_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(2 + 2 * group) : "memory"); };
     auto scale_pair = [&](uint32_t sc, int which, int n) {
@@ -769,8 +768,8 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
                 uint32_t rh[4], rl[4], ph[4], pl[4];
                 ldsm4(rh, tile_at<8>(r_hi, a_row, j * 2 + a_vec));
                 ldsm4(rl, tile_at<8>(r_lo, a_row, j * 2 + a_vec));
-                ldsm4(ph, p_hi + j * 256);
-                ldsm4(pl, p_hi + C::kLoPart + j * 256);
+                ldsm4(ph, p_hi + tri_block(0, j) * 512);
+                ldsm4(pl, p_hi + C::kLoPart + tri_block(0, j) * 512);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     mma16816(x[n], rh, ph[2 * n], ph[2 * n + 1]);
@@ -877,8 +876,8 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
             uint32_t rh[4], rl[4], th[4], tl[4];
             ldsm4(rh, tile_at<8>(r_hi, a_row, j * 2 + a_vec));
             ldsm4(rl, tile_at<8>(r_lo, a_row, j * 2 + a_vec));
-            ldsm4(th, t_hi + j * 256);
-            ldsm4(tl, t_hi + C::kLoPart + j * 256);
+            ldsm4(th, t_hi + tri_block(0, j) * 512);
+            ldsm4(tl, t_hi + C::kLoPart + tri_block(0, j) * 512);
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 mma16816(x[n], rh, th[2 * n], th[2 * n + 1]);
@@ -941,8 +940,9 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 // One block per head (128 value columns), the columns as the MMA's M = 128 rows, so
 // that every product has N = 128 and runs at the tensor core's rate:
 //   D1 = S^T [K; Q]^T;  D2 = R^T [T; P T]^T;  D3 = W^T K  with W = diag(cs) U,
-// the left operands from tensor memory (S^T, then R^T and W^T in its place: a
-// shared-memory operand each side would take all of its bandwidth), K's tile of
+// the left operands from tensor memory (R^T and W^T in the place of the halves of D1
+// and D2 that they are made from: a shared-memory operand each side would take all of
+// its bandwidth), the state's halves of D1 and D2 ahead of the outputs', K's tile of
 // tokens by rows serving both as [K; Q] and, read with N contiguous, as W's
 // factor.  The state itself lives in D3: keep S is put there before the product
 // adds to it.  A row of an accumulator, one value column, belongs to one
@@ -968,16 +968,16 @@ struct Walk {
     static constexpr int kThreads = 768;          // state 16 warps, outputs 4, loading 3, MMA issue 1
     static constexpr int kSub = DK / 64;          // 128-byte tiles of 64 dims
     static constexpr int kTile = 128 * 128;
-    static constexpr int kTp = kSub * kTile;      // [K; Q], then [T; P T] hi, lo: 128 rows of 64, in 8x8 matrices
-    static constexpr int kV = kTp + 2 * kTile;    // 64 tokens of 128 values
-    static constexpr int kScales = kV + kChunk * 256;
-    static constexpr int kStage = kScales + 2048;
+    static constexpr int kTp = kSub * kTile;      // [K; Q], then the chunk's record: triangles and scales
+    static constexpr int kScales = kTp + kTriBytes;
+    static constexpr int kV = kTp + 22 * 1024;    // 64 tokens of 128 values
+    static constexpr int kStage = kV + kChunk * 256;
     static constexpr int kSmem = 2 * kStage + 1024;
     static constexpr int kPart = DK / 4;          // state rows of a thread
     static constexpr int kBatches = kPart / 16;
     // tensor-memory columns
-    static constexpr uint32_t kD1 = 0, kD2 = 128, kD3 = 256, kSHi = 384, kSLo = 448, kRHi = 384, kRLo = 416;
-    static_assert(kScaleBytes <= 2048 && kSmem <= 232448 - 16384, "shared memory");
+    static constexpr uint32_t kD1 = 0, kD2 = 128, kD3 = 256, kSHi = 384, kSLo = 448;
+    static_assert(kChunkBytes <= 22 * 1024 && kStage % 1024 == 0 && kSmem <= 232448 - 16384, "shared memory");
 };
 
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
@@ -1034,10 +1034,10 @@ __device__ __forceinline__ float2 row_scale(float bound) {
 }
 
 // K-major operand of 8x8 matrices of 128 bytes without swizzle: the next 8 of K 128
-// bytes on, the next 8 rows 1024.
+// bytes on, the next 8 rows 256.
 __device__ __forceinline__ uint64_t smem_desc_plain(uint32_t saddr) {
     return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>(128 >> 4) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
+           (static_cast<uint64_t>(256 >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
 }
 
 template <int DK>
@@ -1045,7 +1045,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     using C = Walk<DK>;
     constexpr int kVecs = DK / 8;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[2], empty[2], s_ready[2], r_ready, w_ready, made[3], o_done, scaled;
+    __shared__ __align__(8) uint64_t full[2], empty[2], s_ready[2], r_ready, w_ready, made[4], o_done, scaled;
     __shared__ float2 most[3][4][128];      // [chunk % 3][part][row]: max|S|, max|v|
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1063,7 +1063,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         }
         mbar_init(&r_ready, 16);
         mbar_init(&w_ready, 16);
-        for (int i = 0; i < 3; ++i) mbar_init(&made[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&made[i], 1);
         mbar_init(&o_done, 4);
         mbar_init(&scaled, 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1140,13 +1140,13 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_ready[b]);
         };
-        // R or W of this part's 16 tokens
-        auto put_row = [&](const float (&x)[16], uint64_t* ready) {
+        // R or W of this part's 16 tokens as hi and lo operand, in the place of the product that it was made from
+        auto put_row = [&](const float (&x)[16], uint32_t place, uint64_t* ready) {
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) split_f16(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-            tmem_st8(lane_at + C::kRHi + part * 8, hi);
-            tmem_st8(lane_at + C::kRLo + part * 8, lo);
+            tmem_st8(lane_at + place + part * 16, hi);
+            tmem_st8(lane_at + place + part * 16 + 8, lo);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
@@ -1205,7 +1205,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 for (int e = 0; e < 4; ++e)
                     x[i + e] = __half2float(*reinterpret_cast<const __half*>(vp + (i + e) * 256)) * now.x - cp[e] * x[i + e];
             }
-            put_row(x, &r_ready);
+            put_row(x, C::kD1, &r_ready);
             wait(&made[1], c);
             tc_fence_after();
             tmem_ld16(lane_at + C::kD2 + part * 16, x);
@@ -1214,7 +1214,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 const float4 cs = *reinterpret_cast<const float4*>(sc + 2 * kChunk + i);
                 x[i] *= cs.x, x[i + 1] *= cs.y, x[i + 2] *= cs.z, x[i + 3] *= cs.w;
             }
-            put_row(x, &w_ready);
+            put_row(x, C::kD2, &w_ready);
             if (lane == 0) mbar_arrive(&empty[c & 1]);
             // while the last product is made: the next chunk's scale and decay
             const bool last = c + 1 == chunks_here;
@@ -1269,7 +1269,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             const float* sc = scales_of(c);
             wait(&full[c & 1], c >> 1);
             const float unit = scale.next(c, most[c % 3], row).y;
-            wait(&made[1], c);
+            wait(&made[3], c);
             tc_fence_after();
             const int left = col < a.dv ? end - begin - c * kChunk - odd : 0;      // of this lane's tokens
 #pragma unroll 1
@@ -1313,45 +1313,37 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         const __half* q0 = a.q + kh * a.q_hs;
         const __half* v0 = a.v + h * a.v_hs + col0;
         const Chunk* rec = chunks + first_chunk(begin, b) * a.v_heads + h;
-        // 32 runs of 8x8 matrices (two parts, two matrices, eight groups of rows) from the record's packed
-        // triangles to their places among zeros, and the scales: eleven copies per warp, since a warp's
-        // lanes issue theirs one by one
-        const int run = (lt >> 5) * 11 + lane, part = run >> 4, which = (run >> 3) & 1, rg = run & 7;
-        const bool scales = run == 32;
-        const uint32_t run_to = scales ? C::kScales : C::kTp + part * C::kTile + (which * 8 + rg) * 1024;
-        const uint32_t run_bytes = scales ? kScaleBytes : (2 * (rg >> 1) + 2) * 128;
-        const uint32_t run_from = scales ? kTriBytes : ((part * 2 + which) * kTri + tri_at(rg * 8, 0)) * 2;
-        for (int i = lt; i < 2 * 2 * C::kTile / 16; i += C::kLoaders) {
-            const int st = i / (2 * C::kTile / 16), at = i % (2 * C::kTile / 16);
-            *reinterpret_cast<uint4*>(smem + st * C::kStage + C::kTp + at * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        asm volatile("bar.sync 2, 96;" ::: "memory");      // zeros first, copies behind them
+        // rows of `vecs` vectors of 16 bytes, `n` of them there, one vector of every few rows per thread
+        auto copy_rows = [&](uint32_t to, const __half* from, int64_t stride, auto vecs, int n, bool live, auto place) {
+            constexpr int kStep = C::kLoaders / decltype(vecs)::value;
+            const int x = lt % decltype(vecs)::value;
+            const __half* p = from + (lt / decltype(vecs)::value) * stride + x * 8;
+#pragma unroll 2
+            for (int r = lt / decltype(vecs)::value; r < kChunk; r += kStep, p += kStep * stride) {
+                const bool ok = live && r < n;
+                cp_async16_or_zero(to + place(r, x), ok ? p : from, ok);
+            }
+        };
+        auto swizzled = [](int r, int x) { return static_cast<uint32_t>((x >> 3) * C::kTile + r * 128 + (((x & 7) ^ (r & 7)) << 4)); };
+        auto plain = [](int r, int x) { return static_cast<uint32_t>(r * 256 + x * 16); };
+        using Vecs = std::integral_constant<int, kVecs>;
+        using VVecs = std::integral_constant<int, 16>;
+        const bool v_live = col0 + (lt & 15) * 8 < a.dv;
         for (int c = 0; c < chunks_here; ++c) {
             const int st = c & 1;
             if (c >= 2) wait(&empty[st], (c >> 1) - 1);
             const uint32_t stage = base + st * C::kStage;
             fence_proxy_async_smem();      // the stage's reads come before the copies into it
-            if (lt == 0) mbar_expect_tx(&full[st], kChunkBytes);
-            if (lane < 11) bulk_load(smem + st * C::kStage + run_to, reinterpret_cast<const char*>(rec) + run_from, run_bytes, &full[st]);
+            if (lt == 0) {
+                mbar_expect_tx(&full[st], kChunkBytes);
+                bulk_load(smem + st * C::kStage + C::kTp, rec, kChunkBytes, &full[st]);
+            }
             rec += a.v_heads;
-            const int t0 = begin + c * kChunk;
-            const int n = min(kChunk, end - t0);
-#pragma unroll 2
-            for (int i = lt; i < kChunk * kVecs; i += C::kLoaders) {
-                const int r = i / kVecs, x = i % kVecs;
-                const bool ok = r < n;
-                const int64_t tok = t0 + (ok ? r : 0);
-                const uint32_t dst = stage + (x >> 3) * C::kTile + r * 128 + (((x & 7) ^ (r & 7)) << 4);
-                cp_async16_or_zero(dst, k0 + tok * a.k_ts + x * 8, ok);
-                cp_async16_or_zero(dst + kChunk * 128, q0 + tok * a.q_ts + x * 8, ok);
-            }
-#pragma unroll 2
-            for (int i = lt; i < kChunk * 16; i += C::kLoaders) {
-                const int r = i >> 4, x = i & 15;
-                const bool ok = r < n && col0 + x * 8 < a.dv;
-                cp_async16_or_zero(stage + C::kV + r * 256 + x * 16, ok ? v0 + static_cast<int64_t>(t0 + r) * a.v_ts + x * 8 : a.v, ok);
-            }
+            const int64_t t0 = begin + c * kChunk;
+            const int n = min(kChunk, end - begin - c * kChunk);
+            copy_rows(stage, k0 + t0 * a.k_ts, a.k_ts, Vecs(), n, true, swizzled);
+            copy_rows(stage + kChunk * 128, q0 + t0 * a.q_ts, a.q_ts, Vecs(), n, true, swizzled);
+            copy_rows(stage + C::kV, v0 + t0 * a.v_ts, a.v_ts, VVecs(), n, v_live, plain);
             cp_async_commit();
             cp_async_wait<0>();
             fence_proxy_async_smem();      // the MMAs read through the async proxy
@@ -1363,7 +1355,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         // ---- MMA issue ----
         // The warp stays together and an elected lane issues: 36 clocks an MMA beside 23 busy warps (74 from a
         // branch of lane 0, 130 from a rolled loop).
-        constexpr uint32_t kIdesc = instr_desc_f16(128, 128), kIdescT = instr_desc_f16(128, DK) | (1u << 16);   // B with N contiguous
+        constexpr uint32_t kIdesc = instr_desc_f16(128, kChunk), kIdescT = instr_desc_f16(128, DK) | (1u << 16);   // B with N contiguous
+        constexpr uint64_t kQ = (kChunk * 128) >> 4;      // from K to Q
         // descriptors count in 16 bytes; all are constants away from these
         const uint64_t tiles = smem_desc_sw128(base);
         const uint64_t tri = smem_desc_plain(base + C::kTp);
@@ -1372,33 +1365,50 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         for (int c = 0; c < chunks_here; ++c) {
             const uint64_t st = static_cast<uint64_t>((c & 1) * (C::kStage >> 4));
             const uint64_t kq = tiles + st, tp = tri + st, kt = turned + st;
+            auto state_product = [&](int k, int half) {
+                const uint64_t d = kq + half * kQ + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
+                const uint32_t to = tmem + C::kD1 + half * kChunk;
+                mma_f16_ts(to, tmem + C::kSHi + k * 8, d, kIdesc, k > 0);
+                mma_f16_ts(to, tmem + C::kSLo + k * 8, d, kIdesc, 1);
+            };
+            // 16 tokens reach the outputs from themselves on
+            auto row_product = [&](int half) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t to = tmem + C::kD2 + half * kChunk + k * 16, r = tmem + C::kD1 + k * 16;
+                    const uint32_t idesc = instr_desc_f16(128, kChunk - k * 16);
+                    const uint64_t hi = tp + ((half * kTri * 2 + tri_column(k) * 512) >> 4), lo = hi + ((2 * kTri * 2) >> 4);
+                    mma_f16_ts(to, r, hi, idesc, k > 0);
+                    mma_f16_ts(to, r + 8, hi, idesc, 1);
+                    mma_f16_ts(to, r, lo, idesc, 1);
+                }
+            };
             wait_one(&full[c & 1], c >> 1);
-            wait_one(&o_done, c);      // the outputs have read D1 and D2
 #pragma unroll
             for (int b = 0; b < C::kBatches; ++b) {
                 wait_one(&s_ready[b], c);
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = b; k < DK / 16; k += C::kBatches) {
-                        const uint64_t d = kq + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
-                        mma_f16_ts(tmem + C::kD1, tmem + C::kSHi + k * 8, d, kIdesc, k > 0);
-                        mma_f16_ts(tmem + C::kD1, tmem + C::kSLo + k * 8, d, kIdesc, 1);
-                    }
+                    for (int k = b; k < DK / 16; k += C::kBatches) state_product(k, 0);
                     if (b == C::kBatches - 1) mma_commit(&made[0]);
                 }
                 __syncwarp();
             }
-            wait_one(&r_ready, c);
+            wait_one(&o_done, c);      // the outputs have read their halves of D1 and D2
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + k * 16, kIdesc, k > 0);
-                    mma_f16_ts(tmem + C::kD2, tmem + C::kRLo + k * 8, tp + k * 16, kIdesc, 1);
-                    mma_f16_ts(tmem + C::kD2, tmem + C::kRHi + k * 8, tp + (C::kTile >> 4) + k * 16, kIdesc, 1);
-                }
+                for (int k = 0; k < DK / 16; ++k) state_product(k, 1);
+            }
+            __syncwarp();
+            wait_one(&r_ready, c);
+            tc_fence_after();
+            if (elect_one()) {
+                row_product(0);
                 mma_commit(&made[1]);
+                row_product(1);
+                mma_commit(&made[3]);
             }
             __syncwarp();
             wait_one(&w_ready, c);
@@ -1406,8 +1416,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    mma_f16_ts(tmem + C::kD3, tmem + C::kRHi + k * 8, kt + k * 128, kIdescT, 1);
-                    mma_f16_ts(tmem + C::kD3, tmem + C::kRLo + k * 8, kt + k * 128, kIdescT, 1);
+                    mma_f16_ts(tmem + C::kD3, tmem + C::kD2 + k * 16, kt + k * 128, kIdescT, 1);
+                    mma_f16_ts(tmem + C::kD3, tmem + C::kD2 + k * 16 + 8, kt + k * 128, kIdescT, 1);
                 }
                 mma_commit(&made[2]);
                 mma_commit(&empty[c & 1]);
