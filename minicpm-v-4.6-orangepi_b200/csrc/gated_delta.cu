@@ -1047,6 +1047,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[2], empty[2], s_ready[2], r_ready, w_ready, made[4], o_done, scaled;
     __shared__ float2 most[3][4][128];      // [chunk % 3][part][row]: max|S|, max|v|
+    __shared__ __align__(16) float out_scales[2][2 * kChunk];      // [chunk % 2]: cq, oq
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -1266,8 +1267,12 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         const int64_t step = 2 * static_cast<int64_t>(a.v_heads) * a.dv;
         __half* to = a.out + ((static_cast<int64_t>(begin) + odd) * a.v_heads + h) * a.dv + (col & ~1);
         for (int c = 0; c < chunks_here; ++c) {
-            const float* sc = scales_of(c);
+            // the outputs are done last: their scales are copied, and the stage is free for the next chunk before that
+            float* sc = out_scales[c & 1];
             wait(&full[c & 1], c >> 1);
+            sc[row] = scales_of(c)[(row < kChunk ? kChunk : 2 * kChunk) + row];
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+            if (lane == 0) mbar_arrive(&empty[c & 1]);
             const float unit = scale.next(c, most[c % 3], row).y;
             wait(&made[3], c);
             tc_fence_after();
@@ -1280,8 +1285,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 float cq[16], oq[16], o[16];
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    *reinterpret_cast<float4*>(cq + i) = *reinterpret_cast<const float4*>(sc + kChunk + b * 16 + i);
-                    *reinterpret_cast<float4*>(oq + i) = *reinterpret_cast<const float4*>(sc + 3 * kChunk + b * 16 + i);
+                    *reinterpret_cast<float4*>(cq + i) = *reinterpret_cast<const float4*>(sc + b * 16 + i);
+                    *reinterpret_cast<float4*>(oq + i) = *reinterpret_cast<const float4*>(sc + kChunk + b * 16 + i);
                 }
                 tmem_wait(x);
                 tmem_wait(y);
@@ -1301,10 +1306,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             if (c + 1 < chunks_here) wait(&scaled, c + 1);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&o_done);
-                mbar_arrive(&empty[c & 1]);
-            }
+            if (lane == 0) mbar_arrive(&o_done);
         }
     } else if (warp < 23) {
         // ---- loading ----
