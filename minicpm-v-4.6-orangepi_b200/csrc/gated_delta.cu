@@ -972,7 +972,8 @@ struct Walk {
     static constexpr int kScales = kTp + kTriBytes;
     static constexpr int kV = kTp + 22 * 1024;    // 64 tokens of 128 values
     static constexpr int kStage = kV + kChunk * 256;
-    static constexpr int kSmem = 2 * kStage + 1024;
+    static constexpr int kStages = 3;
+    static constexpr int kSmem = kStages * kStage + 1024;
     static constexpr int kPart = DK / 4;          // state rows of a thread
     static constexpr int kBatches = kPart / 16;
     // tensor-memory columns
@@ -1023,6 +1024,10 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
+// Arrives when all of this thread's cp.async so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -1045,7 +1050,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     using C = Walk<DK>;
     constexpr int kVecs = DK / 8;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[2], empty[2], s_ready[2], r_ready, w_ready, made[4], o_done, scaled;
+    __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], s_ready[2], r_ready, w_ready, made[4], o_done, scaled;
     __shared__ float2 most[3][4][128];      // [chunk % 3][part][row]: max|S|, max|v|
     __shared__ __align__(16) float out_scales[2][2 * kChunk];      // [chunk % 2]: cq, oq
     __shared__ uint32_t tmem_slot;
@@ -1057,11 +1062,11 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&full[i], C::kLoaders + 1);      // the loading threads, and the announcement of the bulk copies
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(&full[i], C::kLoaders + 1);      // the loading threads, and the announcement of the bulk copy
             mbar_init(&empty[i], 21);      // state and output warps, and the MMAs
-            mbar_init(&s_ready[i], 16);
         }
+        for (int i = 0; i < 2; ++i) mbar_init(&s_ready[i], 16);
         mbar_init(&r_ready, 16);
         mbar_init(&w_ready, 16);
         for (int i = 0; i < 4; ++i) mbar_init(&made[i], 1);
@@ -1095,7 +1100,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     auto wait_one = [&](uint64_t* bar, uint32_t parity) {
         if (!dead && !mbar_wait(bar, parity & 1)) gave_up();
     };
-    auto scales_of = [&](int c) { return reinterpret_cast<const float*>(smem + (c & 1) * C::kStage + C::kScales); };
+    auto scales_of = [&](int c) { return reinterpret_cast<const float*>(smem + c % C::kStages * C::kStage + C::kScales); };
     // A row's scale and its inverse, chunk by chunk.
     struct Scale {
         float s = 0.0f, v = 0.0f;      // bound of the state before the chunk; max|v| of the chunk
@@ -1154,8 +1159,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             if (lane == 0) mbar_arrive(ready);
         };
         auto most_v = [&](int c) {
-            wait(&full[c & 1], c >> 1);
-            const unsigned char* p = v_at + (c & 1) * C::kStage;
+            wait(&full[c % C::kStages], c / C::kStages);
+            const unsigned char* p = v_at + c % C::kStages * C::kStage;
             __half m = __float2half_rn(0.0f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) m = __hmax(m, __habs(*reinterpret_cast<const __half*>(p + i * 256)));
@@ -1197,7 +1202,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             wait(&made[0], c);
             tc_fence_after();
             tmem_ld16(lane_at + C::kD1 + part * 16, x);
-            const unsigned char* vp = v_at + (c & 1) * C::kStage;
+            const unsigned char* vp = v_at + c % C::kStages * C::kStage;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const float4 ck = *reinterpret_cast<const float4*>(sc + i);
@@ -1216,7 +1221,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 x[i] *= cs.x, x[i + 1] *= cs.y, x[i + 2] *= cs.z, x[i + 3] *= cs.w;
             }
             put_row(x, C::kD2, &w_ready);
-            if (lane == 0) mbar_arrive(&empty[c & 1]);
+            if (lane == 0) mbar_arrive(&empty[c % C::kStages]);
             // while the last product is made: the next chunk's scale and decay
             const bool last = c + 1 == chunks_here;
             float2 next = now;
@@ -1269,10 +1274,10 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         for (int c = 0; c < chunks_here; ++c) {
             // the outputs are done last: their scales are copied, and the stage is free for the next chunk before that
             float* sc = out_scales[c & 1];
-            wait(&full[c & 1], c >> 1);
+            wait(&full[c % C::kStages], c / C::kStages);
             sc[row] = scales_of(c)[(row < kChunk ? kChunk : 2 * kChunk) + row];
             asm volatile("bar.sync 2, 128;" ::: "memory");
-            if (lane == 0) mbar_arrive(&empty[c & 1]);
+            if (lane == 0) mbar_arrive(&empty[c % C::kStages]);
             const float unit = scale.next(c, most[c % 3], row).y;
             wait(&made[3], c);
             tc_fence_after();
@@ -1332,8 +1337,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         using VVecs = std::integral_constant<int, 16>;
         const bool v_live = col0 + (lt & 15) * 8 < a.dv;
         for (int c = 0; c < chunks_here; ++c) {
-            const int st = c & 1;
-            if (c >= 2) wait(&empty[st], (c >> 1) - 1);
+            const int st = c % C::kStages;
+            if (c >= C::kStages) wait(&empty[st], c / C::kStages - 1);
             const uint32_t stage = base + st * C::kStage;
             fence_proxy_async_smem();      // the stage's reads come before the copies into it
             if (lt == 0) {
@@ -1346,13 +1351,10 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             copy_rows(stage, k0 + t0 * a.k_ts, a.k_ts, Vecs(), n, true, swizzled);
             copy_rows(stage + kChunk * 128, q0 + t0 * a.q_ts, a.q_ts, Vecs(), n, true, swizzled);
             copy_rows(stage + C::kV, v0 + t0 * a.v_ts, a.v_ts, VVecs(), n, v_live, plain);
-            cp_async_commit();
-            cp_async_wait<0>();
-            fence_proxy_async_smem();      // the MMAs read through the async proxy
-            mbar_arrive(&full[st]);
+            cp_async_arrive(&full[st]);      // once this thread's copies have landed
         }
-        // the bulk copies have landed before the block's shared memory goes
-        for (int c = max(0, chunks_here - 2); c < chunks_here; ++c) wait(&full[c & 1], c >> 1);
+        // all copies have landed before the block's shared memory goes
+        for (int c = max(0, chunks_here - C::kStages); c < chunks_here; ++c) wait(&full[c % C::kStages], c / C::kStages);
     } else {
         // ---- MMA issue ----
         // The warp stays together and an elected lane issues: 36 clocks an MMA beside 23 busy warps (74 from a
@@ -1365,7 +1367,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         // K by tokens: groups of eight 1024 bytes apart, the second 64 dims a tile on
         const uint64_t turned = (tiles & ~(static_cast<uint64_t>(0x3fff) << 16)) | (static_cast<uint64_t>(C::kTile >> 4) << 16);
         for (int c = 0; c < chunks_here; ++c) {
-            const uint64_t st = static_cast<uint64_t>((c & 1) * (C::kStage >> 4));
+            const uint64_t st = static_cast<uint64_t>(c % C::kStages * (C::kStage >> 4));
             const uint64_t kq = tiles + st, tp = tri + st, kt = turned + st;
             auto state_product = [&](int k, int half) {
                 const uint64_t d = kq + half * kQ + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
@@ -1385,7 +1387,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                     mma_f16_ts(to, r, lo, idesc, 1);
                 }
             };
-            wait_one(&full[c & 1], c >> 1);
+            wait_one(&full[c % C::kStages], c / C::kStages);
+            fence_proxy_async_smem();      // K and Q were written by threads, the MMAs read through the async proxy
 #pragma unroll
             for (int b = 0; b < C::kBatches; ++b) {
                 wait_one(&s_ready[b], c);
@@ -1422,7 +1425,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                     mma_f16_ts(tmem + C::kD3, tmem + C::kD2 + k * 16 + 8, kt + k * 128, kIdescT, 1);
                 }
                 mma_commit(&made[2]);
-                mma_commit(&empty[c & 1]);
+                mma_commit(&empty[c % C::kStages]);
             }
             __syncwarp();
         }
