@@ -937,22 +937,28 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 
 // ---- the same walk on the tcgen05 tensor cores, for many heads -----------------------
 //
-// One block per head (128 value columns), the columns as the MMA's M = 128 rows, so
-// that every product has N = 128 and runs at the tensor core's rate:
+// One block per head (128 value columns), the columns as the MMA's M = 128 rows:
 //   D1 = S^T [K; Q]^T;  D2 = R^T [T; P T]^T;  D3 = W^T K  with W = diag(cs) U,
-// the left operands from tensor memory (R^T and W^T in the place of the halves of D1
-// and D2 that they are made from: a shared-memory operand each side would take all of
-// its bandwidth), the state's halves of D1 and D2 ahead of the outputs', K's tile of
-// tokens by rows serving both as [K; Q] and, read with N contiguous, as W's
-// factor.  The state itself lives in D3: keep S is put there before the product
-// adds to it.  A row of an accumulator, one value column, belongs to one
-// thread of each of four warpgroups (a quarter of the tokens and of the state's
-// rows each), which turn D1 into R, D2 into W and D3 into the next S; four warps
-// write the outputs from the other halves of D1 and D2 beside them, three load
-// the next chunk, one thread issues the MMAs, 16 of K at a time as soon as that
-// part of an operand is there.  The passes over the accumulators are what a chunk
-// waits for, so they are short rolled loops (straight code is fetched more slowly
-// than it runs) on many warps.
+// the left operands from tensor memory (a shared-memory operand each side would take
+// all of its bandwidth): S beside the accumulators, R and W as hi and lo in the place
+// of the halves of D1 and D2 that they are made from.  K's tile of tokens by rows serves
+// both as [K; Q] and, read with N contiguous, as W's factor; a block column of a
+// triangle is an operand of the rows from its diagonal on.  The state itself lives
+// in D3: keep S is put there before the product adds to it.
+//
+// A row of an accumulator, one value column, belongs to one thread of each of
+// four warpgroups (a quarter of the tokens and of the state's rows each), which turn
+// D1 into R, D2 into W and D3 into the next S; four warps write the outputs from the
+// other halves of D1 and D2, whose products follow the state's, three load up to
+// three chunks ahead, one issues the MMAs, 16 of K at a time as soon as that part
+// of an operand is there.  The passes over the accumulators are what a chunk waits for,
+// so they are short rolled loops (straight code is fetched more slowly than it
+// runs) on many warps.
+//
+// A chunk takes 3.1 us (5600 clocks at DK = 128: E1 and E2, to R and to W, 1000 and 500, the
+// products before them 500 and 600, the state's product 1000, its pass 1500): 16000 warp
+// instructions, 72 % of the issue slots, tensor pipe about 40 %.  7600 clocks with both
+// halves of a product in one, two stages, and copies that a warp waited for.
 //
 // Here a split operand is hi + lo in one scale and one accumulator, so a row's values
 // are first multiplied by a power of two that keeps a bound of all of a chunk's,
@@ -1158,17 +1164,17 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             __syncwarp();
             if (lane == 0) mbar_arrive(ready);
         };
-        auto most_v = [&](int c) {
+        // This thread's part of a chunk's max|v| and its own max|S|, for the row's other threads and the outputs
+        auto measure_row = [&](int c) {
             wait(&full[c % C::kStages], c / C::kStages);
             const unsigned char* p = v_at + c % C::kStages * C::kStage;
             __half m = __float2half_rn(0.0f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) m = __hmax(m, __habs(*reinterpret_cast<const __half*>(p + i * 256)));
-            return __half2float(m);
+            most[c % 3][part][row] = make_float2(most_s, __half2float(m));
         };
         Scale scale;
-        auto agree = [&](int c, float v) {      // with the row's other threads; the outputs follow
-            most[c % 3][part][row] = make_float2(most_s, v);
+        auto agree = [&](int c) {
             asm volatile("bar.sync 1, 512;" ::: "memory");
             if (lane == 0) mbar_arrive(&scaled);
             return scale.next(c, most[c % 3], row);
@@ -1185,7 +1191,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 x[i / 16][i % 16] = a.state_in && live ? a.state_in[at + static_cast<int64_t>(i) * a.dv] : 0.0f;
                 most_s = fmaxf(most_s, fabsf(x[i / 16][i % 16]));
             }
-            now = agree(0, most_v(0));
+            measure_row(0);
+            now = agree(0);
             const float keep = scales_of(0)[4 * kChunk];
 #pragma unroll
             for (int b = 0; b < C::kBatches; ++b) {
@@ -1212,6 +1219,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                     x[i + e] = __half2float(*reinterpret_cast<const __half*>(vp + (i + e) * 256)) * now.x - cp[e] * x[i + e];
             }
             put_row(x, C::kD1, &r_ready);
+            const bool last = c + 1 == chunks_here;
+            if (!last) measure_row(c + 1);      // while U is made
             wait(&made[1], c);
             tc_fence_after();
             tmem_ld16(lane_at + C::kD2 + part * 16, x);
@@ -1223,11 +1232,10 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             put_row(x, C::kD2, &w_ready);
             if (lane == 0) mbar_arrive(&empty[c % C::kStages]);
             // while the last product is made: the next chunk's scale and decay
-            const bool last = c + 1 == chunks_here;
             float2 next = now;
             float keep = 0.0f;
             if (!last) {
-                next = agree(c + 1, most_v(c + 1));
+                next = agree(c + 1);
                 keep = scales_of(c + 1)[4 * kChunk];
             }
             const float change = next.x * now.y;
@@ -1460,13 +1468,14 @@ int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
                     kSmem, stream, a, chunks);
     if (st) return st;
-    // One column group a block while those all run at once (a chunk then takes 1.4 us), else two (2.5 us), unless
-    // whole heads on the other walk (4.0 us) get through in less, which they do from twice as many rounds on.
+    // One column group a block while those all run at once (a chunk then takes 1.4 us; 8000 tokens of 16 heads 213 us,
+    // 373 with two groups), else two (2.4 us), unless whole heads on the other walk (3.1 us) get through in less (4
+    // sequences of 4000 tokens of 16 heads: 262 us, where two rounds of two groups took 376).
     const int64_t heads = static_cast<int64_t>(a.batch) * a.v_heads;
     const int sms = sm_count();
     if (heads * (a.dv / 16) > sms) {
         const int64_t pairs = (heads * ((a.dv + 31) / 32) + sms - 1) / sms, whole = (heads * ((a.dv + 127) / 128) + sms - 1) / sms;
-        if (pairs * 5 <= whole * 8) return launch_scan<DK, 2>(a, chunks, stream);
+        if (pairs * 4 <= whole * 5) return launch_scan<DK, 2>(a, chunks, stream);
         static std::atomic<uint64_t> done_walk{0};
         if ((st = allow_smem(walk_kernel<DK>, Walk<DK>::kSmem, done_walk))) return st;
         return launch(walk_kernel<DK>, dim3((a.dv + 127) / 128, a.v_heads, a.batch), dim3(Walk<DK>::kThreads), Walk<DK>::kSmem,
