@@ -1468,9 +1468,9 @@ int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
                     kSmem, stream, a, chunks);
     if (st) return st;
-    // One column group a block while those all run at once (a chunk then takes 1.4 us; 8000 tokens of 16 heads 213 us,
-    // 373 with two groups), else two (2.4 us), unless whole heads on the other walk (3.1 us) get through in less (4
-    // sequences of 4000 tokens of 16 heads: 262 us, where two rounds of two groups took 376).
+    // One column group a block while those all run at once (1.4 us a chunk), else two (2.4 us) where those take no more
+    // rounds than whole heads on the other walk (3.1 us) or few more.  16 heads of 128, all three forced:
+    //   1 sequence of 8000 tokens 213, 337, 406 us;  2 of 8000: 417, 371, 440;  4 of 4000: 422, 378, 261.
     const int64_t heads = static_cast<int64_t>(a.batch) * a.v_heads;
     const int sms = sm_count();
     if (heads * (a.dv / 16) > sms) {
