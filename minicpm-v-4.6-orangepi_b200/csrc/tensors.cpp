@@ -1,7 +1,7 @@
 // Python module mcv_b200._tensors: the per-call checks of tensors in the
-// token-mixing binding.  A decode step's kernels take 3 us on the GPU; asking a
-// tensor for its type, shape, strides, device and address from Python took 4.7 us for
-// the nine of a gated delta step, here it takes 1.
+// token-mixing binding.  A decode step's kernel takes 2 to 5 us on the GPU; checking and
+// packing the nine tensors of a gated delta step took 4.7 us with each attribute asked for
+// from Python, 2.0 with them looked at here.
 #include <Python.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
