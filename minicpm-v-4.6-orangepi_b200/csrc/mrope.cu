@@ -17,8 +17,9 @@
 // are on their way, and keeps the eight pairs of each lane's place for all heads.
 // With few tokens up to eight warps share one, a part of the heads each.
 // Other head sizes go through a kernel that deals out items.
-// 8191 tokens of 8 + 2 + 2 heads of 256 (101 MB, 15.4 us at the copy rate): 21.7 us; in blocks of
-// eight warps 25.4, with all sizes dealt out as items, whose divisions cost more than the rows, 31.6.
+// 8191 tokens of 8 + 2 + 2 heads of 256 (101 MB, 15.4 us at the copy rate): 19.5 us; in blocks of
+// eight warps 25.4, with the places looked up and the angles' entries read behind all rows 21.8,
+// with all sizes dealt out as items, whose divisions cost more than the rows, 31.6.
 // What is left is latency: a warp's rows, place and angles are one chain of about 5 us, and the registers
 // that hold the rows on their way leave an SM 18 to 20 warps.
 #include "mixing.cuh"
@@ -73,10 +74,8 @@ __device__ __forceinline__ void rotate8(uint4& a, uint4& b, const float2* cs) {
 }
 
 // Element offset of the token's slot in head 0 of the cache, -1: not written.
-__device__ __forceinline__ int64_t place_of(const RopeArgs& a, int tok) {
-    const int i = a.index[tok];
+__device__ __forceinline__ int64_t place_of(const RopeArgs& a, int i, int row) {
     if (i < 0) return -1;
-    const int row = a.seq ? a.seq[tok] : tok;
     const int page = a.page.div(i);
     int p = -1;
     if (row >= 0 && row < a.table_rows && page < a.table_cols) p = a.table[row * a.table_cols + page];
@@ -85,7 +84,12 @@ __device__ __forceinline__ int64_t place_of(const RopeArgs& a, int tok) {
     return -1;
 }
 __device__ __forceinline__ float2 turn_of(const mcv_mrope_spec& spec, const RopeArgs& a, int tok, int i) {
-    const double turns = static_cast<double>(a.positions[static_cast<int64_t>(spec.axis[i]) * a.tokens + tok]) * spec.turns[i];
+    // lanes read different entries: as constants one after the other, from memory together (200 tokens 4.7 -> 4.1 us)
+    uint32_t axis;
+    double f;
+    asm("ld.u8 %0, [%1];" : "=r"(axis) : "l"(&spec.axis[i]));
+    asm("ld.f64 %0, [%1];" : "=d"(f) : "l"(&spec.turns[i]));
+    const double turns = static_cast<double>(a.positions[static_cast<int64_t>(axis) * a.tokens + tok]) * f;
     float s, c;
     sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
     return make_float2(c, s);
@@ -105,7 +109,7 @@ __device__ __forceinline__ void turn_vector(uint4& x, bool turn, int partner, co
 }
 
 // BLOCKS resident: 8 leave a thread the 128 registers that hold all its rows on their way (200 tokens of 16 + 2 + 2
-// heads 4.7 us, with 9 5.2); 9 hide more of the tokens' latency when there are many (8191 tokens 21.7 us, with 8 24.1).
+// heads 4.1 us, with 9 4.5); 9 hide more of the tokens' latency when there are many (8191 tokens 19.5 us, with 8 21.6).
 template <int VECS, int BLOCKS>
 __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const __grid_constant__ mcv_mrope_spec spec, const RopeArgs a) {
     constexpr int kPer = 32 / VECS;      // rows of a step
@@ -125,6 +129,7 @@ __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const _
     const int q_heads = a.in_place && !turned ? 0 : a.q_heads;      // what passes in place is there already
     const uint4* qp = reinterpret_cast<const uint4*>(a.q + tok * a.q_ts + q0 * a.q_hs) + vec;
     const int64_t qs = step * a.q_hs / 8;
+    const int index = a.k ? a.index[tok] : -1, row = a.k && a.seq ? a.seq[tok] : tok;
     uint4 xq[kQRows], xk[kKvRows], xv[kKvRows];
 #pragma unroll
     for (int r = 0; r < kQRows; ++r) xq[r] = q0 + r * step < q_heads ? __ldg(qp + r * qs) : make_uint4(0, 0, 0, 0);
@@ -132,6 +137,7 @@ __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const _
     int64_t ks = 0, vs = 0, place = -1;
     const int shift = (a.q_heads + kPer - 1) / kPer, kv0 = ((mine - shift) & ((1 << a.share) - 1)) * kPer + sub;
     if (a.k) {
+        place = place_of(a, index, row);
         kp = reinterpret_cast<const uint4*>(a.k + tok * a.k_ts + kv0 * a.k_hs) + vec;
         vp = reinterpret_cast<const uint4*>(a.v + tok * a.v_ts + kv0 * a.v_hs) + vec;
         ks = step * a.k_hs / 8;
@@ -142,7 +148,6 @@ __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const _
             xk[r] = there ? __ldg(kp + r * ks) : make_uint4(0, 0, 0, 0);
             xv[r] = there ? __ldg(vp + r * vs) : make_uint4(0, 0, 0, 0);
         }
-        place = place_of(a, tok);
     }
     for (int i = lane; i < half; i += 32) turns[warp][i] = turn_of(spec, a, tok, i);
     __syncwarp();
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(kThreads) mrope_kernel(const __grid_constant__
     const int nt = min(a.per_block, a.tokens - t0);
     if (a.k && threadIdx.x >= kThreads - nt) {
         const int t = kThreads - 1 - threadIdx.x;
-        place[t] = place_of(a, t0 + t);
+        place[t] = place_of(a, a.index[t0 + t], a.seq ? a.seq[t0 + t] : t0 + t);
     }
     for (int j = threadIdx.x; j < nt * half; j += kThreads) {
         const int t = j / half, i = j - t * half;
