@@ -634,7 +634,8 @@ struct Scan {
     static constexpr int kSx = 16 * DK * 2;
     static constexpr int kRx = 16 * kChunk * 2;
     static constexpr int kGroup = 2 * kSx + 4 * kRx;
-    static constexpr int kSmem = 2 * kStage + NG * kGroup;
+    static constexpr int kStages = 3;
+    static constexpr int kSmem = kStages * kStage + NG * kGroup;
 };
 
 template <int DK, int NG>
@@ -643,10 +644,9 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
     constexpr int kVecs = DK / 8;
     constexpr int kN = DK / 32;       // n8 tiles of a state warp's rows
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ __align__(8) uint64_t landed[2];
+    __shared__ __align__(8) uint64_t landed[C::kStages];
     if (threadIdx.x == 0) {
-        mbar_init(&landed[0], 1);
-        mbar_init(&landed[1], 1);
+        for (int i = 0; i < C::kStages; ++i) mbar_init(&landed[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
     const uint32_t base = smem_u32(smem);
 
     if (tid >= NG * 256) {
-        // ---- the loading warps: one chunk ahead ----
+        // ---- the loading warps: two chunks ahead ----
         constexpr int kStep = 128 / kVecs;           // rows of one sweep of the 128 threads; a multiple of 8,
         static_assert(kStep % 8 == 0, "swizzle");    // so a thread keeps its place in the swizzle
         const int kh = h / a.share, lt = tid - NG * 256;
@@ -672,39 +672,48 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
         const int64_t k_step = kStep * a.k_ts, q_step = kStep * a.q_ts;
         const Chunk* rec = chunks + first_chunk(begin, b) * a.v_heads + h;
         bool dead = false;
-        for (int c = 0; c < chunks_here; ++c) {
-            const uint32_t stage = base + (c & 1) * C::kStage;
-            if (lt == 0) {
-                fence_proxy_async_smem();      // the stage's reads come before the copy into it
-                mbar_expect_tx(&landed[c & 1], kChunkBytes);
-                bulk_load(smem + (c & 1) * C::kStage + C::kRecord, rec, kChunkBytes, &landed[c & 1]);
-            }
-            rec += a.v_heads;
-            const uint32_t dst = tile_at<kVecs>(stage, lr, lx);
-            const int t0 = begin + c * kChunk;
-            const int n = min(kChunk, end - t0);
+        auto issue = [&](int c) {
+            if (c < chunks_here) {
+                const int st = c % C::kStages;
+                const uint32_t stage = base + st * C::kStage;
+                if (lt == 0) {
+                    fence_proxy_async_smem();      // the stage's reads come before the copy into it
+                    mbar_expect_tx(&landed[st], kChunkBytes);
+                    bulk_load(smem + st * C::kStage + C::kRecord, rec, kChunkBytes, &landed[st]);
+                }
+                rec += a.v_heads;
+                const uint32_t dst = tile_at<kVecs>(stage, lr, lx);
+                const int t0 = begin + c * kChunk;
+                const int n = min(kChunk, end - t0);
 #pragma unroll
-            for (int i = 0; i < kChunk / kStep; ++i) {
-                const bool ok = i * kStep + lr < n;
-                cp_async16_or_zero(dst + i * kStep * kVecs * 16, ok ? kp : a.k, ok);
-                cp_async16_or_zero(dst + i * kStep * kVecs * 16 + C::kTile, ok ? qp : a.q, ok);
-                kp += k_step;
-                qp += q_step;
-            }
+                for (int i = 0; i < kChunk / kStep; ++i) {
+                    const bool ok = i * kStep + lr < n;
+                    cp_async16_or_zero(dst + i * kStep * kVecs * 16, ok ? kp : a.k, ok);
+                    cp_async16_or_zero(dst + i * kStep * kVecs * 16 + C::kTile, ok ? qp : a.q, ok);
+                    kp += k_step;
+                    qp += q_step;
+                }
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int item = i * 128 + lt, r = item / (2 * NG), x = item % (2 * NG);
-                const bool ok = r < n && col0 + x * 8 < a.dv;
-                cp_async16_or_zero(tile_at<2 * NG>(stage + C::kV, r, x),
-                                   ok ? a.v + static_cast<int64_t>(t0 + r) * a.v_ts + h * a.v_hs + col0 + x * 8 : a.v, ok);
+                for (int i = 0; i < NG; ++i) {
+                    const int item = i * 128 + lt, r = item / (2 * NG), x = item % (2 * NG);
+                    const bool ok = r < n && col0 + x * 8 < a.dv;
+                    cp_async16_or_zero(tile_at<2 * NG>(stage + C::kV, r, x),
+                                       ok ? a.v + static_cast<int64_t>(t0 + r) * a.v_ts + h * a.v_hs + col0 + x * 8 : a.v, ok);
+                }
             }
             cp_async_commit();
-            cp_async_wait<0>();
-            if (lt == 0 && !dead && !mbar_wait(&landed[c & 1], (c >> 1) & 1)) {
+        };
+        issue(0);
+        issue(1);
+#pragma unroll 1
+        for (int c = 0; c < chunks_here; ++c) {
+            cp_async_wait<1>();
+            if (lt == 0 && !dead && !mbar_wait(&landed[c % C::kStages], (c / C::kStages) & 1)) {
                 dead = true;      // gives up waiting, not the barriers: the block still ends
                 atomicOr(&g_gated_delta_dev_error, kDevErrTimeout);
             }
             __syncthreads();   // chunk c is there, and c - 1 is done with
+            issue(c + 2);
         }
         return;
     }
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
     const bool outputs = (tid >> 7) & 1;
     const int col = col0 + group * 16;
     const bool live = col < a.dv;
-    const uint32_t s_hi = base + 2 * C::kStage + group * C::kGroup, s_lo = s_hi + C::kSx, r_hi = s_lo + C::kSx,
+    const uint32_t s_hi = base + C::kStages * C::kStage + group * C::kGroup, s_lo = s_hi + C::kSx, r_hi = s_lo + C::kSx,
                    r_lo = r_hi + C::kRx, w_hi = r_lo + C::kRx, w_lo = w_hi + C::kRx;
     const int blk = outputs ? 3 - warp : warp;       // this warp's 16 tokens of a chunk
     const int a_row = lane & 15, a_vec = lane >> 4;                                // A operand
@@ -733,7 +742,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
     if (outputs) {
         for (int c = 0; c < chunks_here; ++c) {
             __syncthreads();
-            const uint32_t stage = base + (c & 1) * C::kStage, sc = stage + C::kScales;
+            const uint32_t stage = base + c % C::kStages * C::kStage, sc = stage + C::kScales;
             const uint32_t p_hi = stage + C::kRecord + kTri * 2 + tri_row;
             float o[2][4], ol[2][4], x[2][4];
 #pragma unroll
@@ -830,7 +839,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
     put_state();
     for (int c = 0; c < chunks_here; ++c) {
         __syncthreads();
-        const uint32_t stage = base + (c & 1) * C::kStage, sc = stage + C::kScales;
+        const uint32_t stage = base + c % C::kStages * C::kStage, sc = stage + C::kScales;
         const uint32_t t_hi = stage + C::kRecord + tri_row;
 
         // S0^T K^T for this warp's tokens
