@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 // The walk.  Eight warps own 16 value columns of a head: four carry the state
 // (each a quarter of its rows, in registers), four make the outputs; a block
 // has NG such groups, which share the chunk's tiles, and four warps that load the
-// chunks after next while this one is in use.  All products are taken
+// next two chunks' while this one's are in use.  All products are taken
 // transposed, with the 16 columns as the MMA's m:
 //   R^T = V^T - (S0^T K^T) diag(ck);  U^T = R^T T^T;  S'^T = keep S0^T + (U^T diag(cs)) K
 // by the state's warps, each for 16 tokens or a quarter of the rows, with R, U
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 // the output warp beside it on the same scheduler take tokens 16 w and 16 (3 - w), so
 // that the triangles' work adds up to the same on each.
 //
-// 8000 tokens of 16 heads, one group a block: 170 us, 1.35 us a chunk (the operators' bytes would take 20), with
+// 8000 tokens of 16 heads, one group a block: 170 us, 1.35 us a chunk (the operator's bytes would take 20), with
 // shared memory busy in three quarters of the cycles, most of that for fragments of S that eight warps
 // need; two groups 2.4 us a chunk.
 template <int DK, int NG>

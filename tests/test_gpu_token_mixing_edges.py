@@ -188,3 +188,53 @@ def test_mrope_however_many_tokens(cuda, dim, rotary, hq, hk):
     assert torch.equal(got[3][0][:5], got[0][0][:5])
     mcv.mrope(q, pos, rope, q)
     assert torch.equal(q, got[0][0])
+
+
+@pytest.mark.parametrize("page,hq,hk,dim", [(1, 8, 2, 64), (1000, 16, 2, 256), (5000, 5, 1, 128), (3, 34, 2, 64)])
+def test_pages_of_any_size(cuda, page, hq, hk, dim):
+    """A cache written token by token through its pages reads like one piece: pages of one key, pages longer than the
+    sequences, 17 query heads a kv head."""
+    import mcv_b200 as mcv
+    from test_gpu_token_mixing import attention_check
+    torch = cuda
+    g = gen(page + hq)
+    lens = [1, 40, 333]
+    cols = -(-333 // page)
+    total = sum(lens)
+    cache = mcv.PagedKVCache.empty(3 * cols, hk, page, dim)
+    cache.k.fill_(float("nan"))
+    cache.v.fill_(float("nan"))
+    table = torch.randperm(3 * cols, generator=g, device="cuda").int().view(3, cols)
+    q, k, v = randn(g, total, hq, dim), randn(g, total, hk, dim), randn(g, total, hk, dim)
+    rope = mcv.MRope(32, [16])
+    index = torch.cat([torch.arange(n) for n in lens]).int().cuda()
+    seq = torch.cat([torch.full((n,), i) for i, n in enumerate(lens)]).int().cuda()
+    still = torch.zeros(1, total, dtype=torch.int32, device="cuda")       # position 0: keys stay as they are
+    mcv.mrope_append_kv(q, k, v, still, rope, cache, table, index, torch.empty_like(q), seq=seq)
+    qs = randn(g, 3, hq, dim)
+    out, lse = torch.empty(3, hq, dim, dtype=torch.float16, device="cuda"), torch.empty(3, hq, device="cuda")
+    mcv.paged_attention_decode(qs, cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), out,
+                               mcv.paged_attention_workspace(3, hq, hk, dim), lse=lse)
+    keys, at = [], 0
+    for n in lens:
+        keys.append((k[at:at + n], v[at:at + n]))
+        at += n
+    attention_check(torch, qs, keys, dim ** -0.5, out, lse, "pages")
+    assert mcv.device_errors() == 0
+
+
+def test_mrope_turns_back(cuda):
+    """Negative positions turn the other way: there and back leaves two roundings, each half a step of a vector of the
+    pair's length, and what fp32 leaves of two rotations (2^-19 of it)."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(31)
+    x = randn(g, 77, 4, 128)
+    pos = torch.randint(0, 200000, (1, 77), generator=g, device="cuda").int()
+    rope = mcv.MRope(128, [64])
+    there, back = torch.empty_like(x), torch.empty_like(x)
+    mcv.mrope(x, pos, rope, there)
+    mcv.mrope(there, -pos, rope, back)
+    length = (x[..., :64].double() ** 2 + x[..., 64:].double() ** 2).sqrt().repeat(1, 1, 2)
+    # the first rounding errs by 2^-11 in each of a pair's two, turned: sqrt 2 times that at most
+    assert ((back.double() - x.double()).abs() <= (2.0 ** -11 * (1 + 2.0 ** 0.5) + 2.0 ** -19) * length + 2.0 ** -23).all()
