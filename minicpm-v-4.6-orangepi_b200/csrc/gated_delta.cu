@@ -970,7 +970,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 //
 // A chunk takes 3.1 us (5600 clocks at DK = 128: E1 and E2, to R and to W, 1000 and 500, the
 // products before them 500 and 600, the state's product 1000, its pass 1500): 16000 warp
-// instructions, 72 % of the issue slots, tensor pipe about 40 %.  7600 clocks with both
+// instructions, 67 % of the issue slots, tensor pipe 36 %.  7600 clocks with both
 // halves of a product in one, two stages, and copies that a warp waited for.
 //
 // Here a split operand is hi + lo in one scale and one accumulator, so a row's values
