@@ -106,9 +106,13 @@ PyObject* rows_out(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (dev == -1 && PyErr_Occurred()) return nullptr;
         const at::Tensor *x = tensor(args[0], "x"), *out = x ? tensor(args[1], what) : nullptr;
         if (!out) return nullptr;
-        if (out->scalar_type() == x->scalar_type() && out->get_device() == x->get_device() && out->sizes() == x->sizes() &&
-            out->strides() == x->strides() && out->data_ptr() == x->data_ptr())
-            return address(*x);
+        if (out->data_ptr() == x->data_ptr() && x->numel() > 0) {
+            if (out->scalar_type() == x->scalar_type() && out->sizes() == x->sizes() && out->strides() == x->strides())
+                return address(*x);
+            // the call takes an output at x's address to have x's strides
+            PyErr_Format(PyExc_RuntimeError, "mcv_b200: %s begins where its input does but is laid out differently", what);
+            return nullptr;
+        }
         return dense_address(*out, at::kHalf, "float16", x->sizes().data(), x->dim(), what, dev);
     });
 }

@@ -59,3 +59,14 @@ def test_delta_outputs_and_states():
         mcv_b200.gated_delta_step(*delta()[:4], [0.0], state, out)
     with pytest.raises(RuntimeError, match="cu_seqlens"):
         mcv_b200.gated_delta_prefill(*delta(), torch.zeros(1, dtype=torch.int32), None, out, torch.zeros(1, dtype=torch.uint8))
+
+
+def test_output_over_its_input():
+    """An output at the input's address is that input in place; one of another layout there is refused."""
+    wide = half(3, 2, 128)
+    x, dense = wide[:, :, :64], wide.view(-1)[:3 * 2 * 64].view(3, 2, 64)
+    pos, rope = torch.zeros(1, 3, dtype=torch.int32), mcv_b200.MRope(64, [32])
+    with pytest.raises(RuntimeError, match="out begins where its input does"):
+        mcv_b200.mrope(x, pos, rope, dense)
+    with pytest.raises(RuntimeError, match="CUDA device"):      # the input itself passes this check
+        mcv_b200.mrope(x, pos, rope, x)
