@@ -610,8 +610,10 @@ size_t mcv_paged_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int
  * a page out of range reads as zeros (and sets it).  head_dim 64, 128 or 256;
  * batch up to 4096; batch * kv_heads * table_cols * page_size / 16 (twice that
  * from 17 query heads per kv head on, and so forth) below 2^31; k and v within
- * 64 GB each.  Scores, softmax and sums are fp32; the cache is read once
- * up to 16 query heads per kv head. */
+ * 64 GB each.  Scores, softmax and sums are fp32; a key's weight is kept to 22
+ * bits, or to 2^-40 of the largest weight's size where that is more; values are
+ * expected to be finite (an infinite one gives NaN).  The cache is read once up to
+ * 16 query heads per kv head. */
 int mcv_paged_attention_decode(const mcv_rows* q, const mcv_kv_cache* cache, const void* page_table,
                                int64_t table_cols, const void* lengths, void* out, void* lse, int64_t batch,
                                int64_t q_heads, float scale, void* workspace, size_t workspace_bytes,

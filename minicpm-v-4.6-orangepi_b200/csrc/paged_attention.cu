@@ -12,15 +12,17 @@
 // S^T (16 keys x 8 heads) = K Q^T, and O^T (D x 8 heads) = V^T P^T.  K comes
 // as an A fragment through ldmatrix and V^T through its transposing form; S^T
 // turns into the B fragment of the second product by an 8x8 register
-// transpose.  P is split into hi + lo fp16, so that the probabilities keep 22
-// bits (the second MMA costs nothing here); scores, maxima, sums and outputs
-// are fp32.
+// transpose.  P = 2^(s - max) is taken times 2^15 and split into hi + lo fp16 (the
+// second MMA costs nothing here): weights down to 2^-18 of the maximum's keep 22 bits,
+// smaller ones an absolute 2^-40 of it.  Without the factor fp16's end, 2^-24, would
+// cut off the long tail behind one dominant key.  Scores, maxima, sums and outputs
+// are fp32, the sums in the factor's scale too.
 //
 // Work is cut evenly however ragged the batch is: all (sequence, head group)
 // rows' 16-key units form one line that is divided into one contiguous range
 // per block.  Within its range the four warps of a block take every fourth
 // unit, each through a ring of its own in shared memory that runs ahead
-// across row ends; page numbers are looked up one unit ahead of the copies.
+// across row ends; page numbers are looked up two units ahead of the copies.
 // At a row's end the block joins its warps' (max, sum, O).  A row that
 // lies in one block's range is written at once; of a row cut over several
 // blocks every block leaves a partial result, and the last one to arrive
@@ -42,6 +44,7 @@ constexpr int kFan = 16;       // partial results joined at a time
 constexpr int kLevels = 3;     // levels of joining: kFan^3 blocks at most
 constexpr int kMaxBatch = 4096;
 constexpr int kMinUnits = 4;   // least units of a block: one per warp
+constexpr float kPLog2 = 15.0f;   // probabilities and their sums are kept times 2^15, below fp16's 65504
 
 static __device__ unsigned g_attention_dev_error;
 
@@ -216,7 +219,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot
             *reinterpret_cast<uint2*>(a.out + row * D + d) =
                 make_uint2(h2_as_u32(__floats2half2_rn(acc[i].x * inv, acc[i].y * inv)),
                            h2_as_u32(__floats2half2_rn(acc[i].z * inv, acc[i].w * inv)));
-            if (d == 0 && a.lse) a.lse[row] = (all.x + log2f(all.y)) * 0.6931471805599453f;
+            if (d == 0 && a.lse) a.lse[row] = (all.x + (log2f(all.y) - kPLog2)) * 0.6931471805599453f;
         } else {
             // each element of slot_of(0) is read and written by one thread alone, and
             // its maxima and sums were read by all before the barriers above
@@ -531,8 +534,8 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
                 for (int c = 0; c < 2; ++c) {
                     // no number above -inf so far: nothing to weigh yet
                     const float base = m[n][c] == -INFINITY ? 0.0f : m[n][c];
-                    p[c] = exp2f(s[n][c] - base);
-                    p[2 + c] = exp2f(s[n][2 + c] - base);
+                    p[c] = exp2f(s[n][c] - base + kPLog2);
+                    p[2 + c] = exp2f(s[n][2 + c] - base + kPLog2);
                     l[n][c] += p[c] + p[2 + c];
                 }
                 uint32_t lo;
@@ -614,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
                     *reinterpret_cast<uint2*>(a.out + orow * D + d) =
                         make_uint2(h2_as_u32(__floats2half2_rn(o.x * inv, o.y * inv)),
                                    h2_as_u32(__floats2half2_rn(o.z * inv, o.w * inv)));
-                    if (d == 0 && a.lse) a.lse[orow] = (top + log2f(sum)) * 0.6931471805599453f;
+                    if (d == 0 && a.lse) a.lse[orow] = (top + (log2f(sum) - kPLog2)) * 0.6931471805599453f;
                 } else {
                     *reinterpret_cast<float4*>(mine_part.o(n * 8 + h) + d) = o;
                     if (d == 0) {

@@ -1,0 +1,104 @@
+"""What the token-mixing operators keep of small terms beside large ones: the
+tail of a softmax under one dominant key.
+
+Attention's bounds are those of test_gpu_token_mixing, with weights kept to 22
+bits or to 2^-40 of the largest one's size.  An output is one rounding to fp16
+away from fp32's, so what single outputs cannot show is looked for in their
+mean: roundings to nearest are independent of each other and off by at most half
+a step, 2^-11 of the value, 2^-11 / sqrt(3) in root mean square, so the mean
+relative error of N outputs stays within six times 2^-11 / sqrt(3 N).
+"""
+import math
+
+import pytest
+
+from test_gpu_token_mixing import attention_setup, close16, gen
+
+pytestmark = pytest.mark.gpu
+
+
+def weights_check(torch, q, keys, scale, out, lse, what):
+    """Every row against fp64; the mean relative error of the outputs."""
+    group = q.shape[1] // keys[0][0].shape[1]
+    errors = []
+    for b, (k, v) in enumerate(keys):
+        if k.shape[0] == 0:
+            assert not out[b].any() and (lse[b] == -math.inf).all(), what
+            continue
+        kk, vv = (x.double().repeat_interleave(group, dim=1).transpose(0, 1) for x in (k, v))
+        s = torch.einsum("hd,hnd->hn", q[b].double(), kk) * scale
+        # fp32 scores: D products and their scaling
+        e = torch.einsum("hd,hnd->hn", q[b].double().abs(), kk.abs()).amax(1) * scale * q.shape[2] * 2.0 ** -24
+        p = torch.softmax(s, 1)
+        ref, spread = torch.einsum("hn,hnd->hd", p, vv), torch.einsum("hn,hnd->hd", p, vv.abs())
+        kept = 2.0 ** -22 * spread + 2.0 ** -40 * p.amax(1)[:, None] * vv.abs().sum(1)
+        close16(out[b], ref, spread * (2 * e[:, None] + 2.0 ** -18) + kept, f"{what} row {b}")
+        ref_lse = torch.logsumexp(s, 1)
+        assert ((lse[b].double() - ref_lse).abs() <= 2 * e + 2.0 ** -20 * (1 + ref_lse.abs())).all(), what
+        errors.append(((out[b].double() - ref) / ref).flatten())
+    errors = torch.cat(errors)
+    return errors.mean().abs().item(), errors.numel()
+
+
+# ---- attention: one dominant key over a long tail ---------------------------------
+
+@pytest.mark.parametrize("nats", [10.0, 14.0, 18.0, 24.0])
+@pytest.mark.parametrize("dim,hq,hk,page,lens,sinks", [
+    (128, 8, 8, 16, [4096], 1), (64, 8, 2, 16, [16384, 300], 4), (256, 16, 1, 48, [4096, 0, 1, 5000], 1),
+    (128, 32, 8, 16, [1200] * 40, 4)])
+def test_attention_sink(cuda, nats, dim, hq, hk, page, lens, sinks):
+    """The first keys of a trained model's sequence take most of the weight and have values near 0: what
+    the output is made of are the many small weights behind them."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(int(nats) + dim + len(lens))
+    q, ck, cv, table, lengths, keys = attention_setup(torch, g, lens, hq, hk, dim, page, qscale=0.3)
+    # dimension 0 of q is 1 and that of the dominant keys sqrt(dim) * nats (both exact in fp16 to a part in 2^11, and taken
+    # as they are by the reference), of the others 0; tail values of a mean other than 0, so that sums do not cancel
+    q[:, :, 0] = 1.0
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        k, v = keys[b]
+        k[:, :, 0] = 0.0
+        v += 2.0
+        for i in range(0, min(n, 16 * sinks), 16):
+            k[i, :, 0] = math.sqrt(dim) * nats
+            v[i] = 0.0
+        v *= 1000.0
+        i = torch.arange(n, device="cuda")
+        p = table[b].long()[i // page]
+        ck[p, :, i % page], cv[p, :, i % page] = k, v
+    out, lse = torch.empty_like(q), torch.empty(len(lens), hq, device="cuda")
+    ws = mcv.paged_attention_workspace(len(lens), hq, hk, dim)
+    mcv.paged_attention_decode(q, mcv.PagedKVCache(ck, cv), table, lengths, out, ws, lse=lse)
+    weights_check(torch, q, keys, dim ** -0.5, out, lse, f"sink {nats}")
+
+
+@pytest.mark.parametrize("exponent", [-1, -9, -20])
+def test_attention_weights_keep_their_low_bits(cuda, exponent):
+    """One key of every 16 dominates and has the value 0; all others weigh 2^exponent (1 + 2^-11) of it each, where a
+    single fp16 is off by half a step and always the same way: the outputs' mean error shows what the weights lost."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(9)
+    n, heads, dim = 2001, 16, 128
+    q, ck, cv, table, lengths, keys = attention_setup(torch, g, [n], heads, heads, dim, 16)
+    q.zero_()
+    q[:, :, 0] = 8.0
+    k, v = keys[0]
+    k.zero_()
+    k[::16, :, 0] = 8.0
+    # values of one sign, so large that the outputs are normal fp16 numbers
+    v.copy_((v.abs() + 1.0) * 4000.0)
+    v[::16] = 0.0
+    i = torch.arange(n, device="cuda")
+    p = table[0].long()[i // 16]
+    ck[p, :, i % 16], cv[p, :, i % 16] = k, v
+    scale = float(torch.tensor(-math.log(2.0 ** exponent * (1 + 0.99 * 2.0 ** -11)) / 64.0, dtype=torch.float32))
+    out, lse = torch.empty_like(q), torch.empty(1, heads, device="cuda")
+    mcv.paged_attention_decode(q, mcv.PagedKVCache(ck, cv), table, lengths, out,
+                               mcv.paged_attention_workspace(1, heads, heads, dim), scale=scale, lse=lse)
+    mean, count = weights_check(torch, q, keys, scale, out, lse, "equal weights")
+    # the score, 2^exponent's logarithm, is a product and a sum in fp32: up to 20 (2^-24 + 2^-24) of the weights more
+    assert mean <= 6 * 2.0 ** -11 / math.sqrt(3 * count) + 2.0 ** -18, mean
