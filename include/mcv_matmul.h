@@ -655,7 +655,8 @@ int mcv_gated_delta_step(const mcv_gated_delta* args, int64_t batch, mcv_stream_
  * calls that may overlap on the GPU need workspaces of their own.
  * The chunks' triangular systems and split operands need log decays g <= 0,
  * 0 <= beta <= 2, keys of norm 1 or less, and states and sums of |v| below 65504
- * (the step has no such limits); accuracy is fp32's down to an absolute 2^-36.
+ * (the step has no such limits); accuracy is fp32's down to an absolute 2^-36 of
+ * the largest of 1, |v| and the states.
  * Replaces linear_gated_delta_rule. */
 size_t mcv_gated_delta_workspace_size(int64_t tokens, int64_t batch, int64_t v_heads, int64_t key_dim,
                                       int64_t value_dim);

@@ -173,7 +173,8 @@ int run_step(const DeltaArgs& a, int dk, cudaStream_t stream) {
 // below fp16's 65504 then; with |k| <= 1, beta <= 2 and g <= 0 they are bounded by
 // the state's start and twice the sum of |v|.)
 constexpr int kChunk = 64;
-constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;
+constexpr int kLoBits = 11;
+constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;      // 2^kLoBits
 
 __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uint32_t& lo) {
     hi = h2_as_u32(__floats2half2_rn(x, y));
@@ -973,14 +974,17 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 // instructions, 67 % of the issue slots, tensor pipe 36 %.  7600 clocks with both
 // halves of a product in one, two stages, and copies that a warp waited for.
 //
-// Here a split operand is hi + lo in one scale and one accumulator, so a row's values
-// are first multiplied by a power of two that keeps a bound of all of a chunk's,
-// |S|, |S'|, |R|, |U| <= sqrt(Dk) max|S| + (C + 1) max|v|, between 2^4 and 2^13 (the
+// A split operand is hi + 2^-11 lo here too, in one accumulator: the products with a
+// lo come first, and the first one with a hi scales what is there by 2^-11 (the MMA's
+// scaling of its input).  A row's values are first multiplied by a power of two that
+// keeps a bound of all of a chunk's,
+// |S|, |S'|, |R|, |U| <= sqrt(Dk) max|S| + (C + 1) max|v|, between 2^9 and 2^13 (the
 // state's update is a contraction).  max|S| is measured every fourth chunk and
 // raised by C max|v| for each chunk since, so that the scale is there before the
-// state is; the state stays in its scale in registers.  Values down to 2^-12 of
-// the bound keep 20 bits or more, smaller ones an absolute 2^-29 of it at worst, and
-// a factor of 8 above it stays below fp16's end.
+// state is; the state stays in its scale in registers.  So values keep 22 bits, or an
+// absolute 2^-45 of the bound (2^-36 in this scale) where that is more, and a factor
+// of 8 above the bound stays below fp16's end.  (With lo in the scale of hi the absolute
+// error is 2^-29 of the bound: too much for small values beside one of 30000.)
 template <int DK>
 struct Walk {
     static constexpr int kLoaders = 96;           // three warps
@@ -1051,9 +1055,9 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// The power of two that takes a bound of a row's values to 2^9 .. 2^10, and its inverse.
+// The power of two that takes a bound of a row's values to 2^11 .. 2^12, and its inverse.
 __device__ __forceinline__ float2 row_scale(float bound) {
-    const int e = min(max(136 - static_cast<int>((__float_as_uint(bound) >> 23) & 255u), -100), 100);
+    const int e = min(max(138 - static_cast<int>((__float_as_uint(bound) >> 23) & 255u), -100), 100);
     return make_float2(__uint_as_float(static_cast<uint32_t>(127 + e) << 23), __uint_as_float(static_cast<uint32_t>(127 - e) << 23));
 }
 
@@ -1146,7 +1150,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             s += kChunk * v;
             v = m.y;
             const float bound = s + (kChunk + 1) * v, at = bound * now.x;
-            if (!(at >= 16.0f && at < 8192.0f)) now = row_scale(bound);
+            if (!(at >= 512.0f && at < 8192.0f)) now = row_scale(bound);
             return now;
         }
     };
@@ -1160,17 +1164,18 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         const int64_t at = ((static_cast<int64_t>(slot) * a.v_heads + h) * DK + part * C::kPart) * a.dv + col;
         const unsigned char* v_at = smem + C::kV + part * 16 * 256 + row * 2;      // this thread's 16 tokens
         float most_s = 0.0f;
-        // 16 state rows of this part (batch b) as hi and lo operand, and times `keep` where the product adds to them
-        auto put_state = [&](int b, const float (&x)[16], float keep) {
+        // 16 state rows of this part (batch b) as hi and lo operand, and times `kept` = 2^11 keep where the product, its
+        // low part first, adds to them
+        auto put_state = [&](int b, const float (&x)[16], float kept) {
             uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) split_f16(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+            for (int i = 0; i < 8; ++i) split_scaled(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
             tmem_st8(lane_at + C::kSHi + part * (C::kPart / 2) + b * 8, hi);
             tmem_st8(lane_at + C::kSLo + part * (C::kPart / 2) + b * 8, lo);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) hi[i] = __float_as_uint(keep * x[e * 8 + i]);
+                for (int i = 0; i < 8; ++i) hi[i] = __float_as_uint(kept * x[e * 8 + i]);
                 tmem_st8(lane_at + C::kD3 + part * C::kPart + b * 16 + e * 8, hi);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -1182,7 +1187,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         auto put_row = [&](const float (&x)[16], uint32_t place, uint64_t* ready) {
             uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) split_f16(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+            for (int i = 0; i < 8; ++i) split_scaled(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
             tmem_st8(lane_at + place + part * 16, hi);
             tmem_st8(lane_at + place + part * 16 + 8, lo);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -1219,12 +1224,12 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             }
             measure_row(0);
             now = agree(0);
-            const float keep = scales_of(0)[4 * kChunk];
+            const float kept = kLo * scales_of(0)[4 * kChunk];
 #pragma unroll
             for (int b = 0; b < C::kBatches; ++b) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[b][i] *= now.x;
-                put_state(b, x[b], keep);
+                put_state(b, x[b], kept);
             }
         }
 
@@ -1259,10 +1264,10 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             if (lane == 0) mbar_arrive(&empty[c % C::kStages]);
             // while the last product is made: the next chunk's scale and decay
             float2 next = now;
-            float keep = 0.0f;
+            float kept = 0.0f;
             if (!last) {
                 next = agree(c + 1);
-                keep = scales_of(c + 1)[4 * kChunk];
+                kept = kLo * scales_of(c + 1)[4 * kChunk];
             }
             const float change = next.x * now.y;
             const bool changes = __any_sync(0xffffffffu, change != 1.0f), measure = (c & 3) == 0;
@@ -1287,7 +1292,7 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] *= change;
                 }
-                put_state(b, x, keep);
+                put_state(b, x, kept);
             }
             if (measure) most_s *= now.y;
             now = next;
@@ -1403,22 +1408,35 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
         for (int c = 0; c < chunks_here; ++c) {
             const uint64_t st = static_cast<uint64_t>(c % C::kStages * (C::kStage >> 4));
             const uint64_t kq = tiles + st, tp = tri + st, kt = turned + st;
-            auto state_product = [&](int k, int half) {
+            // products with a low part first, each accumulator brought to scale by its first product with a high part
+            auto state_low = [&](int k, int half) {
                 const uint64_t d = kq + half * kQ + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
-                const uint32_t to = tmem + C::kD1 + half * kChunk;
-                mma_f16_ts(to, tmem + C::kSHi + k * 8, d, kIdesc, k > 0);
-                mma_f16_ts(to, tmem + C::kSLo + k * 8, d, kIdesc, 1);
+                mma_f16_ts(tmem + C::kD1 + half * kChunk, tmem + C::kSLo + k * 8, d, kIdesc, k > 0);
             };
-            // 16 tokens reach the outputs from themselves on
+            auto state_high = [&](int half) {
+#pragma unroll
+                for (int k = 0; k < DK / 16; ++k) {
+                    const uint64_t d = kq + half * kQ + (((k >> 2) * C::kTile + (k & 3) * 32) >> 4);
+                    const uint32_t to = tmem + C::kD1 + half * kChunk;
+                    if (k == 0) mma_f16_ts_shifted<kLoBits>(to, tmem + C::kSHi, d, kIdesc);
+                    else mma_f16_ts(to, tmem + C::kSHi + k * 8, d, kIdesc, 1);
+                }
+            };
+            // 16 tokens reach the outputs from themselves on; the first 16 reach all, so their products begin and scale
             auto row_product = [&](int half) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int step = 0; step < 8; ++step) {
+                    const int k = step & 3;
                     const uint32_t to = tmem + C::kD2 + half * kChunk + k * 16, r = tmem + C::kD1 + k * 16;
                     const uint32_t idesc = instr_desc_f16(128, kChunk - k * 16);
                     const uint64_t hi = tp + ((half * kTri * 2 + tri_column(k) * 512) >> 4), lo = hi + ((2 * kTri * 2) >> 4);
-                    mma_f16_ts(to, r, hi, idesc, k > 0);
-                    mma_f16_ts(to, r + 8, hi, idesc, 1);
-                    mma_f16_ts(to, r, lo, idesc, 1);
+                    if (step < 4) {
+                        mma_f16_ts(to, r + 8, hi, idesc, k > 0);
+                    } else {
+                        if (k == 0) mma_f16_ts_shifted<kLoBits>(to, r, hi, idesc);
+                        else mma_f16_ts(to, r, hi, idesc, 1);
+                        mma_f16_ts(to, r, lo, idesc, 1);
+                    }
                 }
             };
             wait_one(&full[c % C::kStages], c / C::kStages);
@@ -1429,8 +1447,11 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = b; k < DK / 16; k += C::kBatches) state_product(k, 0);
-                    if (b == C::kBatches - 1) mma_commit(&made[0]);
+                    for (int k = b; k < DK / 16; k += C::kBatches) state_low(k, 0);
+                    if (b == C::kBatches - 1) {
+                        state_high(0);
+                        mma_commit(&made[0]);
+                    }
                 }
                 __syncwarp();
             }
@@ -1438,7 +1459,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < DK / 16; ++k) state_product(k, 1);
+                for (int k = 0; k < DK / 16; ++k) state_low(k, 1);
+                state_high(1);
             }
             __syncwarp();
             wait_one(&r_ready, c);
@@ -1454,10 +1476,10 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    mma_f16_ts(tmem + C::kD3, tmem + C::kD2 + k * 16, kt + k * 128, kIdescT, 1);
-                    mma_f16_ts(tmem + C::kD3, tmem + C::kD2 + k * 16 + 8, kt + k * 128, kIdescT, 1);
-                }
+                for (int k = 0; k < 4; ++k) mma_f16_ts(tmem + C::kD3, tmem + C::kD2 + k * 16 + 8, kt + k * 128, kIdescT, 1);
+                mma_f16_ts_shifted<kLoBits>(tmem + C::kD3, tmem + C::kD2, kt, kIdescT);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) mma_f16_ts(tmem + C::kD3, tmem + C::kD2 + k * 16, kt + k * 128, kIdescT, 1);
                 mma_commit(&made[2]);
                 mma_commit(&empty[c % C::kStages]);
             }

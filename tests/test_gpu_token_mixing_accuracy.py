@@ -1,5 +1,5 @@
 """What the token-mixing operators keep of small terms beside large ones: the
-tail of a softmax under one dominant key.
+tail of a softmax under one dominant key, the fp32 states of prompts.
 
 Attention's bounds are those of test_gpu_token_mixing, with weights kept to 22
 bits or to 2^-40 of the largest one's size.  An output is one rounding to fp16
@@ -7,12 +7,18 @@ away from fp32's, so what single outputs cannot show is looked for in their
 mean: roundings to nearest are independent of each other and off by at most half
 a step, 2^-11 of the value, 2^-11 / sqrt(3) in root mean square, so the mean
 relative error of N outputs stays within six times 2^-11 / sqrt(3 N).
+
+A prompt's final states are compared with the recurrence in fp64; they may be
+off by eight times what the plain recurrence in fp32 is off by on the same
+inputs (chunks round other terms in another order: half to twice of it is
+expected, one fp16 operand without its low part makes it a thousand times),
+and by the absolute error that the header allows.
 """
 import math
 
 import pytest
 
-from test_gpu_token_mixing import attention_setup, close16, gen
+from test_gpu_token_mixing import attention_setup, close16, delta_inputs, gen, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +108,83 @@ def test_attention_weights_keep_their_low_bits(cuda, exponent):
     mean, count = weights_check(torch, q, keys, scale, out, lse, "equal weights")
     # the score, 2^exponent's logarithm, is a product and a sum in fp32: up to 20 (2^-24 + 2^-24) of the weights more
     assert mean <= 6 * 2.0 ** -11 / math.sqrt(3 * count) + 2.0 ** -18, mean
+
+
+# ---- the gated delta rule: states of prompts -------------------------------------------
+
+def recurrence(torch, q, k, v, g, beta, s, dtype):
+    """Token by token, in this type, with q and k normalised."""
+    r = v.shape[1] // q.shape[1]
+
+    def prep(x):
+        x = x.to(dtype)
+        return (x / torch.sqrt((x * x).sum(-1, keepdim=True) + 1e-6)).repeat_interleave(r, dim=1)
+
+    q, k, v, beta = prep(q), prep(k), v.to(dtype), beta.to(dtype)
+    decay = torch.exp(g.to(dtype))
+    s = s.to(dtype).clone()
+    out = torch.empty_like(v)
+    for t in range(v.shape[0]):
+        s = s * decay[t][:, None, None]
+        u = beta[t][:, None] * (v[t] - (s * k[t][:, :, None]).sum(1))
+        s = s + k[t][:, :, None] * u[:, None]
+        out[t] = (s * q[t][:, :, None]).sum(1)
+    return out, s
+
+
+def prompt(torch, g, kind, n, hk, hv, dk, dv):
+    q, k, v, gl, beta = delta_inputs(torch, g, n, hk, hv, dk, dv)
+    v = v.clone()
+    start = randn(g, 1, hv, dk, dv, dtype=torch.float32)
+    if kind.startswith("reset"):          # one large value, small ones behind it, and a decay between them
+        v *= 0.01
+        v[0] = 30000.0
+        start.zero_()
+        gl[8] = -float(kind[5:])
+    elif kind == "forget":
+        gl[::7] = -300.0
+        gl[50] = -math.inf
+    elif kind == "keep":
+        gl.zero_()
+    elif kind == "write":
+        beta.fill_(1.0)
+        gl.zero_()
+        k = k[:1].expand(n, hk, dk).contiguous()
+    elif kind == "mixed":
+        gl = gl * torch.randint(0, 2, gl.shape, generator=g, device="cuda") * 40
+    elif kind == "steps":                 # values of another size every 50 tokens, long-lived states
+        e = torch.randint(-7, 8, (n // 50 + 1,), generator=g, device="cuda").repeat_interleave(50)[:n]
+        v *= (2.0 ** e.float()).half()[:, None, None]
+        gl *= 0.1
+    return q, k, v, gl, beta, start
+
+
+@pytest.mark.parametrize("heads", [2, 20, 40])     # one and two column groups a block, whole heads
+@pytest.mark.parametrize("kind,n", [("plain", 64), ("plain", 700), ("reset40", 64), ("reset40", 200), ("forget", 200),
+                                    ("keep", 200), ("write", 200), ("mixed", 200), ("steps", 900)])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_prefill_states(cuda, heads, kind, n, dk):
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(n + heads + dk)
+    hk = heads // 2 if kind == "plain" else heads
+    q, k, v, gl, beta, start = prompt(torch, g, kind, n, hk, heads, dk, 128)
+    out, new = torch.empty(n, heads, 128, dtype=torch.float16, device="cuda"), torch.empty_like(start)
+    ws = mcv.gated_delta_workspace(n, 1, heads, dk, 128)
+    mcv.device_errors()
+    mcv.gated_delta_prefill(q, k, v, gl, beta, torch.tensor([0, n], dtype=torch.int32, device="cuda"), start, out, ws,
+                            state_out=new, scale=1.0, l2_eps=1e-6)
+    assert mcv.device_errors() == 0
+    ref_out, ref = recurrence(torch, q, k, v, gl, beta, start[0], torch.float64)
+    fp32_out, fp32 = recurrence(torch, q, k, v, gl, beta, start[0], torch.float32)
+    # 2^-36, where whole heads are taken of the largest value or state
+    large = max(1.0, v.abs().max().item(), start.abs().max().item()) if heads == 40 else 1.0
+    least = 2.0 ** -36 * large
+    err, plain = (new[0].double() - ref).abs().max().item(), (fp32.double() - ref).abs().max().item()
+    assert err <= 8 * plain + least, f"states off by {err:.3g}, fp32's by {plain:.3g}, absolute {least:.3g}"
+    # an output's error is that of a state's column times q of norm 1, and its rounding
+    wrong = (out.double() - ref_out).abs() - 2.0 ** -11 * ref_out.abs() - 2.0 ** -25
+    off = (fp32_out.double() - ref_out).abs()
+    for rows in (slice(0, 9), slice(9, None)):
+        err, plain = wrong[rows].max().item(), off[rows].max().item()
+        assert err <= 8 * plain + math.sqrt(dk) * least, f"outputs off by {err:.3g}, fp32's by {plain:.3g}"
