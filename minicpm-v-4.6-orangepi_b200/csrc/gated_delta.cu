@@ -169,7 +169,9 @@ int run_step(const DeltaArgs& a, int dk, cudaStream_t stream) {
 // accumulation.  The other operands (S, T, P T, R, U) are split as hi + 2^-11 lo,
 // both fp16, the lo products in accumulators of their own: 22 bits of each
 // value, down to an absolute 2^-36, so results keep fp32's accuracy where
-// a single fp16 operand would leave 2^-11.  (State values and written rows are
+// a single fp16 operand would leave 2^-11.  T, P T and the blocks that they are made
+// from are bounded and kept times 2^13 and 2^12, for they meet the largest values: a
+// decayed element of 2^-20 has its 22 bits too.  (State values and written rows are
 // below fp16's 65504 then; with |k| <= 1, beta <= 2 and g <= 0 they are bounded by
 // the state's start and twice the sum of |v|.)
 constexpr int kChunk = 64;
@@ -178,18 +180,23 @@ constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;      // 2^kLoBits
 
 __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uint32_t& lo) {
     hi = h2_as_u32(__floats2half2_rn(x, y));
-    fma2_f16_f32(x, y, hi, 0xbc00bc00u);      // - 1 hi
-    lo = h2_as_u32(__floats2half2_rn(x * kLo, y * kLo));
+    // 2^11 x - 2^11 hi, exact
+    asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %2};\n\tmul.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(kLo));
+    fma2_f16_f32(x, y, hi, 0xe800e800u);
+    lo = h2_as_u32(__floats2half2_rn(x, y));
 }
 
 // One chunk's share of the workspace: T and P T (its rows for q of norm 1 or less),
-// both at most 4 in magnitude (1 with beta <= 1) and kept times 2^13 as hi + lo, and the scales.  Of the
+// both at most 4 in magnitude (1 with beta <= 1) and kept times 2^13 as hi + 2^-11 lo, and the scales.  Of the
 // two matrices only the 16x16 blocks on and below the diagonal are kept, block column
 // after block column, each block as four 8x8 matrices of 128 contiguous bytes:
 // fragments are written and read whole, ldmatrix hits no bank twice, a block
 // column is an MMA's operand of 64 - 16 j rows, and a chunk is one copy.
 constexpr int kTri = 40 * 64;        // elements of a triangle
 constexpr float kTriScale = 8192.0f;
+constexpr float kBlockScale = 4096.0f;      // of the chunk kernel's blocks: A, P, X and A X are at most 2 in magnitude
 struct Chunk {
     __half tp[2][2][kTri];           // [hi, lo][T, P T]
     float ck[kChunk];                // e^G r_k
@@ -379,7 +386,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
         if (tid == kChunk - 1) out.keep = eg;
         if (tid >= 16) {
             const float f = decay_between(make_float2(r.x, r.y), g_at((tid & ~15) - 1));
-            row_by[tid] = make_float2(f * r.z * bt[tid], f * r.w);
+            row_by[tid] = make_float2(f * r.z * bt[tid] * kBlockScale, f * r.w * kBlockScale);
         }
     }
     if (tid >= 32) {
@@ -469,7 +476,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
                         const float4 col = rows[bi * 16 + c];
                         const float w = decay_between(make_float2(mine.x, mine.y), make_float2(col.x, col.y)) * col.z;
                         diag[r * M::kDiagRow + c] = c < r ? w * write * kk[j][q][e + i] : 0.0f;
-                        qk[j][q][e + i] = c <= r ? w * mine.w * qk[j][q][e + i] : 0.0f;
+                        qk[j][q][e + i] = c <= r ? w * (mine.w * kBlockScale) * qk[j][q][e + i] : 0.0f;
                     }
             }
         }
@@ -506,7 +513,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[q][e] = yl[q][e] = 0.0f;
     };
-    // (y, yl) += block at `left` times block at `right`
+    // (y, yl) += block at `left` times block at `right`; finish leaves y in the blocks' scale
     auto times = [&](int left, int right) {
         Split4 l, r;
         ldsm4(l.hi, base + left + lane * 16);
@@ -519,9 +526,9 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[q][e] = sign * (y[q][e] + kLoInv * yl[q][e]);
+            for (int e = 0; e < 4; ++e) y[q][e] = (sign / kBlockScale) * (y[q][e] + kLoInv * yl[q][e]);
     };
-    // y times beta 2^13 as block (i, j) of the record's T (0) or P T (1)
+    // y times beta (2^13 in all) as block (i, j) of the record's T (0) or P T (1)
     auto record = [&](int which, int i, int j) {
         const int in = tri_block(i, j) * 256 + g * 8 + t * 2;
 #pragma unroll
@@ -530,7 +537,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
                 uint32_t u, l;
-                split_f16(y[q][e] * (b.x * kTriScale), y[q][e + 1] * (b.y * kTriScale), u, l);
+                split_scaled(y[q][e] * (b.x * (kTriScale / kBlockScale)), y[q][e + 1] * (b.y * (kTriScale / kBlockScale)), u, l);
                 const int at = in + (e / 2) * 128 + q * 64;
                 *reinterpret_cast<uint32_t*>(&out.tp[0][which][at]) = u;
                 *reinterpret_cast<uint32_t*>(&out.tp[1][which][at]) = l;
@@ -551,7 +558,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[q][e] = diag[(g + (e >> 1) * 8) * M::kDiagRow + q * 8 + 2 * t + (e & 1)];
+        for (int e = 0; e < 4; ++e) y[q][e] = kBlockScale * diag[(g + (e >> 1) * 8) * M::kDiagRow + q * 8 + 2 * t + (e & 1)];
     put_x(own, own);
     __syncthreads();
     auto y_at = [](int i, int j) { return M::kY + ((i - 2) * 2 + j) * 1024; };
@@ -788,7 +795,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
                 for (int n = 0; n < 2; ++n) {
                     mma16816(x[n], rh, ph[2 * n], ph[2 * n + 1]);
                     mma16816(ol[n], rl, ph[2 * n], ph[2 * n + 1]);
-                    mma16816(x[n], rh, pl[2 * n], pl[2 * n + 1]);
+                    mma16816(ol[n], rh, pl[2 * n], pl[2 * n + 1]);
                 }
             }
 #pragma unroll
@@ -896,7 +903,7 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
             for (int n = 0; n < 2; ++n) {
                 mma16816(x[n], rh, th[2 * n], th[2 * n + 1]);
                 mma16816(xl[n], rl, th[2 * n], th[2 * n + 1]);
-                mma16816(x[n], rh, tl[2 * n], tl[2 * n + 1]);
+                mma16816(xl[n], rh, tl[2 * n], tl[2 * n + 1]);
             }
         }
 #pragma unroll
@@ -1432,10 +1439,11 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                     const uint64_t hi = tp + ((half * kTri * 2 + tri_column(k) * 512) >> 4), lo = hi + ((2 * kTri * 2) >> 4);
                     if (step < 4) {
                         mma_f16_ts(to, r + 8, hi, idesc, k > 0);
-                    } else {
-                        if (k == 0) mma_f16_ts_shifted<kLoBits>(to, r, hi, idesc);
-                        else mma_f16_ts(to, r, hi, idesc, 1);
                         mma_f16_ts(to, r, lo, idesc, 1);
+                    } else if (k == 0) {
+                        mma_f16_ts_shifted<kLoBits>(to, r, hi, idesc);
+                    } else {
+                        mma_f16_ts(to, r, hi, idesc, 1);
                     }
                 }
             };

@@ -160,8 +160,9 @@ def prompt(torch, g, kind, n, hk, hv, dk, dv):
 
 
 @pytest.mark.parametrize("heads", [2, 20, 40])     # one and two column groups a block, whole heads
-@pytest.mark.parametrize("kind,n", [("plain", 64), ("plain", 700), ("reset40", 64), ("reset40", 200), ("forget", 200),
-                                    ("keep", 200), ("write", 200), ("mixed", 200), ("steps", 900)])
+@pytest.mark.parametrize("kind,n", [("plain", 64), ("plain", 700), ("reset40", 64), ("reset40", 200), ("reset14", 64),
+                                    ("reset14", 200), ("forget", 200), ("keep", 200), ("write", 200), ("mixed", 200),
+                                    ("steps", 900)])
 @pytest.mark.parametrize("dk", [64, 128])
 def test_prefill_states(cuda, heads, kind, n, dk):
     import mcv_b200 as mcv
