@@ -130,9 +130,11 @@ __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const _
     const uint4* qp = reinterpret_cast<const uint4*>(a.q + tok * a.q_ts + q0 * a.q_hs) + vec;
     const int64_t qs = step * a.q_hs / 8;
     const int index = a.k ? a.index[tok] : -1, row = a.k && a.seq ? a.seq[tok] : tok;
+    // plain loads: in place other warps write rows in the same 32-byte sectors, and a preceding kernel may still write q, k
+    // and v while this one starts, both of which the read-only path does not allow
     uint4 xq[kQRows], xk[kKvRows], xv[kKvRows];
 #pragma unroll
-    for (int r = 0; r < kQRows; ++r) xq[r] = q0 + r * step < q_heads ? __ldg(qp + r * qs) : make_uint4(0, 0, 0, 0);
+    for (int r = 0; r < kQRows; ++r) xq[r] = q0 + r * step < q_heads ? qp[r * qs] : make_uint4(0, 0, 0, 0);
     const uint4 *kp = nullptr, *vp = nullptr;
     int64_t ks = 0, vs = 0, place = -1;
     const int shift = (a.q_heads + kPer - 1) / kPer, kv0 = ((mine - shift) & ((1 << a.share) - 1)) * kPer + sub;
@@ -145,8 +147,8 @@ __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const _
 #pragma unroll
         for (int r = 0; r < kKvRows; ++r) {
             const bool there = kv0 + r * step < a.kv_heads;
-            xk[r] = there ? __ldg(kp + r * ks) : make_uint4(0, 0, 0, 0);
-            xv[r] = there ? __ldg(vp + r * vs) : make_uint4(0, 0, 0, 0);
+            xk[r] = there ? kp[r * ks] : make_uint4(0, 0, 0, 0);
+            xv[r] = there ? vp[r * vs] : make_uint4(0, 0, 0, 0);
         }
     }
     for (int i = lane; i < half; i += 32) turns[warp][i] = turn_of(spec, a, tok, i);
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const _
         qp += kQRows * qs;
         op += kQRows * os;
 #pragma unroll
-        for (int r = 0; r < kQRows; ++r) xq[r] = q0 + base + r * step < q_heads ? __ldg(qp + r * qs) : make_uint4(0, 0, 0, 0);
+        for (int r = 0; r < kQRows; ++r) xq[r] = q0 + base + r * step < q_heads ? qp[r * qs] : make_uint4(0, 0, 0, 0);
     }
     if (place < 0) return;
     const int64_t head = static_cast<int64_t>(a.page_size) * a.dim, cs = step * head / 8;
@@ -196,8 +198,8 @@ __global__ void __launch_bounds__(kWarps * 32, BLOCKS) mrope_rows_kernel(const _
 #pragma unroll
         for (int r = 0; r < kKvRows; ++r) {
             const bool there = kv0 + base + r * step < a.kv_heads;
-            xk[r] = there ? __ldg(kp + r * ks) : make_uint4(0, 0, 0, 0);
-            xv[r] = there ? __ldg(vp + r * vs) : make_uint4(0, 0, 0, 0);
+            xk[r] = there ? kp[r * ks] : make_uint4(0, 0, 0, 0);
+            xv[r] = there ? vp[r * vs] : make_uint4(0, 0, 0, 0);
         }
     }
 }

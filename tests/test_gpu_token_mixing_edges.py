@@ -238,3 +238,25 @@ def test_mrope_turns_back(cuda):
     length = (x[..., :64].double() ** 2 + x[..., 64:].double() ** 2).sqrt().repeat(1, 1, 2)
     # the first rounding errs by 2^-11 in each of a pair's two, turned: sqrt 2 times that at most
     assert ((back.double() - x.double()).abs() <= (2.0 ** -11 * (1 + 2.0 ** 0.5) + 2.0 ** -19) * length + 2.0 ** -23).all()
+
+
+@pytest.mark.parametrize("dim,tokens,gap", [(64, 700, 8), (128, 33, 24), (256, 4000, 8)])
+def test_mrope_in_place_again_and_again(cuda, dim, tokens, gap):
+    """In place, with rows that share 32-byte sectors, each call's input written by the call before it, without a wait
+    between them: the same bits as call by call into fresh tensors."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(dim)
+    heads, rope = 9, mcv.MRope(dim, [dim // 2 - 8, 4, 4], interleaved=False)
+    pos = torch.randint(0, 5000, (3, tokens), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.zeros(tokens, heads, dim + gap, dtype=torch.float16, device="cuda")[:, :, :dim]
+    x.copy_(randn(g, tokens, heads, dim))
+    step = x.contiguous()
+    for _ in range(6):
+        out = torch.empty_like(step)
+        mcv.mrope(step, pos, rope, out)
+        torch.cuda.synchronize()
+        step = out
+    for _ in range(6):
+        mcv.mrope(x, pos, rope, x)
+    assert torch.equal(x, step)
