@@ -1023,21 +1023,25 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
-// Waits for an mbarrier phase suspended, 10 ms at a time and 200 times at most.
+// As mbar_wait, suspended for up to 1 ms at a time: a hint, the hardware may come back sooner, so the clock bounds the wait.
 __device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity) {
+    uint64_t t0 = 0;
 #pragma unroll 1
-    for (int i = 0; i < 200; ++i) {
+    for (uint32_t i = 0;; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity), "r"(10000000u)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
             : "memory");
         if (ok) return true;
+        if (i & 7) continue;
+        const uint64_t now = globaltimer_ns();
+        if (i == 0) t0 = now;
+        else if (now - t0 > 2000000000ull) return false;
     }
-    return false;
 }
 // 16 columns of this warp's 32 lanes, to be waited for with tmem_wait.
 __device__ __forceinline__ void tmem_get(uint32_t addr, uint32_t (&r)[16]) {
