@@ -846,9 +846,10 @@ def _setup():
         from . import _tensors
     except ImportError as e:
         raise RuntimeError("mcv_b200/_tensors.so not built; run __graft_entry__.build()") from e
-    _torch, _f16_rows, _dense, _rows_out = torch, _tensors.rows, _tensors.dense, _tensors.rows_out
+    _f16_rows, _dense, _rows_out = _tensors.rows, _tensors.dense, _tensors.rows_out
     for name in ("mrope", "mrope_append_kv", "paged_attention_decode", "gated_delta_step", "gated_delta_prefill"):
         _fns[name] = getattr(lib(), "mcv_" + name)
+    _torch = torch      # last: another thread that sees it makes its call with all of the above
     return torch
 
 
