@@ -103,7 +103,9 @@ int mcv_set_tuning(int key, int value);
  * bit 0 = a bounded wait inside a kernel gave up (that kernel returned early
  * and its outputs are incomplete); bit 1 = an index in device memory (page,
  * sequence row, state slot, sequence bound) was out of range and was not
- * followed.  Synchronises the current device. */
+ * followed; bit 2 = a gated delta prompt ended in a state that is not finite: its
+ * states or values left the range given at mcv_gated_delta_prefill, or its inputs
+ * were not finite.  Synchronises the current device. */
 unsigned mcv_device_errors(void);
 int mcv_get_tuning(int key);
 
@@ -655,8 +657,10 @@ int mcv_gated_delta_step(const mcv_gated_delta* args, int64_t batch, mcv_stream_
  * calls that may overlap on the GPU need workspaces of their own.
  * The chunks' triangular systems and split operands need log decays g <= 0,
  * 0 <= beta <= 2, keys of norm 1 or less, and states and sums of |v| below 65504
- * (the step has no such limits); accuracy is fp32's down to an absolute 2^-36 of
- * the largest of 1, |v| and the states.
+ * (the step has no such limits; where many heads are taken together larger states
+ * are right too).  A state that is infinite or NaN at the end sets bit 2 of
+ * mcv_device_errors().  Accuracy is fp32's down to an absolute 2^-36 of the largest
+ * of 1, |v| and the states.
  * Replaces linear_gated_delta_rule. */
 size_t mcv_gated_delta_workspace_size(int64_t tokens, int64_t batch, int64_t v_heads, int64_t key_dim,
                                       int64_t value_dim);

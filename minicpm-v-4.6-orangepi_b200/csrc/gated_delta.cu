@@ -947,6 +947,13 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
             for (int e = 0; e < 4; ++e) s[n][e] += kLoInv * sl[n][e];
         put_state();
     }
+    // a value beyond fp16's range makes an operand infinite and its low part too, and so the state NaN for good
+    bool finite = true;
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) finite &= isfinite(s[n][e]);
+    if (!finite && chunks_here > 0) atomicOr(&g_gated_delta_dev_error, kDevErrRange);
     if (a.state_out && live) {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
@@ -1293,6 +1300,10 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                     for (int i = 0; i < 16; ++i) most_s = fmaxf(most_s, fabsf(x[i]));
                 }
                 if (last) {
+                    bool finite = true;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) finite &= isfinite(x[i]);
+                    if (!finite) atomicOr(&g_gated_delta_dev_error, kDevErrRange);
                     if (a.state_out && live) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) a.state_out[at + static_cast<int64_t>(b * 16 + i) * a.dv] = x[i] * now.y;

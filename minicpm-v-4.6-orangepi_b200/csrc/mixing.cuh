@@ -12,6 +12,8 @@ namespace mcv {
 // device memory (page, sequence row, state slot, sequence bound) was out of
 // range.  It is never followed.
 enum : unsigned { kDevErrIndex = 2u };
+// A gated delta prompt ended in a state that is not finite.
+enum : unsigned { kDevErrRange = 4u };
 
 // Host checks; both set the error message and return a status.
 int check_rows(const char* who, const char* what, const mcv_rows* r, int64_t heads, int64_t dim);

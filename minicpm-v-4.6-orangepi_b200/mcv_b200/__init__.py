@@ -190,7 +190,8 @@ TUNE_W4A16_KSPLIT_WARPS = 10
 
 def device_errors() -> int:
     """Device-side error bits since the last call (bit 0: a bounded wait gave up;
-    bit 1: an index in device memory was out of range and not followed)."""
+    bit 1: an index in device memory was out of range and not followed; bit 2: a
+    gated delta prompt ended in a state that is not finite)."""
     return int(lib().mcv_device_errors())
 
 

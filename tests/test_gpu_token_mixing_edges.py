@@ -260,3 +260,46 @@ def test_mrope_in_place_again_and_again(cuda, dim, tokens, gap):
     for _ in range(6):
         mcv.mrope(x, pos, rope, x)
     assert torch.equal(x, step)
+
+
+@pytest.mark.parametrize("dk", [64, 128])
+@pytest.mark.parametrize("heads", [2, 20, 40])     # one and two column groups a block, whole heads
+@pytest.mark.parametrize("kind", ["start", "sum", "within"])
+def test_prefill_beyond_its_range(cuda, heads, dk, kind):
+    """States and sums of values beyond the documented range: either the result is right or the call is reported; the
+    largest within it are right and not reported."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(heads)
+    n = 130
+    q, k, v, gl, beta = delta_inputs(torch, g, n, heads, heads, dk, 128)
+    v = v.clone()
+    k = k[:1].expand(n, heads, dk).contiguous()
+    gl.zero_()
+    beta.fill_(1.0)
+    state = torch.zeros(1, heads, dk, 128, device="cuda")
+    if kind == "start":
+        state[0, 0, 3, 5] = 1.0e6
+    elif kind == "sum":           # opposite keys of one direction: u takes twice the value again and again
+        k[1::2] *= -1
+        v[:, 0, 7] = 60000.0
+    else:
+        v[0, 0, 7] = 60000.0
+    out, new = torch.empty(n, heads, 128, dtype=torch.float16, device="cuda"), torch.empty_like(state)
+    ws = mcv.gated_delta_workspace(n, 1, heads, dk, 128)
+    mcv.device_errors()
+    mcv.gated_delta_prefill(q, k, v, gl, beta, cu_of(torch, 0, n), state, out, ws, state_out=new, scale=2.0 ** -10,
+                            l2_eps=1e-6)
+    errors = mcv.device_errors()
+    assert errors == (0 if torch.isfinite(new).all() else 4)
+    if kind == "within":
+        assert errors == 0
+    elif kind == "start" and heads < 40:
+        assert errors == 4
+    if errors == 0:
+        ref, s, size = delta_ref(torch, q, k, v, gl, beta, state[0], 2.0 ** -10, 1e-6)
+        fp32 = (n + 1) * (dk + 8) * 2.0 ** -24 * size
+        assert ((new[0].double() - s).abs() <= fp32[:, None] + 2.0 ** -24 * s.abs()).all()
+    if kind != "start":           # reported without final states too
+        mcv.gated_delta_prefill(q, k, v, gl, beta, cu_of(torch, 0, n), None, out, ws, scale=2.0 ** -10, l2_eps=1e-6)
+        assert mcv.device_errors() == errors
