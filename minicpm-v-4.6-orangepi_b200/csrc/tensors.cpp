@@ -47,7 +47,7 @@ PyObject* dense_address(const at::Tensor& t, at::ScalarType type, const char* ty
     return nullptr;
 }
 
-// rows(t, what, dev): address, token and head stride of [tokens, heads, dim] fp16 with contiguous rows.
+// rows(t, what, dev): address, token and head stride (0 where there is one) of [tokens, heads, dim] fp16 with contiguous rows.
 PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!arguments(n, 3, "rows")) return nullptr;
     return guarded([&]() -> PyObject* {
@@ -61,12 +61,14 @@ PyObject* rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
             PyErr_Format(PyExc_RuntimeError, "mcv_b200: %s must be float16 [tokens, heads, dim] on cuda:%ld", what, dev);
             return nullptr;
         }
-        const auto stride = t->strides();
-        if (stride[2] != 1 && t->sizes()[2] != 1) {
+        const auto stride = t->strides(), size = t->sizes();
+        if (stride[2] != 1 && size[2] != 1) {
             PyErr_Format(PyExc_RuntimeError, "mcv_b200: rows of %s must be contiguous", what);
             return nullptr;
         }
-        return Py_BuildValue("(NLL)", address(*t), static_cast<long long>(stride[0]), static_cast<long long>(stride[1]));
+        // a dimension of size 1 is never stepped along, and may have any stride
+        return Py_BuildValue("(NLL)", address(*t), size[0] == 1 ? 0ll : static_cast<long long>(stride[0]),
+                             size[1] == 1 ? 0ll : static_cast<long long>(stride[1]));
     });
 }
 

@@ -879,12 +879,15 @@ class PagedKVCache:
             raise RuntimeError("PagedKVCache: k and v must be float16 [pages, kv_heads, page_size, head_dim]")
         if k.device != v.device or not k.is_cuda:
             raise RuntimeError("PagedKVCache: k and v must be on one CUDA device")
-        _, heads, page, dim = k.shape
-        if k.stride()[1:] != (page * dim, dim, 1) or v.stride() != k.stride():
+        pages, heads, page, dim = k.shape
+        # a dimension of size 1 is never stepped along, and may have any stride
+        apart = k.stride(0) if pages > 1 else heads * page * dim
+        want = (apart, page * dim, dim, 1)
+        if any(n > 1 and (a != w or b != w) for n, a, b, w in zip(k.shape, k.stride(), v.stride(), want)):
             raise RuntimeError("PagedKVCache: pages must be contiguous and k and v laid out alike")
         self.k, self.v = k, v
         self.dev, self.kv_heads, self.head_dim = k.get_device(), heads, dim
-        self._c = _KVCache(k.data_ptr(), v.data_ptr(), k.stride(0), k.shape[0], page, heads, dim)
+        self._c = _KVCache(k.data_ptr(), v.data_ptr(), apart, pages, page, heads, dim)
         self._ref = _ref(self._c)
 
     @classmethod

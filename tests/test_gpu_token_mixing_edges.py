@@ -303,3 +303,40 @@ def test_prefill_beyond_its_range(cuda, heads, dk, kind):
     if kind != "start":           # reported without final states too
         mcv.gated_delta_prefill(q, k, v, gl, beta, cu_of(torch, 0, n), None, out, ws, scale=2.0 ** -10, l2_eps=1e-6)
         assert mcv.device_errors() == errors
+
+
+@pytest.mark.parametrize("pages,heads,page", [(9, 1, 16), (9, 2, 1), (1, 1, 128), (1, 2, 128)])
+def test_caches_and_rows_of_size_one(cuda, pages, heads, page):
+    """Dimensions of size 1 with strides of their own - one kv head, pages of one slot, one page, one token of a row whose
+    width is no multiple of 8 - give what the dense tensors give; other layouts are refused."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(page)
+    n, dim = min(pages * page, 100), 64
+    dense = mcv.PagedKVCache(randn(g, pages, heads, page, dim), randn(g, pages, heads, page, dim))
+    shape, stride = (pages, heads, page, dim), list(dense.k.stride())
+    for i in range(3):
+        if shape[i] == 1:
+            stride[i] = 8 * (i + 1) + 1
+    odd = mcv.PagedKVCache(*(x.clone().as_strided(shape, stride) for x in (dense.k, dense.v)))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    wide = randn(g, 1, 3 * 4 * dim + 1)
+    assert wide[:, :dim].stride(0) % 8
+    q = wide[:, :4 * dim].view(1, 4, dim)
+    k, v = (wide[:, at * 4 * dim:][:, :heads * dim].view(1, heads, dim) for at in (1, 2))
+    rope, pos = mcv.MRope(dim, [dim // 2]), torch.tensor([[5]], dtype=torch.int32, device="cuda")
+    index, lengths = (torch.tensor([x], dtype=torch.int32, device="cuda") for x in (n - 1, n))
+    ws, got = mcv.paged_attention_workspace(1, 4, heads, dim), []
+    for cache, rows in ((dense, [x.contiguous() for x in (q, k, v)]), (odd, [q, k, v])):
+        turned, out = torch.empty(1, 4, dim, dtype=torch.float16, device="cuda"), torch.empty_like(q).contiguous()
+        mcv.mrope_append_kv(*rows, pos, rope, cache, table, index, turned)
+        mcv.paged_attention_decode(turned, cache, table, lengths, out, ws)
+        got.append((turned, out, cache.k.clone(), cache.v.clone()))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    for bad in (torch.empty(4, 2, dim, 16, dtype=torch.float16, device="cuda").transpose(2, 3),
+                torch.empty(4, 16, 2, dim, dtype=torch.float16, device="cuda").transpose(1, 2)):
+        with pytest.raises(RuntimeError, match="contiguous"):
+            mcv.PagedKVCache(bad, bad)
+        with pytest.raises(RuntimeError, match="laid out alike"):
+            mcv.PagedKVCache(bad.contiguous(), bad)

@@ -70,3 +70,14 @@ def test_output_over_its_input():
         mcv_b200.mrope(x, pos, rope, dense)
     with pytest.raises(RuntimeError, match="CUDA device"):      # the input itself passes this check
         mcv_b200.mrope(x, pos, rope, x)
+
+
+def test_strides_of_single_tokens_and_heads():
+    """A dimension of size 1 may have any stride: a slice of one row of a wide projection, one head of many."""
+    import mcv_b200 as mcv
+    mcv._torch or mcv._setup()
+    wide = half(1, 2049)
+    assert wide.stride(0) == 2049
+    assert mcv._f16_rows(wide[:, :2048].view(1, 8, 256), "q", -1)[1:] == (0, 256)
+    assert mcv._f16_rows(half(3, 64).as_strided((3, 1, 64), (64, 5, 1)), "q", -1)[1:] == (64, 0)
+    assert mcv._f16_rows(half(3, 2, 64), "q", -1)[1:] == (128, 64)
