@@ -1539,20 +1539,20 @@ int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     st = launch(chunk_kernel<DK>, dim3(static_cast<unsigned>(chunk_slots(a.tokens, a.batch)), a.v_heads), dim3(128),
                     kSmem, stream, a, chunks);
     if (st) return st;
-    // One column group a block while those all run at once (1.4 us a chunk), else two (2.4 us) where those take no more
-    // rounds than whole heads on the other walk (3.1 us) or few more.  16 heads of 128, all three forced:
-    //   1 sequence of 8000 tokens 209, 335, 406 us;  2 of 8000: 408, 368, 440;  4 of 4000: 413, 375, 261.
+    // The walk that takes the least time: rounds of blocks on the SMs, at 1.4 us a chunk with one column group a block,
+    // 2.4 with two, 3.1 with whole heads.  Prompts of equal lengths, all three forced (key size 128):
+    //   heads x values   16 x 128, 1 of 8000: 209, 335, 406 us   32 x 128, 2 of 8000: 408, 368, 440   64 x 128, 4 of 4000: 413, 375, 261
+    //   of 2000 tokens   200 x 16: 199, 258, 317   140 x 32: 166, 155, 183   200 x 32: 242, 261, 318   80 x 64: 181, 200, 154
     const int64_t heads = static_cast<int64_t>(a.batch) * a.v_heads;
     const int sms = sm_count();
-    if (heads * (a.dv / 16) > sms) {
-        const int64_t pairs = (heads * ((a.dv + 31) / 32) + sms - 1) / sms, whole = (heads * ((a.dv + 127) / 128) + sms - 1) / sms;
-        if (pairs * 4 <= whole * 5) return launch_scan<DK, 2>(a, chunks, stream);
-        static std::atomic<uint64_t> done_walk{0};
-        if ((st = allow_smem(walk_kernel<DK>, Walk<DK>::kSmem, done_walk))) return st;
-        return launch(walk_kernel<DK>, dim3((a.dv + 127) / 128, a.v_heads, a.batch), dim3(Walk<DK>::kThreads), Walk<DK>::kSmem,
-                      stream, a, chunks);
-    }
-    return launch_scan<DK, 1>(a, chunks, stream);
+    auto rounds = [&](int cols) { return (heads * ((a.dv + cols - 1) / cols) + sms - 1) / sms; };
+    const int64_t single = 14 * rounds(16), pairs = 24 * rounds(32), whole = 31 * rounds(128);
+    if (single <= pairs && single <= whole) return launch_scan<DK, 1>(a, chunks, stream);
+    if (pairs <= whole) return launch_scan<DK, 2>(a, chunks, stream);
+    static std::atomic<uint64_t> done_walk{0};
+    if ((st = allow_smem(walk_kernel<DK>, Walk<DK>::kSmem, done_walk))) return st;
+    return launch(walk_kernel<DK>, dim3((a.dv + 127) / 128, a.v_heads, a.batch), dim3(Walk<DK>::kThreads), Walk<DK>::kSmem, stream,
+                  a, chunks);
 }
 
 int fill_args(const char* who, const mcv_gated_delta* p, int64_t tokens, int64_t batch, DeltaArgs& a) {

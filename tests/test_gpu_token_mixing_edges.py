@@ -340,3 +340,21 @@ def test_caches_and_rows_of_size_one(cuda, pages, heads, page):
             mcv.PagedKVCache(bad, bad)
         with pytest.raises(RuntimeError, match="laid out alike"):
             mcv.PagedKVCache(bad.contiguous(), bad)
+
+
+@pytest.mark.parametrize("dk,dv,batch,heads", [(64, 16, 10, 20), (128, 16, 10, 40), (128, 32, 10, 20), (64, 32, 10, 14),
+                                               (128, 48, 5, 20), (64, 80, 3, 60)])
+def test_prefill_narrow_values(cuda, dk, dv, batch, heads):
+    """More heads than SMs with few value columns each."""
+    import mcv_b200 as mcv
+    torch = cuda
+    g = gen(dv + heads)
+    n = 70
+    q, k, v, gl, beta = delta_inputs(torch, g, batch * n, heads, heads, dk, dv)
+    state = randn(g, batch, heads, dk, dv, dtype=torch.float32)
+    out, new = torch.empty(batch * n, heads, dv, dtype=torch.float16, device="cuda"), torch.empty_like(state)
+    mcv.gated_delta_prefill(q, k, v, gl, beta, cu_of(torch, *range(0, batch * n + 1, n)), state, out,
+                            mcv.gated_delta_workspace(batch * n, batch, heads, dk, dv), state_out=new, l2_eps=1e-6)
+    for b in (0, batch // 2, batch - 1):
+        rows = slice(b * n, (b + 1) * n)
+        delta_check(torch, [x[rows] for x in (q, k, v, gl, beta)], state[b], out[rows], new[b], dk ** -0.5, 1e-6, f"sequence {b}")
