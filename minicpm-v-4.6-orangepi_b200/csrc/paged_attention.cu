@@ -44,7 +44,7 @@ constexpr int kFan = 16;       // partial results joined at a time
 constexpr int kLevels = 3;     // levels of joining: kFan^3 blocks at most
 constexpr int kMaxBatch = 4096;
 constexpr int kMinUnits = 4;   // least units of a block: one per warp
-constexpr float kPLog2 = 15.0f;   // probabilities and their sums are kept times 2^15, below fp16's 65504
+constexpr float kPLog2 = 15.0f, kPInv = 1.0f / 32768.0f;   // probabilities and their sums are kept times 2^15, below fp16's 65504
 
 static __device__ unsigned g_attention_dev_error;
 
@@ -219,7 +219,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int n, SlotOf slot
             *reinterpret_cast<uint2*>(a.out + row * D + d) =
                 make_uint2(h2_as_u32(__floats2half2_rn(acc[i].x * inv, acc[i].y * inv)),
                            h2_as_u32(__floats2half2_rn(acc[i].z * inv, acc[i].w * inv)));
-            if (d == 0 && a.lse) a.lse[row] = (all.x + (log2f(all.y) - kPLog2)) * 0.6931471805599453f;
+            if (d == 0 && a.lse) a.lse[row] = (all.x + log2f(all.y * kPInv)) * 0.6931471805599453f;
         } else {
             // each element of slot_of(0) is read and written by one thread alone, and
             // its maxima and sums were read by all before the barriers above
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, Tile<D>::kBlocksPerSm) attention_ker
                     *reinterpret_cast<uint2*>(a.out + orow * D + d) =
                         make_uint2(h2_as_u32(__floats2half2_rn(o.x * inv, o.y * inv)),
                                    h2_as_u32(__floats2half2_rn(o.z * inv, o.w * inv)));
-                    if (d == 0 && a.lse) a.lse[orow] = (top + (log2f(sum) - kPLog2)) * 0.6931471805599453f;
+                    if (d == 0 && a.lse) a.lse[orow] = (top + log2f(sum * kPInv)) * 0.6931471805599453f;
                 } else {
                     *reinterpret_cast<float4*>(mine_part.o(n * 8 + h) + d) = o;
                     if (d == 0) {

@@ -110,6 +110,28 @@ def test_attention_weights_keep_their_low_bits(cuda, exponent):
     assert mean <= 6 * 2.0 ** -11 / math.sqrt(3 * count) + 2.0 ** -18, mean
 
 
+@pytest.mark.parametrize("n", [1, 37, 3000])
+def test_attention_small_lse(cuda, n):
+    """Sums near 1: the log-sum-exp is as small as the weights behind the largest, and keeps fp32's accuracy for it."""
+    import mcv_b200 as mcv
+    torch = cuda
+    q, ck, cv, table, lengths, keys = attention_setup(torch, gen(n), [n], 2, 2, 64, 16)
+    q.zero_()
+    q[:, :, 0] = 1.0
+    i = torch.arange(n, device="cuda")
+    ck[table[0].long()[i // 16], :, i % 16] = 0.0
+    ck[table[0].long()[i[1:] // 16], :, i[1:] % 16, 0] = -16.0
+    out, lse = torch.empty_like(q), torch.empty(1, 2, device="cuda")
+    mcv.paged_attention_decode(q, mcv.PagedKVCache(ck, cv), table, lengths, out, mcv.paged_attention_workspace(1, 2, 2, 64),
+                               scale=1.0, lse=lse)
+    ref = math.log1p((n - 1) * math.exp(-16.0))
+    # Each addition to a sum near 1 rounds by at most 2^-24, half a step there; the terms are equal, so roundings may all
+    # go one way.  A sum with the largest weight in it meets one addition per unit of 16 keys of its warp, three across
+    # lanes, three across warps and one per further block (of four units or more): no more than n / 16 + 6.  The
+    # logarithm adds a few 2^-24 of its value.
+    assert ((lse.double() - ref).abs() <= (n / 16 + 8) * 2.0 ** -24).all(), (lse, ref)
+
+
 # ---- the gated delta rule: states of prompts -------------------------------------------
 
 def recurrence(torch, q, k, v, g, beta, s, dtype):
