@@ -178,13 +178,16 @@ constexpr int kChunk = 64;
 constexpr int kLoBits = 11;
 constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;      // 2^kLoBits
 
+// x *= a, y *= b in one instruction.
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %3};\n\tmul.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
 __device__ __forceinline__ void split_scaled(float x, float y, uint32_t& hi, uint32_t& lo) {
     hi = h2_as_u32(__floats2half2_rn(x, y));
-    // 2^11 x - 2^11 hi, exact
-    asm("{\n\t.reg .b64 v, f;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 f, {%2, %2};\n\tmul.rn.f32x2 v, v, f;\n\tmov.b64 {%0, %1}, v;\n\t}"
-        : "+f"(x), "+f"(y)
-        : "f"(kLo));
-    fma2_f16_f32(x, y, hi, 0xe800e800u);
+    mul2(x, y, kLo, kLo);
+    fma2_f16_f32(x, y, hi, 0xe800e800u);      // - 2^11 hi: exact
     lo = h2_as_u32(__floats2half2_rn(x, y));
 }
 
@@ -1193,7 +1196,11 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) hi[i] = __float_as_uint(kept * x[e * 8 + i]);
+                for (int i = 0; i < 8; i += 2) {
+                    float a = x[e * 8 + i], b = x[e * 8 + i + 1];
+                    mul2(a, b, kept, kept);
+                    hi[i] = __float_as_uint(a), hi[i + 1] = __float_as_uint(b);
+                }
                 tmem_st8(lane_at + C::kD3 + part * C::kPart + b * 16 + e * 8, hi);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -1264,8 +1271,13 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
                 const float4 ck = *reinterpret_cast<const float4*>(sc + i);
                 const float* cp = &ck.x;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[i + e] = __half2float(*reinterpret_cast<const __half*>(vp + (i + e) * 256)) * now.x - cp[e] * x[i + e];
+                for (int e = 0; e < 4; e += 2) {
+                    float v0 = __half2float(*reinterpret_cast<const __half*>(vp + (i + e) * 256));
+                    float v1 = __half2float(*reinterpret_cast<const __half*>(vp + (i + e + 1) * 256));
+                    mul2(v0, v1, now.x, now.x);
+                    x[i + e] = v0 - cp[e] * x[i + e];
+                    x[i + e + 1] = v1 - cp[e + 1] * x[i + e + 1];
+                }
             }
             put_row(x, C::kD1, &r_ready);
             const bool last = c + 1 == chunks_here;
@@ -1276,7 +1288,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const float4 cs = *reinterpret_cast<const float4*>(sc + 2 * kChunk + i);
-                x[i] *= cs.x, x[i + 1] *= cs.y, x[i + 2] *= cs.z, x[i + 3] *= cs.w;
+                mul2(x[i], x[i + 1], cs.x, cs.y);
+                mul2(x[i + 2], x[i + 3], cs.z, cs.w);
             }
             put_row(x, C::kD2, &w_ready);
             if (lane == 0) mbar_arrive(&empty[c % C::kStages]);
