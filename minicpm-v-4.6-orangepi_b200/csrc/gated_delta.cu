@@ -266,7 +266,7 @@ __device__ __forceinline__ void mma_split(float (&acc)[2][4], float (&acc_lo)[2]
 // X_10 and X_32, then the lower left quarter -X_B (A_BA X_A), so that no warp
 // waits for more than four steps; and P X beside and behind them.
 //
-// 8256 chunks of 64 tokens (16 heads of 128, 409 MB with what stays in L2): 136 us, 2.4 us a chunk and
+// 8256 chunks of 64 tokens (16 heads of 128, 409 MB with what stays in L2): 143 us, 2.6 us a chunk and
 // SM, where the copy rate would take 67.  Bound by its instructions and shared memory: 9200 warp
 // instructions a chunk, issued in 54 % of the cycles, shared memory busy in 67 %, DRAM in 37 %
 // (152 us before the triangle's blocks were dealt out evenly, 262 with a warp a block row).
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(128, 5) chunk_kernel(const DeltaArgs a, Chunk*
 //
 // 8000 tokens of 16 heads, one group a block: 170 us, 1.35 us a chunk (the operator's bytes would take 20), with
 // shared memory busy in three quarters of the cycles, most of that for fragments of S that eight warps
-// need; two groups 2.4 us a chunk.
+// need; two groups 2.3 us a chunk (24 bytes of a thread's registers spilled).
 template <int DK, int NG>
 struct Scan {
     static constexpr int kThreads = NG * 256 + 128;
@@ -986,9 +986,9 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 // so they are short rolled loops (straight code is fetched more slowly than it
 // runs) on many warps.
 //
-// A chunk takes 3.1 us (5600 clocks at DK = 128: E1 and E2, to R and to W, 1000 and 500, the
-// products before them 500 and 600, the state's product 1000, its pass 1500): 16000 warp
-// instructions, 67 % of the issue slots, tensor pipe 36 %.  7600 clocks with both
+// A chunk takes 3.1 us (5800 clocks at DK = 128: E1 and E2, to R and to W, 1250 and 550, the
+// products before them 700 and 600, the state's product 950, its pass 1500): 15100 warp
+// instructions, 66 % of the issue slots, tensor pipe 35 %.  7600 clocks with both
 // halves of a product in one, two stages, and copies that a warp waited for.
 //
 // A split operand is hi + 2^-11 lo here too, in one accumulator: the products with a
@@ -1001,7 +1001,8 @@ __global__ void __launch_bounds__(NG * 256 + 128, 1) scan_kernel(const DeltaArgs
 // state is; the state stays in its scale in registers.  So values keep 22 bits, or an
 // absolute 2^-45 of the bound (2^-36 in this scale) where that is more, and a factor
 // of 8 above the bound stays below fp16's end.  (With lo in the scale of hi the absolute
-// error is 2^-29 of the bound: too much for small values beside one of 30000.)
+// error is 2^-29 of the bound: too much for small values beside one of 30000.  The low parts'
+// scaling costs 3 % of a chunk's time, all of it in the passes.)
 template <int DK>
 struct Walk {
     static constexpr int kLoaders = 96;           // three warps
@@ -1129,8 +1130,8 @@ __global__ void __launch_bounds__(Walk<DK>::kThreads, 1) walk_kernel(const Delta
     int b = blockIdx.z;
     if (a.batch > 1 && a.batch <= 32) {
         // The longest sequences first: a long one begun when the others end is waited for alone (12 sequences of 50 to
-        // 4000 tokens of 16 heads: 306 us, in their own order 359).  Each warp ranks them by itself; more than a
-        // warp's lanes even out (100 sequences up to 500 tokens, ranked by the block: 360 us, not ranked 352).
+        // 4000 tokens of 16 heads: 317 us, in their own order 378).  Each warp ranks them by itself; more than a
+        // warp's lanes even out (100 sequences up to 500 tokens, ranked by the block, took 2 % longer).
         const int mine = lane < a.batch ? a.cu[lane + 1] - a.cu[lane] : 0;
         int rank = 0;
         for (int i = 0; i < a.batch; ++i) {
@@ -1553,13 +1554,13 @@ int run_chunked(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
                     kSmem, stream, a, chunks);
     if (st) return st;
     // The walk that takes the least time: rounds of blocks on the SMs, at 1.4 us a chunk with one column group a block,
-    // 2.4 with two, 3.1 with whole heads.  Prompts of equal lengths, all three forced (key size 128):
-    //   heads x values   16 x 128, 1 of 8000: 209, 335, 406 us   32 x 128, 2 of 8000: 408, 368, 440   64 x 128, 4 of 4000: 413, 375, 261
-    //   of 2000 tokens   200 x 16: 199, 258, 317   140 x 32: 166, 155, 183   200 x 32: 242, 261, 318   80 x 64: 181, 200, 154
+    // 2.3 with two, 3.1 with whole heads.  Heads of 128 keys, all three forced:
+    //   16 of 128 values, 8000 tokens: 210, 326, 427 us;  32 of 128, 8000: 408, 358, 460;  64 of 128, 4000: 413, 365, 273;
+    //   2000 tokens, 200 of 16: 199, 258, 315;  140 of 32: 167, 155, 182;  200 of 32: 242, 261, 315;  80 of 64: 181, 200, 152.
     const int64_t heads = static_cast<int64_t>(a.batch) * a.v_heads;
     const int sms = sm_count();
     auto rounds = [&](int cols) { return (heads * ((a.dv + cols - 1) / cols) + sms - 1) / sms; };
-    const int64_t single = 14 * rounds(16), pairs = 24 * rounds(32), whole = 31 * rounds(128);
+    const int64_t single = 14 * rounds(16), pairs = 23 * rounds(32), whole = 31 * rounds(128);
     if (single <= pairs && single <= whole) return launch_scan<DK, 1>(a, chunks, stream);
     if (pairs <= whole) return launch_scan<DK, 2>(a, chunks, stream);
     static std::atomic<uint64_t> done_walk{0};
