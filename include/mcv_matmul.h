@@ -659,8 +659,9 @@ int mcv_gated_delta_step(const mcv_gated_delta* args, int64_t batch, mcv_stream_
  * 0 <= beta <= 2, keys of norm 1 or less, and states and sums of |v| below 65504
  * (the step has no such limits; where many heads are taken together larger states
  * are right too).  A state that is infinite or NaN at the end sets bit 2 of
- * mcv_device_errors().  Accuracy is fp32's down to an absolute 2^-36 of the largest
- * of 1, |v| and the states.
+ * mcv_device_errors().  Operands keep 22 bits, down to an absolute 2^-36 of the
+ * largest of 1, |v| and the states, and sums are fp32, so that results are as
+ * accurate as the recurrence in fp32.
  * Replaces linear_gated_delta_rule. */
 size_t mcv_gated_delta_workspace_size(int64_t tokens, int64_t batch, int64_t v_heads, int64_t key_dim,
                                       int64_t value_dim);
